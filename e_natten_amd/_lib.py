@@ -10,6 +10,7 @@ LIB_PATH = os.path.join(_HERE, "libenatten.so")
 
 ABI_VERSION = 5  # ENATTEN_ABI_VERSION of include/enatten.h
 F32, BF16, F16, F64 = 0, 1, 2, 3
+I32, I64, I8, E4M3 = 16, 17, 18, 19
 STATIC_BWD_MAX_QUERIES = 1 << 20
 PATH_NONE, PATH_SIMT, PATH_MFMA, PATH_MFMA_FUSED, PATH_MFMA_SPLIT = 0, 1, 2, 3, 4
 PATH_MFMA_SPLIT_QUEUE = 5
@@ -43,6 +44,11 @@ SIGNATURES = {
     "enatten1d_bwd_workspace_bytes": (ctypes.c_size_t, [_i] * 3),
     "enatten1d_bwd": (_i, [_vp] * 10 + [_i] * 6 + [_sp] * 5 + [ctypes.c_float, _vp]),
     "enatten1d_bwd_into": (_i, [_vp] * 10 + [_i] * 6 + [_sp] * 6 + [ctypes.c_float, _vp]),
+    "enatten_rotary": (_i, [_vp] * 6 + [_i] * 11 + [_sp] * 4 + [ctypes.c_int64, ctypes.c_double, _vp]),
+    "enatten_cache_append": (_i, [_vp] * 9 + [_i] * 9 + [_sp] * 6 + [ctypes.c_int64, _vp]),
+    "enatten_cache_attention_workspace_bytes": (ctypes.c_size_t, [_i] * 9),
+    "enatten_cache_attention": (_i, [_vp] * 10 + [_i] * 11 + [_sp] * 6
+                                + [ctypes.c_int64, ctypes.c_float, _vp]),
     "enatten_profile_enable": (_i, [_i]),
     "enatten_profile_read": (_i, [_i, ctypes.POINTER(_i), ctypes.POINTER(ctypes.c_double)]),
     "enatten_profile_read_overhead": (_i, [_i, ctypes.POINTER(ctypes.c_double)]),
@@ -81,6 +87,11 @@ def last_error() -> str:
 def strides3(t) -> ctypes.Array:
     """Element strides of the (batch, head, position) axes as int64_t[3]."""
     return (ctypes.c_int64 * 3)(*t.stride()[:3])
+
+
+def strides2(t) -> ctypes.Array:
+    """Element strides of the first two axes as int64_t[2]."""
+    return (ctypes.c_int64 * 2)(*t.stride()[:2])
 
 
 def strides4(t) -> ctypes.Array:

@@ -20,7 +20,9 @@ SOURCES = ["na2d_mfma.hip", "na2d_mfma_narrow.hip", "na2d_mfma_dilated.hip", "na
            "na2d_mfma_two_terms.hip", "na2d_mfma_small.hip",
            "enatten_capi.hip", "enatten_prof.cpp", "na2d_simt.hip",
            "na2d_f64.hip", "na2d_mfma_fused.hip", "na2d_mfma_onepass.hip", "na2d_mfma_f32.hip", "na1d_mfma.hip",
-           "na1d_mfma_narrow.hip", "na1d_band_mfma.hip"]
+           "na1d_mfma_narrow.hip", "na1d_band_mfma.hip", "rotary.hip", "cache_append.hip",
+           "cache_attention.hip"]
+TORCH_SOURCES = ["torch_shim.cpp", "torch_sequence.cpp"]
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -67,18 +69,28 @@ def _build_torch_shim() -> str:
     import torch
     from torch.utils import cpp_extension
     tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch.compiled_with_cxx11_abi()),
-           "-I", os.path.join(ROOT, "include")]
+    flags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch.compiled_with_cxx11_abi()),
+             "-I", os.path.join(ROOT, "include")]
     for inc in cpp_extension.include_paths():
-        cmd += ["-isystem", inc]
-    cmd += ["-isystem", "/opt/rocm/include", os.path.join(CSRC, "torch_shim.cpp"), "-o", TORCH_LIB,
-            "-L", HERE, "-lenatten", "-L", tlib, "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch",
-            "-Wl,-rpath,$ORIGIN", "-Wl,--no-as-needed"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError("building the torch binding failed:\n%s" % r.stderr[-4000:])
+        flags += ["-isystem", inc]
+    flags += ["-isystem", "/opt/rocm/include"]
+
+    def run(cmd):
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError("building the torch binding failed:\n%s" % r.stderr[-4000:])
+
+    def compile_one(src):
+        obj = os.path.join(OBJ, os.path.splitext(src)[0] + ".o")
+        run(["g++", *flags, "-c", os.path.join(CSRC, src), "-o", obj])
+        return obj
+
+    with ThreadPoolExecutor(max_workers=len(TORCH_SOURCES)) as ex:
+        objs = list(ex.map(compile_one, TORCH_SOURCES))
+    run(["g++", "-shared", *objs, "-o", TORCH_LIB, "-L", HERE, "-lenatten", "-L", tlib, "-lc10",
+         "-lc10_hip", "-ltorch_cpu", "-ltorch", "-Wl,-rpath,$ORIGIN", "-Wl,--no-as-needed"])
     return TORCH_LIB
 
 
@@ -93,7 +105,8 @@ def build(verbose: bool = False, incremental: bool = False) -> str:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("link failed:\n%s" % r.stderr[-4000:])
-    shim_deps = [os.path.join(CSRC, "torch_shim.cpp"), os.path.join(ROOT, "include", "enatten.h")]
+    shim_deps = [os.path.join(CSRC, f) for f in (*TORCH_SOURCES, "torch_shim.h")]
+    shim_deps.append(os.path.join(ROOT, "include", "enatten.h"))
     if not (incremental and os.path.exists(TORCH_LIB) and
             all(os.path.getmtime(d) <= os.path.getmtime(TORCH_LIB) for d in shim_deps)):
         _build_torch_shim()

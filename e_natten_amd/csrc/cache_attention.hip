@@ -1,0 +1,699 @@
+// Attention of a sequence's last tokens over its cache of 8-bit codes (enatten_cache_attention).
+//
+//   o = sum_j p_j z'_j v_j / sum_j p_j,   p_j = exp(scale z_j q.k_j - m),   j over the visible tokens
+//
+// with codes k_j, v_j and the scales z_j, z'_j of their blocks (page, head).  All query heads that share
+// a head of the cache, and all new tokens, are rows of one problem per (sequence, cache head): a row tile
+// of 16, 32 or 64 of them goes over the tokens once, with the running maximum and sum of the softmax.
+//
+// Products.  Codes are numbers that float16 holds exactly (int8 as they are, E4M3 times 2^-8, by integer
+// operations on their bits), so both products run on the float16 matrix instructions whatever the type
+// of q: rows of q are multiplied by a power of two that brings their largest value to 2^14 .. 2^15, which
+// leaves bfloat16 values exact down to 2^-28 of the largest; float32 rows are the sum of two such terms.
+// The logits come out in float32 and take scale, z_j and the power of two there.
+//
+// The first product forms S^T = K Q^T: a lane then holds 4 tokens of one row, and the softmax's
+// statistics are one value per lane.  The order of the tokens within the second product's sum is free,
+// so O^T = V^T P^T takes the probabilities from the registers where the first product left them, and V
+// with the same permutation: lane (m, g) reads channels m * D/16 .. of tokens 4g .. 4g+3 of both halves
+// of a tile of 32.  Neither K, V nor P passes through LDS.
+//
+// The probabilities go into the second product as float16, times z'_j over the largest power of two
+// among the z' so far, times 2^14: 11 bits for all that is above 2^-28 of the largest (two terms for
+// float32).  Where z' outgrows that power of two, the sums so far are scaled down, as they are for the
+// maximum.
+//
+// What bounds it.  One token of a sequence: every code is read once, two products of 16 rows cost a few
+// percent of the matrix cores: HBM.  Work is split along the tokens so that the chip is filled whatever
+// the number of sequences and heads; the parts leave their sums, maximum and output in the workspace and
+// a second launch joins them.  The split goes by the lengths of this call, which are on the device:
+// every workgroup computes it for itself.
+#include "sequence_common.h"
+
+namespace enatten {
+namespace {
+
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kFloor = -1e37f;  // the maximum of a row that has seen nothing: finite, below every logit
+constexpr int kTile = 32;         // tokens of a step
+constexpr int kTop = 14;          // float16 operands are brought to 2^kTop
+
+struct AttnArgs {
+    Rows q, o;
+    Cache k, v;
+    Table tb;
+    int B, heads, group, heads_kv, T, D, window;  // group: query heads of a cache head
+    int dtype;
+    int row_tiles;   // per (sequence, cache head)
+    int parts;       // workgroups per cache head that the split aims at; 0: one per row tile
+    float scale;
+    float *ws;       // [item][cache head]: row maxima, row sums, rows x D sums
+};
+
+// The tokens that one row tile sees: [lo, hi), hi <= lo if none.
+struct Span {
+    int len, count, start, lo, hi;
+    bool ok;
+};
+template <int ROWS>
+__device__ __forceinline__ Span span_of(const AttnArgs &a, int entry) {
+    Span s;
+    const int b = entry / a.row_tiles, tile = entry - b * a.row_tiles;
+    s.ok = sequence_of(a.tb, b, s.len, s.count);
+    s.start = s.len - s.count;
+    const int first = tile * ROWS / a.group, last = min((tile * ROWS + ROWS - 1) / a.group, s.count - 1);
+    s.lo = s.hi = 0;
+    if (first < s.count) {
+        s.lo = a.window ? max(s.start + first - a.window + 1, 0) : 0;
+        s.hi = s.start + last + 1;
+    }
+    return s;
+}
+__device__ __forceinline__ int steps_of(const Span &s) { return s.hi > s.lo ? (s.hi - (s.lo & -16) + kTile - 1) / kTile : 0; }
+
+// How the row tiles ("entries") are cut into items of at most `chunk` steps; the same in every wave.
+__device__ __forceinline__ int wave_sum(int x) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
+    return x;
+}
+template <int ROWS>
+__device__ __forceinline__ int chunk_of(const AttnArgs &a) {
+    const int entries = a.B * a.row_tiles, lane = threadIdx.x & 63;
+    long long total = 0;
+    for (int e0 = 0; e0 < entries; e0 += 64) {
+        const int e = e0 + lane;
+        total += wave_sum(e < entries ? steps_of(span_of<ROWS>(a, e)) : 0);
+    }
+    // at least 8 steps each: two per wave
+    return max(8, (int)((total + a.parts - 1) / a.parts));
+}
+__device__ __forceinline__ int items_of(int steps, int chunk) { return max(1, (steps + chunk - 1) / chunk); }
+// The entry of item `item` and the number of its first item, or (by_entry) the first item of entry
+// `item`; entry -1 if there is none.
+template <int ROWS>
+__device__ __forceinline__ void find(const AttnArgs &a, int chunk, int item, bool by_entry, int &entry, int &first) {
+    const int entries = a.B * a.row_tiles, lane = threadIdx.x & 63;
+    int before = 0;
+    entry = -1;
+    first = 0;
+    for (int e0 = 0; e0 < entries; e0 += 64) {
+        const int e = e0 + lane;
+        const int n = e < entries ? items_of(steps_of(span_of<ROWS>(a, e)), chunk) : 0;
+        int upto = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_up(upto, o, 64);
+            if (lane >= o) upto += x;
+        }
+        const bool mine = by_entry ? e == item : n > 0 && item >= before + upto - n && item < before + upto;
+        const unsigned long long who = __ballot(mine);
+        if (who) {
+            const int l = __ffsll(who) - 1;
+            entry = e0 + l;
+            first = before + __shfl(upto - n, l, 64);
+            return;
+        }
+        before += __shfl(upto, 63, 64);
+    }
+}
+
+__device__ __forceinline__ f16x2 as_half(unsigned x) { return __builtin_bit_cast(f16x2, x); }
+
+// Two codes side by side, each in the upper byte of a half (E4M3) or the lower byte of a half of
+// 0x6400 (int8, offset 128), as float16.  E4M3: sign, 4 exponent and 3 mantissa bits move to the places
+// of float16's, whose exponents are offset by 8 more: the value times 2^-8.
+__device__ __forceinline__ f16x2 from_e4m3(unsigned x) {
+    const s16x2 s = __builtin_bit_cast(s16x2, x) >> 1;
+    return as_half(__builtin_bit_cast(unsigned, s) & 0xbfffbfffu);
+}
+__device__ __forceinline__ f16x2 from_int8(unsigned x) {
+    return as_half(x) + f16x2{(_Float16)-1152.f, (_Float16)-1152.f};
+}
+// 8 consecutive codes
+template <bool E4M3>
+__device__ __forceinline__ f16x8 widen_row(unsigned x0, unsigned x1) {
+    f16x2 h[4];
+    if constexpr (E4M3) {
+        h[0] = from_e4m3(__builtin_amdgcn_perm(x0, x0, 0x010c000cu));
+        h[1] = from_e4m3(__builtin_amdgcn_perm(x0, x0, 0x030c020cu));
+        h[2] = from_e4m3(__builtin_amdgcn_perm(x1, x1, 0x010c000cu));
+        h[3] = from_e4m3(__builtin_amdgcn_perm(x1, x1, 0x030c020cu));
+    } else {
+        x0 ^= 0x80808080u;
+        x1 ^= 0x80808080u;
+        h[0] = from_int8(__builtin_amdgcn_perm(0x64646464u, x0, 0x04010400u));
+        h[1] = from_int8(__builtin_amdgcn_perm(0x64646464u, x0, 0x04030402u));
+        h[2] = from_int8(__builtin_amdgcn_perm(0x64646464u, x1, 0x04010400u));
+        h[3] = from_int8(__builtin_amdgcn_perm(0x64646464u, x1, 0x04030402u));
+    }
+    return f16x8{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
+}
+// 4 channels (one word) of 8 tokens, transposed: out[i] is channel i of the 8 tokens
+template <bool E4M3>
+__device__ __forceinline__ void widen_columns(const unsigned (&t)[8], f16x8 (&out)[4]) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        f16x2 h[4];
+        if constexpr (E4M3) {
+            h[0] = from_e4m3(__builtin_amdgcn_perm(t[j + 1], t[j], 0x040c000cu));
+            h[1] = from_e4m3(__builtin_amdgcn_perm(t[j + 1], t[j], 0x050c010cu));
+            h[2] = from_e4m3(__builtin_amdgcn_perm(t[j + 1], t[j], 0x060c020cu));
+            h[3] = from_e4m3(__builtin_amdgcn_perm(t[j + 1], t[j], 0x070c030cu));
+        } else {
+            const unsigned lo = __builtin_amdgcn_perm(t[j + 1], t[j], 0x05010400u) ^ 0x80808080u;
+            const unsigned hi = __builtin_amdgcn_perm(t[j + 1], t[j], 0x07030602u) ^ 0x80808080u;
+            h[0] = from_int8(__builtin_amdgcn_perm(0x64646464u, lo, 0x04010400u));
+            h[1] = from_int8(__builtin_amdgcn_perm(0x64646464u, lo, 0x04030402u));
+            h[2] = from_int8(__builtin_amdgcn_perm(0x64646464u, hi, 0x04010400u));
+            h[3] = from_int8(__builtin_amdgcn_perm(0x64646464u, hi, 0x04030402u));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            out[i][j] = h[i][0];
+            out[i][j + 1] = h[i][1];
+        }
+    }
+}
+
+__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+// max / sum over the four lanes of a row
+__device__ __forceinline__ float row_max(float x) {
+    x = fmaxf(x, __shfl_xor(x, 16, 64));
+    return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+__device__ __forceinline__ float row_sum(float x) {
+    x += __shfl_xor(x, 16, 64);
+    return x + __shfl_xor(x, 32, 64);
+}
+
+__device__ __forceinline__ float load_row(const Rows &r, int dtype, int64_t at) {
+    if (dtype == ENATTEN_F32) return static_cast<const float *>(r.ptr)[at];
+    if (dtype == ENATTEN_BF16) return (float)static_cast<const __bf16 *>(r.ptr)[at];
+    return (float)static_cast<const _Float16 *>(r.ptr)[at];
+}
+__device__ __forceinline__ void store_row(const Rows &r, int dtype, int64_t at, float x) {
+    void *p = const_cast<void *>(r.ptr);
+    if (dtype == ENATTEN_F32) static_cast<float *>(p)[at] = x;
+    else if (dtype == ENATTEN_BF16) static_cast<__bf16 *>(p)[at] = (__bf16)x;
+    else static_cast<_Float16 *>(p)[at] = (_Float16)x;
+}
+
+__device__ __forceinline__ int lane_int(int x, int l) { return __builtin_amdgcn_readlane(x, l); }
+__device__ __forceinline__ float lane_float(float x, int l) {
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), l));
+}
+__device__ __forceinline__ int64_t lane_offset(int64_t x, int l) {
+    const unsigned lo = __builtin_amdgcn_readlane((int)x, l), hi = __builtin_amdgcn_readlane((int)(x >> 32), l);
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// Floats of one item's part of the workspace
+constexpr int64_t item_floats(int rows, int D) { return (int64_t)rows * (D + 2); }
+
+// DP: head_dim rounded up to 64, 128 or 256 (channels beyond D: zeros in q, any codes); R: row tiles of
+// 16 per workgroup; TERMS: float16 terms of q and p.
+template <int DP, int R, bool E4M3, int TERMS>
+__global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attend(AttnArgs a) {
+    constexpr int ROWS = 16 * R, KC = DP / 64, VW = DP / 64, DT = DP / 16;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n16 = lane & 15, g4 = lane >> 4;
+
+    // which row tile, and which of its steps
+    const int head = blockIdx.x % a.heads_kv, item = blockIdx.x / a.heads_kv;
+    int entry = item, first_item = item, chunk = 1 << 26;
+    if (a.parts) {
+        chunk = chunk_of<ROWS>(a);
+        find<ROWS>(a, chunk, item, false, entry, first_item);
+        if (entry < 0) return;
+    }
+    const Span s = span_of<ROWS>(a, entry);
+    const int b = entry / a.row_tiles, row0 = (entry - b * a.row_tiles) * ROWS;
+    const int total = steps_of(s), items = items_of(total, chunk);
+    const int step0 = min((item - first_item) * chunk, total), step1 = min(step0 + chunk, total);
+    const int base = s.lo & -16;
+
+    // q: lane (row n16, g4) has channels 64 c + 16 g4 .. + 15
+    f16x8 qf[R][KC][2][TERMS];
+    float unit[R];           // what a product of codes is multiplied by, besides z: log2 units
+    int lo_r[R], hi_r[R];    // tokens that the lane's row sees
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int row = min(row0 + r * 16 + n16, a.T * a.group - 1), t = row / a.group;
+        const int tv = min(t, max(s.count - 1, 0));
+        hi_r[r] = s.start + tv + 1;
+        lo_r[r] = a.window ? max(hi_r[r] - a.window, 0) : 0;
+        const int64_t at = b * a.q.sb + (head * a.group + row - t * a.group) * a.q.sh + t * a.q.st;
+        float x[KC][16], top = 0.f, nan = 0.f;
+#pragma unroll
+        for (int c = 0; c < KC; c++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const int d = c * 64 + g4 * 16 + j;
+                x[c][j] = d < a.D ? load_row(a.q, a.dtype, at + d) : 0.f;
+                top = fmaxf(top, fabsf(x[c][j]));
+                nan += x[c][j] * 0.f;  // a value that is not finite makes its row NaN
+            }
+        nan = row_sum(nan);
+        top = row_max(top);
+        const int e = top > 0.f ? __builtin_amdgcn_frexp_expf(top) : 0;
+        const int up = kTop + 1 - e;  // the largest to 2^14 .. 2^15
+        unit[r] = __builtin_ldexpf(a.scale * kLog2e, -up + (E4M3 ? 8 : 0)) + nan;
+#pragma unroll
+        for (int c = 0; c < KC; c++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const float y = __builtin_ldexpf(x[c][j], up);
+                const _Float16 h = (_Float16)y;
+                qf[r][c][j / 8][0][j % 8] = h;
+                if constexpr (TERMS == 2) qf[r][c][j / 8][1][j % 8] = (_Float16)(y - (float)h);
+            }
+    }
+    // between these all rows see every token
+    const int all_lo = a.window ? max(s.start + min((row0 + ROWS - 1) / a.group, s.count - 1) + 1 - a.window, 0) : 0;
+    const int all_hi = s.start + row0 / a.group + 1;
+
+    f32x4 acc[R][DT];
+    float m[R], l[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        m[r] = kFloor;
+        l[r] = 0.f;
+#pragma unroll
+        for (int i = 0; i < DT; i++) acc[r][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    int ref = -126;  // the z' so far are at most 2^ref
+
+    // the wave's steps, and the places of their two groups of 16 tokens: lane i holds group `filled` + i
+    const int quarter = (step1 - step0 + 3) / 4;
+    const int w0 = min(step0 + wave * quarter, step1), w1 = min(w0 + quarter, step1);
+    int filled = -64;
+    int64_t k_at = 0, v_at = 0;
+    float k_z = 0.f, v_z = 0.f;
+    auto fill = [&](int group) {
+        filled = group;
+        const int token = base + (group + lane) * 16;
+        k_at = v_at = 0;
+        k_z = v_z = 0.f;
+        if (token < s.hi && token >= 0) {
+            const int column = token / a.tb.page, within = token - column * a.tb.page;
+            const int at = a.tb.pages[b * a.tb.stride + column];
+            if ((unsigned)at < (unsigned)a.tb.num_pages) {
+                k_at = at * a.k.sp + head * a.k.sh + within * a.k.st;
+                v_at = at * a.v.sp + head * a.v.sh + within * a.v.st;
+                k_z = a.k.scales[at * a.k.zp + head * a.k.zh];
+                v_z = a.v.scales[at * a.v.zp + head * a.v.zh];
+            } else {
+                k_z = __uint_as_float(0x7fc00000u);
+            }
+        }
+    };
+    struct Tile {
+        u32x4 k[2][KC];
+        unsigned v[8][VW];
+        float kz[2], vz[2];
+    };
+    auto fetch = [&](int step, Tile &t) {
+        const int group = 2 * step;
+        if (group >= filled + 64) fill(group);
+        const char *kc = static_cast<const char *>(a.k.codes), *vc = static_cast<const char *>(a.v.codes);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int at = group + h - filled;
+            const char *kp = kc + lane_offset(k_at, at), *vp = vc + lane_offset(v_at, at);
+            t.kz[h] = lane_float(k_z, at);
+            t.vz[h] = lane_float(v_z, at);
+#pragma unroll
+            for (int c = 0; c < KC; c++) {
+                const unsigned off = n16 * (unsigned)a.k.st + min(c * 64 + g4 * 16, a.D - 16);
+                t.k[h][c] = *reinterpret_cast<const u32x4 *>(kp + off);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const unsigned off = (g4 * 4 + j) * (unsigned)a.v.st + min(n16 * DT, a.D - DT);
+                if constexpr (VW == 1) {
+                    t.v[h * 4 + j][0] = *reinterpret_cast<const unsigned *>(vp + off);
+                } else if constexpr (VW == 2) {
+                    const u32x2 x = *reinterpret_cast<const u32x2 *>(vp + off);
+                    t.v[h * 4 + j][0] = x[0];
+                    t.v[h * 4 + j][1] = x[1];
+                } else {
+                    const u32x4 x = *reinterpret_cast<const u32x4 *>(vp + off);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) t.v[h * 4 + j][c] = x[c];
+                }
+            }
+        }
+    };
+    auto work = [&](int step, const Tile &t) {
+        // a larger z' than any so far
+        const float zmax = fmaxf(fabsf(t.vz[0]), fabsf(t.vz[1]));
+        float shrink = 1.f;
+        const int e = __builtin_amdgcn_frexp_expf(zmax);
+        if (zmax < INFINITY && zmax > 0.f && e > ref) {
+            shrink = __builtin_ldexpf(1.f, max(ref - e, -200));
+            ref = e;
+        }
+        const float z0 = __builtin_ldexpf(t.vz[0], kTop - ref), z1 = __builtin_ldexpf(t.vz[1], kTop - ref);
+
+        f32x4 st[R][2];
+#pragma unroll
+        for (int r = 0; r < R; r++) st[r][0] = st[r][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int c = 0; c < KC; c++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const f16x8 kf = widen_row<E4M3>(t.k[h][c][2 * u], t.k[h][c][2 * u + 1]);
+#pragma unroll
+                    for (int r = 0; r < R; r++)
+#pragma unroll
+                        for (int i = TERMS - 1; i >= 0; i--) st[r][h] = mfma(kf, qf[r][c][u][i], st[r][h]);
+                }
+        const int token = base + step * kTile;
+        const bool whole = token >= all_lo && token + kTile <= all_hi;
+        f16x8 pf[R][TERMS];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const float u0 = unit[r] * t.kz[0], u1 = unit[r] * t.kz[1];
+            st[r][0] *= u0;
+            st[r][1] *= u1;
+            if (!whole) {
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int j = token + h * 16 + g4 * 4 + i;
+                        st[r][h][i] = j >= lo_r[r] && j < hi_r[r] ? st[r][h][i] : -INFINITY;
+                    }
+            }
+            float top = fmaxf(fmaxf(fmaxf(st[r][0][0], st[r][0][1]), fmaxf(st[r][0][2], st[r][0][3])),
+                              fmaxf(fmaxf(st[r][1][0], st[r][1][1]), fmaxf(st[r][1][2], st[r][1][3])));
+            top = fmaxf(row_max(top), m[r]);
+            const float alpha = __builtin_amdgcn_exp2f(m[r] - top);
+            m[r] = top;
+            float sum = 0.f;
+            f32x4 p[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    p[h][i] = __builtin_amdgcn_exp2f(st[r][h][i] - top);
+                    sum += p[h][i];
+                }
+            l[r] = l[r] * alpha + sum;
+            if (__any(alpha != 1.f) || shrink != 1.f) {
+                const float f = alpha * shrink;
+#pragma unroll
+                for (int i = 0; i < DT; i++) acc[r][i] *= f;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    // (a masked token's block may have a scale that is not finite)
+                    float y = p[h][i] * (h ? z1 : z0);
+                    if (!whole) y = st[r][h][i] == -INFINITY ? 0.f : y;
+                    const _Float16 w = (_Float16)y;
+                    pf[r][0][h * 4 + i] = w;
+                    if constexpr (TERMS == 2) pf[r][1][h * 4 + i] = (_Float16)(y - (float)w);
+                }
+        }
+#pragma unroll
+        for (int c = 0; c < VW; c++) {
+            unsigned x[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] = t.v[j][c];
+            f16x8 vf[4];
+            widen_columns<E4M3>(x, vf);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int k = TERMS - 1; k >= 0; k--) acc[r][c * 4 + i] = mfma(vf[i], pf[r][k], acc[r][c * 4 + i]);
+        }
+    };
+    if (w0 < w1) {
+        Tile t0, t1;
+        fetch(w0, t0);
+        int step = w0;
+        for (; step + 1 < w1; step += 2) {
+            fetch(step + 1, t1);
+            work(step, t0);
+            if (step + 2 < w1) fetch(step + 2, t0);
+            work(step + 1, t1);
+        }
+        if (step < w1) work(step, t0);
+    }
+
+    // the four waves' parts, one row tile of 16 after the other
+    __shared__ __align__(16) float part_o[4][16][DP + 4];
+    __shared__ float part_m[4][16], part_l[4][16];
+    const float back = __builtin_ldexpf(1.f, ref - kTop + (E4M3 ? 8 : 0));
+    const int mr = threadIdx.x >> 4, mc = threadIdx.x & 15;  // row and 1/16 of the channels in the merge
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        __syncthreads();
+        const float sum = row_sum(l[r]);
+        if (g4 == 0) {
+            part_m[wave][n16] = m[r];
+            part_l[wave][n16] = sum;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int c = 0; c < DT; c += 4)
+                *reinterpret_cast<f32x4 *>(&part_o[wave][n16][(g4 * 4 + i) * DT + c]) =
+                    f32x4{acc[r][c][i], acc[r][c + 1][i], acc[r][c + 2][i], acc[r][c + 3][i]} * back;
+        __syncthreads();
+        float top = part_m[0][mr], f[4], all = 0.f;
+#pragma unroll
+        for (int w = 1; w < 4; w++) top = fmaxf(top, part_m[w][mr]);
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            f[w] = __builtin_amdgcn_exp2f(part_m[w][mr] - top);
+            all += f[w] * part_l[w][mr];
+        }
+        const int row = row0 + r * 16 + mr;
+        if (row >= a.T * a.group) continue;
+        const int t = row / a.group;
+        const int64_t at = b * a.o.sb + (head * a.group + row - t * a.group) * a.o.sh + t * a.o.st;
+        const float poison = s.ok ? 0.f : __uint_as_float(0x7fc00000u);
+        const bool live = t < s.count;
+        float *part = a.ws + ((int64_t)item * a.heads_kv + head) * item_floats(ROWS, a.D);
+        if (items > 1 && mc == 0) {
+            part[r * 16 + mr] = top;
+            part[ROWS + r * 16 + mr] = all;
+        }
+        const float norm = all == 0.f ? 0.f : 1.f / all;
+#pragma unroll
+        for (int c = 0; c < DT; c++) {
+            const int d = mc * DT + c;
+            if (d >= a.D) break;
+            float y = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; w++) y += f[w] * part_o[w][mr][d];
+            if (items > 1) part[2 * ROWS + (r * 16 + mr) * a.D + d] = y;
+            else store_row(a.o, a.dtype, at + d, (live ? y * norm : 0.f) + poison);
+        }
+    }
+}
+
+// The parts of a row joined: one workgroup per (row tile, cache head, row)
+template <int ROWS>
+__global__ __launch_bounds__(256) void attend_join(AttnArgs a) {
+    const int per = min(ROWS, a.T * a.group);
+    int block = blockIdx.x;
+    const int r = block % per;
+    block /= per;
+    const int head = block % a.heads_kv, entry = block / a.heads_kv;
+    const int b = entry / a.row_tiles, row = (entry - b * a.row_tiles) * ROWS + r;
+    if (row >= a.T * a.group) return;
+    const int chunk = chunk_of<ROWS>(a);
+    const Span s = span_of<ROWS>(a, entry);
+    const int items = items_of(steps_of(s), chunk);
+    if (items == 1) return;
+    int same, first;
+    find<ROWS>(a, chunk, entry, true, same, first);
+    const int t = row / a.group;
+    const int64_t at = b * a.o.sb + (head * a.group + row - t * a.group) * a.o.sh + t * a.o.st;
+    const float *ws = a.ws + ((int64_t)first * a.heads_kv + head) * item_floats(ROWS, a.D);
+    const int64_t stride = a.heads_kv * item_floats(ROWS, a.D);
+
+    __shared__ __align__(16) float red[256][4];
+    __shared__ float top_s[4], sums[256];
+    float top = kFloor;
+    for (int i = threadIdx.x; i < items; i += 256) top = fmaxf(top, ws[i * stride + r]);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    if (threadIdx.x % 64 == 0) top_s[threadIdx.x / 64] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(top_s[0], top_s[1]), fmaxf(top_s[2], top_s[3]));
+
+    // lanes over the channels, 4 each, and the remaining factor of 256 over the items
+    const int lanes = a.D / 4, groups = 256 / lanes, c = threadIdx.x % lanes, g = threadIdx.x / lanes;
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+    if (g < groups) {
+#pragma unroll 4
+        for (int i = g; i < items; i += groups) {
+            const float *p = ws + i * stride;
+            const float f = __builtin_amdgcn_exp2f(p[r] - top);
+            sum += f * p[ROWS + r];
+            y += f * *reinterpret_cast<const f32x4 *>(p + 2 * ROWS + r * a.D + c * 4);
+        }
+    }
+    sums[threadIdx.x] = sum;
+    *reinterpret_cast<f32x4 *>(red[threadIdx.x]) = y;
+    __syncthreads();
+    if (g == 0) {
+        for (int i = 1; i < groups; i++) {
+            y += *reinterpret_cast<const f32x4 *>(red[i * lanes + c]);
+            sum += sums[i * lanes + c];
+        }
+        const float norm = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+        for (int j = 0; j < 4; j++) store_row(a.o, a.dtype, at + c * 4 + j, t < s.count ? y[j] * norm : 0.f);
+    }
+}
+
+// How a call is cut, from its sizes alone (the lengths are on the device).
+struct Plan {
+    int rows;       // of a tile
+    int row_tiles;
+    int parts;      // 0: one workgroup per row tile and cache head, no workspace
+    int64_t items;  // workgroups per cache head
+};
+Plan plan_of(int B, int heads, int heads_kv, int T, int D, int page, int columns, int window, int dtype) {
+    Plan p;
+    const int64_t all = (int64_t)T * (heads / heads_kv);
+    const int most = dtype == ENATTEN_F32 || D > 128 ? 32 : 64;
+    p.rows = all <= 16 ? 16 : all <= 32 ? 32 : most;
+    p.row_tiles = (int)((all + p.rows - 1) / p.rows);
+    const int64_t entries = (int64_t)B * p.row_tiles;
+    int64_t tokens = (int64_t)columns * page;
+    if (window && window + (int64_t)p.rows < tokens) tokens = window + (int64_t)p.rows;
+    const int64_t steps = (tokens + 15) / kTile + 1;
+    p.parts = 0;
+    p.items = entries;
+    constexpr int target = 512;
+    if (entries * heads_kv < target && steps > 8) {
+        p.parts = (target + heads_kv - 1) / heads_kv;
+        // no more than the longest possible sequences fill at 8 steps each
+        const int64_t useful = entries * ((steps + 7) / 8);
+        if (useful < p.parts) p.parts = (int)useful;
+        p.items = p.parts + entries;
+    }
+    return p;
+}
+
+template <int DP, int R, bool E4M3, int TERMS>
+int launch(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st) {
+    const int64_t blocks = p.items * a.heads_kv, rows = a.T * (int64_t)a.group;
+    const int64_t join = (int64_t)a.B * p.row_tiles * a.heads_kv * (rows < p.rows ? rows : p.rows);
+    if (blocks > 0x7fffffff || (p.parts && join > 0x7fffffff)) {
+        set_error("%s: too many row tiles", fn);
+        return ENATTEN_EUNSUPPORTED;
+    }
+    {
+        ProfScope prof(ENATTEN_KERNEL_CACHE_ATTENTION, "attend", st);
+        attend<DP, R, E4M3, TERMS><<<(int)blocks, 256, 0, st>>>(a);
+    }
+    if (p.parts) {
+        ProfScope prof(ENATTEN_KERNEL_CACHE_JOIN, "attend_join", st);
+        attend_join<16 * R><<<(int)join, 256, 0, st>>>(a);
+    }
+    return launched(fn);
+}
+template <int DP, int R, bool E4M3>
+int launch_terms(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st) {
+    if constexpr (R <= 2)
+        if (a.dtype == ENATTEN_F32) return launch<DP, R, E4M3, 2>(fn, a, p, st);
+    return launch<DP, R, E4M3, 1>(fn, a, p, st);
+}
+template <int DP, bool E4M3>
+int launch_rows(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st) {
+    if (p.rows == 16) return launch_terms<DP, 1, E4M3>(fn, a, p, st);
+    if constexpr (DP <= 128)
+        if (p.rows == 64) return launch_terms<DP, 4, E4M3>(fn, a, p, st);
+    return launch_terms<DP, 2, E4M3>(fn, a, p, st);
+}
+
+}  // namespace
+}  // namespace enatten
+
+using namespace enatten;
+
+extern "C" {
+#pragma GCC visibility push(default)
+
+size_t enatten_cache_attention_workspace_bytes(int B, int heads, int heads_kv, int T, int D, int page, int columns,
+                                               int kernel_size, int dtype) {
+    if (B < 1 || heads < 1 || heads_kv < 1 || heads % heads_kv || T < 1 || D < 1 || page < 1 || columns < 1 ||
+        kernel_size < 0)
+        return 0;
+    const Plan p = plan_of(B, heads, heads_kv, T, D, page, columns, kernel_size, dtype);
+    return p.parts ? (size_t)p.items * heads_kv * item_floats(p.rows, D) * sizeof(float) : 0;
+}
+
+int enatten_cache_attention(const void *q, const void *k_cache, const void *v_cache, const float *k_scale,
+                            const float *v_scale, const int *pages, const int *lengths, const int *counts, void *o,
+                            void *workspace, int B, int heads, int heads_kv, int T, int D, int num_pages, int page,
+                            int columns, int kernel_size, int dtype, int cache_dtype, const int64_t *q_strides,
+                            const int64_t *o_strides, const int64_t *k_cache_strides, const int64_t *v_cache_strides,
+                            const int64_t *k_scale_strides, const int64_t *v_scale_strides, int64_t pages_stride,
+                            float scale, void *stream) {
+    const char *fn = "enatten_cache_attention";
+    int rc = check_cache_sizes(fn, B, heads, T, D, num_pages, page, columns, dtype, cache_dtype, pages_stride);
+    if (rc) return rc;
+    if (heads_kv < 1 || heads % heads_kv) {
+        set_error("%s: %d heads are no multiple of the cache's %d", fn, heads, heads_kv);
+        return ENATTEN_EINVAL;
+    }
+    if (kernel_size < 0) {
+        set_error("%s: kernel_size must be >= 1, or 0 for all tokens, got %d", fn, kernel_size);
+        return ENATTEN_EINVAL;
+    }
+    AttnArgs a{};
+    if ((rc = set_rows(fn, "q", q, q_strides, heads, T, D, &a.q))) return rc;
+    if ((rc = set_rows(fn, "o", o, o_strides, heads, T, D, &a.o))) return rc;
+    if ((rc = set_cache(fn, "k", const_cast<void *>(k_cache), const_cast<float *>(k_scale), k_cache_strides,
+                        k_scale_strides, heads_kv, page, D, 16, &a.k))) return rc;
+    if ((rc = set_cache(fn, "v", const_cast<void *>(v_cache), const_cast<float *>(v_scale), v_cache_strides,
+                        v_scale_strides, heads_kv, page, D, 16, &a.v))) return rc;
+    if (!pages || !lengths) {
+        set_error("%s: pages and lengths must not be NULL", fn);
+        return ENATTEN_EINVAL;
+    }
+    const Plan p = plan_of(B, heads, heads_kv, T, D, page, columns, kernel_size, dtype);
+    if (p.parts && (!workspace || (uintptr_t)workspace % 16)) {
+        set_error("%s: workspace is NULL or not 16-byte aligned", fn);
+        return ENATTEN_EINVAL;
+    }
+    a.tb = Table{pages, lengths, counts, pages_stride, num_pages, page, columns, T};
+    a.B = B; a.heads = heads; a.group = heads / heads_kv; a.heads_kv = heads_kv; a.T = T; a.D = D;
+    a.window = kernel_size;
+    a.dtype = dtype;
+    a.row_tiles = p.row_tiles;
+    a.parts = p.parts;
+    a.scale = scale;
+    a.ws = static_cast<float *>(workspace);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const bool e = cache_dtype == ENATTEN_E4M3;
+    if (D <= 64) return e ? launch_rows<64, true>(fn, a, p, st) : launch_rows<64, false>(fn, a, p, st);
+    if (D <= 128) return e ? launch_rows<128, true>(fn, a, p, st) : launch_rows<128, false>(fn, a, p, st);
+    return e ? launch_rows<256, true>(fn, a, p, st) : launch_rows<256, false>(fn, a, p, st);
+}
+
+#pragma GCC visibility pop
+}  // extern "C"

@@ -19,23 +19,13 @@
 #include <algorithm>
 #include <tuple>
 
-#include "enatten.h"
+#include "torch_shim.h"
 
 namespace {
 
 using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
-
-int dtype_code(const Tensor &t) {
-    switch (t.scalar_type()) {
-        case at::kFloat: return ENATTEN_F32;
-        case at::kBFloat16: return ENATTEN_BF16;
-        case at::kHalf: return ENATTEN_F16;
-        case at::kDouble: return ENATTEN_F64;
-        default: return -1;
-    }
-}
 
 // The checks of the Python host side, with the same error classes: ValueError for
 // bad shapes, dtypes and kernel sizes, RuntimeError for tensors that are not on
@@ -65,19 +55,6 @@ void validate(const char *what, const Tensor &q, const Tensor &k, const Tensor &
     // the right shape for them without touching the library
     TORCH_CHECK(!check_device || q.is_cuda() || q.is_meta(), what,
                 ": tensors must be on the GPU; this build has no CPU path");
-}
-
-// The kernels take any strides on the leading axes but need unit stride on the
-// channel axis.
-Tensor kernel_layout(const Tensor &t) {
-    return (t.stride(-1) != 1 && t.size(-1) != 1) ? t.contiguous() : t;
-}
-
-void check_rc(int rc) {
-    if (rc == ENATTEN_OK) return;
-    const char *msg = enatten_last_error();
-    TORCH_CHECK_VALUE(rc != ENATTEN_EINVAL, msg);
-    TORCH_CHECK(false, msg);
 }
 
 void check_bwd_extras(const char *what, const Tensor &q, const Tensor &o, const Tensor &d_o) {

@@ -32,6 +32,9 @@ extern "C" {
  * arithmetic on kernels of its own (for numerical gradient checks, as the reference's
  * gradcheck.py:6-15 does; not tuned); lse stays float32. */
 enum { ENATTEN_F32 = 0, ENATTEN_BF16 = 1, ENATTEN_F16 = 2, ENATTEN_F64 = 3 };
+/* element types of positions (enatten_rotary) and of a cache (enatten_cache_*); E4M3 is the
+ * 8-bit float with 4 exponent and 3 mantissa bits, no infinities and a largest value of 448 */
+enum { ENATTEN_I32 = 16, ENATTEN_I64 = 17, ENATTEN_I8 = 18, ENATTEN_E4M3 = 19 };
 
 /* return codes */
 enum {
@@ -280,6 +283,83 @@ int enatten1d_bwd_into(const void *q, const void *k, const void *v, const void *
                        float scale, void *stream);
 
 /*
+ * Rotary positions.  They and the cache below have no counterpart in the reference: they are what
+ * a sequence model needs beside its 1D attention (e_natten/triton.py:425-483).
+ * The first R channels of every [D] row of q and k form R / 2 pairs, (i, i + R/2), or (2i, 2i + 1)
+ * if `interleaved`; pair i of the row at position p is turned by the angle p * frequencies[i] and
+ * multiplied by `scale`, the channels from R on are copied.  `inverse` turns the other way round,
+ * which is the gradient: (dq, dk) from the gradients of q_out and k_out.
+ *   q, q_out   [B, heads_q, T, D] of `dtype` (ENATTEN_F32 / BF16 / F16 / F64), strides (batch, head,
+ *              position) as in enatten1d_fwd; k, k_out likewise with heads_k, or both NULL
+ *   positions  whole numbers of any sign (ENATTEN_I32 or ENATTEN_I64), [T] for every sequence
+ *              alike (positions_stride 0) or [B, T] with positions_stride elements between sequences
+ *   frequencies  [R / 2], ENATTEN_F32 or ENATTEN_F64, radians per position.  The product with the
+ *              position and its remainder of a turn are formed in double.
+ * q_out may be q and k_out may be k, of the same strides; they must not overlap otherwise.
+ */
+int enatten_rotary(const void *q, const void *k, void *q_out, void *k_out, const void *positions,
+                   const void *frequencies, int B, int heads_q, int heads_k, int T, int D, int R,
+                   int dtype, int positions_dtype, int frequencies_dtype, int interleaved, int inverse,
+                   const int64_t *q_strides, const int64_t *k_strides, const int64_t *q_out_strides,
+                   const int64_t *k_out_strides, int64_t positions_stride, double scale, void *stream);
+
+/*
+ * A cache of 8 bits for sequences that grow, in pages of `page` tokens:
+ *   k_cache, v_cache  [num_pages, heads, page, D] of cache_dtype (ENATTEN_I8 or ENATTEN_E4M3), D a
+ *              multiple of 16 up to 256, page a multiple of 16 up to 1024; element strides (page,
+ *              head, token), multiples of 16 (of 8 in enatten_cache_append), tokens at most 2^20 apart
+ *   k_scale, v_scale  float32 [num_pages, heads], one factor for each block (page, head): a code
+ *              stands for code * scale; strides (page, head)
+ *   pages      int32 [B, columns], unit stride on the columns: token j of sequence b is row j % page
+ *              of page pages[b, j / page].  Entries behind a sequence's last token are not read.
+ *   lengths    int32 [B]: tokens of each sequence, those that the call is about included
+ *   counts     int32 [B]: how many of T those are, the last ones of the sequence; NULL: T for all
+ * Numbers that do not fit together (a count outside 0 .. T or above the length, a length beyond the
+ * columns) leave that sequence out: enatten_cache_append writes nothing for it,
+ * enatten_cache_attention writes NaN.  A page outside 0 .. num_pages - 1 is neither read nor written;
+ * a query that sees a token on one gets NaN.
+ * All codes are finite numbers: the two codes of E4M3 that are not (0x7f, 0xff) read as +-480, and
+ * are never written.  What a block holds behind a sequence's last token is of no consequence.
+ *
+ * enatten_cache_append writes the new tokens k, v [B, heads, T, D] (`dtype` F32, BF16 or F16; strides
+ * (batch, head, position)).  Block by block, with M = 127 or 448:
+ *   scale' = max(scale, max |x| / M) over the new tokens x, where the page holds older tokens of the
+ *   sequence, else max |x| / M;  code = round(x * (1 / scale'));  where scale' > scale the older codes
+ *   become round(code * (scale * (1 / scale'))).  Rounding is to nearest, ties to even.
+ * A block with a value that is not finite gets the scale NaN, and scales below 2^-126 become 0; the
+ * new codes are 0 then.  A page must belong to one sequence for tokens to be written to it.
+ */
+int enatten_cache_append(const void *k, const void *v, void *k_cache, void *v_cache, float *k_scale,
+                         float *v_scale, const int *pages, const int *lengths, const int *counts,
+                         int B, int heads, int T, int D, int num_pages, int page, int columns,
+                         int dtype, int cache_dtype, const int64_t *k_strides,
+                         const int64_t *v_strides, const int64_t *k_cache_strides,
+                         const int64_t *v_cache_strides, const int64_t *k_scale_strides,
+                         const int64_t *v_scale_strides, int64_t pages_stride, void *stream);
+
+/*
+ * Attention of the last tokens of each sequence over the cache.  q, o: [B, heads, T, D] of `dtype`
+ * (F32, BF16 or F16), strides (batch, head, position); heads is a multiple of heads_kv and head h
+ * reads head h / (heads / heads_kv) of the cache.  Query t < counts[b] stands at position
+ * p = lengths[b] - counts[b] + t and sees the tokens max(p - kernel_size + 1, 0) .. p, or all up to p
+ * with kernel_size 0: the windows of enatten2d_fwd_window's causal axis.  Logits are q.k * scale.
+ * o is 0 for t >= counts[b].
+ *   workspace  enatten_cache_attention_workspace_bytes() of this call's sizes, 16-byte aligned; may
+ *              be NULL if that is 0.  Calls that may overlap need one each.
+ */
+size_t enatten_cache_attention_workspace_bytes(int B, int heads, int heads_kv, int T, int D, int page,
+                                               int columns, int kernel_size, int dtype);
+int enatten_cache_attention(const void *q, const void *k_cache, const void *v_cache,
+                            const float *k_scale, const float *v_scale, const int *pages,
+                            const int *lengths, const int *counts, void *o, void *workspace, int B,
+                            int heads, int heads_kv, int T, int D, int num_pages, int page,
+                            int columns, int kernel_size, int dtype, int cache_dtype,
+                            const int64_t *q_strides, const int64_t *o_strides,
+                            const int64_t *k_cache_strides, const int64_t *v_cache_strides,
+                            const int64_t *k_scale_strides, const int64_t *v_scale_strides,
+                            int64_t pages_stride, float scale, void *stream);
+
+/*
  * Per-kernel timing aid for benchmarks (no counterpart in the reference, whose
  * bench.py:28,59 times whole calls with triton.testing.do_bench).  While
  * enabled, kernels this library launches are bracketed by HIP events on the
@@ -295,7 +375,8 @@ int enatten1d_bwd_into(const void *q, const void *k, const void *v, const void *
  * a launch reads one flag and nothing else.
  */
 enum { ENATTEN_KERNEL_FWD = 0, ENATTEN_KERNEL_BWD_DQ = 1, ENATTEN_KERNEL_BWD_DKDV = 2,
-       ENATTEN_KERNEL_BWD_FUSED = 3, ENATTEN_KERNEL_COUNT = 4 };
+       ENATTEN_KERNEL_BWD_FUSED = 3, ENATTEN_KERNEL_ROTARY = 4, ENATTEN_KERNEL_CACHE_APPEND = 5,
+       ENATTEN_KERNEL_CACHE_ATTENTION = 6, ENATTEN_KERNEL_CACHE_JOIN = 7, ENATTEN_KERNEL_COUNT = 8 };
 int enatten_profile_enable(int on);
 int enatten_profile_read(int kernel, int *launches, double *total_ms);
 /* What the brackets themselves added to total_ms: after each timed launch's closing

@@ -1,0 +1,154 @@
+"""The cache of 8 bits on the GPU: new tokens written into it, and attention over it, against their
+definitions (the codes bit for bit, the attention in 64 bits)."""
+import pytest
+import torch
+
+from _sequence import Cache, append_ref, attention_ref, half_step
+from _util import ensure_built
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+I8, E4M3 = torch.int8, torch.float8_e4m3fn
+
+
+def _ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _new_tokens(B, heads, T, d, dtype, seed, layout="proj", spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    k, v = (torch.randn((B, T, heads, d), generator=g) * spread for _ in range(2))
+    if layout == "odd":   # rows on no particular address
+        x = torch.zeros((2, B, heads, T, d + 3), dtype=dtype)
+        x[0, ..., 1:d + 1], x[1, ..., 1:d + 1] = k.transpose(1, 2).to(dtype), v.transpose(1, 2).to(dtype)
+        return x[0, ..., 1:d + 1], x[1, ..., 1:d + 1]
+    return k.to(dtype).transpose(1, 2), v.to(dtype).transpose(1, 2)
+
+
+@pytest.mark.parametrize("lengths,counts,heads,T,d,page,dtype,cache_dtype,layout", [
+    ([1], None, 1, 1, 16, 16, BF16, I8, "proj"),                       # the first token
+    ([17, 40, 1], None, 2, 1, 128, 16, BF16, E4M3, "proj"),            # first of a page, inside one, first of all
+    ([33, 64, 65], None, 3, 1, 80, 32, F32, I8, "odd"),
+    ([300, 129], None, 2, 100, 64, 64, F16, I8, "proj"),               # several pages, old tokens before them
+    ([300, 129, 50, 7], [100, 0, 33, 7], 2, 100, 64, 48, BF16, E4M3, "proj"),   # ragged; one brings none
+    ([1030], None, 1, 1030, 256, 256, BF16, I8, "proj"),               # blocks of more than a workgroup holds
+    ([1500], [1100], 1, 1101, 256, 1024, F32, E4M3, "proj"),
+    ([70, 31], None, 2, 31, 48, 16, F16, E4M3, "odd"),
+])
+def test_append(lengths, counts, heads, T, d, page, dtype, cache_dtype, layout):
+    ensure_built()
+    from e_natten_amd import cache_append
+    print("case append", lengths, counts, heads, T, d, page, dtype, cache_dtype, layout, flush=True)
+    cache = Cache(lengths, heads, page, d, cache_dtype, seed=T, scale_spread=(0.1, 1.0))
+    k, v = _new_tokens(len(lengths), heads, T, d, dtype, 5, layout)
+    want = append_ref(cache, k, v, counts)
+    kc, vc, ks, vs, pages = cache.on("cuda")
+    cache_append(k.cuda(), v.cuda(), kc, vc, ks, vs, pages, _ints(lengths), None if counts is None else _ints(counts))
+    for (codes, scales), c, s in zip(want, (kc, vc), (ks, vs)):
+        # -0 of float8 and NaN scales: compared as bits
+        assert torch.equal(c.view(torch.uint8).cpu(), codes)
+        assert torch.equal(s.cpu().nan_to_num(nan=-1.0), scales.nan_to_num(nan=-1.0))
+
+
+@pytest.mark.parametrize("cache_dtype", [I8, E4M3])
+def test_append_corner_values(cache_dtype):
+    """Zeros, values that are not finite, values too small for a scale, and a scale that grows."""
+    ensure_built()
+    from e_natten_amd import cache_append
+    heads, d, page = 6, 32, 16
+    cache = Cache([20, 20], heads, page, d, cache_dtype, seed=3, scale_spread=(0.5, 0.6))
+    k, v = _new_tokens(2, heads, 2, d, F32, 6)
+    k[0, 0], v[0, 0] = 0.0, 1e-39
+    k[0, 1, 1, 3] = float("inf")
+    v[0, 1, 0, 31] = float("nan")
+    k[0, 2] *= 1e4          # older tokens of the page lose nearly all their bits
+    v[0, 3] *= 3.4e38 / v[0, 3].abs().max()
+    k[1, 4, 0, 0] = float("-inf")
+    want = append_ref(cache, k, v)
+    kc, vc, ks, vs, pages = cache.on("cuda")
+    cache_append(k.cuda(), v.cuda(), kc, vc, ks, vs, pages, _ints([20, 20]))
+    for (codes, scales), c, s in zip(want, (kc, vc), (ks, vs)):
+        assert torch.equal(c.view(torch.uint8).cpu(), codes)
+        assert torch.equal(s.cpu().nan_to_num(nan=-1.0), scales.nan_to_num(nan=-1.0))
+    # a block that is NaN stays so, another token of the sequence's next page starts afresh
+    page_at = int(cache.pages[0, 1])
+    assert torch.isnan(ks[page_at, 1]) and torch.isnan(vs[page_at, 1])
+
+
+def test_append_leaves_out_what_does_not_fit():
+    """Counts and lengths that contradict each other or the table, and pages outside the cache: nothing
+    of the cache changes for them, the other sequences get their tokens."""
+    ensure_built()
+    from e_natten_amd import cache_append
+    cache = Cache([20, 20, 20, 20, 20, 20], 2, 16, 32, I8, seed=8, extra_columns=0)
+    k, v = _new_tokens(6, 2, 4, 32, BF16, 9)
+    lengths, counts = [20, 2, 33, -5, 20, 20], [4, 4, 4, 0, -1, 5]
+    cache.lengths = [20, 0, 0, 0, 0, 0]
+    want = append_ref(cache, k, v, [4, 0, 0, 0, 0, 0])
+    kc, vc, ks, vs, pages = cache.on("cuda")
+    cache_append(k.cuda(), v.cuda(), kc, vc, ks, vs, pages, _ints(lengths), _ints(counts))
+    for bad in (-1, kc.shape[0], 2 ** 31 - 1, -2 ** 31):
+        pages[1:, 1] = bad
+        cache_append(k.cuda(), v.cuda(), kc, vc, ks, vs, pages, _ints([20] * 6), _ints([4] * 6))
+    for (codes, scales), c, s in zip(want, (kc, vc), (ks, vs)):
+        assert torch.equal(c.view(torch.uint8).cpu(), codes)
+        assert torch.equal(s.cpu().nan_to_num(nan=-1.0), scales.nan_to_num(nan=-1.0))
+
+
+def _check(o, ref, bound, dtype, what):
+    off = (o.detach().cpu().double() - ref).abs()
+    limit = bound + half_step(dtype) * (ref.abs() + bound)
+    worst = (off / limit.clamp(min=1e-300)).max().item()
+    print("   %s: worst element at %.3f of its bound, 2-norm %.2e"
+          % (what, worst, (off.norm() / ref.norm().clamp(min=1e-300)).item()), flush=True)
+    assert torch.isfinite(o.float()).all(), what
+    assert (off <= limit).all(), what
+
+
+@pytest.mark.parametrize("lengths,counts,N,heads,T,d,page,dtype,cache_dtype,window", [
+    ([1], None, 1, 1, 1, 16, 16, BF16, I8, None),                    # a single token sees itself
+    ([5], None, 4, 4, 1, 128, 16, BF16, E4M3, None),
+    ([16, 17, 31, 32, 33], None, 4, 2, 1, 64, 16, F16, I8, None),    # around the groups and steps of tokens
+    ([100, 1000, 257], None, 8, 2, 1, 128, 64, BF16, I8, None),
+    ([3000], None, 8, 1, 1, 128, 16, BF16, E4M3, None),              # split along the tokens
+    ([5000, 0, 12, 2500], None, 16, 2, 1, 64, 48, F16, E4M3, None),  # one sequence without tokens
+    ([700, 33], None, 32, 1, 1, 256, 32, BF16, I8, None),            # two tiles of rows
+    ([700, 300], None, 6, 3, 1, 80, 48, F32, I8, None),
+    ([4000], None, 15, 5, 1, 96, 16, F32, E4M3, 1000),
+    ([900, 128, 127, 1], None, 4, 4, 1, 128, 32, BF16, I8, 128),     # sliding window
+    ([900, 40], None, 4, 4, 1, 128, 32, F16, I8, 1),                 # ... of the token itself
+    ([900, 40], None, 4, 4, 1, 32, 1024, BF16, E4M3, 33),
+    ([600, 9, 250], [5, 3, 0], 8, 2, 5, 64, 128, BF16, E4M3, None),  # drafted tokens, ragged
+    ([600, 9, 250], [5, 3, 1], 8, 2, 5, 64, 128, F16, I8, 7),
+    ([7, 50], None, 15, 5, 7, 80, 48, F32, I8, None),                # the whole sequence at once
+    ([300, 200], [70, 33], 8, 2, 70, 128, 64, BF16, I8, None),       # chunks: several tiles of rows
+    ([300, 200], [70, 33], 8, 2, 70, 128, 64, F16, E4M3, 50),
+    ([260], None, 2, 2, 130, 192, 16, BF16, E4M3, 20),
+    ([513, 400], [257, 1], 4, 1, 257, 64, 16, BF16, I8, None),
+    ([200, 130], [129, 130], 6, 2, 130, 256, 32, F32, E4M3, 70),
+    ([200, 130], [129, 130], 6, 2, 130, 112, 80, F32, I8, None),
+])
+def test_attention(lengths, counts, N, heads, T, d, page, dtype, cache_dtype, window):
+    ensure_built()
+    from e_natten_amd import cache_attention
+    print("case attention", lengths, counts, N, heads, T, d, page, dtype, cache_dtype, window, flush=True)
+    cache = Cache(lengths, heads, page, d, cache_dtype, seed=sum(lengths))
+    g = torch.Generator().manual_seed(T)
+    q = (torch.randn((len(lengths), T, N, d), generator=g) * 2).to(dtype).transpose(1, 2)
+    if 0 in lengths:
+        counts = [min(n, T) for n in lengths]
+    scale = d ** -0.5
+    kc, vc, ks, vs, pages = cache.on("cuda")
+    args = (kc, vc, ks, vs, pages, _ints(lengths), window, scale, None if counts is None else _ints(counts))
+    o = cache_attention(q.cuda(), *args)
+    assert o.shape == q.shape and o.dtype == dtype
+    ref, bound = attention_ref(q, cache, counts, window, scale)
+    _check(o, ref, bound, dtype, "o")
+    if counts is not None:
+        for b, c in enumerate(counts):
+            assert not o[b, :, c:].any()
+    # the same call again, and rows that lie elsewhere: the same bits
+    assert torch.equal(o, cache_attention(q.cuda(), *args))
+    x = torch.zeros((len(lengths), N, T, d + 5), dtype=dtype, device="cuda")
+    x[..., 3:d + 3] = q.cuda()
+    assert torch.equal(o, cache_attention(x[..., 3:d + 3], *args))
