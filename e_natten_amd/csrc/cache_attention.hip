@@ -28,216 +28,38 @@
 // the number of sequences and heads; the parts leave their sums, maximum and output in the workspace and
 // a second launch joins them.  The split goes by the lengths of this call, which are on the device:
 // every workgroup computes it for itself.
-#include "sequence_common.h"
+#include "cache_attention.h"
 
 namespace enatten {
 namespace {
 
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef short s16x2 __attribute__((ext_vector_type(2)));
+constexpr int kTile = 32;  // tokens of a step of a wave
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kFloor = -1e37f;  // the maximum of a row that has seen nothing: finite, below every logit
-constexpr int kTile = 32;         // tokens of a step
-constexpr int kTop = 14;          // float16 operands are brought to 2^kTop
-
-struct AttnArgs {
-    Rows q, o;
-    Cache k, v;
-    Table tb;
-    int B, heads, group, heads_kv, T, D, window;  // group: query heads of a cache head
-    int dtype;
-    int row_tiles;   // per (sequence, cache head)
-    int parts;       // workgroups per cache head that the split aims at; 0: one per row tile
-    float scale;
-    float *ws;       // [item][cache head]: row maxima, row sums, rows x D sums
-};
-
-// The tokens that one row tile sees: [lo, hi), hi <= lo if none.
-struct Span {
-    int len, count, start, lo, hi;
-    bool ok;
-};
-template <int ROWS>
-__device__ __forceinline__ Span span_of(const AttnArgs &a, int entry) {
-    Span s;
-    const int b = entry / a.row_tiles, tile = entry - b * a.row_tiles;
-    s.ok = sequence_of(a.tb, b, s.len, s.count);
-    s.start = s.len - s.count;
-    const int first = tile * ROWS / a.group, last = min((tile * ROWS + ROWS - 1) / a.group, s.count - 1);
-    s.lo = s.hi = 0;
-    if (first < s.count) {
-        s.lo = a.window ? max(s.start + first - a.window + 1, 0) : 0;
-        s.hi = s.start + last + 1;
-    }
-    return s;
+// Waves per SIMD that the registers allow: the sums, q, logits and probabilities of every row tile, and
+// two tiles of codes.
+constexpr int waves_of(int DP, int R, int TERMS) {
+    const int need = R * (DP / 4 + DP / 8 * TERMS + 8 + 4 * TERMS) + DP / 2 + 88;
+    return need <= 168 ? 3 : need <= 256 ? 2 : 1;
 }
-__device__ __forceinline__ int steps_of(const Span &s) { return s.hi > s.lo ? (s.hi - (s.lo & -16) + kTile - 1) / kTile : 0; }
-
-// How the row tiles ("entries") are cut into items of at most `chunk` steps; the same in every wave.
-__device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
-    return x;
-}
-template <int ROWS>
-__device__ __forceinline__ int chunk_of(const AttnArgs &a) {
-    const int entries = a.B * a.row_tiles, lane = threadIdx.x & 63;
-    long long total = 0;
-    for (int e0 = 0; e0 < entries; e0 += 64) {
-        const int e = e0 + lane;
-        total += wave_sum(e < entries ? steps_of(span_of<ROWS>(a, e)) : 0);
-    }
-    // at least 8 steps each: two per wave
-    return max(8, (int)((total + a.parts - 1) / a.parts));
-}
-__device__ __forceinline__ int items_of(int steps, int chunk) { return max(1, (steps + chunk - 1) / chunk); }
-// The entry of item `item` and the number of its first item, or (by_entry) the first item of entry
-// `item`; entry -1 if there is none.
-template <int ROWS>
-__device__ __forceinline__ void find(const AttnArgs &a, int chunk, int item, bool by_entry, int &entry, int &first) {
-    const int entries = a.B * a.row_tiles, lane = threadIdx.x & 63;
-    int before = 0;
-    entry = -1;
-    first = 0;
-    for (int e0 = 0; e0 < entries; e0 += 64) {
-        const int e = e0 + lane;
-        const int n = e < entries ? items_of(steps_of(span_of<ROWS>(a, e)), chunk) : 0;
-        int upto = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int x = __shfl_up(upto, o, 64);
-            if (lane >= o) upto += x;
-        }
-        const bool mine = by_entry ? e == item : n > 0 && item >= before + upto - n && item < before + upto;
-        const unsigned long long who = __ballot(mine);
-        if (who) {
-            const int l = __ffsll(who) - 1;
-            entry = e0 + l;
-            first = before + __shfl(upto - n, l, 64);
-            return;
-        }
-        before += __shfl(upto, 63, 64);
-    }
-}
-
-__device__ __forceinline__ f16x2 as_half(unsigned x) { return __builtin_bit_cast(f16x2, x); }
-
-// Two codes side by side, each in the upper byte of a half (E4M3) or the lower byte of a half of
-// 0x6400 (int8, offset 128), as float16.  E4M3: sign, 4 exponent and 3 mantissa bits move to the places
-// of float16's, whose exponents are offset by 8 more: the value times 2^-8.
-__device__ __forceinline__ f16x2 from_e4m3(unsigned x) {
-    const s16x2 s = __builtin_bit_cast(s16x2, x) >> 1;
-    return as_half(__builtin_bit_cast(unsigned, s) & 0xbfffbfffu);
-}
-__device__ __forceinline__ f16x2 from_int8(unsigned x) {
-    return as_half(x) + f16x2{(_Float16)-1152.f, (_Float16)-1152.f};
-}
-// 8 consecutive codes
-template <bool E4M3>
-__device__ __forceinline__ f16x8 widen_row(unsigned x0, unsigned x1) {
-    f16x2 h[4];
-    if constexpr (E4M3) {
-        h[0] = from_e4m3(__builtin_amdgcn_perm(x0, x0, 0x010c000cu));
-        h[1] = from_e4m3(__builtin_amdgcn_perm(x0, x0, 0x030c020cu));
-        h[2] = from_e4m3(__builtin_amdgcn_perm(x1, x1, 0x010c000cu));
-        h[3] = from_e4m3(__builtin_amdgcn_perm(x1, x1, 0x030c020cu));
-    } else {
-        x0 ^= 0x80808080u;
-        x1 ^= 0x80808080u;
-        h[0] = from_int8(__builtin_amdgcn_perm(0x64646464u, x0, 0x04010400u));
-        h[1] = from_int8(__builtin_amdgcn_perm(0x64646464u, x0, 0x04030402u));
-        h[2] = from_int8(__builtin_amdgcn_perm(0x64646464u, x1, 0x04010400u));
-        h[3] = from_int8(__builtin_amdgcn_perm(0x64646464u, x1, 0x04030402u));
-    }
-    return f16x8{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
-}
-// 4 channels (one word) of 8 tokens, transposed: out[i] is channel i of the 8 tokens
-template <bool E4M3>
-__device__ __forceinline__ void widen_columns(const unsigned (&t)[8], f16x8 (&out)[4]) {
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-        f16x2 h[4];
-        if constexpr (E4M3) {
-            h[0] = from_e4m3(__builtin_amdgcn_perm(t[j + 1], t[j], 0x040c000cu));
-            h[1] = from_e4m3(__builtin_amdgcn_perm(t[j + 1], t[j], 0x050c010cu));
-            h[2] = from_e4m3(__builtin_amdgcn_perm(t[j + 1], t[j], 0x060c020cu));
-            h[3] = from_e4m3(__builtin_amdgcn_perm(t[j + 1], t[j], 0x070c030cu));
-        } else {
-            const unsigned lo = __builtin_amdgcn_perm(t[j + 1], t[j], 0x05010400u) ^ 0x80808080u;
-            const unsigned hi = __builtin_amdgcn_perm(t[j + 1], t[j], 0x07030602u) ^ 0x80808080u;
-            h[0] = from_int8(__builtin_amdgcn_perm(0x64646464u, lo, 0x04010400u));
-            h[1] = from_int8(__builtin_amdgcn_perm(0x64646464u, lo, 0x04030402u));
-            h[2] = from_int8(__builtin_amdgcn_perm(0x64646464u, hi, 0x04010400u));
-            h[3] = from_int8(__builtin_amdgcn_perm(0x64646464u, hi, 0x04030402u));
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            out[i][j] = h[i][0];
-            out[i][j + 1] = h[i][1];
-        }
-    }
-}
-
-__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-// max / sum over the four lanes of a row
-__device__ __forceinline__ float row_max(float x) {
-    x = fmaxf(x, __shfl_xor(x, 16, 64));
-    return fmaxf(x, __shfl_xor(x, 32, 64));
-}
-__device__ __forceinline__ float row_sum(float x) {
-    x += __shfl_xor(x, 16, 64);
-    return x + __shfl_xor(x, 32, 64);
-}
-
-__device__ __forceinline__ float load_row(const Rows &r, int dtype, int64_t at) {
-    if (dtype == ENATTEN_F32) return static_cast<const float *>(r.ptr)[at];
-    if (dtype == ENATTEN_BF16) return (float)static_cast<const __bf16 *>(r.ptr)[at];
-    return (float)static_cast<const _Float16 *>(r.ptr)[at];
-}
-__device__ __forceinline__ void store_row(const Rows &r, int dtype, int64_t at, float x) {
-    void *p = const_cast<void *>(r.ptr);
-    if (dtype == ENATTEN_F32) static_cast<float *>(p)[at] = x;
-    else if (dtype == ENATTEN_BF16) static_cast<__bf16 *>(p)[at] = (__bf16)x;
-    else static_cast<_Float16 *>(p)[at] = (_Float16)x;
-}
-
-__device__ __forceinline__ int lane_int(int x, int l) { return __builtin_amdgcn_readlane(x, l); }
-__device__ __forceinline__ float lane_float(float x, int l) {
-    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), l));
-}
-__device__ __forceinline__ int64_t lane_offset(int64_t x, int l) {
-    const unsigned lo = __builtin_amdgcn_readlane((int)x, l), hi = __builtin_amdgcn_readlane((int)(x >> 32), l);
-    return (int64_t)((uint64_t)hi << 32 | lo);
-}
-
-// Floats of one item's part of the workspace
-constexpr int64_t item_floats(int rows, int D) { return (int64_t)rows * (D + 2); }
 
 // DP: head_dim rounded up to 64, 128 or 256 (channels beyond D: zeros in q, any codes); R: row tiles of
 // 16 per workgroup; TERMS: float16 terms of q and p.
 template <int DP, int R, bool E4M3, int TERMS>
-__global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attend(AttnArgs a) {
-    constexpr int ROWS = 16 * R, KC = DP / 64, VW = DP / 64, DT = DP / 16;
+__global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a) {
+    constexpr int TOK = kTile, ROWS = 16 * R, KC = DP / 64, VW = DP / 64, DT = DP / 16;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n16 = lane & 15, g4 = lane >> 4;
 
     // which row tile, and which of its steps
     const int head = blockIdx.x % a.heads_kv, item = blockIdx.x / a.heads_kv;
     int entry = item, first_item = item, chunk = 1 << 26;
     if (a.parts) {
-        chunk = chunk_of<ROWS>(a);
-        find<ROWS>(a, chunk, item, false, entry, first_item);
+        chunk = chunk_of<ROWS, TOK>(a);
+        find<ROWS, TOK>(a, chunk, item, false, entry, first_item);
         if (entry < 0) return;
     }
     const Span s = span_of<ROWS>(a, entry);
     const int b = entry / a.row_tiles, row0 = (entry - b * a.row_tiles) * ROWS;
-    const int total = steps_of(s), items = items_of(total, chunk);
+    const int total = steps_of<TOK>(s), items = items_of(total, chunk);
     const int step0 = min((item - first_item) * chunk, total), step1 = min(step0 + chunk, total);
     const int base = s.lo & -16;
 
@@ -510,7 +332,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attend(AttnArgs a) {
 }
 
 // The parts of a row joined: one workgroup per (row tile, cache head, row)
-template <int ROWS>
+template <int ROWS, int TOK>
 __global__ __launch_bounds__(256) void attend_join(AttnArgs a) {
     const int per = min(ROWS, a.T * a.group);
     int block = blockIdx.x;
@@ -519,12 +341,12 @@ __global__ __launch_bounds__(256) void attend_join(AttnArgs a) {
     const int head = block % a.heads_kv, entry = block / a.heads_kv;
     const int b = entry / a.row_tiles, row = (entry - b * a.row_tiles) * ROWS + r;
     if (row >= a.T * a.group) return;
-    const int chunk = chunk_of<ROWS>(a);
+    const int chunk = chunk_of<ROWS, TOK>(a);
     const Span s = span_of<ROWS>(a, entry);
-    const int items = items_of(steps_of(s), chunk);
+    const int items = items_of(steps_of<TOK>(s), chunk);
     if (items == 1) return;
     int same, first;
-    find<ROWS>(a, chunk, entry, true, same, first);
+    find<ROWS, TOK>(a, chunk, entry, true, same, first);
     const int t = row / a.group;
     const int64_t at = b * a.o.sb + (head * a.group + row - t * a.group) * a.o.sh + t * a.o.st;
     const float *ws = a.ws + ((int64_t)first * a.heads_kv + head) * item_floats(ROWS, a.D);
@@ -567,65 +389,70 @@ __global__ __launch_bounds__(256) void attend_join(AttnArgs a) {
     }
 }
 
-// How a call is cut, from its sizes alone (the lengths are on the device).
-struct Plan {
-    int rows;       // of a tile
-    int row_tiles;
-    int parts;      // 0: one workgroup per row tile and cache head, no workspace
-    int64_t items;  // workgroups per cache head
-};
 Plan plan_of(int B, int heads, int heads_kv, int T, int D, int page, int columns, int window, int dtype) {
     Plan p;
     const int64_t all = (int64_t)T * (heads / heads_kv);
-    const int most = dtype == ENATTEN_F32 || D > 128 ? 32 : 64;
-    p.rows = all <= 16 ? 16 : all <= 32 ? 32 : most;
+    // Up to `most` rows: one tile of as many sixteens as there are, each wave with its own tokens.
+    // Beyond, tiles of 256 rows; float32 rows of more than 128 channels have too many registers there.
+    const int most = D > 128 ? 32 : 64;
+    p.rows = all <= most ? (int)(all + 15) / 16 * 16 : D > 128 && dtype == ENATTEN_F32 ? 32 : kWideRows;
     p.row_tiles = (int)((all + p.rows - 1) / p.rows);
     const int64_t entries = (int64_t)B * p.row_tiles;
     int64_t tokens = (int64_t)columns * page;
     if (window && window + (int64_t)p.rows < tokens) tokens = window + (int64_t)p.rows;
-    const int64_t steps = (tokens + 15) / kTile + 1;
     p.parts = 0;
     p.items = entries;
-    constexpr int target = 512;
-    if (entries * heads_kv < target && steps > 8) {
+    const int target = p.rows == kWideRows ? 256 : 512;
+    if (entries * heads_kv < target && tokens > kLeast) {
         p.parts = (target + heads_kv - 1) / heads_kv;
-        // no more than the longest possible sequences fill at 8 steps each
-        const int64_t useful = entries * ((steps + 7) / 8);
+        // no more than the longest possible sequences fill
+        const int64_t useful = entries * ((tokens + 16 + kLeast - 1) / kLeast);
         if (useful < p.parts) p.parts = (int)useful;
         p.items = p.parts + entries;
     }
     return p;
 }
 
-template <int DP, int R, bool E4M3, int TERMS>
-int launch(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st) {
-    const int64_t blocks = p.items * a.heads_kv, rows = a.T * (int64_t)a.group;
-    const int64_t join = (int64_t)a.B * p.row_tiles * a.heads_kv * (rows < p.rows ? rows : p.rows);
-    if (blocks > 0x7fffffff || (p.parts && join > 0x7fffffff)) {
-        set_error("%s: too many row tiles", fn);
+template <int ROWS, int TOK>
+int launch_join(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st) {
+    if (!p.parts) return ENATTEN_OK;
+    const int64_t rows = a.T * (int64_t)a.group, blocks = (int64_t)a.B * p.row_tiles * a.heads_kv * (rows < ROWS ? rows : ROWS);
+    if (blocks > 0x7fffffff) {
+        set_error("%s: too many rows", fn);
         return ENATTEN_EUNSUPPORTED;
     }
+    ProfScope prof(ENATTEN_KERNEL_CACHE_JOIN, "attend_join", st);
+    attend_join<ROWS, TOK><<<(int)blocks, 256, 0, st>>>(a);
+    return launched(fn);
+}
+template <int DP, int R, bool E4M3, int TERMS>
+int launch(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st) {
     {
         ProfScope prof(ENATTEN_KERNEL_CACHE_ATTENTION, "attend", st);
-        attend<DP, R, E4M3, TERMS><<<(int)blocks, 256, 0, st>>>(a);
+        attend<DP, R, E4M3, TERMS><<<(int)(p.items * a.heads_kv), 256, 0, st>>>(a);
     }
-    if (p.parts) {
-        ProfScope prof(ENATTEN_KERNEL_CACHE_JOIN, "attend_join", st);
-        attend_join<16 * R><<<(int)join, 256, 0, st>>>(a);
-    }
-    return launched(fn);
+    const int rc = launched(fn);
+    return rc ? rc : launch_join<16 * R, kTile>(fn, a, p, st);
 }
 template <int DP, int R, bool E4M3>
 int launch_terms(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st) {
-    if constexpr (R <= 2)
-        if (a.dtype == ENATTEN_F32) return launch<DP, R, E4M3, 2>(fn, a, p, st);
-    return launch<DP, R, E4M3, 1>(fn, a, p, st);
+    return a.dtype == ENATTEN_F32 ? launch<DP, R, E4M3, 2>(fn, a, p, st) : launch<DP, R, E4M3, 1>(fn, a, p, st);
 }
 template <int DP, bool E4M3>
 int launch_rows(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st) {
+    if (p.items * a.heads_kv > 0x7fffffff) {
+        set_error("%s: too many row tiles", fn);
+        return ENATTEN_EUNSUPPORTED;
+    }
+    if (p.rows == kWideRows) {
+        const int rc = launch_attend_rows(fn, a, E4M3, p.items * a.heads_kv, st);
+        return rc ? rc : launch_join<kWideRows, 8192 / DP>(fn, a, p, st);
+    }
     if (p.rows == 16) return launch_terms<DP, 1, E4M3>(fn, a, p, st);
-    if constexpr (DP <= 128)
+    if constexpr (DP <= 128) {
+        if (p.rows == 48) return launch_terms<DP, 3, E4M3>(fn, a, p, st);
         if (p.rows == 64) return launch_terms<DP, 4, E4M3>(fn, a, p, st);
+    }
     return launch_terms<DP, 2, E4M3>(fn, a, p, st);
 }
 

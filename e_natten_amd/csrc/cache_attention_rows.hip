@@ -1,0 +1,363 @@
+// cache_attention with many rows per cache head (chunks of prompts): tiles of 256 rows.
+//
+// The mathematics is that of cache_attention.hip.  With this many rows the matrix cores bound the call,
+// so the codes are turned into float16 once for all rows: eight waves take 32 rows each, and go
+// together over steps of 8192 / DP tokens whose keys and values lie in LDS as the operands of
+// v_mfma_f32_32x32x16_f16, in the order in which lanes read them.  Waves 0 to 3 turn keys, 4 to 7
+// values; codes come two steps ahead into registers and are turned into the other half of LDS while the
+// step's products run.
+//
+// S^T = K Q^T again leaves the probabilities in the registers that O^T = V^T P^T takes: lane (n, h) has
+// the tokens 4h .. 4h+3 (+ 8, 16, ...) of row n, and V is laid out with the same tokens in a lane's eight.
+//
+// exp2 is a quarter-rate instruction and as many as the products' cycles are spent on it, so the rest is
+// kept short: one fused multiply-add forms its argument, in which the value scale z' is a summand,
+//   p' = exp2(s u + (log2 z'' - m)),  z'' = z' 2^14 / (largest power of two of the z' so far),
+// and the sums divide z'' out again block by block.
+#include "cache_attention.h"
+
+namespace enatten {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// a lane's and its partner's (32 lanes on) maximum and sum
+__device__ __forceinline__ float pair_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pair_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float uniform(float x) {
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
+}
+
+// DP: head_dim rounded up to 64, 128 or 256; TERMS: float16 terms of q and p.
+template <int DP, bool E4M3, int TERMS>
+__global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
+    constexpr int TOK = 8192 / DP;    // tokens of a step: 128, 64, 32
+    constexpr int NB = TOK / 32;      // blocks of 32 of them
+    constexpr int GR = TOK / 16;      // groups of 16, each within a page
+    constexpr int SD = DP / 16;       // products along head_dim of S
+    constexpr int OB = DP / 32;       // blocks of 32 channels of O
+    constexpr int CH = DP / 16;       // loads of 16 codes per token
+    constexpr int QUADS = DP / 4;     // words of 4 channels
+    // operands of one step: K [NB][SD][64 lanes][8], V [OB][TOK / 16][64 lanes][8]
+    __shared__ __align__(16) _Float16 k_lds[2][8192], v_lds[2][8192];
+    __shared__ float z_lds[2][2][GR];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 31, h = lane >> 5;
+
+    // Which row tile, and which of its steps.  Blocks 8 apart share an XCD and its L2: neighbours in
+    // the order of the cache heads go to different ones, the row tiles of a head to the same where
+    // their number allows.  Later rows see more tokens: they come first.
+    const int heads = a.heads_kv;
+    int head, entry, item, first_item, chunk = 1 << 26;
+    if (a.parts) {
+        head = blockIdx.x % heads;
+        item = blockIdx.x / heads;
+        chunk = chunk_of<kWideRows, TOK>(a);
+        find<kWideRows, TOK>(a, chunk, item, false, entry, first_item);
+        if (entry < 0) return;
+    } else {
+        const int pair = blockIdx.x % (heads * a.B);
+        head = pair % heads;
+        entry = pair / heads * a.row_tiles + a.row_tiles - 1 - blockIdx.x / (heads * a.B);
+        item = first_item = entry;
+    }
+    const Span s = span_of<kWideRows>(a, entry);
+    const int b = entry / a.row_tiles, row0 = (entry - b * a.row_tiles) * kWideRows + wave * 32;
+    const int total = steps_of<TOK>(s), items = items_of(total, chunk);
+    const int step0 = min((item - first_item) * chunk, total), step1 = min(step0 + chunk, total);
+    const int base = s.lo & -16;
+    const int all_rows = a.T * a.group;
+
+    // the lane's row; q: lane (n, h) has channels 16 c + 8 h .. + 7
+    const int row = min(row0 + n, all_rows - 1), t_row = row / a.group;
+    const bool live = row0 + n < all_rows && t_row < s.count;
+    const int hi_r = live ? s.start + t_row + 1 : 0, lo_r = live && a.window ? max(hi_r - a.window, 0) : 0;
+    f16x8 qf[SD][TERMS];
+    float unit;
+    {
+        const int64_t at = b * a.q.sb + (head * a.group + row - t_row * a.group) * a.q.sh + t_row * a.q.st;
+        const float flip = a.scale < 0.f ? -1.f : 1.f;  // into q, so that units are not negative
+        float top = 0.f, nan = 0.f;
+#pragma unroll
+        for (int c = 0; c < SD; c++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int d = c * 16 + h * 8 + j;
+                const float x = d < a.D ? load_row(a.q, a.dtype, at + d) : 0.f;
+                top = fmaxf(top, fabsf(x));
+                nan += x * 0.f;
+            }
+        nan = pair_sum(nan);
+        top = pair_max(top);
+        const int up = kTop + 1 - (top > 0.f ? __builtin_amdgcn_frexp_expf(top) : 0);
+        unit = __builtin_ldexpf(fabsf(a.scale) * kLog2e, -up + (E4M3 ? 8 : 0)) + nan;
+#pragma unroll
+        for (int c = 0; c < SD; c++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int d = c * 16 + h * 8 + j;
+                const float x = d < a.D ? load_row(a.q, a.dtype, at + d) : 0.f;
+                const float y = __builtin_ldexpf(x * flip, up);
+                const _Float16 w = (_Float16)y;
+                qf[c][0][j] = w;
+                if constexpr (TERMS == 2) qf[c][1][j] = (_Float16)(y - (float)w);
+            }
+    }
+    // tokens that any, and that all rows of the wave see
+    const int t_first = min(row0, all_rows - 1) / a.group, t_last = min(min(row0 + 31, all_rows - 1) / a.group, s.count - 1);
+    const bool any_row = row0 < all_rows && t_first < s.count;
+    const int some_lo = any_row && a.window ? max(s.start + t_first + 1 - a.window, 0) : 0;
+    const int some_hi = any_row ? s.start + t_last + 1 : 0;
+    const int all_lo = a.window ? max(s.start + t_last + 1 - a.window, 0) : 0, all_hi = s.start + t_first + 1;
+
+    f32x16 acc[OB];
+#pragma unroll
+    for (int i = 0; i < OB; i++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) acc[i][j] = 0.f;
+    float m = kFloor, l = 0.f;
+    int ref = -126;
+
+    // places of the groups of 16 tokens: lane i holds group `filled` + i
+    int filled = -64;
+    int64_t at = 0;
+    float z_k = 0.f, z_v = 0.f;
+    const bool for_v = wave >= 4;
+    auto fill = [&](int group) {
+        filled = group;
+        const int token = base + (group + lane) * 16;
+        at = 0;
+        z_k = z_v = 0.f;
+        if (token < s.hi && token >= 0) {
+            const int column = token / a.tb.page, within = token - column * a.tb.page;
+            const int p = a.tb.pages[b * a.tb.stride + column];
+            if ((unsigned)p < (unsigned)a.tb.num_pages) {
+                at = for_v ? p * a.v.sp + head * a.v.sh + within * a.v.st : p * a.k.sp + head * a.k.sh + within * a.k.st;
+                z_k = a.k.scales[p * a.k.zp + head * a.k.zh];
+                z_v = a.v.scales[p * a.v.zp + head * a.v.zh];
+            } else {
+                z_k = __uint_as_float(0x7fc00000u);
+            }
+        }
+    };
+    // What a thread brings: of keys two runs of 16 codes, of values a word of 4 channels of 8 tokens.
+    unsigned raw[8];
+    float raw_z = 0.f;  // lanes 0 .. GR - 1 of wave 0: key scales of the step's groups, of wave 4: value scales
+    auto fetch = [&](int step) {
+        const int group = step * GR;
+        if (group >= filled + 64) fill(group);
+        const int here = group - filled;
+        const char *codes = static_cast<const char *>(for_v ? a.v.codes : a.k.codes);
+        raw_z = __shfl(for_v ? z_v : z_k, here + (lane & (GR - 1)), 64);
+        if (!for_v) {
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int token = wave * (128 / CH) + j * (64 / CH) + lane / CH, c = lane % CH;
+                const int64_t off = __shfl(at, here + token / 16, 64) + token % 16 * a.k.st + min(c * 16, a.D - 16);
+                const u32x4 x = *reinterpret_cast<const u32x4 *>(codes + off);
+#pragma unroll
+                for (int i = 0; i < 4; i++) raw[j * 4 + i] = x[i];
+            }
+        } else {
+            const int run = (wave - 4) * (64 * 4 / DP) + lane / QUADS, quad = lane % QUADS;  // 8 tokens each
+            const int64_t off = __shfl(at, here + run / 2, 64) + run % 2 * 4 * a.v.st + min(quad * 4, a.D - 4);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                raw[j] = *reinterpret_cast<const unsigned *>(codes + off + (j % 4 + j / 4 * 8) * a.v.st);
+        }
+    };
+    auto put = [&](int buffer) {
+        if (!for_v) {
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int token = wave * (128 / CH) + j * (64 / CH) + lane / CH, c = lane % CH;
+                const int swap = CH < 8 ? c * (8 / CH) & 7 : c & 7;
+                f16x8 *to = reinterpret_cast<f16x8 *>(k_lds[buffer]) + (token / 32 * SD + c) * 64 + ((token % 32) ^ swap);
+                to[0] = widen_row<E4M3>(raw[j * 4], raw[j * 4 + 1]);
+                to[32] = widen_row<E4M3>(raw[j * 4 + 2], raw[j * 4 + 3]);
+            }
+        } else {
+            const int run = (wave - 4) * (64 * 4 / DP) + lane / QUADS, quad = lane % QUADS;
+            f16x8 v[4];
+            widen_columns<E4M3>(raw, v);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int block = DP == 64 ? i / 2 : i + quad / 32 * 4, mm = DP == 64 ? (i & 1) * 16 + quad : quad & 31;
+                reinterpret_cast<f16x8 *>(v_lds[buffer])[(block * (TOK / 16) + run / 2) * 64 + run % 2 * 32 + mm] = v[i];
+            }
+        }
+        if ((wave & 3) == 0 && lane < GR) z_lds[buffer][for_v][lane] = raw_z;
+    };
+
+    if (step0 < step1) {
+        fetch(step0);
+        put(0);
+        if (step0 + 1 < step1) fetch(step0 + 1);
+    }
+    for (int step = step0; step < step1; step++) {
+        const int buffer = (step - step0) & 1;
+        __syncthreads();
+        if (step + 1 < step1) {
+            put(buffer ^ 1);
+            if (step + 2 < step1) fetch(step + 2);
+        }
+        const int token = base + step * TOK;
+        if (token >= some_hi || token + TOK <= some_lo) continue;
+
+        // scales of the step's groups, and a larger z' than any so far
+        float kz[GR], vz[GR], zmax = 0.f;
+#pragma unroll
+        for (int g = 0; g < GR; g++) {
+            kz[g] = uniform(z_lds[buffer][0][g]);
+            vz[g] = uniform(z_lds[buffer][1][g]);
+            zmax = fmaxf(zmax, vz[g]);
+        }
+        float shrink = 1.f;
+        const int e = __builtin_amdgcn_frexp_expf(zmax);
+        if (zmax < INFINITY && zmax > 0.f && e > ref) {
+            shrink = __builtin_ldexpf(1.f, max(ref - e, -200));
+            ref = e;
+        }
+
+        f32x16 st[NB];
+#pragma unroll
+        for (int i = 0; i < NB; i++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) st[i][j] = 0.f;
+        const f16x8 *kp = reinterpret_cast<const f16x8 *>(k_lds[buffer]);
+#pragma unroll
+        for (int c = 0; c < SD; c++) {
+            const int swap = CH < 8 ? c * (8 / CH) & 7 : c & 7;
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                const f16x8 kf = kp[(i * SD + c) * 64 + h * 32 + (n ^ swap)];
+#pragma unroll
+                for (int t = TERMS - 1; t >= 0; t--)
+                    st[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[c][t], st[i], 0, 0, 0);
+            }
+        }
+
+        // lane's tokens: 32 i + 16 g + 8 (j / 4) + 4 h + j % 4 for its 8 values j of a group
+        const bool whole = token >= all_lo && token + TOK <= all_hi;
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < NB; i++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    const int tk = token + i * 32 + j / 4 * 8 + h * 4 + j % 4;
+                    st[i][j] = tk >= lo_r && tk < hi_r ? st[i][j] : -INFINITY;
+                }
+        }
+        float u[GR], top = m;
+#pragma unroll
+        for (int g = 0; g < GR; g++) {
+            u[g] = unit * kz[g];
+            float most = st[g / 2][g % 2 * 8];
+#pragma unroll
+            for (int j = 1; j < 8; j++) most = fmaxf(most, st[g / 2][g % 2 * 8 + j]);
+            top = fmaxf(top, most * u[g]);
+        }
+        top = pair_max(top);
+        const float alpha = __builtin_amdgcn_exp2f(m - top);
+        m = top;
+        float sum = 0.f;
+#pragma unroll
+        for (int g = 0; g < GR; g++) {
+            // (a scale of 0: codes may be anything, and go in with a weight that float16 drops)
+            float z = __builtin_ldexpf(vz[g], kTop - ref);
+            z = z < 0x1p-40f ? 0x1p-40f : z;
+            const float shift = __builtin_amdgcn_logf(z) - top;
+            float part = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float x = st[g / 2][g % 2 * 8 + j];
+                float y = fmaf(x, u[g], shift);
+                if (!whole) y = x == -INFINITY ? -INFINITY : y;
+                const float p = __builtin_amdgcn_exp2f(y);
+                st[g / 2][g % 2 * 8 + j] = p;
+                part += p;
+            }
+            sum = fmaf(part, __builtin_amdgcn_rcpf(z), sum);
+        }
+        l = fmaf(l, alpha, sum);
+        if (__any(alpha != 1.f) || shrink != 1.f) {
+            const float f = alpha * shrink;
+#pragma unroll
+            for (int i = 0; i < OB; i++) acc[i] *= f;
+        }
+        const f16x8 *vp = reinterpret_cast<const f16x8 *>(v_lds[buffer]);
+#pragma unroll
+        for (int c = 0; c < GR; c++) {
+            f16x8 pf[TERMS];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float y = st[c / 2][c % 2 * 8 + j];
+                const _Float16 w = (_Float16)y;
+                pf[0][j] = w;
+                if constexpr (TERMS == 2) pf[1][j] = (_Float16)(y - (float)w);
+            }
+#pragma unroll
+            for (int i = 0; i < OB; i++) {
+                const f16x8 vf = vp[(i * (TOK / 16) + c) * 64 + lane];
+#pragma unroll
+                for (int t = TERMS - 1; t >= 0; t--)
+                    acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[t], acc[i], 0, 0, 0);
+            }
+        }
+    }
+
+    l = pair_sum(l);
+    if (row0 + n >= all_rows) return;
+    const float back = __builtin_ldexpf(1.f, ref - kTop + (E4M3 ? 8 : 0));
+    const float poison = s.ok ? 0.f : __uint_as_float(0x7fc00000u);
+    const float norm = (l == 0.f ? 0.f : 1.f / l) * back;
+    const int r = wave * 32 + n;
+    float *part = a.ws + ((int64_t)item * heads + head) * item_floats(kWideRows, a.D);
+    if (items > 1 && h == 0) {
+        part[r] = m;
+        part[kWideRows + r] = l;
+    }
+    const int64_t to = b * a.o.sb + (head * a.group + row - t_row * a.group) * a.o.sh + t_row * a.o.st;
+#pragma unroll
+    for (int i = 0; i < OB; i++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const int mm = j / 4 * 8 + h * 4 + j % 4;
+            const int d = DP == 64 ? 4 * (mm & 15) + i * 2 + mm / 16 : 4 * mm + i / 4 * 128 + i % 4;
+            if (d >= a.D) continue;
+            if (items > 1) part[2 * kWideRows + r * a.D + d] = acc[i][j] * back;
+            else store_row(a.o, a.dtype, to + d, (live ? acc[i][j] * norm : 0.f) + poison);
+        }
+}
+
+template <int DP, bool E4M3, int TERMS>
+int launch(const char *fn, const AttnArgs &a, int64_t blocks, hipStream_t st) {
+    ProfScope prof(ENATTEN_KERNEL_CACHE_ATTENTION, "attend_rows", st);
+    attend_rows<DP, E4M3, TERMS><<<(int)blocks, 512, 0, st>>>(a);
+    return launched(fn);
+}
+template <int DP, bool E4M3>
+int launch_terms(const char *fn, const AttnArgs &a, int64_t blocks, hipStream_t st) {
+    if constexpr (DP <= 128)
+        if (a.dtype == ENATTEN_F32) return launch<DP, E4M3, 2>(fn, a, blocks, st);
+    return launch<DP, E4M3, 1>(fn, a, blocks, st);
+}
+template <bool E4M3>
+int launch_dim(const char *fn, const AttnArgs &a, int64_t blocks, hipStream_t st) {
+    if (a.D <= 64) return launch_terms<64, E4M3>(fn, a, blocks, st);
+    if (a.D <= 128) return launch_terms<128, E4M3>(fn, a, blocks, st);
+    return launch_terms<256, E4M3>(fn, a, blocks, st);
+}
+
+}  // namespace
+
+int launch_attend_rows(const char *fn, const AttnArgs &a, bool e4m3, int64_t blocks, hipStream_t st) {
+    return e4m3 ? launch_dim<true>(fn, a, blocks, st) : launch_dim<false>(fn, a, blocks, st);
+}
+
+}  // namespace enatten

@@ -121,6 +121,13 @@ def _check(o, ref, bound, dtype, what):
     ([600, 9, 250], [5, 3, 0], 8, 2, 5, 64, 128, BF16, E4M3, None),  # drafted tokens, ragged
     ([600, 9, 250], [5, 3, 1], 8, 2, 5, 64, 128, F16, I8, 7),
     ([7, 50], None, 15, 5, 7, 80, 48, F32, I8, None),                # the whole sequence at once
+    ([600, 9, 1250], [5, 3, 1], 16, 2, 5, 64, 128, F16, E4M3, None),  # 40 rows
+    ([600, 8], None, 16, 2, 8, 64, 16, BF16, I8, 77),                # 64
+    ([600, 8], None, 16, 2, 8, 128, 16, F32, E4M3, None),
+    ([300, 6], None, 16, 2, 6, 128, 64, BF16, I8, None),
+    ([2000], None, 9, 1, 8, 96, 64, F16, I8, None),                  # 72 rows
+    ([3000, 2500, 64], None, 8, 4, 64, 128, 64, BF16, E4M3, 1500),   # 128 rows, split along the tokens
+    ([1500], None, 4, 1, 40, 64, 48, F32, I8, None),
     ([300, 200], [70, 33], 8, 2, 70, 128, 64, BF16, I8, None),       # chunks: several tiles of rows
     ([300, 200], [70, 33], 8, 2, 70, 128, 64, F16, E4M3, 50),
     ([260], None, 2, 2, 130, 192, 16, BF16, E4M3, 20),
