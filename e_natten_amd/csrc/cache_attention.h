@@ -11,10 +11,11 @@ struct AttnArgs {
     Table tb;
     int B, heads, group, heads_kv, T, D, window;  // group: query heads of a cache head
     int dtype;
+    bool wide_q, wide_o;  // rows at multiples of 16 bytes
     int row_tiles;   // per (sequence, cache head)
     int parts;       // workgroups per cache head that the split aims at; 0: one per row tile
     float scale;
-    float *ws;       // [item][cache head]: row maxima, row sums, rows x D sums
+    float *ws;       // (part_of)
 };
 
 // How a call is cut, from its sizes alone (the lengths are on the device).
@@ -62,49 +63,76 @@ __device__ __forceinline__ Span span_of(const AttnArgs &a, int entry) {
 template <int TOK>
 __device__ __forceinline__ int steps_of(const Span &s) { return s.hi > s.lo ? (s.hi - (s.lo & -16) + TOK - 1) / TOK : 0; }
 
-// How the row tiles ("entries") are cut into items of at most `chunk` steps; the same in every wave.
-__device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
-    return x;
+// Sums over the lanes up to and including each.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ int plus_moved(int x) {
+    return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROW_MASK, 0xf, false);
 }
+__device__ __forceinline__ int running_sum(int x) {
+    x = plus_moved<0x111, 0xf>(x);  // row_shr:1, 2, 4, 8: within 16 lanes
+    x = plus_moved<0x112, 0xf>(x);
+    x = plus_moved<0x114, 0xf>(x);
+    x = plus_moved<0x118, 0xf>(x);
+    x = plus_moved<0x142, 0xa>(x);  // row_bcast:15: lane 15 into the next 16, lane 47 likewise
+    return plus_moved<0x143, 0xc>(x);  // row_bcast:31
+}
+
+// One workgroup's share: some steps of a row tile ("entry").  Entries are cut into items of at most
+// `chunk` steps, about as many items as the call's `parts`; all items are equally long but the last of
+// an entry.  Every wave finds its item from the lengths.
+struct Share {
+    int entry, first, items;  // entry < 0: nothing; the number of its first item, and how many it has
+    int step0, step1, item;
+};
 template <int ROWS, int TOK>
-__device__ __forceinline__ int chunk_of(const AttnArgs &a) {
+__device__ __forceinline__ Share share_of(const AttnArgs &a, int item) {
+    Share w;
+    w.item = item;
     const int entries = a.B * a.row_tiles, lane = threadIdx.x & 63;
+    auto steps_at = [&](int e) { return e < entries ? steps_of<TOK>(span_of<ROWS>(a, e)) : 0; };
     long long total = 0;
+    int steps = 0;
     for (int e0 = 0; e0 < entries; e0 += 64) {
-        const int e = e0 + lane;
-        total += wave_sum(e < entries ? steps_of<TOK>(span_of<ROWS>(a, e)) : 0);
+        steps = steps_at(e0 + lane);
+        total += __builtin_amdgcn_readlane(running_sum(steps), 63);
     }
-    return max(kLeast / TOK, (int)((total + a.parts - 1) / a.parts));
-}
-__device__ __forceinline__ int items_of(int steps, int chunk) { return max(1, (steps + chunk - 1) / chunk); }
-// The entry of item `item` and the number of its first item, or (by_entry) the first item of entry
-// `item`; entry -1 if there is none.
-template <int ROWS, int TOK>
-__device__ __forceinline__ void find(const AttnArgs &a, int chunk, int item, bool by_entry, int &entry, int &first) {
-    const int entries = a.B * a.row_tiles, lane = threadIdx.x & 63;
+    const int chunk = max(kLeast / TOK, (int)((total + a.parts - 1) / a.parts));
     int before = 0;
-    entry = -1;
-    first = 0;
     for (int e0 = 0; e0 < entries; e0 += 64) {
         const int e = e0 + lane;
-        const int n = e < entries ? items_of(steps_of<TOK>(span_of<ROWS>(a, e)), chunk) : 0;
-        int upto = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int x = __shfl_up(upto, o, 64);
-            if (lane >= o) upto += x;
-        }
-        const bool mine = by_entry ? e == item : n > 0 && item >= before + upto - n && item < before + upto;
-        const unsigned long long who = __ballot(mine);
+        if (entries > 64) steps = steps_at(e);
+        const int n = e < entries ? max(1, (steps + chunk - 1) / chunk) : 0;
+        const int upto = before + running_sum(n);
+        const unsigned long long who = __ballot(item >= upto - n && item < upto);
         if (who) {
             const int l = __ffsll(who) - 1;
-            entry = e0 + l;
-            first = before + __shfl(upto - n, l, 64);
-            return;
+            w.entry = e0 + l;
+            w.items = __builtin_amdgcn_readlane(n, l);
+            w.first = __builtin_amdgcn_readlane(upto, l) - w.items;
+            const int all = __builtin_amdgcn_readlane(steps, l);
+            w.step0 = min((item - w.first) * chunk, all);
+            w.step1 = min(w.step0 + chunk, all);
+            return w;
         }
-        before += __shfl(upto, 63, 64);
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+    w.entry = -1;
+    return w;
+}
+
+// The workspace: first item and items of every entry, then for every (item, cache head) the maxima and
+// sums of its rows and rows x D sums of values.
+constexpr int64_t item_floats(int rows, int D) { return (int64_t)rows * (D + 2); }
+__host__ __device__ inline int64_t head_floats(int64_t entries) { return (2 * entries + 3) / 4 * 4; }
+__device__ __forceinline__ float *part_of(const AttnArgs &a, int rows, int item, int head) {
+    return a.ws + head_floats((int64_t)a.B * a.row_tiles) + ((int64_t)item * a.heads_kv + head) * item_floats(rows, a.D);
+}
+// (for the launch that joins the parts)
+__device__ __forceinline__ void note_share(const AttnArgs &a, const Share &w, int head) {
+    if (w.item == w.first && head == 0 && threadIdx.x == 0) {
+        int *note = reinterpret_cast<int *>(a.ws) + 2 * w.entry;
+        note[0] = w.first;
+        note[1] = w.items;
     }
 }
 
@@ -169,26 +197,93 @@ __device__ __forceinline__ void widen_columns(const unsigned (&t)[8], f16x8 (&ou
 __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
-// max / sum over the four lanes of a row
+// max / sum over the lanes l, l ^ 32
+__device__ __forceinline__ float pair_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pair_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// ... over the lanes l, l ^ 16, l ^ 32, l ^ 48
 __device__ __forceinline__ float row_max(float x) {
-    x = fmaxf(x, __shfl_xor(x, 16, 64));
-    return fmaxf(x, __shfl_xor(x, 32, 64));
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return pair_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
 }
 __device__ __forceinline__ float row_sum(float x) {
-    x += __shfl_xor(x, 16, 64);
-    return x + __shfl_xor(x, 32, 64);
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return pair_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
-__device__ __forceinline__ float load_row(const Rows &r, int dtype, int64_t at) {
-    if (dtype == ENATTEN_F32) return static_cast<const float *>(r.ptr)[at];
-    if (dtype == ENATTEN_BF16) return (float)static_cast<const __bf16 *>(r.ptr)[at];
-    return (float)static_cast<const _Float16 *>(r.ptr)[at];
+// N channels of a row, N a multiple of 8, by loads of 16 bytes if `wide` (rows at multiples of that)
+template <int N>
+__device__ __forceinline__ void load_channels(const Rows &r, int dtype, bool wide, int64_t at, float (&x)[N]) {
+    if (dtype == ENATTEN_F32) {
+        const float *p = static_cast<const float *>(r.ptr) + at;
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < N; i += 4) {
+                const f32x4 y = *reinterpret_cast<const f32x4 *>(p + i);
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[i + j] = y[j];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) x[i] = p[i];
+        }
+        return;
+    }
+    const unsigned short *p = static_cast<const unsigned short *>(r.ptr) + at;
+    unsigned y[N / 2];
+    if (wide) {
+#pragma unroll
+        for (int i = 0; i < N / 8; i++) {
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(p + i * 8);
+#pragma unroll
+            for (int j = 0; j < 4; j++) y[i * 4 + j] = w[j];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) y[i] = p[2 * i] | (unsigned)p[2 * i + 1] << 16;
+    }
+    if (dtype == ENATTEN_BF16) {
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = __uint_as_float(i % 2 ? y[i / 2] & 0xffff0000u : y[i / 2] << 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = (float)__builtin_bit_cast(f16x2, y[i / 2])[i % 2];
+    }
 }
-__device__ __forceinline__ void store_row(const Rows &r, int dtype, int64_t at, float x) {
-    void *p = const_cast<void *>(r.ptr);
-    if (dtype == ENATTEN_F32) static_cast<float *>(p)[at] = x;
-    else if (dtype == ENATTEN_BF16) static_cast<__bf16 *>(p)[at] = (__bf16)x;
-    else static_cast<_Float16 *>(p)[at] = (_Float16)x;
+// 4 channels of a row; `wide`: rows at multiples of 16 bytes
+__device__ __forceinline__ void store_channels(const Rows &r, int dtype, bool wide, int64_t at, f32x4 x) {
+    if (dtype == ENATTEN_F32) {
+        float *p = static_cast<float *>(const_cast<void *>(r.ptr)) + at;
+        if (wide) {
+            *reinterpret_cast<f32x4 *>(p) = x;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) p[i] = x[i];
+        }
+        return;
+    }
+    u32x2 y;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        if (dtype == ENATTEN_BF16) {
+            typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+            y[i] = __builtin_bit_cast(unsigned, bf16x2{(__bf16)x[2 * i], (__bf16)x[2 * i + 1]});
+        } else {
+            y[i] = __builtin_bit_cast(unsigned, f16x2{(_Float16)x[2 * i], (_Float16)x[2 * i + 1]});
+        }
+    }
+    unsigned short *p = static_cast<unsigned short *>(const_cast<void *>(r.ptr)) + at;
+    if (wide) {
+        *reinterpret_cast<u32x2 *>(p) = y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) p[i] = (unsigned short)(y[i / 2] >> i % 2 * 16);
+    }
 }
 
 __device__ __forceinline__ int lane_int(int x, int l) { return __builtin_amdgcn_readlane(x, l); }
@@ -199,9 +294,6 @@ __device__ __forceinline__ int64_t lane_offset(int64_t x, int l) {
     const unsigned lo = __builtin_amdgcn_readlane((int)x, l), hi = __builtin_amdgcn_readlane((int)(x >> 32), l);
     return (int64_t)((uint64_t)hi << 32 | lo);
 }
-
-// Floats of one item's part of the workspace
-constexpr int64_t item_floats(int rows, int D) { return (int64_t)rows * (D + 2); }
 
 }  // namespace
 

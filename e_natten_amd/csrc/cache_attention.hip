@@ -50,17 +50,24 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n16 = lane & 15, g4 = lane >> 4;
 
     // which row tile, and which of its steps
-    const int head = blockIdx.x % a.heads_kv, item = blockIdx.x / a.heads_kv;
-    int entry = item, first_item = item, chunk = 1 << 26;
+    const int head = blockIdx.x % a.heads_kv;
+    Share w;
     if (a.parts) {
-        chunk = chunk_of<ROWS, TOK>(a);
-        find<ROWS, TOK>(a, chunk, item, false, entry, first_item);
-        if (entry < 0) return;
+        w = share_of<ROWS, TOK>(a, blockIdx.x / a.heads_kv);
+        if (w.entry < 0) return;
+        note_share(a, w, head);
+    } else {
+        w.entry = blockIdx.x / a.heads_kv;
+        w.items = 1;
     }
+    const int entry = w.entry;
     const Span s = span_of<ROWS>(a, entry);
+    if (!a.parts) {
+        w.step0 = 0;
+        w.step1 = steps_of<TOK>(s);
+    }
     const int b = entry / a.row_tiles, row0 = (entry - b * a.row_tiles) * ROWS;
-    const int total = steps_of<TOK>(s), items = items_of(total, chunk);
-    const int step0 = min((item - first_item) * chunk, total), step1 = min(step0 + chunk, total);
+    const int step0 = w.step0, step1 = w.step1;
     const int base = s.lo & -16;
 
     // q: lane (row n16, g4) has channels 64 c + 16 g4 .. + 15
@@ -76,11 +83,15 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
         const int64_t at = b * a.q.sb + (head * a.group + row - t * a.group) * a.q.sh + t * a.q.st;
         float x[KC][16], top = 0.f, nan = 0.f;
 #pragma unroll
+        for (int c = 0; c < KC; c++) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) x[c][j] = 0.f;
+            if (c * 64 + g4 * 16 < a.D) load_channels<16>(a.q, a.dtype, a.wide_q, at + c * 64 + g4 * 16, x[c]);
+        }
+#pragma unroll
         for (int c = 0; c < KC; c++)
 #pragma unroll
             for (int j = 0; j < 16; j++) {
-                const int d = c * 64 + g4 * 16 + j;
-                x[c][j] = d < a.D ? load_row(a.q, a.dtype, at + d) : 0.f;
                 top = fmaxf(top, fabsf(x[c][j]));
                 nan += x[c][j] * 0.f;  // a value that is not finite makes its row NaN
             }
@@ -300,11 +311,11 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
         __syncthreads();
         float top = part_m[0][mr], f[4], all = 0.f;
 #pragma unroll
-        for (int w = 1; w < 4; w++) top = fmaxf(top, part_m[w][mr]);
+        for (int v = 1; v < 4; v++) top = fmaxf(top, part_m[v][mr]);
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
-            f[w] = __builtin_amdgcn_exp2f(part_m[w][mr] - top);
-            all += f[w] * part_l[w][mr];
+        for (int v = 0; v < 4; v++) {
+            f[v] = __builtin_amdgcn_exp2f(part_m[v][mr] - top);
+            all += f[v] * part_l[v][mr];
         }
         const int row = row0 + r * 16 + mr;
         if (row >= a.T * a.group) continue;
@@ -312,83 +323,98 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
         const int64_t at = b * a.o.sb + (head * a.group + row - t * a.group) * a.o.sh + t * a.o.st;
         const float poison = s.ok ? 0.f : __uint_as_float(0x7fc00000u);
         const bool live = t < s.count;
-        float *part = a.ws + ((int64_t)item * a.heads_kv + head) * item_floats(ROWS, a.D);
-        if (items > 1 && mc == 0) {
+        float *part = part_of(a, ROWS, w.item, head);
+        if (w.items > 1 && mc == 0) {
             part[r * 16 + mr] = top;
             part[ROWS + r * 16 + mr] = all;
         }
-        const float norm = all == 0.f ? 0.f : 1.f / all;
+        const float norm = all == 0.f || !live ? 0.f : 1.f / all;
 #pragma unroll
-        for (int c = 0; c < DT; c++) {
+        for (int c = 0; c < DT; c += 4) {
             const int d = mc * DT + c;
             if (d >= a.D) break;
-            float y = 0.f;
+            f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < 4; w++) y += f[w] * part_o[w][mr][d];
-            if (items > 1) part[2 * ROWS + (r * 16 + mr) * a.D + d] = y;
-            else store_row(a.o, a.dtype, at + d, (live ? y * norm : 0.f) + poison);
+            for (int v = 0; v < 4; v++) y += f[v] * *reinterpret_cast<const f32x4 *>(&part_o[v][mr][d]);
+            if (w.items > 1) *reinterpret_cast<f32x4 *>(part + 2 * ROWS + (r * 16 + mr) * a.D + d) = y;
+            else store_channels(a.o, a.dtype, a.wide_o, at + d, (live ? y * norm : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
         }
     }
 }
 
-// The parts of a row joined: one workgroup per (row tile, cache head, row)
-template <int ROWS, int TOK>
+// The parts of a row joined: one workgroup per (row tile, cache head, row).
+template <int ROWS>
 __global__ __launch_bounds__(256) void attend_join(AttnArgs a) {
     const int per = min(ROWS, a.T * a.group);
     int block = blockIdx.x;
     const int r = block % per;
     block /= per;
     const int head = block % a.heads_kv, entry = block / a.heads_kv;
+    const int *note = reinterpret_cast<const int *>(a.ws) + 2 * entry;
+    const int first = note[0], items = note[1];
     const int b = entry / a.row_tiles, row = (entry - b * a.row_tiles) * ROWS + r;
-    if (row >= a.T * a.group) return;
-    const int chunk = chunk_of<ROWS, TOK>(a);
-    const Span s = span_of<ROWS>(a, entry);
-    const int items = items_of(steps_of<TOK>(s), chunk);
-    if (items == 1) return;
-    int same, first;
-    find<ROWS, TOK>(a, chunk, entry, true, same, first);
-    const int t = row / a.group;
-    const int64_t at = b * a.o.sb + (head * a.group + row - t * a.group) * a.o.sh + t * a.o.st;
-    const float *ws = a.ws + ((int64_t)first * a.heads_kv + head) * item_floats(ROWS, a.D);
+    if (items == 1 || row >= a.T * a.group) return;
+    const float *ws = part_of(a, ROWS, first, head);
     const int64_t stride = a.heads_kv * item_floats(ROWS, a.D);
 
+    // lanes over the channels, 4 each, and the remaining factor of 256 over the items, each with the
+    // maximum of its own so far
     __shared__ __align__(16) float red[256][4];
-    __shared__ float top_s[4], sums[256];
-    float top = kFloor;
-    for (int i = threadIdx.x; i < items; i += 256) top = fmaxf(top, ws[i * stride + r]);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    if (threadIdx.x % 64 == 0) top_s[threadIdx.x / 64] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(top_s[0], top_s[1]), fmaxf(top_s[2], top_s[3]));
-
-    // lanes over the channels, 4 each, and the remaining factor of 256 over the items
+    __shared__ float tops[256], sums[256];
     const int lanes = a.D / 4, groups = 256 / lanes, c = threadIdx.x % lanes, g = threadIdx.x / lanes;
     f32x4 y = {0.f, 0.f, 0.f, 0.f};
-    float sum = 0.f;
+    float sum = 0.f, top = kFloor;
     if (g < groups) {
-#pragma unroll 4
-        for (int i = g; i < items; i += groups) {
-            const float *p = ws + i * stride;
-            const float f = __builtin_amdgcn_exp2f(p[r] - top);
-            sum += f * p[ROWS + r];
-            y += f * *reinterpret_cast<const f32x4 *>(p + 2 * ROWS + r * a.D + c * 4);
+        constexpr int DEEP = 4;  // items whose loads are under way at a time
+        for (int i0 = g; i0 < items; i0 += groups * DEEP) {
+            float m[DEEP], l[DEEP];
+            f32x4 x[DEEP];
+#pragma unroll
+            for (int k = 0; k < DEEP; k++) {
+                const int i = i0 + k * groups;
+                const float *p = ws + min(i, items - 1) * stride;
+                m[k] = i < items ? p[r] : kFloor;
+                l[k] = i < items ? p[ROWS + r] : 0.f;
+                x[k] = *reinterpret_cast<const f32x4 *>(p + 2 * ROWS + r * a.D + c * 4);
+                if (i >= items) x[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+            float most = top;
+#pragma unroll
+            for (int k = 0; k < DEEP; k++) most = fmaxf(most, m[k]);
+            const float old = __builtin_amdgcn_exp2f(top - most);
+            sum *= old;
+            y *= old;
+            top = most;
+#pragma unroll
+            for (int k = 0; k < DEEP; k++) {
+                const float f = __builtin_amdgcn_exp2f(m[k] - top);
+                sum += f * l[k];
+                y += f * x[k];
+            }
         }
     }
+    tops[threadIdx.x] = top;
     sums[threadIdx.x] = sum;
     *reinterpret_cast<f32x4 *>(red[threadIdx.x]) = y;
     __syncthreads();
     if (g == 0) {
-        for (int i = 1; i < groups; i++) {
-            y += *reinterpret_cast<const f32x4 *>(red[i * lanes + c]);
-            sum += sums[i * lanes + c];
+        for (int i = 1; i < groups; i++) top = fmaxf(top, tops[i * lanes]);
+        sum = 0.f;
+        y = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < groups; i++) {
+            const float f = __builtin_amdgcn_exp2f(tops[i * lanes] - top);
+            sum += f * sums[i * lanes];
+            y += f * *reinterpret_cast<const f32x4 *>(red[i * lanes + c]);
         }
+        const int t = row / a.group;
+        const int64_t at = b * a.o.sb + (head * a.group + row - t * a.group) * a.o.sh + t * a.o.st;
+        const int count = a.tb.counts ? a.tb.counts[b] : a.T;
         const float norm = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-        for (int j = 0; j < 4; j++) store_row(a.o, a.dtype, at + c * 4 + j, t < s.count ? y[j] * norm : 0.f);
+        store_channels(a.o, a.dtype, a.wide_o, at + c * 4, t < count ? y * norm : f32x4{0.f, 0.f, 0.f, 0.f});
     }
 }
 
+// How a call is cut, from its sizes alone (the lengths are on the device).
 Plan plan_of(int B, int heads, int heads_kv, int T, int D, int page, int columns, int window, int dtype) {
     Plan p;
     const int64_t all = (int64_t)T * (heads / heads_kv);
@@ -413,7 +439,7 @@ Plan plan_of(int B, int heads, int heads_kv, int T, int D, int page, int columns
     return p;
 }
 
-template <int ROWS, int TOK>
+template <int ROWS>
 int launch_join(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st) {
     if (!p.parts) return ENATTEN_OK;
     const int64_t rows = a.T * (int64_t)a.group, blocks = (int64_t)a.B * p.row_tiles * a.heads_kv * (rows < ROWS ? rows : ROWS);
@@ -422,7 +448,7 @@ int launch_join(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st
         return ENATTEN_EUNSUPPORTED;
     }
     ProfScope prof(ENATTEN_KERNEL_CACHE_JOIN, "attend_join", st);
-    attend_join<ROWS, TOK><<<(int)blocks, 256, 0, st>>>(a);
+    attend_join<ROWS><<<(int)blocks, 256, 0, st>>>(a);
     return launched(fn);
 }
 template <int DP, int R, bool E4M3, int TERMS>
@@ -432,7 +458,7 @@ int launch(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st) {
         attend<DP, R, E4M3, TERMS><<<(int)(p.items * a.heads_kv), 256, 0, st>>>(a);
     }
     const int rc = launched(fn);
-    return rc ? rc : launch_join<16 * R, kTile>(fn, a, p, st);
+    return rc ? rc : launch_join<16 * R>(fn, a, p, st);
 }
 template <int DP, int R, bool E4M3>
 int launch_terms(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st) {
@@ -446,7 +472,7 @@ int launch_rows(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st
     }
     if (p.rows == kWideRows) {
         const int rc = launch_attend_rows(fn, a, E4M3, p.items * a.heads_kv, st);
-        return rc ? rc : launch_join<kWideRows, 8192 / DP>(fn, a, p, st);
+        return rc ? rc : launch_join<kWideRows>(fn, a, p, st);
     }
     if (p.rows == 16) return launch_terms<DP, 1, E4M3>(fn, a, p, st);
     if constexpr (DP <= 128) {
@@ -470,7 +496,8 @@ size_t enatten_cache_attention_workspace_bytes(int B, int heads, int heads_kv, i
         kernel_size < 0)
         return 0;
     const Plan p = plan_of(B, heads, heads_kv, T, D, page, columns, kernel_size, dtype);
-    return p.parts ? (size_t)p.items * heads_kv * item_floats(p.rows, D) * sizeof(float) : 0;
+    if (!p.parts) return 0;
+    return (size_t)(head_floats((int64_t)B * p.row_tiles) + p.items * heads_kv * item_floats(p.rows, D)) * sizeof(float);
 }
 
 int enatten_cache_attention(const void *q, const void *k_cache, const void *v_cache, const float *k_scale,
@@ -511,6 +538,9 @@ int enatten_cache_attention(const void *q, const void *k_cache, const void *v_ca
     a.B = B; a.heads = heads; a.group = heads / heads_kv; a.heads_kv = heads_kv; a.T = T; a.D = D;
     a.window = kernel_size;
     a.dtype = dtype;
+    const int pack = dtype == ENATTEN_F32 ? 4 : 8;
+    a.wide_q = (uintptr_t)q % 16 == 0 && (a.q.sb | a.q.sh | a.q.st) % pack == 0;
+    a.wide_o = (uintptr_t)o % 16 == 0 && (a.o.sb | a.o.sh | a.o.st) % pack == 0;
     a.row_tiles = p.row_tiles;
     a.parts = p.parts;
     a.scale = scale;

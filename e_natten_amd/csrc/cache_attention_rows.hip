@@ -21,15 +21,6 @@ namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-// a lane's and its partner's (32 lanes on) maximum and sum
-__device__ __forceinline__ float pair_max(float x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float pair_sum(float x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
 __device__ __forceinline__ float uniform(float x) {
     return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
 }
@@ -53,23 +44,27 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
     // the order of the cache heads go to different ones, the row tiles of a head to the same where
     // their number allows.  Later rows see more tokens: they come first.
     const int heads = a.heads_kv;
-    int head, entry, item, first_item, chunk = 1 << 26;
+    int head;
+    Share w;
     if (a.parts) {
         head = blockIdx.x % heads;
-        item = blockIdx.x / heads;
-        chunk = chunk_of<kWideRows, TOK>(a);
-        find<kWideRows, TOK>(a, chunk, item, false, entry, first_item);
-        if (entry < 0) return;
+        w = share_of<kWideRows, TOK>(a, blockIdx.x / heads);
+        if (w.entry < 0) return;
+        note_share(a, w, head);
     } else {
         const int pair = blockIdx.x % (heads * a.B);
         head = pair % heads;
-        entry = pair / heads * a.row_tiles + a.row_tiles - 1 - blockIdx.x / (heads * a.B);
-        item = first_item = entry;
+        w.entry = pair / heads * a.row_tiles + a.row_tiles - 1 - blockIdx.x / (heads * a.B);
+        w.items = 1;
     }
+    const int entry = w.entry;
     const Span s = span_of<kWideRows>(a, entry);
+    if (!a.parts) {
+        w.step0 = 0;
+        w.step1 = steps_of<TOK>(s);
+    }
     const int b = entry / a.row_tiles, row0 = (entry - b * a.row_tiles) * kWideRows + wave * 32;
-    const int total = steps_of<TOK>(s), items = items_of(total, chunk);
-    const int step0 = min((item - first_item) * chunk, total), step1 = min(step0 + chunk, total);
+    const int step0 = w.step0, step1 = w.step1;
     const int base = s.lo & -16;
     const int all_rows = a.T * a.group;
 
@@ -82,15 +77,19 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
     {
         const int64_t at = b * a.q.sb + (head * a.group + row - t_row * a.group) * a.q.sh + t_row * a.q.st;
         const float flip = a.scale < 0.f ? -1.f : 1.f;  // into q, so that units are not negative
-        float top = 0.f, nan = 0.f;
+        float x[SD][8], top = 0.f, nan = 0.f;
+#pragma unroll
+        for (int c = 0; c < SD; c++) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[c][j] = 0.f;
+            if (c * 16 < a.D) load_channels<8>(a.q, a.dtype, a.wide_q, at + c * 16 + h * 8, x[c]);
+        }
 #pragma unroll
         for (int c = 0; c < SD; c++)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const int d = c * 16 + h * 8 + j;
-                const float x = d < a.D ? load_row(a.q, a.dtype, at + d) : 0.f;
-                top = fmaxf(top, fabsf(x));
-                nan += x * 0.f;
+                top = fmaxf(top, fabsf(x[c][j]));
+                nan += x[c][j] * 0.f;  // a value that is not finite makes its row NaN
             }
         nan = pair_sum(nan);
         top = pair_max(top);
@@ -100,12 +99,10 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
         for (int c = 0; c < SD; c++)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const int d = c * 16 + h * 8 + j;
-                const float x = d < a.D ? load_row(a.q, a.dtype, at + d) : 0.f;
-                const float y = __builtin_ldexpf(x * flip, up);
-                const _Float16 w = (_Float16)y;
-                qf[c][0][j] = w;
-                if constexpr (TERMS == 2) qf[c][1][j] = (_Float16)(y - (float)w);
+                const float y = __builtin_ldexpf(x[c][j] * flip, up);
+                const _Float16 v = (_Float16)y;
+                qf[c][0][j] = v;
+                if constexpr (TERMS == 2) qf[c][1][j] = (_Float16)(y - (float)v);
             }
     }
     // tokens that any, and that all rows of the wave see
@@ -317,21 +314,26 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
     const float poison = s.ok ? 0.f : __uint_as_float(0x7fc00000u);
     const float norm = (l == 0.f ? 0.f : 1.f / l) * back;
     const int r = wave * 32 + n;
-    float *part = a.ws + ((int64_t)item * heads + head) * item_floats(kWideRows, a.D);
-    if (items > 1 && h == 0) {
+    float *part = part_of(a, kWideRows, w.item, head);
+    if (w.items > 1 && h == 0) {
         part[r] = m;
         part[kWideRows + r] = l;
     }
     const int64_t to = b * a.o.sb + (head * a.group + row - t_row * a.group) * a.o.sh + t_row * a.o.st;
+    const float f = w.items > 1 ? back : live ? norm : 0.f;
+    // 4 neighbouring channels: words of one value row, blocks i of O, or for DP 64 rows 16 apart too
 #pragma unroll
-    for (int i = 0; i < OB; i++)
+    for (int i = 0; i < OB; i += DP == 64 ? 2 : 4)
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
+        for (int j = 0; j < (DP == 64 ? 8 : 16); j++) {
             const int mm = j / 4 * 8 + h * 4 + j % 4;
-            const int d = DP == 64 ? 4 * (mm & 15) + i * 2 + mm / 16 : 4 * mm + i / 4 * 128 + i % 4;
+            f32x4 y;
+            if constexpr (DP == 64) y = f32x4{acc[0][j], acc[0][j + 8], acc[1][j], acc[1][j + 8]};
+            else y = f32x4{acc[i][j], acc[i + 1][j], acc[i + 2][j], acc[i + 3][j]};
+            const int d = 4 * mm + i / 4 * 128;
             if (d >= a.D) continue;
-            if (items > 1) part[2 * kWideRows + r * a.D + d] = acc[i][j] * back;
-            else store_row(a.o, a.dtype, to + d, (live ? acc[i][j] * norm : 0.f) + poison);
+            if (w.items > 1) *reinterpret_cast<f32x4 *>(part + 2 * kWideRows + r * a.D + d) = y * f;
+            else store_channels(a.o, a.dtype, a.wide_o, to + d, (live ? y * f : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
         }
 }
 
