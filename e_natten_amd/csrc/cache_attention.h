@@ -38,7 +38,9 @@ typedef short s16x2 __attribute__((ext_vector_type(2)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFloor = -1e37f;  // the maximum of a row that has seen nothing: finite, below every logit
 constexpr int kLeast = 256;       // tokens of a part at least: what a workgroup takes to get going pays from there
-constexpr int kTop = 14;          // float16 operands are brought to 2^kTop
+constexpr int kTop = 14;          // rows of q are brought to 2^kTop .. 2 * 2^kTop
+constexpr int kPTop = 7;          // probabilities to 2^kPTop, and up to 2^kSlack times that where the
+constexpr int kSlack = 8;         // running maximum is let lag behind
 
 // The tokens that one row tile sees: [lo, hi), hi <= lo if none.
 struct Span {
@@ -84,19 +86,22 @@ struct Share {
     int entry, first, items;  // entry < 0: nothing; the number of its first item, and how many it has
     int step0, step1, item;
 };
-template <int ROWS, int TOK>
+// WAVES: how many waves share the steps of an item (each takes whole ones).
+template <int ROWS, int TOK, int WAVES>
 __device__ __forceinline__ Share share_of(const AttnArgs &a, int item) {
     Share w;
     w.item = item;
     const int entries = a.B * a.row_tiles, lane = threadIdx.x & 63;
     auto steps_at = [&](int e) { return e < entries ? steps_of<TOK>(span_of<ROWS>(a, e)) : 0; };
-    long long total = 0;
+    float total = 0.f;
     int steps = 0;
     for (int e0 = 0; e0 < entries; e0 += 64) {
         steps = steps_at(e0 + lane);
-        total += __builtin_amdgcn_readlane(running_sum(steps), 63);
+        total += (float)(unsigned)__builtin_amdgcn_readlane(running_sum(steps), 63);
     }
-    const int chunk = max(kLeast / TOK, (int)((total + a.parts - 1) / a.parts));
+    // (a little more than the quotient: the items are at most `parts` and one for every entry)
+    const int each = (int)(total * 1.00001f / a.parts) + 1;
+    const int chunk = max(kLeast / TOK, each + WAVES - 1) / WAVES * WAVES;
     int before = 0;
     for (int e0 = 0; e0 < entries; e0 += 64) {
         const int e = e0 + lane;
@@ -138,21 +143,32 @@ __device__ __forceinline__ void note_share(const AttnArgs &a, const Share &w, in
 
 __device__ __forceinline__ f16x2 as_half(unsigned x) { return __builtin_bit_cast(f16x2, x); }
 
-// Two codes side by side, each in the upper byte of a half (E4M3) or the lower byte of a half of
-// 0x6400 (int8, offset 128), as float16.  E4M3: sign, 4 exponent and 3 mantissa bits move to the places
-// of float16's, whose exponents are offset by 8 more: the value times 2^-8.
+// Two codes side by side as float16: int8 in the lower byte of halves of 0x6400, offset by 128; E4M3 in
+// the upper byte of each half: sign, 4 exponent and 3 mantissa bits move to the places of float16's,
+// whose exponents are offset by 8 more, which gives the value times 2^-8.
+__device__ __forceinline__ f16x2 from_int8(unsigned x) {
+    return as_half(x) + f16x2{(_Float16)-1152.f, (_Float16)-1152.f};
+}
 __device__ __forceinline__ f16x2 from_e4m3(unsigned x) {
     const s16x2 s = __builtin_bit_cast(s16x2, x) >> 1;
     return as_half(__builtin_bit_cast(unsigned, s) & 0xbfffbfffu);
 }
-__device__ __forceinline__ f16x2 from_int8(unsigned x) {
-    return as_half(x) + f16x2{(_Float16)-1152.f, (_Float16)-1152.f};
+// The conversion instruction gives the same and takes half the operations, but NaN for the codes 0x7f
+// and 0xff: only where every row sees the tokens (a weight of 0 would not hide a NaN).
+template <bool HIGH>
+__device__ __forceinline__ f16x2 from_e4m3_word(unsigned x) {
+    return __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 0x1p-8f, HIGH));
 }
 // 8 consecutive codes
-template <bool E4M3>
+template <bool E4M3, bool SEEN>
 __device__ __forceinline__ f16x8 widen_row(unsigned x0, unsigned x1) {
     f16x2 h[4];
-    if constexpr (E4M3) {
+    if constexpr (E4M3 && SEEN) {
+        h[0] = from_e4m3_word<false>(x0);
+        h[1] = from_e4m3_word<true>(x0);
+        h[2] = from_e4m3_word<false>(x1);
+        h[3] = from_e4m3_word<true>(x1);
+    } else if constexpr (E4M3) {
         h[0] = from_e4m3(__builtin_amdgcn_perm(x0, x0, 0x010c000cu));
         h[1] = from_e4m3(__builtin_amdgcn_perm(x0, x0, 0x030c020cu));
         h[2] = from_e4m3(__builtin_amdgcn_perm(x1, x1, 0x010c000cu));
@@ -168,23 +184,33 @@ __device__ __forceinline__ f16x8 widen_row(unsigned x0, unsigned x1) {
     return f16x8{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
 }
 // 4 channels (one word) of 8 tokens, transposed: out[i] is channel i of the 8 tokens
-template <bool E4M3>
+template <bool E4M3, bool SEEN>
 __device__ __forceinline__ void widen_columns(const unsigned (&t)[8], f16x8 (&out)[4]) {
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
         f16x2 h[4];
-        if constexpr (E4M3) {
+        if constexpr (E4M3 && !SEEN) {
             h[0] = from_e4m3(__builtin_amdgcn_perm(t[j + 1], t[j], 0x040c000cu));
             h[1] = from_e4m3(__builtin_amdgcn_perm(t[j + 1], t[j], 0x050c010cu));
             h[2] = from_e4m3(__builtin_amdgcn_perm(t[j + 1], t[j], 0x060c020cu));
             h[3] = from_e4m3(__builtin_amdgcn_perm(t[j + 1], t[j], 0x070c030cu));
         } else {
-            const unsigned lo = __builtin_amdgcn_perm(t[j + 1], t[j], 0x05010400u) ^ 0x80808080u;
-            const unsigned hi = __builtin_amdgcn_perm(t[j + 1], t[j], 0x07030602u) ^ 0x80808080u;
-            h[0] = from_int8(__builtin_amdgcn_perm(0x64646464u, lo, 0x04010400u));
-            h[1] = from_int8(__builtin_amdgcn_perm(0x64646464u, lo, 0x04030402u));
-            h[2] = from_int8(__builtin_amdgcn_perm(0x64646464u, hi, 0x04010400u));
-            h[3] = from_int8(__builtin_amdgcn_perm(0x64646464u, hi, 0x04030402u));
+            // channel by channel the two tokens' codes
+            unsigned lo = __builtin_amdgcn_perm(t[j + 1], t[j], 0x05010400u);
+            unsigned hi = __builtin_amdgcn_perm(t[j + 1], t[j], 0x07030602u);
+            if constexpr (E4M3) {
+                h[0] = from_e4m3_word<false>(lo);
+                h[1] = from_e4m3_word<true>(lo);
+                h[2] = from_e4m3_word<false>(hi);
+                h[3] = from_e4m3_word<true>(hi);
+            } else {
+                lo ^= 0x80808080u;
+                hi ^= 0x80808080u;
+                h[0] = from_int8(__builtin_amdgcn_perm(0x64646464u, lo, 0x04010400u));
+                h[1] = from_int8(__builtin_amdgcn_perm(0x64646464u, lo, 0x04030402u));
+                h[2] = from_int8(__builtin_amdgcn_perm(0x64646464u, hi, 0x04010400u));
+                h[3] = from_int8(__builtin_amdgcn_perm(0x64646464u, hi, 0x04030402u));
+            }
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -192,6 +218,51 @@ __device__ __forceinline__ void widen_columns(const unsigned (&t)[8], f16x8 (&ou
             out[i][j + 1] = h[i][1];
         }
     }
+}
+
+// A value scale that is not finite counts as NaN.
+__device__ __forceinline__ float finite_or_nan(float z) { return fabsf(z) < INFINITY ? z : __uint_as_float(0x7fc00000u); }
+
+// The value scales z' of the groups go into the probabilities relative to the largest power of two of
+// them so far, 2^ref, times 2^kPTop.  `grow` brings ref up to date and returns what the sums so far are
+// multiplied by.  (ref is the same in all lanes; `top` is log2 of the step's largest z'.)
+__device__ __forceinline__ float grow(float &ref, float top) {
+    if (!(top > ref)) return 1.f;
+    const float old = ref;
+    ref = ceilf(top);
+    return __builtin_amdgcn_exp2f(old - ref);
+}
+// log2 of a group's factor.  Scales of 0 and far below the largest go in with a weight that float16
+// drops, whatever the codes; NaN stays.
+__device__ __forceinline__ float log_weight(float log_z, float ref) {
+    const float x = log_z + ((float)kPTop - ref);
+    return x < -40.f ? -40.f : x;
+}
+// For float32, where the last bits of log2 and exp2 would show, the factor itself.
+__device__ __forceinline__ float plain_weight(float z, float ref) {
+    const float x = __builtin_ldexpf(z, kPTop - (int)ref);
+    return x < 0x1p-40f ? 0x1p-40f : x;
+}
+// Two values as two float16 terms each.  The compiler may form the rounded value twice, once of the
+// rounded product that x is and once fused with that product; what is left has to be that of the one
+// that is used.
+__device__ __forceinline__ void two_terms(float x, float y, f16x2 &high, f16x2 &low) {
+    unsigned w = __builtin_bit_cast(unsigned, f16x2{(_Float16)x, (_Float16)y});
+    asm("" : "+v"(w));
+    high = as_half(w);
+    low = f16x2{(_Float16)(x - (float)high[0]), (_Float16)(y - (float)high[1])};
+}
+// Whether the sum of probabilities may be formed of what the second product takes, rounded to float16:
+// then a rounding moves a weight in both, and the result stays a mean of values.  A group far below the
+// largest scale has weights that float16 drops; they count in the sum all the same.
+__device__ __forceinline__ bool close(float lz) { return __builtin_amdgcn_readfirstlane(lz >= 0.f); }
+// What divides the factor out of a sum; 0 for NaN, which the sum of a row that sees such a group has
+// itself, and one that does not is 0.
+__device__ __forceinline__ float inverse_weight(float lz) { return lz == lz ? __builtin_amdgcn_exp2f(-lz) : 0.f; }
+// sum of four float16 values in float32
+__device__ __forceinline__ float sum4(_Float16 a, _Float16 b, _Float16 c, _Float16 d, float more) {
+    const f16x2 one = {(_Float16)1.f, (_Float16)1.f};
+    return __builtin_amdgcn_fdot2(f16x2{c, d}, one, __builtin_amdgcn_fdot2(f16x2{a, b}, one, more, false), false);
 }
 
 __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {

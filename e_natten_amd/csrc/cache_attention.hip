@@ -30,6 +30,8 @@
 // every workgroup computes it for itself.
 #include "cache_attention.h"
 
+#include <type_traits>
+
 namespace enatten {
 namespace {
 
@@ -53,7 +55,7 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
     const int head = blockIdx.x % a.heads_kv;
     Share w;
     if (a.parts) {
-        w = share_of<ROWS, TOK>(a, blockIdx.x / a.heads_kv);
+        w = share_of<ROWS, TOK, 4>(a, blockIdx.x / a.heads_kv);
         if (w.entry < 0) return;
         note_share(a, w, head);
     } else {
@@ -72,7 +74,8 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
 
     // q: lane (row n16, g4) has channels 64 c + 16 g4 .. + 15
     f16x8 qf[R][KC][2][TERMS];
-    float unit[R];           // what a product of codes is multiplied by, besides z: log2 units
+    float unit[R];           // what a product of codes is multiplied by, besides z: log2 units, not negative
+    const float flip = a.scale < 0.f ? -1.f : 1.f;
     int lo_r[R], hi_r[R];    // tokens that the lane's row sees
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -99,15 +102,24 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
         top = row_max(top);
         const int e = top > 0.f ? __builtin_amdgcn_frexp_expf(top) : 0;
         const int up = kTop + 1 - e;  // the largest to 2^14 .. 2^15
-        unit[r] = __builtin_ldexpf(a.scale * kLog2e, -up + (E4M3 ? 8 : 0)) + nan;
+        unit[r] = __builtin_ldexpf(fabsf(a.scale) * kLog2e, -up + (E4M3 ? 8 : 0)) + nan;
 #pragma unroll
         for (int c = 0; c < KC; c++)
 #pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const float y = __builtin_ldexpf(x[c][j], up);
-                const _Float16 h = (_Float16)y;
-                qf[r][c][j / 8][0][j % 8] = h;
-                if constexpr (TERMS == 2) qf[r][c][j / 8][1][j % 8] = (_Float16)(y - (float)h);
+            for (int j = 0; j < 16; j += 2) {
+                const float y0 = __builtin_ldexpf(x[c][j] * flip, up), y1 = __builtin_ldexpf(x[c][j + 1] * flip, up);
+                f16x8 &w = qf[r][c][j / 8][0];
+                if constexpr (TERMS == 2) {
+                    f16x2 high, low;
+                    two_terms(y0, y1, high, low);
+                    w[j % 8] = high[0];
+                    w[j % 8 + 1] = high[1];
+                    qf[r][c][j / 8][1][j % 8] = low[0];
+                    qf[r][c][j / 8][1][j % 8 + 1] = low[1];
+                } else {
+                    w[j % 8] = (_Float16)y0;
+                    w[j % 8 + 1] = (_Float16)y1;
+                }
             }
     }
     // between these all rows see every token
@@ -123,7 +135,7 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
 #pragma unroll
         for (int i = 0; i < DT; i++) acc[r][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    int ref = -126;  // the z' so far are at most 2^ref
+    float ref = -126.f;  // the z' so far are at most 2^ref
 
     // the wave's steps, and the places of their two groups of 16 tokens: lane i holds group `filled` + i
     const int quarter = (step1 - step0 + 3) / 4;
@@ -135,7 +147,8 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
         filled = group;
         const int token = base + (group + lane) * 16;
         k_at = v_at = 0;
-        k_z = v_z = 0.f;
+        k_z = 0.f;
+        v_z = TERMS == 1 ? -INFINITY : 0.f;  // (its log2, but for float32)
         if (token < s.hi && token >= 0) {
             const int column = token / a.tb.page, within = token - column * a.tb.page;
             const int at = a.tb.pages[b * a.tb.stride + column];
@@ -143,7 +156,8 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
                 k_at = at * a.k.sp + head * a.k.sh + within * a.k.st;
                 v_at = at * a.v.sp + head * a.v.sh + within * a.v.st;
                 k_z = a.k.scales[at * a.k.zp + head * a.k.zh];
-                v_z = a.v.scales[at * a.v.zp + head * a.v.zh];
+                v_z = finite_or_nan(a.v.scales[at * a.v.zp + head * a.v.zh]);
+                if (TERMS == 1) v_z = __builtin_amdgcn_logf(v_z);
             } else {
                 k_z = __uint_as_float(0x7fc00000u);
             }
@@ -186,17 +200,16 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
             }
         }
     };
-    auto work = [&](int step, const Tile &t) {
-        // a larger z' than any so far
-        const float zmax = fmaxf(fabsf(t.vz[0]), fabsf(t.vz[1]));
-        float shrink = 1.f;
-        const int e = __builtin_amdgcn_frexp_expf(zmax);
-        if (zmax < INFINITY && zmax > 0.f && e > ref) {
-            shrink = __builtin_ldexpf(1.f, max(ref - e, -200));
-            ref = e;
+    // SEEN: every row sees every token of the step
+    auto work = [&](auto seen, int step, const Tile &t) {
+        constexpr bool SEEN = decltype(seen)::value;
+        const float most_z = fmaxf(t.vz[0], t.vz[1]), shrink = grow(ref, TERMS == 1 ? most_z : __builtin_amdgcn_logf(most_z));
+        float lz[2], inv_z[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            lz[h] = TERMS == 1 ? log_weight(t.vz[h], ref) : plain_weight(t.vz[h], ref);
+            inv_z[h] = inverse_weight(lz[h]);
         }
-        const float z0 = __builtin_ldexpf(t.vz[0], kTop - ref), z1 = __builtin_ldexpf(t.vz[1], kTop - ref);
-
         f32x4 st[R][2];
 #pragma unroll
         for (int r = 0; r < R; r++) st[r][0] = st[r][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -206,21 +219,17 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
             for (int c = 0; c < KC; c++)
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    const f16x8 kf = widen_row<E4M3>(t.k[h][c][2 * u], t.k[h][c][2 * u + 1]);
+                    const f16x8 kf = widen_row<E4M3, SEEN>(t.k[h][c][2 * u], t.k[h][c][2 * u + 1]);
 #pragma unroll
                     for (int r = 0; r < R; r++)
 #pragma unroll
                         for (int i = TERMS - 1; i >= 0; i--) st[r][h] = mfma(kf, qf[r][c][u][i], st[r][h]);
                 }
-        const int token = base + step * kTile;
-        const bool whole = token >= all_lo && token + kTile <= all_hi;
         f16x8 pf[R][TERMS];
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            const float u0 = unit[r] * t.kz[0], u1 = unit[r] * t.kz[1];
-            st[r][0] *= u0;
-            st[r][1] *= u1;
-            if (!whole) {
+            if (!SEEN) {
+                const int token = base + step * kTile;
 #pragma unroll
                 for (int h = 0; h < 2; h++)
 #pragma unroll
@@ -229,37 +238,60 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
                         st[r][h][i] = j >= lo_r[r] && j < hi_r[r] ? st[r][h][i] : -INFINITY;
                     }
             }
-            float top = fmaxf(fmaxf(fmaxf(st[r][0][0], st[r][0][1]), fmaxf(st[r][0][2], st[r][0][3])),
-                              fmaxf(fmaxf(st[r][1][0], st[r][1][1]), fmaxf(st[r][1][2], st[r][1][3])));
-            top = fmaxf(row_max(top), m[r]);
-            const float alpha = __builtin_amdgcn_exp2f(m[r] - top);
-            m[r] = top;
-            float sum = 0.f;
-            f32x4 p[2];
+            const float u[2] = {unit[r] * t.kz[0], unit[r] * t.kz[1]};
+            float top = kFloor;
 #pragma unroll
             for (int h = 0; h < 2; h++)
+                top = fmaxf(top, u[h] * fmaxf(fmaxf(st[r][h][0], st[r][h][1]), fmaxf(st[r][h][2], st[r][h][3])));
+            float scale = shrink;
+            if (__any(top > m[r] + kSlack)) {
+                // (row by row: what other rows see changes nothing here)
+                top = row_max(top);
+                top = top > m[r] + kSlack ? top : m[r];
+                const float alpha = __builtin_amdgcn_exp2f(m[r] - top);
+                m[r] = top;
+                l[r] *= alpha;
+                scale *= alpha;
+            }
+            if (__any(scale != 1.f)) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    p[h][i] = __builtin_amdgcn_exp2f(st[r][h][i] - top);
-                    sum += p[h][i];
-                }
-            l[r] = l[r] * alpha + sum;
-            if (__any(alpha != 1.f) || shrink != 1.f) {
-                const float f = alpha * shrink;
-#pragma unroll
-                for (int i = 0; i < DT; i++) acc[r][i] *= f;
+                for (int i = 0; i < DT; i++) acc[r][i] *= scale;
             }
 #pragma unroll
-            for (int h = 0; h < 2; h++)
+            for (int h = 0; h < 2; h++) {
+                const float shift = (TERMS == 1 ? lz[h] : 0.f) - m[r];
+                f32x4 p;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    // (a masked token's block may have a scale that is not finite)
-                    float y = p[h][i] * (h ? z1 : z0);
-                    if (!whole) y = st[r][h][i] == -INFINITY ? 0.f : y;
-                    const _Float16 w = (_Float16)y;
-                    pf[r][0][h * 4 + i] = w;
-                    if constexpr (TERMS == 2) pf[r][1][h * 4 + i] = (_Float16)(y - (float)w);
+                    float y = fmaf(st[r][h][i], u[h], shift);
+                    if (!SEEN) y = st[r][h][i] == -INFINITY ? -INFINITY : y;
+                    p[i] = __builtin_amdgcn_exp2f(y);
                 }
+                if constexpr (TERMS == 1) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) pf[r][0][h * 4 + i] = (_Float16)p[i];
+                    const f16x8 &w = pf[r][0];
+                    const float part = close(lz[h]) ? sum4(w[h * 4], w[h * 4 + 1], w[h * 4 + 2], w[h * 4 + 3], 0.f)
+                                                    : (p[0] + p[1]) + (p[2] + p[3]);
+                    l[r] = fmaf(part, inv_z[h], l[r]);
+                } else {
+                    l[r] += (p[0] + p[1]) + (p[2] + p[3]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        p[i] *= lz[h];
+                        if (!SEEN) p[i] = st[r][h][i] == -INFINITY ? 0.f : p[i];  // (the factor may be NaN)
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i += 2) {
+                        f16x2 high, low;
+                        two_terms(p[i], p[i + 1], high, low);
+                        pf[r][0][h * 4 + i] = high[0];
+                        pf[r][0][h * 4 + i + 1] = high[1];
+                        pf[r][1][h * 4 + i] = low[0];
+                        pf[r][1][h * 4 + i + 1] = low[1];
+                    }
+                }
+            }
         }
 #pragma unroll
         for (int c = 0; c < VW; c++) {
@@ -267,7 +299,7 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] = t.v[j][c];
             f16x8 vf[4];
-            widen_columns<E4M3>(x, vf);
+            widen_columns<E4M3, SEEN>(x, vf);
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -276,67 +308,74 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
                     for (int k = TERMS - 1; k >= 0; k--) acc[r][c * 4 + i] = mfma(vf[i], pf[r][k], acc[r][c * 4 + i]);
         }
     };
+    auto go = [&](int step, const Tile &t) {
+        const int token = base + step * kTile;
+        if (token >= all_lo && token + kTile <= all_hi) work(std::true_type{}, step, t);
+        else work(std::false_type{}, step, t);
+    };
     if (w0 < w1) {
         Tile t0, t1;
         fetch(w0, t0);
         int step = w0;
         for (; step + 1 < w1; step += 2) {
             fetch(step + 1, t1);
-            work(step, t0);
+            go(step, t0);
             if (step + 2 < w1) fetch(step + 2, t0);
-            work(step + 1, t1);
+            go(step + 1, t1);
         }
-        if (step < w1) work(step, t0);
+        if (step < w1) go(step, t0);
     }
 
-    // the four waves' parts, one row tile of 16 after the other
-    __shared__ __align__(16) float part_o[4][16][DP + 4];
-    __shared__ float part_m[4][16], part_l[4][16];
-    const float back = __builtin_ldexpf(1.f, ref - kTop + (E4M3 ? 8 : 0));
-    const int mr = threadIdx.x >> 4, mc = threadIdx.x & 15;  // row and 1/16 of the channels in the merge
+    // the four waves' parts
+    const int rows = min(ROWS, a.T * a.group - row0);
+    __shared__ __align__(16) float part_o[4][ROWS][DP + 4];
+    __shared__ float part_m[4][ROWS], part_l[4][ROWS];
+    const float back = __builtin_amdgcn_exp2f(ref - kPTop + (E4M3 ? 8 : 0));
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        __syncthreads();
         const float sum = row_sum(l[r]);
+        const int row = r * 16 + n16;
+        if (row >= rows) continue;
         if (g4 == 0) {
-            part_m[wave][n16] = m[r];
-            part_l[wave][n16] = sum;
+            part_m[wave][row] = m[r];
+            part_l[wave][row] = sum;
         }
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int c = 0; c < DT; c += 4)
-                *reinterpret_cast<f32x4 *>(&part_o[wave][n16][(g4 * 4 + i) * DT + c]) =
+                *reinterpret_cast<f32x4 *>(&part_o[wave][row][(g4 * 4 + i) * DT + c]) =
                     f32x4{acc[r][c][i], acc[r][c + 1][i], acc[r][c + 2][i], acc[r][c + 3][i]} * back;
-        __syncthreads();
-        float top = part_m[0][mr], f[4], all = 0.f;
+    }
+    __syncthreads();
+    const float poison = s.ok ? 0.f : __uint_as_float(0x7fc00000u);
+    float *part = part_of(a, ROWS, w.item, head);
+    const int mc = threadIdx.x & 15;  // of the channels, 4 in 64
+    for (int r = threadIdx.x >> 4; r < rows; r += 16) {
+        float top = part_m[0][r], f[4], all = 0.f;
 #pragma unroll
-        for (int v = 1; v < 4; v++) top = fmaxf(top, part_m[v][mr]);
+        for (int v = 1; v < 4; v++) top = fmaxf(top, part_m[v][r]);
 #pragma unroll
         for (int v = 0; v < 4; v++) {
-            f[v] = __builtin_amdgcn_exp2f(part_m[v][mr] - top);
-            all += f[v] * part_l[v][mr];
+            f[v] = __builtin_amdgcn_exp2f(part_m[v][r] - top);
+            all += f[v] * part_l[v][r];
         }
-        const int row = row0 + r * 16 + mr;
-        if (row >= a.T * a.group) continue;
-        const int t = row / a.group;
-        const int64_t at = b * a.o.sb + (head * a.group + row - t * a.group) * a.o.sh + t * a.o.st;
-        const float poison = s.ok ? 0.f : __uint_as_float(0x7fc00000u);
-        const bool live = t < s.count;
-        float *part = part_of(a, ROWS, w.item, head);
         if (w.items > 1 && mc == 0) {
-            part[r * 16 + mr] = top;
-            part[ROWS + r * 16 + mr] = all;
+            part[r] = top;
+            part[ROWS + r] = all;
         }
+        const int row = row0 + r, t = row / a.group;
+        const int64_t at = b * a.o.sb + (head * a.group + row - t * a.group) * a.o.sh + t * a.o.st;
+        const bool live = t < s.count;
         const float norm = all == 0.f || !live ? 0.f : 1.f / all;
 #pragma unroll
-        for (int c = 0; c < DT; c += 4) {
-            const int d = mc * DT + c;
+        for (int c = 0; c < DP; c += 64) {
+            const int d = c + mc * 4;
             if (d >= a.D) break;
             f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int v = 0; v < 4; v++) y += f[v] * *reinterpret_cast<const f32x4 *>(&part_o[v][mr][d]);
-            if (w.items > 1) *reinterpret_cast<f32x4 *>(part + 2 * ROWS + (r * 16 + mr) * a.D + d) = y;
+            for (int v = 0; v < 4; v++) y += f[v] * *reinterpret_cast<const f32x4 *>(&part_o[v][r][d]);
+            if (w.items > 1) *reinterpret_cast<f32x4 *>(part + 2 * ROWS + r * a.D + d) = y;
             else store_channels(a.o, a.dtype, a.wide_o, at + d, (live ? y * norm : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
         }
     }

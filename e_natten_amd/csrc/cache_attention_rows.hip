@@ -10,11 +10,11 @@
 // S^T = K Q^T again leaves the probabilities in the registers that O^T = V^T P^T takes: lane (n, h) has
 // the tokens 4h .. 4h+3 (+ 8, 16, ...) of row n, and V is laid out with the same tokens in a lane's eight.
 //
-// exp2 is a quarter-rate instruction and as many as the products' cycles are spent on it, so the rest is
-// kept short: one fused multiply-add forms its argument, in which the value scale z' is a summand,
-//   p' = exp2(s u + (log2 z'' - m)),  z'' = z' 2^14 / (largest power of two of the z' so far),
-// and the sums divide z'' out again block by block.
+// exp2 is a quarter-rate instruction on which as many cycles are spent as on the products, so the rest
+// of the softmax is kept short: see cache_attention.hip.
 #include "cache_attention.h"
+
+#include <type_traits>
 
 namespace enatten {
 namespace {
@@ -48,7 +48,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
     Share w;
     if (a.parts) {
         head = blockIdx.x % heads;
-        w = share_of<kWideRows, TOK>(a, blockIdx.x / heads);
+        w = share_of<kWideRows, TOK, 1>(a, blockIdx.x / heads);
         if (w.entry < 0) return;
         note_share(a, w, head);
     } else {
@@ -98,11 +98,19 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
 #pragma unroll
         for (int c = 0; c < SD; c++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float y = __builtin_ldexpf(x[c][j] * flip, up);
-                const _Float16 v = (_Float16)y;
-                qf[c][0][j] = v;
-                if constexpr (TERMS == 2) qf[c][1][j] = (_Float16)(y - (float)v);
+            for (int j = 0; j < 8; j += 2) {
+                const float y0 = __builtin_ldexpf(x[c][j] * flip, up), y1 = __builtin_ldexpf(x[c][j + 1] * flip, up);
+                if constexpr (TERMS == 2) {
+                    f16x2 high, low;
+                    two_terms(y0, y1, high, low);
+                    qf[c][0][j] = high[0];
+                    qf[c][0][j + 1] = high[1];
+                    qf[c][1][j] = low[0];
+                    qf[c][1][j + 1] = low[1];
+                } else {
+                    qf[c][0][j] = (_Float16)y0;
+                    qf[c][0][j + 1] = (_Float16)y1;
+                }
             }
     }
     // tokens that any, and that all rows of the wave see
@@ -118,7 +126,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
 #pragma unroll
         for (int j = 0; j < 16; j++) acc[i][j] = 0.f;
     float m = kFloor, l = 0.f;
-    int ref = -126;
+    float ref = -126.f;
 
     // places of the groups of 16 tokens: lane i holds group `filled` + i
     int filled = -64;
@@ -129,14 +137,16 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
         filled = group;
         const int token = base + (group + lane) * 16;
         at = 0;
-        z_k = z_v = 0.f;
+        z_k = 0.f;
+        z_v = TERMS == 1 ? -INFINITY : 0.f;  // (its log2, but for float32)
         if (token < s.hi && token >= 0) {
             const int column = token / a.tb.page, within = token - column * a.tb.page;
             const int p = a.tb.pages[b * a.tb.stride + column];
             if ((unsigned)p < (unsigned)a.tb.num_pages) {
                 at = for_v ? p * a.v.sp + head * a.v.sh + within * a.v.st : p * a.k.sp + head * a.k.sh + within * a.k.st;
                 z_k = a.k.scales[p * a.k.zp + head * a.k.zh];
-                z_v = a.v.scales[p * a.v.zp + head * a.v.zh];
+                z_v = finite_or_nan(a.v.scales[p * a.v.zp + head * a.v.zh]);
+                if (TERMS == 1) z_v = __builtin_amdgcn_logf(z_v);
             } else {
                 z_k = __uint_as_float(0x7fc00000u);
             }
@@ -168,20 +178,21 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
                 raw[j] = *reinterpret_cast<const unsigned *>(codes + off + (j % 4 + j / 4 * 8) * a.v.st);
         }
     };
-    auto put = [&](int buffer) {
+    auto put_as = [&](auto seen, int buffer) {
+        constexpr bool SEEN = decltype(seen)::value;
         if (!for_v) {
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const int token = wave * (128 / CH) + j * (64 / CH) + lane / CH, c = lane % CH;
                 const int swap = CH < 8 ? c * (8 / CH) & 7 : c & 7;
                 f16x8 *to = reinterpret_cast<f16x8 *>(k_lds[buffer]) + (token / 32 * SD + c) * 64 + ((token % 32) ^ swap);
-                to[0] = widen_row<E4M3>(raw[j * 4], raw[j * 4 + 1]);
-                to[32] = widen_row<E4M3>(raw[j * 4 + 2], raw[j * 4 + 3]);
+                to[0] = widen_row<E4M3, SEEN>(raw[j * 4], raw[j * 4 + 1]);
+                to[32] = widen_row<E4M3, SEEN>(raw[j * 4 + 2], raw[j * 4 + 3]);
             }
         } else {
             const int run = (wave - 4) * (64 * 4 / DP) + lane / QUADS, quad = lane % QUADS;
             f16x8 v[4];
-            widen_columns<E4M3>(raw, v);
+            widen_columns<E4M3, SEEN>(raw, v);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int block = DP == 64 ? i / 2 : i + quad / 32 * 4, mm = DP == 64 ? (i & 1) * 16 + quad : quad & 31;
@@ -190,36 +201,28 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
         }
         if ((wave & 3) == 0 && lane < GR) z_lds[buffer][for_v][lane] = raw_z;
     };
-
-    if (step0 < step1) {
-        fetch(step0);
-        put(0);
-        if (step0 + 1 < step1) fetch(step0 + 1);
-    }
-    for (int step = step0; step < step1; step++) {
-        const int buffer = (step - step0) & 1;
-        __syncthreads();
-        if (step + 1 < step1) {
-            put(buffer ^ 1);
-            if (step + 2 < step1) fetch(step + 2);
-        }
+    // (the workgroup's first and last rows, for the shorter way of turning E4M3)
+    const int wg_row = row0 - wave * 32, wg_last = min((wg_row + kWideRows - 1) / a.group, s.count - 1);
+    const int wg_lo = a.window ? max(s.start + wg_last + 1 - a.window, 0) : 0, wg_hi = s.start + wg_row / a.group + 1;
+    auto put = [&](int buffer, int step) {
         const int token = base + step * TOK;
-        if (token >= some_hi || token + TOK <= some_lo) continue;
+        if (E4M3 && token >= wg_lo && token + TOK <= wg_hi) put_as(std::true_type{}, buffer);
+        else put_as(std::false_type{}, buffer);
+    };
 
-        // scales of the step's groups, and a larger z' than any so far
-        float kz[GR], vz[GR], zmax = 0.f;
+    // One step for the wave's rows; SEEN: all of them see all its tokens.
+    auto work = [&](auto seen, int token, int buffer) {
+        constexpr bool SEEN = decltype(seen)::value;
+        float kz[GR], lz[GR], most_z = -INFINITY;
 #pragma unroll
         for (int g = 0; g < GR; g++) {
             kz[g] = uniform(z_lds[buffer][0][g]);
-            vz[g] = uniform(z_lds[buffer][1][g]);
-            zmax = fmaxf(zmax, vz[g]);
+            lz[g] = uniform(z_lds[buffer][1][g]);
+            most_z = fmaxf(most_z, lz[g]);
         }
-        float shrink = 1.f;
-        const int e = __builtin_amdgcn_frexp_expf(zmax);
-        if (zmax < INFINITY && zmax > 0.f && e > ref) {
-            shrink = __builtin_ldexpf(1.f, max(ref - e, -200));
-            ref = e;
-        }
+        float scale = grow(ref, TERMS == 1 ? most_z : __builtin_amdgcn_logf(most_z));
+#pragma unroll
+        for (int g = 0; g < GR; g++) lz[g] = TERMS == 1 ? log_weight(lz[g], ref) : plain_weight(lz[g], ref);
 
         f32x16 st[NB];
 #pragma unroll
@@ -240,8 +243,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
         }
 
         // lane's tokens: 32 i + 16 g + 8 (j / 4) + 4 h + j % 4 for its 8 values j of a group
-        const bool whole = token >= all_lo && token + TOK <= all_hi;
-        if (!whole) {
+        if constexpr (!SEEN) {
 #pragma unroll
             for (int i = 0; i < NB; i++)
 #pragma unroll
@@ -250,7 +252,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
                     st[i][j] = tk >= lo_r && tk < hi_r ? st[i][j] : -INFINITY;
                 }
         }
-        float u[GR], top = m;
+        float u[GR], top = kFloor;
 #pragma unroll
         for (int g = 0; g < GR; g++) {
             u[g] = unit * kz[g];
@@ -259,58 +261,86 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
             for (int j = 1; j < 8; j++) most = fmaxf(most, st[g / 2][g % 2 * 8 + j]);
             top = fmaxf(top, most * u[g]);
         }
-        top = pair_max(top);
-        const float alpha = __builtin_amdgcn_exp2f(m - top);
-        m = top;
-        float sum = 0.f;
+        if (__any(top > m + kSlack)) {
+            // (row by row: what other rows see changes nothing here)
+            top = pair_max(top);
+            top = top > m + kSlack ? top : m;
+            const float alpha = __builtin_amdgcn_exp2f(m - top);
+            m = top;
+            l *= alpha;
+            scale *= alpha;
+        }
+        if (__any(scale != 1.f)) {
+#pragma unroll
+            for (int i = 0; i < OB; i++) acc[i] *= scale;
+        }
+        // group by group, so that the exponentials of one go beside the products of another
+        const f16x8 *vp = reinterpret_cast<const f16x8 *>(v_lds[buffer]);
 #pragma unroll
         for (int g = 0; g < GR; g++) {
-            // (a scale of 0: codes may be anything, and go in with a weight that float16 drops)
-            float z = __builtin_ldexpf(vz[g], kTop - ref);
-            z = z < 0x1p-40f ? 0x1p-40f : z;
-            const float shift = __builtin_amdgcn_logf(z) - top;
-            float part = 0.f;
+            const float shift = (TERMS == 1 ? lz[g] : 0.f) - m;
+            f16x8 pf[TERMS];
+            float p[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const float x = st[g / 2][g % 2 * 8 + j];
                 float y = fmaf(x, u[g], shift);
-                if (!whole) y = x == -INFINITY ? -INFINITY : y;
-                const float p = __builtin_amdgcn_exp2f(y);
-                st[g / 2][g % 2 * 8 + j] = p;
-                part += p;
+                if (!SEEN) y = x == -INFINITY ? -INFINITY : y;
+                p[j] = __builtin_amdgcn_exp2f(y);
             }
-            sum = fmaf(part, __builtin_amdgcn_rcpf(z), sum);
-        }
-        l = fmaf(l, alpha, sum);
-        if (__any(alpha != 1.f) || shrink != 1.f) {
-            const float f = alpha * shrink;
+            const float part = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            if constexpr (TERMS == 1) {
 #pragma unroll
-            for (int i = 0; i < OB; i++) acc[i] *= f;
-        }
-        const f16x8 *vp = reinterpret_cast<const f16x8 *>(v_lds[buffer]);
+                for (int j = 0; j < 8; j++) pf[0][j] = (_Float16)p[j];
+                l = fmaf(part, inverse_weight(lz[g]), l);
+            } else {
+                l += part;
 #pragma unroll
-        for (int c = 0; c < GR; c++) {
-            f16x8 pf[TERMS];
+                for (int j = 0; j < 8; j += 2) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float y = st[c / 2][c % 2 * 8 + j];
-                const _Float16 w = (_Float16)y;
-                pf[0][j] = w;
-                if constexpr (TERMS == 2) pf[1][j] = (_Float16)(y - (float)w);
+                    for (int k = j; k < j + 2; k++) {
+                        p[k] *= lz[g];
+                        if (!SEEN) p[k] = st[g / 2][g % 2 * 8 + k] == -INFINITY ? 0.f : p[k];  // (the factor may be NaN)
+                    }
+                    f16x2 high, low;
+                    two_terms(p[j], p[j + 1], high, low);
+                    pf[0][j] = high[0];
+                    pf[0][j + 1] = high[1];
+                    pf[1][j] = low[0];
+                    pf[1][j + 1] = low[1];
+                }
             }
 #pragma unroll
             for (int i = 0; i < OB; i++) {
-                const f16x8 vf = vp[(i * (TOK / 16) + c) * 64 + lane];
+                const f16x8 vf = vp[(i * (TOK / 16) + g) * 64 + lane];
 #pragma unroll
                 for (int t = TERMS - 1; t >= 0; t--)
                     acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[t], acc[i], 0, 0, 0);
             }
         }
+    };
+
+    if (step0 < step1) {
+        fetch(step0);
+        put(0, step0);
+        if (step0 + 1 < step1) fetch(step0 + 1);
+    }
+    for (int step = step0; step < step1; step++) {
+        const int buffer = (step - step0) & 1;
+        __syncthreads();
+        if (step + 1 < step1) {
+            put(buffer ^ 1, step + 1);
+            if (step + 2 < step1) fetch(step + 2);
+        }
+        const int token = base + step * TOK;
+        if (token >= some_hi || token + TOK <= some_lo) continue;
+        if (token >= all_lo && token + TOK <= all_hi) work(std::true_type{}, token, buffer);
+        else work(std::false_type{}, token, buffer);
     }
 
     l = pair_sum(l);
     if (row0 + n >= all_rows) return;
-    const float back = __builtin_ldexpf(1.f, ref - kTop + (E4M3 ? 8 : 0));
+    const float back = __builtin_amdgcn_exp2f(ref - kPTop + (E4M3 ? 8 : 0));
     const float poison = s.ok ? 0.f : __uint_as_float(0x7fc00000u);
     const float norm = (l == 0.f ? 0.f : 1.f / l) * back;
     const int r = wave * 32 + n;

@@ -159,3 +159,120 @@ def test_attention(lengths, counts, N, heads, T, d, page, dtype, cache_dtype, wi
     x = torch.zeros((len(lengths), N, T, d + 5), dtype=dtype, device="cuda")
     x[..., 3:d + 3] = q.cuda()
     assert torch.equal(o, cache_attention(x[..., 3:d + 3], *args))
+
+
+@pytest.mark.parametrize("T,d,window,dtype,cache_dtype", [
+    (1, 64, 40, BF16, I8), (1, 128, 40, F32, E4M3), (6, 64, 24, BF16, E4M3), (6, 128, None, F32, I8),
+    (40, 64, 24, F16, I8), (40, 64, 24, F32, E4M3), (70, 128, 33, BF16, E4M3), (70, 128, None, F16, I8),
+    (70, 64, 100, F32, I8), (70, 256, 33, BF16, E4M3), (20, 256, 33, F32, I8),
+])
+def test_masked_places_do_not_matter(T, d, window, dtype, cache_dtype):
+    """Blocks whose scale is NaN or infinite, and codes of E4M3 that are no numbers: queries that do not
+    see them get what they get without them; those that see a NaN block get NaN.
+
+    Bit for bit where keys change: rows do not know of each other.  A value scale has a part in the power
+    of two that the value scales of a step are taken relative to.  Another power of two scales the weights
+    and all sums exactly, but for float16's subnormals and the rounding of a sum of two logarithms; both
+    results are then within the bound of one, and twice that apart at most."""
+    ensure_built()
+    from e_natten_amd import cache_attention
+    n, page, group = 200, 16, 4
+    cache = Cache([n, n], 2, page, d, cache_dtype, seed=d + T)
+    g = torch.Generator().manual_seed(1)
+    q = torch.randn((2, 2 * group, T, d), generator=g).to(dtype).cuda()
+    kc, vc, ks, vs, pages = cache.on("cuda")
+    call = lambda: cache_attention(q, kc, vc, ks, vs, pages, _ints([n, n]), window, d ** -0.5)
+    clean = call()
+    ref, bound = attention_ref(q, cache, None, window, d ** -0.5)
+    apart = (2 * (bound + half_step(dtype) * (ref.abs() + bound)))[0]
+    place = torch.arange(n - T, n)
+    first = torch.zeros(T, dtype=torch.long) if window is None else (place - window + 1).clamp(min=0)
+    for which, value, block in (("k", float("nan"), 10), ("v", float("nan"), 12), ("k", float("inf"), 11),
+                                ("v", float("inf"), 9), ("codes", None, 11)):
+        at = int(pages[0, block])
+        cache_now = {"k": ks, "v": vs}.get(which)
+        if which == "codes":
+            if cache_dtype == I8:
+                continue
+            keep = kc[at].clone(), vc[at].clone()
+            kc.view(torch.uint8)[at], vc.view(torch.uint8)[at] = 0x7f, 0xff
+        else:
+            keep = cache_now[at].clone()
+            cache_now[at] = value
+        o = call()
+        sees = (first < (block + 1) * page) & (place >= block * page)
+        assert torch.equal(o[1], clean[1])
+        if which == "v":
+            off = (o[0].double() - clean[0].double()).abs().cpu()
+            assert (off <= apart)[:, ~sees].all(), (which, value)
+        else:
+            assert torch.equal(o[0][:, ~sees], clean[0][:, ~sees]), (which, value)
+        if value != value:
+            assert torch.isnan(o[0][:, sees]).all()
+        if which == "codes":
+            kc[at], vc[at] = keep
+        else:
+            cache_now[at] = keep
+    assert torch.equal(call(), clean)
+
+
+def test_numbers_that_do_not_fit_give_nan():
+    """Counts and lengths that contradict each other or the table: NaN for that sequence, for no other;
+    pages outside the cache: NaN for the queries that see them."""
+    ensure_built()
+    from e_natten_amd import cache_attention
+    for T in (1, 4, 80):
+        cache = Cache([200] * 6, 2, 16, 64, I8, seed=8, extra_columns=0)
+        q = torch.randn((6, 4, T, 64), generator=torch.Generator().manual_seed(2)).to(BF16).cuda()
+        kc, vc, ks, vs, pages = cache.on("cuda")
+        full = cache_attention(q, kc, vc, ks, vs, pages, _ints([200] * 6), None, 0.1, _ints([T] * 6))
+        lengths, counts = [200, T - 1, 209, -5, 200, 200], [T, T, T, 0, -1, T + 1]
+        o = cache_attention(q, kc, vc, ks, vs, pages, _ints(lengths), None, 0.1, _ints(counts))
+        assert torch.equal(o[0], full[0]) and torch.isnan(o[1:]).all()
+        for bad in (-1, kc.shape[0], 2 ** 31 - 1, -2 ** 31):
+            broken = pages.clone()
+            broken[1, 12] = bad      # tokens 192 ..
+            broken[2, 3] = bad       # not in the window
+            o = cache_attention(q, kc, vc, ks, vs, broken, _ints([200] * 6), 30, 0.1)
+            want = cache_attention(q, kc, vc, ks, vs, pages, _ints([200] * 6), 30, 0.1)
+            sees = torch.arange(200 - T, 200) >= 192
+            assert torch.isnan(o[1][:, sees]).all() and torch.equal(o[1][:, ~sees], want[1][:, ~sees])
+            inner = torch.arange(200 - T, 200) >= 64 + 29
+            assert torch.equal(o[2][:, inner], want[2][:, inner]) and torch.equal(o[3:], want[3:])
+
+
+def test_queries_that_are_not_finite_stay_in_their_rows():
+    ensure_built()
+    from e_natten_amd import cache_attention
+    for T, dtype in ((1, BF16), (5, F32), (40, F16), (90, BF16)):
+        cache = Cache([150], 2, 32, 64, E4M3, seed=T)
+        q = torch.randn((1, 4, T, 64), generator=torch.Generator().manual_seed(3)).to(dtype).cuda()
+        args = (*cache.on("cuda"), _ints([150]))
+        want = cache_attention(q, *args)
+        q[0, 1, 0, 5], q[0, 2, T - 1, 63] = float("nan"), float("inf")
+        o = cache_attention(q, *args)
+        bad = torch.zeros((4, T), dtype=torch.bool)
+        bad[1, 0] = bad[2, T - 1] = True
+        assert torch.isnan(o[0][bad]).all() and torch.equal(o[0][~bad], want[0][~bad])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_extreme_scales(dtype):
+    """Logits of hundreds, a maximum that comes late, a negative and a zero factor, value scales many
+    powers of two apart (zero among them)."""
+    ensure_built()
+    from e_natten_amd import cache_attention
+    for T, scale, spread in ((1, 3.0, (1e-12, 1e12)), (6, -2.0, (1e-3, 1e3)), (80, 0.0, (1e-30, 1e30)),
+                             (80, 1.5, (1e-6, 1e2))):
+        cache = Cache([500, 90], 2, 16, 64, I8, seed=T, scale_spread=spread)
+        cache.scales[0] = torch.where(torch.isnan(cache.scales[0]), cache.scales[0], torch.full_like(cache.scales[0], 0.03))
+        cache.scales[1][int(cache.pages[0, 2])] = 0.0
+        q = (torch.randn((2, 4, T, 64), generator=torch.Generator().manual_seed(5)) * 3).to(dtype)
+        o = cache_attention(q.cuda(), *cache.on("cuda"), _ints([500, 90]), None, scale)
+        ref, bound = attention_ref(q, cache, None, None, scale)
+        # tokens whose value scale is far below the largest: their weights go in as float16 of the
+        # product of probability and scale, off by at most 2^-31 (2^-41) of the largest value
+        top = torch.stack([cache.values(1, b).abs().amax((1, 2)) for b in range(2)]).view(2, 2, 1, 1)
+        n = torch.tensor([500.0, 90.0]).view(2, 1, 1, 1)
+        bound = bound + (n * top * 2.0 ** -31).repeat_interleave(2, 1)
+        _check(o, ref, bound, dtype, "o, factor %g" % scale)
