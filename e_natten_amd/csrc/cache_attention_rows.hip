@@ -21,10 +21,6 @@ namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-__device__ __forceinline__ float uniform(float x) {
-    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
-}
-
 // DP: head_dim rounded up to 64, 128 or 256; TERMS: float16 terms of q and p.
 template <int DP, bool E4M3, int TERMS>
 __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
@@ -35,9 +31,11 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
     constexpr int OB = DP / 32;       // blocks of 32 channels of O
     constexpr int CH = DP / 16;       // loads of 16 codes per token
     constexpr int QUADS = DP / 4;     // words of 4 channels
-    // operands of one step: K [NB][SD][64 lanes][8], V [OB][TOK / 16][64 lanes][8]
-    __shared__ __align__(16) _Float16 k_lds[2][8192], v_lds[2][8192];
-    __shared__ float z_lds[2][2][GR];
+    // operands of one step: K [NB][SD][64 lanes][8], V [OB][TOK / 16][64 lanes][8]; eight lanes that turn
+    // one or two tokens write to as many operands of K, which therefore start 1 or 2 lanes apart in the banks
+    constexpr int PART = 64 + (CH < 8 ? 8 / CH : 1);
+    __shared__ f16x8 k_lds[2][NB * SD * PART], v_lds[2][1024];
+    __shared__ float z_lds[2][3][GR];  // of the step's groups: key scales, value scales (log2), their inverses
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 31, h = lane >> 5;
 
     // Which row tile, and which of its steps.  Blocks 8 apart share an XCD and its L2: neighbours in
@@ -155,27 +153,32 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
     // What a thread brings: of keys two runs of 16 codes, of values a word of 4 channels of 8 tokens.
     unsigned raw[8];
     float raw_z = 0.f;  // lanes 0 .. GR - 1 of wave 0: key scales of the step's groups, of wave 4: value scales
+    // (offsets within a group of 16 tokens; a wave's 64 runs of keys lie in one group, its 64 words of
+    // values too, but for DP 64, where each half of the wave has its own)
+    const int run = (wave & 3) * (64 * 4 / DP) + lane / QUADS, quad = lane % QUADS;  // runs of 8 tokens
+    const unsigned within = for_v ? run % 2 * 4 * (unsigned)a.v.st + min(quad * 4, a.D - 4)
+                                  : (wave * (128 / CH) + lane / CH) % 16 * (unsigned)a.k.st + min(lane % CH * 16, a.D - 16);
     auto fetch = [&](int step) {
         const int group = step * GR;
         if (group >= filled + 64) fill(group);
         const int here = group - filled;
-        const char *codes = static_cast<const char *>(for_v ? a.v.codes : a.k.codes);
         raw_z = __shfl(for_v ? z_v : z_k, here + (lane & (GR - 1)), 64);
         if (!for_v) {
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                const int token = wave * (128 / CH) + j * (64 / CH) + lane / CH, c = lane % CH;
-                const int64_t off = __shfl(at, here + token / 16, 64) + token % 16 * a.k.st + min(c * 16, a.D - 16);
-                const u32x4 x = *reinterpret_cast<const u32x4 *>(codes + off);
+                const char *from = static_cast<const char *>(a.k.codes) +
+                                   lane_offset(at, here + (wave * (128 / CH) + j * (64 / CH)) / 16);
+                const u32x4 x = *reinterpret_cast<const u32x4 *>(from + (DP == 64 ? 0 : j * (64 / CH)) * a.k.st + within);
 #pragma unroll
                 for (int i = 0; i < 4; i++) raw[j * 4 + i] = x[i];
             }
         } else {
-            const int run = (wave - 4) * (64 * 4 / DP) + lane / QUADS, quad = lane % QUADS;  // 8 tokens each
-            const int64_t off = __shfl(at, here + run / 2, 64) + run % 2 * 4 * a.v.st + min(quad * 4, a.D - 4);
+            int64_t off = lane_offset(at, here + (wave & 3) * (64 * 4 / DP) / 2);
+            if constexpr (DP == 64) off = lane < 32 ? off : lane_offset(at, here + (wave & 3) * 2 + 1);
+            const char *from = static_cast<const char *>(a.v.codes) + off;
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                raw[j] = *reinterpret_cast<const unsigned *>(codes + off + (j % 4 + j / 4 * 8) * a.v.st);
+                raw[j] = *reinterpret_cast<const unsigned *>(from + (j % 4 + j / 4 * 8) * a.v.st + within);
         }
     };
     auto put_as = [&](auto seen, int buffer) {
@@ -184,29 +187,30 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const int token = wave * (128 / CH) + j * (64 / CH) + lane / CH, c = lane % CH;
-                const int swap = CH < 8 ? c * (8 / CH) & 7 : c & 7;
-                f16x8 *to = reinterpret_cast<f16x8 *>(k_lds[buffer]) + (token / 32 * SD + c) * 64 + ((token % 32) ^ swap);
+                f16x8 *to = &k_lds[buffer][(token / 32 * SD + c) * PART + token % 32];
                 to[0] = widen_row<E4M3, SEEN>(raw[j * 4], raw[j * 4 + 1]);
                 to[32] = widen_row<E4M3, SEEN>(raw[j * 4 + 2], raw[j * 4 + 3]);
             }
         } else {
-            const int run = (wave - 4) * (64 * 4 / DP) + lane / QUADS, quad = lane % QUADS;
             f16x8 v[4];
             widen_columns<E4M3, SEEN>(raw, v);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int block = DP == 64 ? i / 2 : i + quad / 32 * 4, mm = DP == 64 ? (i & 1) * 16 + quad : quad & 31;
-                reinterpret_cast<f16x8 *>(v_lds[buffer])[(block * (TOK / 16) + run / 2) * 64 + run % 2 * 32 + mm] = v[i];
+                v_lds[buffer][(block * (TOK / 16) + run / 2) * 64 + run % 2 * 32 + mm] = v[i];
             }
         }
-        if ((wave & 3) == 0 && lane < GR) z_lds[buffer][for_v][lane] = raw_z;
+        if ((wave & 3) == 0 && lane < GR) {
+            z_lds[buffer][for_v][lane] = raw_z;
+            if (for_v) z_lds[buffer][2][lane] = __builtin_amdgcn_exp2f(-raw_z);
+        }
     };
     // (the workgroup's first and last rows, for the shorter way of turning E4M3)
     const int wg_row = row0 - wave * 32, wg_last = min((wg_row + kWideRows - 1) / a.group, s.count - 1);
     const int wg_lo = a.window ? max(s.start + wg_last + 1 - a.window, 0) : 0, wg_hi = s.start + wg_row / a.group + 1;
     auto put = [&](int buffer, int step) {
         const int token = base + step * TOK;
-        if (E4M3 && token >= wg_lo && token + TOK <= wg_hi) put_as(std::true_type{}, buffer);
+        if (E4M3 && DP < 256 && token >= wg_lo && token + TOK <= wg_hi) put_as(std::true_type{}, buffer);
         else put_as(std::false_type{}, buffer);
     };
 
@@ -216,8 +220,8 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
         float kz[GR], lz[GR], most_z = -INFINITY;
 #pragma unroll
         for (int g = 0; g < GR; g++) {
-            kz[g] = uniform(z_lds[buffer][0][g]);
-            lz[g] = uniform(z_lds[buffer][1][g]);
+            kz[g] = z_lds[buffer][0][g];
+            lz[g] = z_lds[buffer][1][g];
             most_z = fmaxf(most_z, lz[g]);
         }
         float scale = grow(ref, TERMS == 1 ? most_z : __builtin_amdgcn_logf(most_z));
@@ -229,13 +233,12 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
         for (int i = 0; i < NB; i++)
 #pragma unroll
             for (int j = 0; j < 16; j++) st[i][j] = 0.f;
-        const f16x8 *kp = reinterpret_cast<const f16x8 *>(k_lds[buffer]);
+        const f16x8 *kp = &k_lds[buffer][lane];
 #pragma unroll
         for (int c = 0; c < SD; c++) {
-            const int swap = CH < 8 ? c * (8 / CH) & 7 : c & 7;
 #pragma unroll
             for (int i = 0; i < NB; i++) {
-                const f16x8 kf = kp[(i * SD + c) * 64 + h * 32 + (n ^ swap)];
+                const f16x8 kf = kp[(i * SD + c) * PART];
 #pragma unroll
                 for (int t = TERMS - 1; t >= 0; t--)
                     st[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[c][t], st[i], 0, 0, 0);
@@ -252,6 +255,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
                     st[i][j] = tk >= lo_r && tk < hi_r ? st[i][j] : -INFINITY;
                 }
         }
+        const float unit_z = __builtin_amdgcn_exp2f(ref - kPTop);
         float u[GR], top = kFloor;
 #pragma unroll
         for (int g = 0; g < GR; g++) {
@@ -275,7 +279,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
             for (int i = 0; i < OB; i++) acc[i] *= scale;
         }
         // group by group, so that the exponentials of one go beside the products of another
-        const f16x8 *vp = reinterpret_cast<const f16x8 *>(v_lds[buffer]);
+        const f16x8 *vp = &v_lds[buffer][lane];
 #pragma unroll
         for (int g = 0; g < GR; g++) {
             const float shift = (TERMS == 1 ? lz[g] : 0.f) - m;
@@ -292,7 +296,9 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
             if constexpr (TERMS == 1) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) pf[0][j] = (_Float16)p[j];
-                l = fmaf(part, inverse_weight(lz[g]), l);
+                // (at most 2^40, as the weight is at least 2^-40; NaN too: the sum of a row that sees such a
+                // group is NaN itself, and one that does not is 0)
+                l = fmaf(part, fminf(z_lds[buffer][2][g] * unit_z, 0x1p40f), l);
             } else {
                 l += part;
 #pragma unroll
@@ -312,7 +318,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
             }
 #pragma unroll
             for (int i = 0; i < OB; i++) {
-                const f16x8 vf = vp[(i * (TOK / 16) + g) * 64 + lane];
+                const f16x8 vf = vp[(i * (TOK / 16) + g) * 64];
 #pragma unroll
                 for (int t = TERMS - 1; t >= 0; t--)
                     acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[t], acc[i], 0, 0, 0);
@@ -334,7 +340,8 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
         }
         const int token = base + step * TOK;
         if (token >= some_hi || token + TOK <= some_lo) continue;
-        if (token >= all_lo && token + TOK <= all_hi) work(std::true_type{}, token, buffer);
+        // (head dims above 128 have no registers to spare for both)
+        if (DP < 256 && token >= all_lo && token + TOK <= all_hi) work(std::true_type{}, token, buffer);
         else work(std::false_type{}, token, buffer);
     }
 
