@@ -36,7 +36,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kFloor = -1e37f;  // the maximum of a row that has seen nothing: finite, below every logit
+constexpr float kFloor = -1e15f;  // the maximum of a row that has seen nothing: finite, below every logit
 constexpr int kLeast = 256;       // tokens of a part at least: what a workgroup takes to get going pays from there
 constexpr int kTop = 14;          // rows of q are brought to 2^kTop .. 2 * 2^kTop
 constexpr int kPTop = 7;          // probabilities to 2^kPTop, and up to 2^kSlack times that where the

@@ -49,7 +49,8 @@ constexpr int waves_of(int DP, int R, int TERMS) {
 template <int DP, int R, bool E4M3, int TERMS>
 __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a) {
     constexpr int TOK = kTile, ROWS = 16 * R, KC = DP / 64, VW = DP / 64, DT = DP / 16;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n16 = lane & 15, g4 = lane >> 4;
+    const int lane = threadIdx.x & 63, n16 = lane & 15, g4 = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (branches on it are the wave's)
 
     // which row tile, and which of its steps
     const int head = blockIdx.x % a.heads_kv;

@@ -36,7 +36,9 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
     constexpr int PART = 64 + (CH < 8 ? 8 / CH : 1);
     __shared__ f16x8 k_lds[2][NB * SD * PART], v_lds[2][1024];
     __shared__ float z_lds[2][3][GR];  // of the step's groups: key scales, value scales (log2), their inverses
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 31, h = lane >> 5;
+    __shared__ int z_bad[2][2];        // ... and which of either are not finite (0 in their place)
+    const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (branches on it are the wave's)
 
     // Which row tile, and which of its steps.  Blocks 8 apart share an XCD and its L2: neighbours in
     // the order of the cache heads go to different ones, the row tiles of a head to the same where
@@ -71,7 +73,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
     const bool live = row0 + n < all_rows && t_row < s.count;
     const int hi_r = live ? s.start + t_row + 1 : 0, lo_r = live && a.window ? max(hi_r - a.window, 0) : 0;
     f16x8 qf[SD][TERMS];
-    float unit;
+    float unit, bad_q;
     {
         const int64_t at = b * a.q.sb + (head * a.group + row - t_row * a.group) * a.q.sh + t_row * a.q.st;
         const float flip = a.scale < 0.f ? -1.f : 1.f;  // into q, so that units are not negative
@@ -92,7 +94,8 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
         nan = pair_sum(nan);
         top = pair_max(top);
         const int up = kTop + 1 - (top > 0.f ? __builtin_amdgcn_frexp_expf(top) : 0);
-        unit = __builtin_ldexpf(fabsf(a.scale) * kLog2e, -up + (E4M3 ? 8 : 0)) + nan;
+        unit = __builtin_ldexpf(fabsf(a.scale) * kLog2e, -up + (E4M3 ? 8 : 0));
+        bad_q = nan;
 #pragma unroll
         for (int c = 0; c < SD; c++)
 #pragma unroll
@@ -200,9 +203,15 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
                 v_lds[buffer][(block * (TOK / 16) + run / 2) * 64 + run % 2 * 32 + mm] = v[i];
             }
         }
-        if ((wave & 3) == 0 && lane < GR) {
-            z_lds[buffer][for_v][lane] = raw_z;
-            if (for_v) z_lds[buffer][2][lane] = __builtin_amdgcn_exp2f(-raw_z);
+        if ((wave & 3) == 0) {
+            const bool finite = for_v && TERMS == 1 ? raw_z < INFINITY : fabsf(raw_z) < INFINITY;
+            const float z = finite ? raw_z : for_v && TERMS == 1 ? -INFINITY : 0.f;
+            if (lane < GR) {
+                z_lds[buffer][for_v][lane] = z;
+                if (for_v) z_lds[buffer][2][lane] = __builtin_amdgcn_exp2f(-z);
+            }
+            const int bad = (int)__ballot(!finite) & ((1 << GR) - 1);
+            if (lane == 0) z_bad[buffer][for_v] = bad;
         }
     };
     // (the workgroup's first and last rows, for the shorter way of turning E4M3)
@@ -210,13 +219,14 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
     const int wg_lo = a.window ? max(s.start + wg_last + 1 - a.window, 0) : 0, wg_hi = s.start + wg_row / a.group + 1;
     auto put = [&](int buffer, int step) {
         const int token = base + step * TOK;
-        if (E4M3 && DP < 256 && token >= wg_lo && token + TOK <= wg_hi) put_as(std::true_type{}, buffer);
+        if (E4M3 && token >= wg_lo && token + TOK <= wg_hi) put_as(std::true_type{}, buffer);
         else put_as(std::false_type{}, buffer);
     };
 
-    // One step for the wave's rows; SEEN: all of them see all its tokens.
-    auto work = [&](auto seen, int token, int buffer) {
-        constexpr bool SEEN = decltype(seen)::value;
+    // One step for the wave's rows.  Masked logits are a large negative number, not an infinity: units
+    // are at least 1e-20, so that they end below -1e18 and their exponentials are 0 whatever the maximum
+    // (kFloor at least), and a unit of 0 asks for nothing special.
+    auto work = [&](bool whole, int token, int buffer) {
         float kz[GR], lz[GR], most_z = -INFINITY;
 #pragma unroll
         for (int g = 0; g < GR; g++) {
@@ -246,25 +256,37 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
         }
 
         // lane's tokens: 32 i + 16 g + 8 (j / 4) + 4 h + j % 4 for its 8 values j of a group
-        if constexpr (!SEEN) {
+        float cap = INFINITY;
+        if (!whole) {
+            if (token >= hi_r || token + TOK <= lo_r) cap = kFloor;  // the row sees none of them
 #pragma unroll
             for (int i = 0; i < NB; i++)
 #pragma unroll
                 for (int j = 0; j < 16; j++) {
                     const int tk = token + i * 32 + j / 4 * 8 + h * 4 + j % 4;
-                    st[i][j] = tk >= lo_r && tk < hi_r ? st[i][j] : -INFINITY;
+                    st[i][j] = tk >= lo_r && tk < hi_r ? st[i][j] : -3e38f;
                 }
+        }
+        // scales that are not finite: NaN for the rows that see a token of the group
+        const int bad = __builtin_amdgcn_readfirstlane(z_bad[buffer][0] | z_bad[buffer][1]);
+        if (bad) {
+#pragma unroll
+            for (int g = 0; g < GR; g++) {
+                const int first = token + g * 16;
+                if ((bad >> g & 1) && first < hi_r && first + 16 > lo_r) l = __uint_as_float(0x7fc00000u);
+            }
         }
         const float unit_z = __builtin_amdgcn_exp2f(ref - kPTop);
         float u[GR], top = kFloor;
 #pragma unroll
         for (int g = 0; g < GR; g++) {
-            u[g] = unit * kz[g];
-            float most = st[g / 2][g % 2 * 8];
+            u[g] = fmaxf(unit * kz[g], 1e-20f);
+            float most = -3e38f;  // (a constant to start from: else the compiler makes values canonical)
 #pragma unroll
-            for (int j = 1; j < 8; j++) most = fmaxf(most, st[g / 2][g % 2 * 8 + j]);
+            for (int j = 0; j < 8; j++) most = fmaxf(most, st[g / 2][g % 2 * 8 + j]);
             top = fmaxf(top, most * u[g]);
         }
+        top = fminf(top, cap);
         if (__any(top > m + kSlack)) {
             // (row by row: what other rows see changes nothing here)
             top = pair_max(top);
@@ -287,27 +309,20 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
             float p[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float x = st[g / 2][g % 2 * 8 + j];
-                float y = fmaf(x, u[g], shift);
-                if (!SEEN) y = x == -INFINITY ? -INFINITY : y;
-                p[j] = __builtin_amdgcn_exp2f(y);
+                p[j] = __builtin_amdgcn_exp2f(fmaf(st[g / 2][g % 2 * 8 + j], u[g], shift));
             }
             const float part = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
             if constexpr (TERMS == 1) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) pf[0][j] = (_Float16)p[j];
-                // (at most 2^40, as the weight is at least 2^-40; NaN too: the sum of a row that sees such a
-                // group is NaN itself, and one that does not is 0)
+                // (at most 2^40, as the weight is at least 2^-40)
                 l = fmaf(part, fminf(z_lds[buffer][2][g] * unit_z, 0x1p40f), l);
             } else {
                 l += part;
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
 #pragma unroll
-                    for (int k = j; k < j + 2; k++) {
-                        p[k] *= lz[g];
-                        if (!SEEN) p[k] = st[g / 2][g % 2 * 8 + k] == -INFINITY ? 0.f : p[k];  // (the factor may be NaN)
-                    }
+                    for (int k = j; k < j + 2; k++) p[k] *= lz[g];
                     f16x2 high, low;
                     two_terms(p[j], p[j + 1], high, low);
                     pf[0][j] = high[0];
@@ -340,11 +355,10 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
         }
         const int token = base + step * TOK;
         if (token >= some_hi || token + TOK <= some_lo) continue;
-        // (head dims above 128 have no registers to spare for both)
-        if (DP < 256 && token >= all_lo && token + TOK <= all_hi) work(std::true_type{}, token, buffer);
-        else work(std::false_type{}, token, buffer);
+        work(token >= all_lo && token + TOK <= all_hi, token, buffer);
     }
 
+    l += bad_q;
     l = pair_sum(l);
     if (row0 + n >= all_rows) return;
     const float back = __builtin_amdgcn_exp2f(ref - kPTop + (E4M3 ? 8 : 0));
