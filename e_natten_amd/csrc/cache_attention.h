@@ -38,6 +38,8 @@ typedef short s16x2 __attribute__((ext_vector_type(2)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFloor = -1e15f;  // the maximum of a row that has seen nothing: finite, below every logit
 constexpr int kLeast = 256;       // tokens of a part at least: what a workgroup takes to get going pays from there
+constexpr int kLeastWide = 512;   // ... of a range of steps on tiles of many rows
+constexpr int kWideRows = 256;    // rows of those tiles
 constexpr int kTop = 14;          // rows of q are brought to 2^kTop .. 2 * 2^kTop
 constexpr int kPTop = 7;          // probabilities to 2^kPTop, and up to 2^kSlack times that where the
 constexpr int kSlack = 8;         // running maximum is let lag behind
@@ -125,9 +127,63 @@ __device__ __forceinline__ Share share_of(const AttnArgs &a, int item) {
     return w;
 }
 
+// Equal shares of a different kind, for tiles of many rows: the steps of all row tiles of all cache heads
+// in one line (heads, then sequences, then row tiles; a tile without steps counts as one, so that its
+// rows are written), cut into `parts` ranges.  A range takes what is left of a tile, whole tiles, and the
+// beginning of one; only tiles that are cut have parts to join, and every workgroup has the same work.
+constexpr int64_t item_floats(int rows, int D) { return (int64_t)rows * (D + 2); }  // maxima, sums, sums of values
+struct Ranges {
+    int64_t line, each;  // steps of one cache head, of one range
+    bool whole;          // no more tiles than ranges, and nearly as long as those: a tile each, none cut
+};
+template <int ROWS, int TOK>
+__device__ __forceinline__ int counted_steps(const AttnArgs &a, int e) {
+    return e < a.B * a.row_tiles ? max(1, steps_of<TOK>(span_of<ROWS>(a, e))) : 0;
+}
+template <int ROWS, int TOK>
+__device__ __forceinline__ Ranges ranges_of(const AttnArgs &a) {
+    const int entries = a.B * a.row_tiles, lane = threadIdx.x & 63;
+    Ranges r{0, 0, false};
+    int most = 0;
+    for (int e0 = 0; e0 < entries; e0 += 64) {
+        const int n = counted_steps<ROWS, TOK>(a, e0 + lane);
+        most = max(most, n);
+        r.line += (unsigned)__builtin_amdgcn_readlane(running_sum(n), 63);
+    }
+    r.each = (r.line * a.heads_kv + a.parts - 1) / a.parts;
+    // The parts of a cut tile are 256 rows of sums, written and read: with a tile for every workgroup that
+    // costs more than up to 30% that some are longer than the mean (2048 tokens of two sequences of 16384 and
+    // 12288: 565 us whole, 576 cut)
+    r.whole = (int64_t)entries * a.heads_kv <= a.parts && !__any(10 * (int64_t)most > 13 * r.each);
+    if (r.each < kLeastWide / TOK) r.each = kLeastWide / TOK;
+    return r;
+}
+// The row tile at step `y` of a head's line, and how far into it that is
+template <int ROWS, int TOK>
+__device__ __forceinline__ int tile_at(const AttnArgs &a, int64_t y, int &into) {
+    const int entries = a.B * a.row_tiles, lane = threadIdx.x & 63;
+    for (int e0 = 0; e0 < entries; e0 += 64) {
+        const unsigned n = counted_steps<ROWS, TOK>(a, e0 + lane), upto = running_sum(n);
+        const unsigned all = __builtin_amdgcn_readlane(upto, 63);
+        if (y < all) {
+            const unsigned long long who = __ballot((unsigned)y < upto);
+            const int l = __ffsll(who) - 1;
+            into = (int)((unsigned)y - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l)));
+            return e0 + l;
+        }
+        y -= all;
+    }
+    into = 0;
+    return -1;
+}
+// Workspace of the ranges: for each the number of the tile that it starts within, or -1; then two slots
+// each, for the tile that it starts within and for the one that it ends within.
+__device__ __forceinline__ float *slot_of(const AttnArgs &a, int slot) {
+    return a.ws + (a.parts + 3) / 4 * 4 + slot * item_floats(kWideRows, a.D);
+}
+
 // The workspace: first item and items of every entry, then for every (item, cache head) the maxima and
 // sums of its rows and rows x D sums of values.
-constexpr int64_t item_floats(int rows, int D) { return (int64_t)rows * (D + 2); }
 __host__ __device__ inline int64_t head_floats(int64_t entries) { return (2 * entries + 3) / 4 * 4; }
 __device__ __forceinline__ float *part_of(const AttnArgs &a, int rows, int item, int head) {
     return a.ws + head_floats((int64_t)a.B * a.row_tiles) + ((int64_t)item * a.heads_kv + head) * item_floats(rows, a.D);
@@ -368,8 +424,7 @@ __device__ __forceinline__ int64_t lane_offset(int64_t x, int l) {
 
 }  // namespace
 
-// Tiles of kWideRows rows (cache_attention_rows.hip)
-constexpr int kWideRows = 256;
-int launch_attend_rows(const char *fn, const AttnArgs &a, bool e4m3, int64_t blocks, hipStream_t st);
+// Tiles of kWideRows rows (cache_attention_rows.hip), a.parts ranges
+int launch_attend_rows(const char *fn, const AttnArgs &a, bool e4m3, hipStream_t st);
 
 }  // namespace enatten

@@ -468,8 +468,10 @@ Plan plan_of(int B, int heads, int heads_kv, int T, int D, int page, int columns
     if (window && window + (int64_t)p.rows < tokens) tokens = window + (int64_t)p.rows;
     p.parts = 0;
     p.items = entries;
-    const int target = p.rows == kWideRows ? 256 : 512;
-    if (entries * heads_kv < target && tokens > kLeast) {
+    constexpr int target = 512;
+    if (p.rows == kWideRows) {
+        p.parts = 256;  // ranges: one workgroup per CU
+    } else if (entries * heads_kv < target && tokens > kLeast) {
         p.parts = (target + heads_kv - 1) / heads_kv;
         // no more than the longest possible sequences fill
         const int64_t useful = entries * ((tokens + 16 + kLeast - 1) / kLeast);
@@ -510,10 +512,7 @@ int launch_rows(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st
         set_error("%s: too many row tiles", fn);
         return ENATTEN_EUNSUPPORTED;
     }
-    if (p.rows == kWideRows) {
-        const int rc = launch_attend_rows(fn, a, E4M3, p.items * a.heads_kv, st);
-        return rc ? rc : launch_join<kWideRows>(fn, a, p, st);
-    }
+    if (p.rows == kWideRows) return launch_attend_rows(fn, a, E4M3, st);
     if (p.rows == 16) return launch_terms<DP, 1, E4M3>(fn, a, p, st);
     if constexpr (DP <= 128) {
         if (p.rows == 48) return launch_terms<DP, 3, E4M3>(fn, a, p, st);
@@ -537,6 +536,7 @@ size_t enatten_cache_attention_workspace_bytes(int B, int heads, int heads_kv, i
         return 0;
     const Plan p = plan_of(B, heads, heads_kv, T, D, page, columns, kernel_size, dtype);
     if (!p.parts) return 0;
+    if (p.rows == kWideRows) return ((size_t)(p.parts + 3) / 4 * 4 + 2 * p.parts * item_floats(kWideRows, D)) * sizeof(float);
     return (size_t)(head_floats((int64_t)B * p.row_tiles) + p.items * heads_kv * item_floats(p.rows, D)) * sizeof(float);
 }
 

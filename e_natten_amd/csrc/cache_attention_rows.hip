@@ -21,9 +21,18 @@ namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
+// The kernel's arguments, read anew: what is used once per row tile or per 64 groups of tokens does not
+// stay in scalar registers across the steps (held there, 124 of them were spilled, for 7% at head_dim 128).
+__device__ __forceinline__ const AttnArgs &args_again() {
+    typedef const AttnArgs __attribute__((address_space(4))) *Kernarg;
+    Kernarg p = (Kernarg)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const AttnArgs *)p;
+}
+
 // DP: head_dim rounded up to 64, 128 or 256; TERMS: float16 terms of q and p.
 template <int DP, bool E4M3, int TERMS>
-__global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
+__global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
     constexpr int TOK = 8192 / DP;    // tokens of a step: 128, 64, 32
     constexpr int NB = TOK / 32;      // blocks of 32 of them
     constexpr int GR = TOK / 16;      // groups of 16, each within a page
@@ -37,43 +46,52 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
     __shared__ f16x8 k_lds[2][NB * SD * PART], v_lds[2][1024];
     __shared__ float z_lds[2][3][GR];  // of the step's groups: key scales, value scales (log2), their inverses
     __shared__ int z_bad[2][2];        // ... and which of either are not finite (0 in their place)
+    // Rows of q stay in registers, at head dims above 128 all but the last operands, for which there are
+    // none left: those a lane puts into LDS and reads again.
+    constexpr int KEPT = DP == 256 ? 10 : SD;
+    __shared__ f16x8 q_lds[8 * 64 * (SD - KEPT) + 1];
     const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (branches on it are the wave's)
 
-    // Which row tile, and which of its steps.  Blocks 8 apart share an XCD and its L2: neighbours in
-    // the order of the cache heads go to different ones, the row tiles of a head to the same where
-    // their number allows.  Later rows see more tokens: they come first.
+    // The workgroup's range of steps.  Blocks 8 apart share an XCD and its L2: they get neighbouring ranges,
+    // which read the same keys and values where they belong to the same head.
+    const AttnArgs &a = args;
+    const int range = blockIdx.x % 8 * (a.parts / 8) + blockIdx.x / 8;
+    const Ranges line = ranges_of<kWideRows, TOK>(a);
     const int heads = a.heads_kv;
-    int head;
-    Share w;
-    if (a.parts) {
-        head = blockIdx.x % heads;
-        w = share_of<kWideRows, TOK, 1>(a, blockIdx.x / heads);
-        if (w.entry < 0) return;
-        note_share(a, w, head);
+    int64_t end = min((range + 1) * line.each, line.line * heads);
+    int64_t at_step = range * line.each;
+    const int entries = a.B * a.row_tiles, all_rows = a.T * a.group;
+    int *note = reinterpret_cast<int *>(a.ws) + range;
+    int head, entry, into = 0;
+    if (line.whole) {  // a tile each
+        head = range / entries;
+        entry = range - head * entries;
+        at_step = head < heads ? 0 : end;
+        end = min(end, (int64_t)1);
     } else {
-        const int pair = blockIdx.x % (heads * a.B);
-        head = pair % heads;
-        w.entry = pair / heads * a.row_tiles + a.row_tiles - 1 - blockIdx.x / (heads * a.B);
-        w.items = 1;
+        head = (int)(at_step / line.line);
+        entry = at_step < end ? tile_at<kWideRows, TOK>(a, at_step - head * line.line, into) : 0;
     }
-    const int entry = w.entry;
+    if (threadIdx.x == 0) *note = into ? head * entries + entry : -1;
+
+    for (; at_step < end; into = 0) {
+    const AttnArgs &a = args_again();
     const Span s = span_of<kWideRows>(a, entry);
-    if (!a.parts) {
-        w.step0 = 0;
-        w.step1 = steps_of<TOK>(s);
-    }
+    const int total = steps_of<TOK>(s), counted = max(1, total), step0 = into;
+    const int step1 = line.whole ? total : min(total, (int)min((int64_t)counted, step0 + (end - at_step)));
+    const bool parted = !line.whole && (into || step0 + (end - at_step) < counted);
+    const int slot = into ? 2 * range : 2 * range + 1;
+    at_step += counted - into;
     const int b = entry / a.row_tiles, row0 = (entry - b * a.row_tiles) * kWideRows + wave * 32;
-    const int step0 = w.step0, step1 = w.step1;
     const int base = s.lo & -16;
-    const int all_rows = a.T * a.group;
 
     // the lane's row; q: lane (n, h) has channels 16 c + 8 h .. + 7
     const int row = min(row0 + n, all_rows - 1), t_row = row / a.group;
     const bool live = row0 + n < all_rows && t_row < s.count;
-    const int hi_r = live ? s.start + t_row + 1 : 0, lo_r = live && a.window ? max(hi_r - a.window, 0) : 0;
-    f16x8 qf[SD][TERMS];
-    float unit, bad_q;
+    const int hi_r = live ? s.start + t_row + 1 : 0, seen = a.window ? a.window : hi_r;  // tokens hi_r - seen .. hi_r - 1
+    f16x8 qf[KEPT][TERMS], *q_rest = &q_lds[threadIdx.x];
+    float unit, l;
     {
         const int64_t at = b * a.q.sb + (head * a.group + row - t_row * a.group) * a.q.sh + t_row * a.q.st;
         const float flip = a.scale < 0.f ? -1.f : 1.f;  // into q, so that units are not negative
@@ -95,24 +113,34 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
         top = pair_max(top);
         const int up = kTop + 1 - (top > 0.f ? __builtin_amdgcn_frexp_expf(top) : 0);
         unit = __builtin_ldexpf(fabsf(a.scale) * kLog2e, -up + (E4M3 ? 8 : 0));
-        bad_q = nan;
+        l = nan;  // (and stays NaN for a row of q that is not finite)
 #pragma unroll
         for (int c = 0; c < SD; c++)
 #pragma unroll
+            for (int j = 0; j < 8; j++) x[c][j] = __builtin_ldexpf(x[c][j] * flip, up);
+#pragma unroll
+        for (int c = 0; c < SD; c++) {
+            f16x8 w[TERMS];
+#pragma unroll
             for (int j = 0; j < 8; j += 2) {
-                const float y0 = __builtin_ldexpf(x[c][j] * flip, up), y1 = __builtin_ldexpf(x[c][j + 1] * flip, up);
                 if constexpr (TERMS == 2) {
                     f16x2 high, low;
-                    two_terms(y0, y1, high, low);
-                    qf[c][0][j] = high[0];
-                    qf[c][0][j + 1] = high[1];
-                    qf[c][1][j] = low[0];
-                    qf[c][1][j + 1] = low[1];
+                    two_terms(x[c][j], x[c][j + 1], high, low);
+                    w[0][j] = high[0];
+                    w[0][j + 1] = high[1];
+                    w[1][j] = low[0];
+                    w[1][j + 1] = low[1];
                 } else {
-                    qf[c][0][j] = (_Float16)y0;
-                    qf[c][0][j + 1] = (_Float16)y1;
+                    w[0][j] = (_Float16)x[c][j];
+                    w[0][j + 1] = (_Float16)x[c][j + 1];
                 }
             }
+#pragma unroll
+            for (int t = 0; t < TERMS; t++) {
+                if (c < KEPT) qf[c][t] = w[t];
+                else q_rest[(c - KEPT) * 512] = w[t];
+            }
+        }
     }
     // tokens that any, and that all rows of the wave see
     const int t_first = min(row0, all_rows - 1) / a.group, t_last = min(min(row0 + 31, all_rows - 1) / a.group, s.count - 1);
@@ -126,30 +154,32 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
     for (int i = 0; i < OB; i++)
 #pragma unroll
         for (int j = 0; j < 16; j++) acc[i][j] = 0.f;
-    float m = kFloor, l = 0.f;
+    float m = kFloor;
     float ref = -126.f;
 
     // places of the groups of 16 tokens: lane i holds group `filled` + i
     int filled = -64;
     int64_t at = 0;
-    float z_k = 0.f, z_v = 0.f;
+    float z_at = 0.f;  // of keys, or log2 of values (for float32 the scale itself)
     const bool for_v = wave >= 4;
     auto fill = [&](int group) {
+        const AttnArgs &a = args_again();
         filled = group;
         const int token = base + (group + lane) * 16;
         at = 0;
-        z_k = 0.f;
-        z_v = TERMS == 1 ? -INFINITY : 0.f;  // (its log2, but for float32)
+        z_at = for_v && TERMS == 1 ? -INFINITY : 0.f;
         if (token < s.hi && token >= 0) {
             const int column = token / a.tb.page, within = token - column * a.tb.page;
             const int p = a.tb.pages[b * a.tb.stride + column];
-            if ((unsigned)p < (unsigned)a.tb.num_pages) {
-                at = for_v ? p * a.v.sp + head * a.v.sh + within * a.v.st : p * a.k.sp + head * a.k.sh + within * a.k.st;
-                z_k = a.k.scales[p * a.k.zp + head * a.k.zh];
-                z_v = finite_or_nan(a.v.scales[p * a.v.zp + head * a.v.zh]);
-                if (TERMS == 1) z_v = __builtin_amdgcn_logf(z_v);
+            if ((unsigned)p >= (unsigned)a.tb.num_pages) {
+                z_at = __uint_as_float(0x7fc00000u);
+            } else if (for_v) {
+                at = p * a.v.sp + head * a.v.sh + within * a.v.st;
+                z_at = finite_or_nan(a.v.scales[p * a.v.zp + head * a.v.zh]);
+                if (TERMS == 1) z_at = __builtin_amdgcn_logf(z_at);
             } else {
-                z_k = __uint_as_float(0x7fc00000u);
+                at = p * a.k.sp + head * a.k.sh + within * a.k.st;
+                z_at = a.k.scales[p * a.k.zp + head * a.k.zh];
             }
         }
     };
@@ -165,7 +195,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
         const int group = step * GR;
         if (group >= filled + 64) fill(group);
         const int here = group - filled;
-        raw_z = __shfl(for_v ? z_v : z_k, here + (lane & (GR - 1)), 64);
+        raw_z = __shfl(z_at, here + (lane & (GR - 1)), 64);
         if (!for_v) {
 #pragma unroll
             for (int j = 0; j < 2; j++) {
@@ -251,20 +281,20 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
                 const f16x8 kf = kp[(i * SD + c) * PART];
 #pragma unroll
                 for (int t = TERMS - 1; t >= 0; t--)
-                    st[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[c][t], st[i], 0, 0, 0);
+                    st[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, c < KEPT ? qf[c][t] : q_rest[(c - KEPT) * 512], st[i], 0, 0, 0);
             }
         }
 
         // lane's tokens: 32 i + 16 g + 8 (j / 4) + 4 h + j % 4 for its 8 values j of a group
         float cap = INFINITY;
         if (!whole) {
-            if (token >= hi_r || token + TOK <= lo_r) cap = kFloor;  // the row sees none of them
+            if (token >= hi_r || token + TOK <= hi_r - seen) cap = kFloor;  // the row sees none of them
 #pragma unroll
             for (int i = 0; i < NB; i++)
 #pragma unroll
                 for (int j = 0; j < 16; j++) {
                     const int tk = token + i * 32 + j / 4 * 8 + h * 4 + j % 4;
-                    st[i][j] = tk >= lo_r && tk < hi_r ? st[i][j] : -3e38f;
+                    st[i][j] = tk >= hi_r - seen && tk < hi_r ? st[i][j] : -3e38f;
                 }
         }
         // scales that are not finite: NaN for the rows that see a token of the group
@@ -273,7 +303,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
 #pragma unroll
             for (int g = 0; g < GR; g++) {
                 const int first = token + g * 16;
-                if ((bad >> g & 1) && first < hi_r && first + 16 > lo_r) l = __uint_as_float(0x7fc00000u);
+                if ((bad >> g & 1) && first < hi_r && first + 16 > hi_r - seen) l = __uint_as_float(0x7fc00000u);
             }
         }
         const float unit_z = __builtin_amdgcn_exp2f(ref - kPTop);
@@ -341,6 +371,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
         }
     };
 
+    __syncthreads();  // (the last tile's operands are read)
     if (step0 < step1) {
         fetch(step0);
         put(0, step0);
@@ -358,59 +389,155 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs a) {
         work(token >= all_lo && token + TOK <= all_hi, token, buffer);
     }
 
-    l += bad_q;
     l = pair_sum(l);
-    if (row0 + n >= all_rows) return;
+    {
+    const AttnArgs &a = args_again();
     const float back = __builtin_amdgcn_exp2f(ref - kPTop + (E4M3 ? 8 : 0));
     const float poison = s.ok ? 0.f : __uint_as_float(0x7fc00000u);
     const float norm = (l == 0.f ? 0.f : 1.f / l) * back;
-    const int r = wave * 32 + n;
-    float *part = part_of(a, kWideRows, w.item, head);
-    if (w.items > 1 && h == 0) {
-        part[r] = m;
-        part[kWideRows + r] = l;
-    }
-    const int64_t to = b * a.o.sb + (head * a.group + row - t_row * a.group) * a.o.sh + t_row * a.o.st;
-    const float f = w.items > 1 ? back : live ? norm : 0.f;
-    // 4 neighbouring channels: words of one value row, blocks i of O, or for DP 64 rows 16 apart too
-#pragma unroll
-    for (int i = 0; i < OB; i += DP == 64 ? 2 : 4)
-#pragma unroll
-        for (int j = 0; j < (DP == 64 ? 8 : 16); j++) {
-            const int mm = j / 4 * 8 + h * 4 + j % 4;
-            f32x4 y;
-            if constexpr (DP == 64) y = f32x4{acc[0][j], acc[0][j + 8], acc[1][j], acc[1][j + 8]};
-            else y = f32x4{acc[i][j], acc[i + 1][j], acc[i + 2][j], acc[i + 3][j]};
-            const int d = 4 * mm + i / 4 * 128;
-            if (d >= a.D) continue;
-            if (w.items > 1) *reinterpret_cast<f32x4 *>(part + 2 * kWideRows + r * a.D + d) = y * f;
-            else store_channels(a.o, a.dtype, a.wide_o, to + d, (live ? y * f : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
+    const int r = wave * 32 + n, row = row0 + n, t_row = row / a.group;
+    const bool live = t_row < s.count;
+    float *part = slot_of(a, slot);
+    if (row < a.T * a.group) {
+        if (parted && h == 0) {
+            part[r] = m;
+            part[kWideRows + r] = l;
         }
+        const int64_t to = b * a.o.sb + (head * a.group + row - t_row * a.group) * a.o.sh + t_row * a.o.st;
+        const float f = parted ? back : live ? norm : 0.f;
+        // 4 neighbouring channels: words of one value row, blocks i of O, or for DP 64 rows 16 apart too
+#pragma unroll
+        for (int i = 0; i < OB; i += DP == 64 ? 2 : 4)
+#pragma unroll
+            for (int j = 0; j < (DP == 64 ? 8 : 16); j++) {
+                const int mm = j / 4 * 8 + h * 4 + j % 4;
+                f32x4 y;
+                if constexpr (DP == 64) y = f32x4{acc[0][j], acc[0][j + 8], acc[1][j], acc[1][j + 8]};
+                else y = f32x4{acc[i][j], acc[i + 1][j], acc[i + 2][j], acc[i + 3][j]};
+                const int d = 4 * mm + i / 4 * 128;
+                if (d >= a.D) continue;
+                if (parted) *reinterpret_cast<f32x4 *>(part + 2 * kWideRows + r * a.D + d) = y * f;
+                else store_channels(a.o, a.dtype, a.wide_o, to + d, (live ? y * f : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
+            }
+    }
+    }
+    if (++entry == entries) {
+        entry = 0;
+        head++;
+    }
+    }
+}
+
+// Tiles that ranges cut, joined: one workgroup per (start of a range, 16 rows), the one of the first
+// start within a tile for all its parts.  A wave takes a row at a time: 16 lanes over the channels, 4 in
+// 64 each, and every fourth part.
+__global__ __launch_bounds__(256) void join_rows(AttnArgs a) {
+    constexpr int BLOCKS = kWideRows / 16;
+    const int range = blockIdx.x / BLOCKS, c = threadIdx.x % 16 * 4, g = threadIdx.x / 16 % 4;
+    const int *note = reinterpret_cast<const int *>(a.ws);
+    const int tile = note[range];
+    if (tile < 0 || note[range - 1] == tile) return;  // (the first range starts with a tile)
+    const int entries = a.B * a.row_tiles, head = tile / entries, entry = tile - head * entries;
+    const int b = entry / a.row_tiles, row0 = (entry - b * a.row_tiles) * kWideRows;
+    const int count = a.tb.counts ? a.tb.counts[b] : a.T;
+    // the parts: the end of the range before, then the beginnings of the ranges that start within the tile
+    int parts = 1;
+    for (;; parts += 64) {
+        const int q = range + parts - 1 + (threadIdx.x & 63);
+        const unsigned long long others = __ballot(q >= a.parts || note[q] != tile);
+        if (others) {
+            parts += __ffsll(others) - 1;
+            break;
+        }
+    }
+    for (int k = 0; k < 4; k++) {
+        const int r = blockIdx.x % BLOCKS * 16 + k * 4 + threadIdx.x / 64, row = row0 + r;
+        if (row >= a.T * a.group) return;
+        f32x4 y[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        float top = kFloor, sum = 0.f;
+        constexpr int DEEP = 4;  // parts whose loads are under way at a time
+        for (int q0 = g; q0 < parts; q0 += 4 * DEEP) {
+            float m[DEEP], l[DEEP];
+            f32x4 x[DEEP][4];
+#pragma unroll
+            for (int n = 0; n < DEEP; n++) {
+                const int q = q0 + 4 * n;
+                m[n] = kFloor;
+                l[n] = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (q >= parts) continue;
+                const float *part = slot_of(a, q ? 2 * (range + q - 1) : 2 * range - 1);
+                m[n] = part[r];
+                l[n] = part[kWideRows + r];
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (c + 64 * i < a.D) x[n][i] = *reinterpret_cast<const f32x4 *>(part + 2 * kWideRows + r * a.D + c + 64 * i);
+            }
+            float most = top;
+#pragma unroll
+            for (int n = 0; n < DEEP; n++) most = fmaxf(most, m[n]);
+            const float old = __builtin_amdgcn_exp2f(top - most);
+            top = most;
+            sum *= old;
+#pragma unroll
+            for (int i = 0; i < 4; i++) y[i] *= old;
+#pragma unroll
+            for (int n = 0; n < DEEP; n++) {
+                const float f = __builtin_amdgcn_exp2f(m[n] - top);
+                sum += f * l[n];
+#pragma unroll
+                for (int i = 0; i < 4; i++) y[i] += f * x[n][i];
+            }
+        }
+        const float most = row_max(top), f = __builtin_amdgcn_exp2f(top - most);
+        sum = row_sum(sum * f);
+        const int t = row / a.group;
+        const int64_t to = b * a.o.sb + (head * a.group + row - t * a.group) * a.o.sh + t * a.o.st;
+        const float norm = sum == 0.f || t >= count ? 0.f : 1.f / sum;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (c + 64 * i >= a.D) break;
+            f32x4 z;
+#pragma unroll
+            for (int j = 0; j < 4; j++) z[j] = row_sum(y[i][j] * f) * norm;
+            if (t >= count) z = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (g == 0) store_channels(a.o, a.dtype, a.wide_o, to + c + 64 * i, z);
+        }
+    }
 }
 
 template <int DP, bool E4M3, int TERMS>
-int launch(const char *fn, const AttnArgs &a, int64_t blocks, hipStream_t st) {
-    ProfScope prof(ENATTEN_KERNEL_CACHE_ATTENTION, "attend_rows", st);
-    attend_rows<DP, E4M3, TERMS><<<(int)blocks, 512, 0, st>>>(a);
+int launch(const char *fn, const AttnArgs &a, hipStream_t st) {
+    {
+        ProfScope prof(ENATTEN_KERNEL_CACHE_ATTENTION, "attend_rows", st);
+        attend_rows<DP, E4M3, TERMS><<<a.parts, 512, 0, st>>>(a);
+    }
+    const int rc = launched(fn);
+    if (rc) return rc;
+    ProfScope prof(ENATTEN_KERNEL_CACHE_JOIN, "join_rows", st);
+    join_rows<<<a.parts * (kWideRows / 16), 256, 0, st>>>(a);
     return launched(fn);
 }
 template <int DP, bool E4M3>
-int launch_terms(const char *fn, const AttnArgs &a, int64_t blocks, hipStream_t st) {
+int launch_terms(const char *fn, const AttnArgs &a, hipStream_t st) {
     if constexpr (DP <= 128)
-        if (a.dtype == ENATTEN_F32) return launch<DP, E4M3, 2>(fn, a, blocks, st);
-    return launch<DP, E4M3, 1>(fn, a, blocks, st);
+        if (a.dtype == ENATTEN_F32) return launch<DP, E4M3, 2>(fn, a, st);
+    return launch<DP, E4M3, 1>(fn, a, st);
 }
 template <bool E4M3>
-int launch_dim(const char *fn, const AttnArgs &a, int64_t blocks, hipStream_t st) {
-    if (a.D <= 64) return launch_terms<64, E4M3>(fn, a, blocks, st);
-    if (a.D <= 128) return launch_terms<128, E4M3>(fn, a, blocks, st);
-    return launch_terms<256, E4M3>(fn, a, blocks, st);
+int launch_dim(const char *fn, const AttnArgs &a, hipStream_t st) {
+    if (a.D <= 64) return launch_terms<64, E4M3>(fn, a, st);
+    if (a.D <= 128) return launch_terms<128, E4M3>(fn, a, st);
+    return launch_terms<256, E4M3>(fn, a, st);
 }
 
 }  // namespace
 
-int launch_attend_rows(const char *fn, const AttnArgs &a, bool e4m3, int64_t blocks, hipStream_t st) {
-    return e4m3 ? launch_dim<true>(fn, a, blocks, st) : launch_dim<false>(fn, a, blocks, st);
+int launch_attend_rows(const char *fn, const AttnArgs &a, bool e4m3, hipStream_t st) {
+    return e4m3 ? launch_dim<true>(fn, a, st) : launch_dim<false>(fn, a, st);
 }
 
 }  // namespace enatten

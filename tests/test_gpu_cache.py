@@ -218,7 +218,11 @@ def test_masked_places_do_not_matter(T, d, window, dtype, cache_dtype):
 
 def test_numbers_that_do_not_fit_give_nan():
     """Counts and lengths that contradict each other or the table: NaN for that sequence, for no other;
-    pages outside the cache: NaN for the queries that see them."""
+    pages outside the cache: NaN for the queries that see them.
+
+    The work of a call is cut by the lengths of all its sequences, and where a sequence is cut its sums
+    are rounded elsewhere: two results that are each within the bound of the exact one are at most twice
+    that apart.  With the same lengths they are the same bits."""
     ensure_built()
     from e_natten_amd import cache_attention
     for T in (1, 4, 80):
@@ -228,7 +232,9 @@ def test_numbers_that_do_not_fit_give_nan():
         full = cache_attention(q, kc, vc, ks, vs, pages, _ints([200] * 6), None, 0.1, _ints([T] * 6))
         lengths, counts = [200, T - 1, 209, -5, 200, 200], [T, T, T, 0, -1, T + 1]
         o = cache_attention(q, kc, vc, ks, vs, pages, _ints(lengths), None, 0.1, _ints(counts))
-        assert torch.equal(o[0], full[0]) and torch.isnan(o[1:]).all()
+        ref, bound = attention_ref(q, cache, [T] * 6, None, 0.1)
+        apart = (2 * (bound + half_step(BF16) * (ref.abs() + bound)))[0]
+        assert ((o[0].double() - full[0].double()).abs().cpu() <= apart).all() and torch.isnan(o[1:]).all()
         for bad in (-1, kc.shape[0], 2 ** 31 - 1, -2 ** 31):
             broken = pages.clone()
             broken[1, 12] = bad      # tokens 192 ..
