@@ -11,7 +11,6 @@ struct AttnArgs {
     Table tb;
     int B, heads, group, heads_kv, T, D, window;  // group: query heads of a cache head
     int dtype;
-    bool wide_q, wide_o;  // rows at multiples of 16 bytes
     int row_tiles;   // per (sequence, cache head)
     int parts;       // workgroups per cache head that the split aims at; 0: one per row tile
     float scale;
@@ -38,7 +37,7 @@ typedef short s16x2 __attribute__((ext_vector_type(2)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFloor = -1e15f;  // the maximum of a row that has seen nothing: finite, below every logit
 constexpr int kLeast = 256;       // tokens of a part at least: what a workgroup takes to get going pays from there
-constexpr int kLeastWide = 512;   // ... of a range of steps on tiles of many rows
+constexpr int kLeastWide = 128;   // ... of a range of steps on tiles of many rows
 constexpr int kWideRows = 256;    // rows of those tiles
 constexpr int kTop = 14;          // rows of q are brought to 2^kTop .. 2 * 2^kTop
 constexpr int kPTop = 7;          // probabilities to 2^kPTop, and up to 2^kSlack times that where the
@@ -343,73 +342,48 @@ __device__ __forceinline__ float row_sum(float x) {
     return pair_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
-// N channels of a row, N a multiple of 8, by loads of 16 bytes if `wide` (rows at multiples of that)
-template <int N>
-__device__ __forceinline__ void load_channels(const Rows &r, int dtype, bool wide, int64_t at, float (&x)[N]) {
-    if (dtype == ENATTEN_F32) {
+// N channels of a row, N a multiple of 8; rows lie at multiples of 16 bytes.  DT: the type, a constant, as
+// what is done once per workgroup is paid by its size: code that was not run before comes from memory.
+template <int DT, int N>
+__device__ __forceinline__ void load_channels(const Rows &r, int64_t at, float (&x)[N]) {
+    if constexpr (DT == ENATTEN_F32) {
         const float *p = static_cast<const float *>(r.ptr) + at;
-        if (wide) {
 #pragma unroll
-            for (int i = 0; i < N; i += 4) {
-                const f32x4 y = *reinterpret_cast<const f32x4 *>(p + i);
+        for (int i = 0; i < N; i += 4) {
+            const f32x4 y = *reinterpret_cast<const f32x4 *>(p + i);
 #pragma unroll
-                for (int j = 0; j < 4; j++) x[i + j] = y[j];
+            for (int j = 0; j < 4; j++) x[i + j] = y[j];
+        }
+    } else {
+        const unsigned short *p = static_cast<const unsigned short *>(r.ptr) + at;
+#pragma unroll
+        for (int i = 0; i < N; i += 8) {
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(p + i);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                if constexpr (DT == ENATTEN_BF16) x[i + j] = __uint_as_float(j % 2 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+                else x[i + j] = (float)as_half(w[j / 2])[j % 2];
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; i++) x[i] = p[i];
         }
-        return;
-    }
-    const unsigned short *p = static_cast<const unsigned short *>(r.ptr) + at;
-    unsigned y[N / 2];
-    if (wide) {
-#pragma unroll
-        for (int i = 0; i < N / 8; i++) {
-            const u32x4 w = *reinterpret_cast<const u32x4 *>(p + i * 8);
-#pragma unroll
-            for (int j = 0; j < 4; j++) y[i * 4 + j] = w[j];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N / 2; i++) y[i] = p[2 * i] | (unsigned)p[2 * i + 1] << 16;
-    }
-    if (dtype == ENATTEN_BF16) {
-#pragma unroll
-        for (int i = 0; i < N; i++) x[i] = __uint_as_float(i % 2 ? y[i / 2] & 0xffff0000u : y[i / 2] << 16);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) x[i] = (float)__builtin_bit_cast(f16x2, y[i / 2])[i % 2];
     }
 }
-// 4 channels of a row; `wide`: rows at multiples of 16 bytes
-__device__ __forceinline__ void store_channels(const Rows &r, int dtype, bool wide, int64_t at, f32x4 x) {
-    if (dtype == ENATTEN_F32) {
-        float *p = static_cast<float *>(const_cast<void *>(r.ptr)) + at;
-        if (wide) {
-            *reinterpret_cast<f32x4 *>(p) = x;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++) p[i] = x[i];
-        }
-        return;
-    }
-    u32x2 y;
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        if (dtype == ENATTEN_BF16) {
-            typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-            y[i] = __builtin_bit_cast(unsigned, bf16x2{(__bf16)x[2 * i], (__bf16)x[2 * i + 1]});
-        } else {
-            y[i] = __builtin_bit_cast(unsigned, f16x2{(_Float16)x[2 * i], (_Float16)x[2 * i + 1]});
-        }
-    }
-    unsigned short *p = static_cast<unsigned short *>(const_cast<void *>(r.ptr)) + at;
-    if (wide) {
-        *reinterpret_cast<u32x2 *>(p) = y;
+// 4 channels of a row
+template <int DT>
+__device__ __forceinline__ void store_channels(const Rows &r, int64_t at, f32x4 x) {
+    if constexpr (DT == ENATTEN_F32) {
+        *reinterpret_cast<f32x4 *>(static_cast<float *>(const_cast<void *>(r.ptr)) + at) = x;
     } else {
+        u32x2 y;
 #pragma unroll
-        for (int i = 0; i < 4; i++) p[i] = (unsigned short)(y[i / 2] >> i % 2 * 16);
+        for (int i = 0; i < 2; i++) {
+            if constexpr (DT == ENATTEN_BF16) {
+                typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+                y[i] = __builtin_bit_cast(unsigned, bf16x2{(__bf16)x[2 * i], (__bf16)x[2 * i + 1]});
+            } else {
+                y[i] = __builtin_bit_cast(unsigned, f16x2{(_Float16)x[2 * i], (_Float16)x[2 * i + 1]});
+            }
+        }
+        *reinterpret_cast<u32x2 *>(static_cast<unsigned short *>(const_cast<void *>(r.ptr)) + at) = y;
     }
 }
 

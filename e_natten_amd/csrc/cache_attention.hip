@@ -46,9 +46,9 @@ constexpr int waves_of(int DP, int R, int TERMS) {
 
 // DP: head_dim rounded up to 64, 128 or 256 (channels beyond D: zeros in q, any codes); R: row tiles of
 // 16 per workgroup; TERMS: float16 terms of q and p.
-template <int DP, int R, bool E4M3, int TERMS>
-__global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a) {
-    constexpr int TOK = kTile, ROWS = 16 * R, KC = DP / 64, VW = DP / 64, DT = DP / 16;
+template <int DP, int R, bool E4M3, int DT>
+__global__ __launch_bounds__(256, waves_of(DP, R, DT == ENATTEN_F32 ? 2 : 1)) void attend(AttnArgs a) {
+    constexpr int TERMS = DT == ENATTEN_F32 ? 2 : 1, TOK = kTile, ROWS = 16 * R, KC = DP / 64, VW = DP / 64, CW = DP / 16;
     const int lane = threadIdx.x & 63, n16 = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (branches on it are the wave's)
 
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
         for (int c = 0; c < KC; c++) {
 #pragma unroll
             for (int j = 0; j < 16; j++) x[c][j] = 0.f;
-            if (c * 64 + g4 * 16 < a.D) load_channels<16>(a.q, a.dtype, a.wide_q, at + c * 64 + g4 * 16, x[c]);
+            if (c * 64 + g4 * 16 < a.D) load_channels<DT>(a.q, at + c * 64 + g4 * 16, x[c]);
         }
 #pragma unroll
         for (int c = 0; c < KC; c++)
@@ -127,14 +127,14 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
     const int all_lo = a.window ? max(s.start + min((row0 + ROWS - 1) / a.group, s.count - 1) + 1 - a.window, 0) : 0;
     const int all_hi = s.start + row0 / a.group + 1;
 
-    f32x4 acc[R][DT];
+    f32x4 acc[R][CW];
     float m[R], l[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
         m[r] = kFloor;
         l[r] = 0.f;
 #pragma unroll
-        for (int i = 0; i < DT; i++) acc[r][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < CW; i++) acc[r][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     float ref = -126.f;  // the z' so far are at most 2^ref
 
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
             }
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const unsigned off = (g4 * 4 + j) * (unsigned)a.v.st + min(n16 * DT, a.D - DT);
+                const unsigned off = (g4 * 4 + j) * (unsigned)a.v.st + min(n16 * CW, a.D - CW);
                 if constexpr (VW == 1) {
                     t.v[h * 4 + j][0] = *reinterpret_cast<const unsigned *>(vp + off);
                 } else if constexpr (VW == 2) {
@@ -256,7 +256,7 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
             }
             if (__any(scale != 1.f)) {
 #pragma unroll
-                for (int i = 0; i < DT; i++) acc[r][i] *= scale;
+                for (int i = 0; i < CW; i++) acc[r][i] *= scale;
             }
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -344,8 +344,8 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int c = 0; c < DT; c += 4)
-                *reinterpret_cast<f32x4 *>(&part_o[wave][row][(g4 * 4 + i) * DT + c]) =
+            for (int c = 0; c < CW; c += 4)
+                *reinterpret_cast<f32x4 *>(&part_o[wave][row][(g4 * 4 + i) * CW + c]) =
                     f32x4{acc[r][c][i], acc[r][c + 1][i], acc[r][c + 2][i], acc[r][c + 3][i]} * back;
     }
     __syncthreads();
@@ -377,13 +377,13 @@ __global__ __launch_bounds__(256, waves_of(DP, R, TERMS)) void attend(AttnArgs a
 #pragma unroll
             for (int v = 0; v < 4; v++) y += f[v] * *reinterpret_cast<const f32x4 *>(&part_o[v][r][d]);
             if (w.items > 1) *reinterpret_cast<f32x4 *>(part + 2 * ROWS + r * a.D + d) = y;
-            else store_channels(a.o, a.dtype, a.wide_o, at + d, (live ? y * norm : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
+            else store_channels<DT>(a.o, at + d, (live ? y * norm : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
         }
     }
 }
 
 // The parts of a row joined: one workgroup per (row tile, cache head, row).
-template <int ROWS>
+template <int ROWS, int DT>
 __global__ __launch_bounds__(256) void attend_join(AttnArgs a) {
     const int per = min(ROWS, a.T * a.group);
     int block = blockIdx.x;
@@ -450,7 +450,7 @@ __global__ __launch_bounds__(256) void attend_join(AttnArgs a) {
         const int64_t at = b * a.o.sb + (head * a.group + row - t * a.group) * a.o.sh + t * a.o.st;
         const int count = a.tb.counts ? a.tb.counts[b] : a.T;
         const float norm = sum == 0.f ? 0.f : 1.f / sum;
-        store_channels(a.o, a.dtype, a.wide_o, at + c * 4, t < count ? y * norm : f32x4{0.f, 0.f, 0.f, 0.f});
+        store_channels<DT>(a.o, at + c * 4, t < count ? y * norm : f32x4{0.f, 0.f, 0.f, 0.f});
     }
 }
 
@@ -460,7 +460,7 @@ Plan plan_of(int B, int heads, int heads_kv, int T, int D, int page, int columns
     const int64_t all = (int64_t)T * (heads / heads_kv);
     // Up to `most` rows: one tile of as many sixteens as there are, each wave with its own tokens.
     // Beyond, tiles of 256 rows; float32 rows of more than 128 channels have too many registers there.
-    const int most = D > 128 ? 32 : 64;
+    const int most = D > 128 ? 32 : D > 64 ? 48 : 64;
     p.rows = all <= most ? (int)(all + 15) / 16 * 16 : D > 128 && dtype == ENATTEN_F32 ? 32 : kWideRows;
     p.row_tiles = (int)((all + p.rows - 1) / p.rows);
     const int64_t entries = (int64_t)B * p.row_tiles;
@@ -468,7 +468,7 @@ Plan plan_of(int B, int heads, int heads_kv, int T, int D, int page, int columns
     if (window && window + (int64_t)p.rows < tokens) tokens = window + (int64_t)p.rows;
     p.parts = 0;
     p.items = entries;
-    constexpr int target = 512;
+    const int target = 256 * (waves_of(D <= 64 ? 64 : D <= 128 ? 128 : 256, p.rows / 16, dtype == ENATTEN_F32 ? 2 : 1) > 1 ? 2 : 1);
     if (p.rows == kWideRows) {
         p.parts = 256;  // ranges: one workgroup per CU
     } else if (entries * heads_kv < target && tokens > kLeast) {
@@ -481,30 +481,28 @@ Plan plan_of(int B, int heads, int heads_kv, int T, int D, int page, int columns
     return p;
 }
 
-template <int ROWS>
-int launch_join(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st) {
-    if (!p.parts) return ENATTEN_OK;
-    const int64_t rows = a.T * (int64_t)a.group, blocks = (int64_t)a.B * p.row_tiles * a.heads_kv * (rows < ROWS ? rows : ROWS);
+template <int DP, int R, bool E4M3, int DT>
+int launch(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st) {
+    {
+        ProfScope prof(ENATTEN_KERNEL_CACHE_ATTENTION, "attend", st);
+        attend<DP, R, E4M3, DT><<<(int)(p.items * a.heads_kv), 256, 0, st>>>(a);
+    }
+    const int rc = launched(fn);
+    if (rc || !p.parts) return rc;
+    const int64_t rows = a.T * (int64_t)a.group, blocks = (int64_t)a.B * p.row_tiles * a.heads_kv * (rows < 16 * R ? rows : 16 * R);
     if (blocks > 0x7fffffff) {
         set_error("%s: too many rows", fn);
         return ENATTEN_EUNSUPPORTED;
     }
     ProfScope prof(ENATTEN_KERNEL_CACHE_JOIN, "attend_join", st);
-    attend_join<ROWS><<<(int)blocks, 256, 0, st>>>(a);
+    attend_join<16 * R, DT><<<(int)blocks, 256, 0, st>>>(a);
     return launched(fn);
 }
-template <int DP, int R, bool E4M3, int TERMS>
-int launch(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st) {
-    {
-        ProfScope prof(ENATTEN_KERNEL_CACHE_ATTENTION, "attend", st);
-        attend<DP, R, E4M3, TERMS><<<(int)(p.items * a.heads_kv), 256, 0, st>>>(a);
-    }
-    const int rc = launched(fn);
-    return rc ? rc : launch_join<16 * R>(fn, a, p, st);
-}
 template <int DP, int R, bool E4M3>
-int launch_terms(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st) {
-    return a.dtype == ENATTEN_F32 ? launch<DP, R, E4M3, 2>(fn, a, p, st) : launch<DP, R, E4M3, 1>(fn, a, p, st);
+int launch_type(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st) {
+    if (a.dtype == ENATTEN_BF16) return launch<DP, R, E4M3, ENATTEN_BF16>(fn, a, p, st);
+    if (a.dtype == ENATTEN_F32) return launch<DP, R, E4M3, ENATTEN_F32>(fn, a, p, st);
+    return launch<DP, R, E4M3, ENATTEN_F16>(fn, a, p, st);
 }
 template <int DP, bool E4M3>
 int launch_rows(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st) {
@@ -513,12 +511,12 @@ int launch_rows(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st
         return ENATTEN_EUNSUPPORTED;
     }
     if (p.rows == kWideRows) return launch_attend_rows(fn, a, E4M3, st);
-    if (p.rows == 16) return launch_terms<DP, 1, E4M3>(fn, a, p, st);
+    if (p.rows == 16) return launch_type<DP, 1, E4M3>(fn, a, p, st);
     if constexpr (DP <= 128) {
-        if (p.rows == 48) return launch_terms<DP, 3, E4M3>(fn, a, p, st);
-        if (p.rows == 64) return launch_terms<DP, 4, E4M3>(fn, a, p, st);
+        if (p.rows == 48) return launch_type<DP, 3, E4M3>(fn, a, p, st);
+        if (DP == 64 && p.rows == 64) return launch_type<64, 4, E4M3>(fn, a, p, st);
     }
-    return launch_terms<DP, 2, E4M3>(fn, a, p, st);
+    return launch_type<DP, 2, E4M3>(fn, a, p, st);
 }
 
 }  // namespace
@@ -561,6 +559,11 @@ int enatten_cache_attention(const void *q, const void *k_cache, const void *v_ca
     AttnArgs a{};
     if ((rc = set_rows(fn, "q", q, q_strides, heads, T, D, &a.q))) return rc;
     if ((rc = set_rows(fn, "o", o, o_strides, heads, T, D, &a.o))) return rc;
+    const int pack = dtype == ENATTEN_F32 ? 4 : 8;
+    if (((uintptr_t)q | (uintptr_t)o) % 16 || (a.q.sb | a.q.sh | a.q.st | a.o.sb | a.o.sh | a.o.st) % pack) {
+        set_error("%s: rows of q and o must lie at multiples of 16 bytes", fn);
+        return ENATTEN_EINVAL;
+    }
     if ((rc = set_cache(fn, "k", const_cast<void *>(k_cache), const_cast<float *>(k_scale), k_cache_strides,
                         k_scale_strides, heads_kv, page, D, 16, &a.k))) return rc;
     if ((rc = set_cache(fn, "v", const_cast<void *>(v_cache), const_cast<float *>(v_scale), v_cache_strides,
@@ -578,9 +581,6 @@ int enatten_cache_attention(const void *q, const void *k_cache, const void *v_ca
     a.B = B; a.heads = heads; a.group = heads / heads_kv; a.heads_kv = heads_kv; a.T = T; a.D = D;
     a.window = kernel_size;
     a.dtype = dtype;
-    const int pack = dtype == ENATTEN_F32 ? 4 : 8;
-    a.wide_q = (uintptr_t)q % 16 == 0 && (a.q.sb | a.q.sh | a.q.st) % pack == 0;
-    a.wide_o = (uintptr_t)o % 16 == 0 && (a.o.sb | a.o.sh | a.o.st) % pack == 0;
     a.row_tiles = p.row_tiles;
     a.parts = p.parts;
     a.scale = scale;

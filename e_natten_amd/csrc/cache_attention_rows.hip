@@ -30,9 +30,10 @@ __device__ __forceinline__ const AttnArgs &args_again() {
     return *(const AttnArgs *)p;
 }
 
-// DP: head_dim rounded up to 64, 128 or 256; TERMS: float16 terms of q and p.
-template <int DP, bool E4M3, int TERMS>
+// DP: head_dim rounded up to 64, 128 or 256; DT: type of q and o, float32 in two float16 terms of q and p.
+template <int DP, bool E4M3, int DT>
 __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
+    constexpr int TERMS = DT == ENATTEN_F32 ? 2 : 1;
     constexpr int TOK = 8192 / DP;    // tokens of a step: 128, 64, 32
     constexpr int NB = TOK / 32;      // blocks of 32 of them
     constexpr int GR = TOK / 16;      // groups of 16, each within a page
@@ -100,7 +101,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
         for (int c = 0; c < SD; c++) {
 #pragma unroll
             for (int j = 0; j < 8; j++) x[c][j] = 0.f;
-            if (c * 16 < a.D) load_channels<8>(a.q, a.dtype, a.wide_q, at + c * 16 + h * 8, x[c]);
+            if (c * 16 < a.D) load_channels<DT>(a.q, at + c * 16 + h * 8, x[c]);
         }
 #pragma unroll
         for (int c = 0; c < SD; c++)
@@ -417,7 +418,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
                 const int d = 4 * mm + i / 4 * 128;
                 if (d >= a.D) continue;
                 if (parted) *reinterpret_cast<f32x4 *>(part + 2 * kWideRows + r * a.D + d) = y * f;
-                else store_channels(a.o, a.dtype, a.wide_o, to + d, (live ? y * f : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
+                else store_channels<DT>(a.o, to + d, (live ? y * f : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
             }
     }
     }
@@ -431,6 +432,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
 // Tiles that ranges cut, joined: one workgroup per (start of a range, 16 rows), the one of the first
 // start within a tile for all its parts.  A wave takes a row at a time: 16 lanes over the channels, 4 in
 // 64 each, and every fourth part.
+template <int DT>
 __global__ __launch_bounds__(256) void join_rows(AttnArgs a) {
     constexpr int BLOCKS = kWideRows / 16;
     const int range = blockIdx.x / BLOCKS, c = threadIdx.x % 16 * 4, g = threadIdx.x / 16 % 4;
@@ -504,34 +506,35 @@ __global__ __launch_bounds__(256) void join_rows(AttnArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; j++) z[j] = row_sum(y[i][j] * f) * norm;
             if (t >= count) z = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (g == 0) store_channels(a.o, a.dtype, a.wide_o, to + c + 64 * i, z);
+            if (g == 0) store_channels<DT>(a.o, to + c + 64 * i, z);
         }
     }
 }
 
-template <int DP, bool E4M3, int TERMS>
+template <int DP, bool E4M3, int DT>
 int launch(const char *fn, const AttnArgs &a, hipStream_t st) {
     {
         ProfScope prof(ENATTEN_KERNEL_CACHE_ATTENTION, "attend_rows", st);
-        attend_rows<DP, E4M3, TERMS><<<a.parts, 512, 0, st>>>(a);
+        attend_rows<DP, E4M3, DT><<<a.parts, 512, 0, st>>>(a);
     }
     const int rc = launched(fn);
     if (rc) return rc;
     ProfScope prof(ENATTEN_KERNEL_CACHE_JOIN, "join_rows", st);
-    join_rows<<<a.parts * (kWideRows / 16), 256, 0, st>>>(a);
+    join_rows<DT><<<a.parts * (kWideRows / 16), 256, 0, st>>>(a);
     return launched(fn);
 }
 template <int DP, bool E4M3>
-int launch_terms(const char *fn, const AttnArgs &a, hipStream_t st) {
+int launch_type(const char *fn, const AttnArgs &a, hipStream_t st) {
+    if (a.dtype == ENATTEN_BF16) return launch<DP, E4M3, ENATTEN_BF16>(fn, a, st);
     if constexpr (DP <= 128)
-        if (a.dtype == ENATTEN_F32) return launch<DP, E4M3, 2>(fn, a, st);
-    return launch<DP, E4M3, 1>(fn, a, st);
+        if (a.dtype == ENATTEN_F32) return launch<DP, E4M3, ENATTEN_F32>(fn, a, st);
+    return launch<DP, E4M3, ENATTEN_F16>(fn, a, st);
 }
 template <bool E4M3>
 int launch_dim(const char *fn, const AttnArgs &a, hipStream_t st) {
-    if (a.D <= 64) return launch_terms<64, E4M3>(fn, a, st);
-    if (a.D <= 128) return launch_terms<128, E4M3>(fn, a, st);
-    return launch_terms<256, E4M3>(fn, a, st);
+    if (a.D <= 64) return launch_type<64, E4M3>(fn, a, st);
+    if (a.D <= 128) return launch_type<128, E4M3>(fn, a, st);
+    return launch_type<256, E4M3>(fn, a, st);
 }
 
 }  // namespace

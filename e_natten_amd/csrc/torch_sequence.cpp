@@ -195,6 +195,14 @@ void validate_attention(const Tensor &q, const Tensor &kc, const Tensor &vc, con
 // the columns of a row of pages are neighbours
 Tensor page_rows(const Tensor &t) { return t.stride(1) == 1 || t.size(1) == 1 ? t : t.contiguous(); }
 
+// rows at multiples of 16 bytes (head dims are multiples of 16): nearly always the tensor itself
+Tensor aligned_rows(const Tensor &t) {
+    const int64_t pack = 16 / t.element_size();
+    const bool ok = t.stride(3) == 1 && (t.stride(0) | t.stride(1) | t.stride(2)) % pack == 0 &&
+                    reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
 void cache_append(const Tensor &k_, const Tensor &v_, const Tensor &kc, const Tensor &vc, const Tensor &ks,
                   const Tensor &vs, const Tensor &pages_, const Tensor &lengths_, const optional<Tensor> &counts_) {
     validate_append(k_, v_, kc, vc, ks, vs, pages_, lengths_, counts_);
@@ -215,9 +223,9 @@ Tensor cache_attention(const Tensor &q_, const Tensor &kc, const Tensor &vc, con
     validate_attention(q_, kc, vc, ks, vs, pages_, lengths_, counts_, kernel_size);
     if (q_.is_meta()) return empty_rows(kernel_layout(q_));
     const c10::DeviceGuard guard(q_.device());
-    const Tensor q = kernel_layout(q_), pages = page_rows(pages_);
+    const Tensor q = aligned_rows(q_), pages = page_rows(pages_);
     const Tensor lengths = lengths_.contiguous(), counts = counts_.has_value() ? counts_->contiguous() : Tensor();
-    Tensor o = empty_rows(q);
+    Tensor o = aligned_rows(empty_rows(q));
     const int window = (int)std::min<int64_t>(kernel_size, 0x7fffffff);
     const int B = q.size(0), N = q.size(1), Nk = kc.size(1), T = q.size(2), D = q.size(3);
     const int page = kc.size(2), columns = pages.size(1);

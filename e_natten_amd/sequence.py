@@ -216,6 +216,14 @@ def _page_rows(t):
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
+def _aligned_rows(t):
+    """Rows at multiples of 16 bytes (head dims are multiples of 16): nearly always the tensor itself."""
+    pack = 16 // t.element_size()
+    if t.stride(3) == 1 and not any(s % pack for s in t.stride()[:3]) and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def _append_impl(k, v, k_cache, v_cache, k_scale, v_scale, pages, lengths, counts) -> None:
     _validate_cache("k", k, k_cache, v_cache, k_scale, v_scale, pages, lengths, counts)
     if v.shape != k.shape:
@@ -253,12 +261,12 @@ def _attention_impl(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, count
     _require_gpu(q, "cache_attention")
     _no_gradient("cache_attention", q, k_scale, v_scale)
     lib = _lib.load()
-    q, pages = _kernel_layout(q), _page_rows(pages)
+    q, pages = _aligned_rows(q), _page_rows(pages)
     lengths, counts = lengths.contiguous(), None if counts is None else counts.contiguous()
     B, N, T, D = q.shape
     heads, page, columns, window = k_cache.shape[1], k_cache.shape[2], pages.shape[1], min(kernel_size, 0x7fffffff)
     with torch.cuda.device(q.device):
-        o = _kernel_layout(torch.empty_like(q))
+        o = _aligned_rows(_kernel_layout(torch.empty_like(q)))
         need = lib.enatten_cache_attention_workspace_bytes(B, N, heads, T, D, page, columns, window, _DTYPES[q.dtype])
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         _check(lib.enatten_cache_attention(

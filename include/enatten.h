@@ -308,8 +308,8 @@ int enatten_rotary(const void *q, const void *k, void *q_out, void *k_out, const
  *   k_cache, v_cache  [num_pages, heads, page, D] of cache_dtype (ENATTEN_I8 or ENATTEN_E4M3), D a
  *              multiple of 16 up to 256, page a multiple of 16 up to 1024; element strides (page,
  *              head, token), multiples of 16 (of 8 in enatten_cache_append), tokens at most 2^20 apart
- *   k_scale, v_scale  float32 [num_pages, heads], one factor for each block (page, head): a code
- *              stands for code * scale; strides (page, head)
+ *   k_scale, v_scale  float32 [num_pages, heads], one factor for each block (page, head), not
+ *              negative: a code stands for code * scale; strides (page, head)
  *   pages      int32 [B, columns], unit stride on the columns: token j of sequence b is row j % page
  *              of page pages[b, j / page].  Entries behind a sequence's last token are not read.
  *   lengths    int32 [B]: tokens of each sequence, those that the call is about included
@@ -318,8 +318,8 @@ int enatten_rotary(const void *q, const void *k, void *q_out, void *k_out, const
  * columns) leave that sequence out: enatten_cache_append writes nothing for it,
  * enatten_cache_attention writes NaN.  A page outside 0 .. num_pages - 1 is neither read nor written;
  * a query that sees a token on one gets NaN.
- * All codes are finite numbers: the two codes of E4M3 that are not (0x7f, 0xff) read as +-480, and
- * are never written.  What a block holds behind a sequence's last token is of no consequence.
+ * All codes are finite numbers: the two codes of E4M3 that are not (0x7f, 0xff) are never written, and
+ * read as +-480 or NaN by the queries that see them.  What a block holds behind a sequence's last token is of no consequence.
  *
  * enatten_cache_append writes the new tokens k, v [B, heads, T, D] (`dtype` F32, BF16 or F16; strides
  * (batch, head, position)).  Block by block, with M = 127 or 448:
@@ -339,7 +339,8 @@ int enatten_cache_append(const void *k, const void *v, void *k_cache, void *v_ca
 
 /*
  * Attention of the last tokens of each sequence over the cache.  q, o: [B, heads, T, D] of `dtype`
- * (F32, BF16 or F16), strides (batch, head, position); heads is a multiple of heads_kv and head h
+ * (F32, BF16 or F16), strides (batch, head, position), rows at multiples of 16 bytes; heads is a multiple
+ * of heads_kv and head h
  * reads head h / (heads / heads_kv) of the cache.  Query t < counts[b] stands at position
  * p = lengths[b] - counts[b] + t and sees the tokens max(p - kernel_size + 1, 0) .. p, or all up to p
  * with kernel_size 0: the windows of enatten2d_fwd_window's causal axis.  Logits are q.k * scale.
