@@ -84,10 +84,15 @@ std::vector<Tensor> rotary_turn(const Tensor &q_, const optional<Tensor> &k_, co
 using RotarySig = std::vector<Tensor>(const Tensor &, const optional<Tensor> &, const Tensor &, const Tensor &, bool,
                                       double, bool);
 // (through the dispatcher: tracers see one operator)
-std::vector<Tensor> call_rotary(const char *name, const Tensor &q, const optional<Tensor> &k, const Tensor &positions,
+std::vector<Tensor> call_turn(const Tensor &q, const optional<Tensor> &k, const Tensor &positions,
+                              const Tensor &frequencies, bool interleaved, double scale, bool inverse) {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("enatten::rotary_turn", "").typed<RotarySig>();
+    return op.call(q, k, positions, frequencies, interleaved, scale, inverse);
+}
+std::vector<Tensor> call_rotary(const Tensor &q, const optional<Tensor> &k, const Tensor &positions,
                                 const Tensor &frequencies, bool interleaved, double scale, bool inverse) {
-    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<RotarySig>().call(
-        q, k, positions, frequencies, interleaved, scale, inverse);
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("enatten::rotary", "").typed<RotarySig>();
+    return op.call(q, k, positions, frequencies, interleaved, scale, inverse);
 }
 
 // The gradient is the turn the other way round of the upstream gradients: the same operator, so that it
@@ -102,7 +107,7 @@ struct RotaryFn : public torch::autograd::Function<RotaryFn> {
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["inverse"] = inverse;
         ctx->set_materialize_grads(false);
-        return call_rotary("enatten::rotary_turn", q, k, positions, frequencies, interleaved, scale, inverse);
+        return call_turn(q, k, positions, frequencies, interleaved, scale, inverse);
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         const variable_list s = ctx->get_saved_variables();
@@ -113,7 +118,7 @@ struct RotaryFn : public torch::autograd::Function<RotaryFn> {
         if (grads[0].defined() || two) {
             const Tensor &first = grads[0].defined() ? grads[0] : grads[1];
             const optional<Tensor> second = grads[0].defined() && two ? optional<Tensor>(grads[1]) : c10::nullopt;
-            const auto out = call_rotary("enatten::rotary", first, second, s[0], s[1], interleaved, scale, !inverse);
+            const auto out = call_rotary(first, second, s[0], s[1], interleaved, scale, !inverse);
             (grads[0].defined() ? dq : dk) = out[0];
             if (second.has_value()) dk = out[1];
         }
@@ -122,12 +127,16 @@ struct RotaryFn : public torch::autograd::Function<RotaryFn> {
 };
 std::vector<Tensor> rotary_autograd(const Tensor &q, const optional<Tensor> &k, const Tensor &positions,
                                     const Tensor &frequencies, bool interleaved, double scale, bool inverse) {
+    if (!at::GradMode::is_enabled() || !(q.requires_grad() || (k.has_value() && k->requires_grad()))) {
+        at::AutoDispatchBelowADInplaceOrView below;  // (no node: inference)
+        return call_turn(q, k, positions, frequencies, interleaved, scale, inverse);
+    }
     validate_rotary(q, k, positions, frequencies);
     return RotaryFn::apply(q, k, positions, frequencies, interleaved, scale, inverse);
 }
 std::vector<Tensor> rotary_plain(const Tensor &q, const optional<Tensor> &k, const Tensor &positions,
                                  const Tensor &frequencies, bool interleaved, double scale, bool inverse) {
-    return call_rotary("enatten::rotary_turn", q, k, positions, frequencies, interleaved, scale, inverse);
+    return call_turn(q, k, positions, frequencies, interleaved, scale, inverse);
 }
 
 // ---- cache -----------------------------------------------------------------

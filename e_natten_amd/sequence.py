@@ -25,6 +25,9 @@ import torch
 from . import _lib
 from .ops import NATIVE_BINDING, _DTYPES, _check, _kernel_layout, _require_gpu, _stream_of
 
+# the operators themselves: a call by overload costs two microseconds less than one by name
+_OPS = tuple(getattr(torch.ops.enatten, name).default for name in ("rotary", "cache_append", "cache_attention")
+             ) if NATIVE_BINDING else None
 _CACHE_DTYPES = {torch.int8: _lib.I8, torch.float8_e4m3fn: _lib.E4M3}
 
 
@@ -172,7 +175,7 @@ def rotary(q, k, positions, frequencies, interleaved=False, scale=1.0):
     _tensors(q=q, positions=positions, frequencies=frequencies)
     if k is not None:
         _tensors(k=k)
-    call = torch.ops.enatten.rotary if NATIVE_BINDING else Rotary.apply
+    call = _OPS[0] if NATIVE_BINDING else Rotary.apply
     out = call(q, k, positions, frequencies, bool(interleaved), float(scale), False)
     return out[0], out[1] if k is not None else None
 
@@ -304,7 +307,7 @@ def cache_append(k, v, k_cache, v_cache, k_scale, v_scale, pages, lengths, count
              lengths=lengths)
     if counts is not None:
         _tensors(counts=counts)
-    call = torch.ops.enatten.cache_append if NATIVE_BINDING else _append_impl
+    call = _OPS[1] if NATIVE_BINDING else _append_impl
     call(k, v, k_cache, v_cache, k_scale, v_scale, pages, lengths, counts)
 
 
@@ -329,5 +332,5 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, kerne
         raise TypeError("kernel_size must be an int or None")
     elif kernel_size < 1:
         raise ValueError("kernel_size must be >= 1, got %d" % kernel_size)
-    call = torch.ops.enatten.cache_attention if NATIVE_BINDING else _attention_impl
+    call = _OPS[2] if NATIVE_BINDING else _attention_impl
     return call(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, counts, kernel_size, float(scale))
