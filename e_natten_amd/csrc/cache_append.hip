@@ -182,7 +182,7 @@ __global__ __launch_bounds__(THREADS) void append_block(AppendArgs a) {
 template <typename S, bool E4M3, bool WIDE>
 int launch_wide(const char *fn, const AppendArgs &a, hipStream_t st) {
     const int64_t blocks = (int64_t)2 * a.heads * a.touched * a.B;
-    if (blocks > 0x7fffffff) {
+    if (blocks > 0x7fffff) {  // (2^32 threads)
         set_error("%s: too many blocks of pages and heads", fn);
         return ENATTEN_EUNSUPPORTED;
     }

@@ -36,8 +36,10 @@ typedef short s16x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFloor = -1e15f;  // the maximum of a row that has seen nothing: finite, below every logit
-constexpr int kLeast = 256;       // tokens of a part at least: what a workgroup takes to get going pays from there
-constexpr int kLeastWide = 128;   // ... of a range of steps on tiles of many rows
+// Tokens of a part at least, and of a range of steps on tiles of many rows: below, what a workgroup takes
+// to get going is more than what it brings (72 rows over 300 tokens: 18.8 us with 128, more with 512)
+constexpr int kLeast = 256;
+constexpr int kLeastWide = 128;
 constexpr int kWideRows = 256;    // rows of those tiles
 constexpr int kTop = 14;          // rows of q are brought to 2^kTop .. 2 * 2^kTop
 constexpr int kPTop = 7;          // probabilities to 2^kPTop, and up to 2^kSlack times that where the
@@ -387,7 +389,6 @@ __device__ __forceinline__ void store_channels(const Rows &r, int64_t at, f32x4 
     }
 }
 
-__device__ __forceinline__ int lane_int(int x, int l) { return __builtin_amdgcn_readlane(x, l); }
 __device__ __forceinline__ float lane_float(float x, int l) {
     return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), l));
 }

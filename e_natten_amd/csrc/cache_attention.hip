@@ -4,30 +4,38 @@
 //
 // with codes k_j, v_j and the scales z_j, z'_j of their blocks (page, head).  All query heads that share
 // a head of the cache, and all new tokens, are rows of one problem per (sequence, cache head): a row tile
-// of 16, 32 or 64 of them goes over the tokens once, with the running maximum and sum of the softmax.
+// of up to 64 of them goes over the tokens once, with the running maximum and sum of the softmax (calls
+// with more rows: cache_attention_rows.hip).
 //
-// Products.  Codes are numbers that float16 holds exactly (int8 as they are, E4M3 times 2^-8, by integer
-// operations on their bits), so both products run on the float16 matrix instructions whatever the type
-// of q: rows of q are multiplied by a power of two that brings their largest value to 2^14 .. 2^15, which
-// leaves bfloat16 values exact down to 2^-28 of the largest; float32 rows are the sum of two such terms.
-// The logits come out in float32 and take scale, z_j and the power of two there.
+// Products.  Codes are numbers that float16 holds exactly (int8 as they are, E4M3 times 2^-8), so both
+// products run on the float16 matrix instructions whatever the type of q: rows of q are multiplied by a
+// power of two that brings their largest value to 2^14 .. 2^15, which leaves bfloat16 values exact down
+// to 2^-28 of the largest; float32 rows are the sum of two such terms.  The logits come out in float32
+// and take scale, z_j and the power of two there.
 //
 // The first product forms S^T = K Q^T: a lane then holds 4 tokens of one row, and the softmax's
 // statistics are one value per lane.  The order of the tokens within the second product's sum is free,
 // so O^T = V^T P^T takes the probabilities from the registers where the first product left them, and V
 // with the same permutation: lane (m, g) reads channels m * D/16 .. of tokens 4g .. 4g+3 of both halves
-// of a tile of 32.  Neither K, V nor P passes through LDS.
+// of a tile of 32.  Neither K, V nor P passes through LDS, and no wave waits for another one on the way.
 //
-// The probabilities go into the second product as float16, times z'_j over the largest power of two
-// among the z' so far, times 2^14: 11 bits for all that is above 2^-28 of the largest (two terms for
-// float32).  Where z' outgrows that power of two, the sums so far are scaled down, as they are for the
-// maximum.
+// Probabilities go into the second product as float16, at 2^7 for the running maximum.  That maximum is
+// let lag by up to 2^8, so that the sums are seldom rescaled; what is below 2^-21 of the largest (2^-29
+// with the lag) has fewer than 11 bits.  float32 takes two terms.  z'_j goes into them too, as a summand
+// of the exponent: log2 of z'_j relative to the largest power of two among the z' so far, and the sums
+// are scaled down where that grows.  The sum of the probabilities is formed of the rounded ones, so that
+// a result stays a mean of values, but for groups whose z' is far below the largest, which float16 drops.
 //
 // What bounds it.  One token of a sequence: every code is read once, two products of 16 rows cost a few
 // percent of the matrix cores: HBM.  Work is split along the tokens so that the chip is filled whatever
 // the number of sequences and heads; the parts leave their sums, maximum and output in the workspace and
 // a second launch joins them.  The split goes by the lengths of this call, which are on the device:
-// every workgroup computes it for itself.
+// every workgroup computes it for itself.  Short calls are bound by the two launches and one chain of
+// loads (lengths, pages, codes).
+//
+// Measured on MI355X, heads of 128 channels: 32 sequences of 4096 .. 16384 tokens, 8 heads, E4M3: 147 us
+// (4.7 TB/s of codes, a plain copy reaches 5.0); 16 + 4 heads, a sequence of 131072 tokens: 33 us; five
+// tokens each for 8 sequences of up to 8192: 21 us; a window of 1024 tokens, one sequence: 5.8 us.
 #include "cache_attention.h"
 
 #include <type_traits>
@@ -44,11 +52,18 @@ constexpr int waves_of(int DP, int R, int TERMS) {
     return need <= 168 ? 3 : need <= 256 ? 2 : 1;
 }
 
+// Whether steps that every row sees go the way of those that only some see.  With a form for either the
+// widest tiles need more registers than there are (22 to 500 were spilled), and a spilled operand of a
+// matrix instruction can come back incomplete: a part that the compiler keeps in an accumulation register
+// is not restored into an operand that lies in such registers.  No kernel here may spill.
+constexpr bool one_form(int DP, int R) { return DP * R > 256 || DP == 256; }
+
 // DP: head_dim rounded up to 64, 128 or 256 (channels beyond D: zeros in q, any codes); R: row tiles of
 // 16 per workgroup; TERMS: float16 terms of q and p.
 template <int DP, int R, bool E4M3, int DT>
 __global__ __launch_bounds__(256, waves_of(DP, R, DT == ENATTEN_F32 ? 2 : 1)) void attend(AttnArgs a) {
     constexpr int TERMS = DT == ENATTEN_F32 ? 2 : 1, TOK = kTile, ROWS = 16 * R, KC = DP / 64, VW = DP / 64, CW = DP / 16;
+    constexpr bool ONE_FORM = one_form(DP, R);
     const int lane = threadIdx.x & 63, n16 = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (branches on it are the wave's)
 
@@ -201,8 +216,8 @@ __global__ __launch_bounds__(256, waves_of(DP, R, DT == ENATTEN_F32 ? 2 : 1)) vo
             }
         }
     };
-    // SEEN: every row sees every token of the step
-    auto work = [&](auto seen, int step, const Tile &t) {
+    // SEEN: every row sees every token of the step; else some may be `hidden`
+    auto work = [&](auto seen, bool hidden, int step, const Tile &t) {
         constexpr bool SEEN = decltype(seen)::value;
         const float most_z = fmaxf(t.vz[0], t.vz[1]), shrink = grow(ref, TERMS == 1 ? most_z : __builtin_amdgcn_logf(most_z));
         float lz[2], inv_z[2];
@@ -229,7 +244,7 @@ __global__ __launch_bounds__(256, waves_of(DP, R, DT == ENATTEN_F32 ? 2 : 1)) vo
         f16x8 pf[R][TERMS];
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            if (!SEEN) {
+            if (!SEEN && hidden) {
                 const int token = base + step * kTile;
 #pragma unroll
                 for (int h = 0; h < 2; h++)
@@ -311,8 +326,13 @@ __global__ __launch_bounds__(256, waves_of(DP, R, DT == ENATTEN_F32 ? 2 : 1)) vo
     };
     auto go = [&](int step, const Tile &t) {
         const int token = base + step * kTile;
-        if (token >= all_lo && token + kTile <= all_hi) work(std::true_type{}, step, t);
-        else work(std::false_type{}, step, t);
+        const bool hidden = token < all_lo || token + kTile > all_hi;
+        if constexpr (ONE_FORM) {
+            work(std::false_type{}, hidden, step, t);
+        } else {
+            if (hidden) work(std::false_type{}, true, step, t);
+            else work(std::true_type{}, false, step, t);
+        }
     };
     if (w0 < w1) {
         Tile t0, t1;
@@ -455,13 +475,19 @@ __global__ __launch_bounds__(256) void attend_join(AttnArgs a) {
 }
 
 // How a call is cut, from its sizes alone (the lengths are on the device).
+//
+// Rows.  A wave holds q, the sums and the probabilities of all rows of its tile in registers, which
+// leaves room for 64 rows of 64 channels, 48 of 128 and 16 of 256 with two tiles of codes under way.
+// Beyond, tiles of 256 rows over codes that LDS holds as float16; 72 rows of 64 channels over 300 tokens
+// take 18.8 us there and took 33.2 in tiles of 32 here.  float32 rows of more than 128 channels have too
+// many registers for that and stay here.
+// Workgroups.  Two per CU where their registers leave room for two waves per SIMD, else one: with 48 rows
+// of 128 channels a second one per CU only waits.
 Plan plan_of(int B, int heads, int heads_kv, int T, int D, int page, int columns, int window, int dtype) {
     Plan p;
     const int64_t all = (int64_t)T * (heads / heads_kv);
-    // Up to `most` rows: one tile of as many sixteens as there are, each wave with its own tokens.
-    // Beyond, tiles of 256 rows; float32 rows of more than 128 channels have too many registers there.
-    const int most = D > 128 ? 32 : D > 64 ? 48 : 64;
-    p.rows = all <= most ? (int)(all + 15) / 16 * 16 : D > 128 && dtype == ENATTEN_F32 ? 32 : kWideRows;
+    const int most = D > 128 ? 16 : D > 64 ? 48 : 64;
+    p.rows = all <= most ? (int)(all + 15) / 16 * 16 : D > 128 && dtype == ENATTEN_F32 ? 16 : kWideRows;
     p.row_tiles = (int)((all + p.rows - 1) / p.rows);
     const int64_t entries = (int64_t)B * p.row_tiles;
     int64_t tokens = (int64_t)columns * page;
@@ -506,17 +532,20 @@ int launch_type(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st
 }
 template <int DP, bool E4M3>
 int launch_rows(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st) {
-    if (p.items * a.heads_kv > 0x7fffffff) {
+    if (p.items * a.heads_kv > 0xffffff) {  // (2^32 threads)
         set_error("%s: too many row tiles", fn);
         return ENATTEN_EUNSUPPORTED;
     }
     if (p.rows == kWideRows) return launch_attend_rows(fn, a, E4M3, st);
     if (p.rows == 16) return launch_type<DP, 1, E4M3>(fn, a, p, st);
     if constexpr (DP <= 128) {
+        if (p.rows == 32) return launch_type<DP, 2, E4M3>(fn, a, p, st);
         if (p.rows == 48) return launch_type<DP, 3, E4M3>(fn, a, p, st);
-        if (DP == 64 && p.rows == 64) return launch_type<64, 4, E4M3>(fn, a, p, st);
     }
-    return launch_type<DP, 2, E4M3>(fn, a, p, st);
+    if constexpr (DP == 64)
+        if (p.rows == 64) return launch_type<DP, 4, E4M3>(fn, a, p, st);
+    set_error("%s: no tile of %d rows of %d channels", fn, p.rows, a.D);
+    return ENATTEN_EUNSUPPORTED;
 }
 
 }  // namespace

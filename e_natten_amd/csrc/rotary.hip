@@ -160,7 +160,7 @@ int launch_tokens(const char *fn, RotaryArgs &a, hipStream_t st) {
         a.slices = (heads + a.slice - 1) / a.slice;
     }
     const int64_t blocks = (int64_t)a.B * a.tiles * a.slices;
-    if (blocks > 0x7fffffff) {
+    if (blocks > 0xffffff) {  // (2^32 threads)
         set_error("%s: too many tokens", fn);
         return ENATTEN_EUNSUPPORTED;
     }
@@ -225,7 +225,7 @@ int enatten_rotary(const void *q, const void *k, void *q_out, void *k_out, const
         return ENATTEN_EINVAL;
     }
     if ((int64_t)B * T * ((int64_t)heads_q + (k ? heads_k : 0)) > (int64_t)1 << 40 || heads_q > (1 << 20) ||
-        heads_k > (1 << 20) || (int64_t)16 * ((int64_t)heads_q + heads_k) * D > 0x7fffffff) {
+        heads_k > (1 << 20) || T > 0x7fffffff - 4096 || (int64_t)16 * ((int64_t)heads_q + heads_k) * D > 0x7fffffff) {
         set_error("%s: tensor too large", fn);
         return ENATTEN_EUNSUPPORTED;
     }

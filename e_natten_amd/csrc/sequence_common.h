@@ -104,8 +104,10 @@ inline int check_cache_sizes(const char *fn, int B, int heads, int T, int D, int
         set_error("%s: negative stride for pages", fn);
         return ENATTEN_EINVAL;
     }
-    if ((int64_t)columns * page > 0x7fffffff - 4096 || (int64_t)B * heads * T > (int64_t)1 << 31) {
-        set_error("%s: more than 2^31 tokens in a sequence's pages, or rows in a call", fn);
+    // (counts of tokens, of rows, and of steps of 64 sequences stay within 31 bits)
+    if ((int64_t)columns * page > (1 << 30) - 4096 || (int64_t)B * heads > (1 << 30) ||
+        (int64_t)B * heads * T > (1 << 30)) {
+        set_error("%s: more than 2^30 tokens in a sequence's pages, or rows in a call", fn);
         return ENATTEN_EUNSUPPORTED;
     }
     return ENATTEN_OK;

@@ -46,7 +46,12 @@ void validate_rotary(const Tensor &q, const optional<Tensor> &k, const Tensor &p
                       ": frequencies must be float32 or float64, got ", frequencies.scalar_type());
     TORCH_CHECK_VALUE(frequencies.dim() == 1 && frequencies.size(0) > 0 && 2 * frequencies.size(0) <= q.size(3), what,
                       ": frequencies must be one for every rotated pair, at most head_dim / 2, got ", frequencies.sizes());
+    TORCH_CHECK_VALUE(q.size(0) <= 0x7fffffff && q.size(1) <= (1 << 20) && q.size(2) <= 0x7fffffff &&
+                          (!k.has_value() || k->size(1) <= (1 << 20)),
+                      what, ": tensor too large");
     TORCH_CHECK_VALUE(q.size(3) <= 1024, what, ": head_dim ", q.size(3), " exceeds the supported maximum of 1024");
+    TORCH_CHECK(!at::GradMode::is_enabled() || !frequencies.requires_grad(), what,
+                ": frequencies have no gradient; call it on detached ones");
     TORCH_CHECK_VALUE(positions.device() == q.device() && frequencies.device() == q.device(), what,
                       ": positions and frequencies must be on the device of q");
     on_gpu(what, q);
@@ -182,7 +187,6 @@ void validate_cache(const char *what, const char *name, const Tensor &x, const T
                       ": too many pages, or more than 1024 tokens in one");
     TORCH_CHECK_VALUE(x.size(0) <= 0x7fffffff && x.size(1) <= (1 << 20) && x.size(2) <= 0x7fffffff && x.size(3) <= 256,
                       what, ": head_dim must be a multiple of 16 up to 256, got ", x.size(3));
-    on_gpu(what, x);
 }
 void validate_append(const Tensor &k, const Tensor &v, const Tensor &kc, const Tensor &vc, const Tensor &ks,
                      const Tensor &vs, const Tensor &pages, const Tensor &lengths, const optional<Tensor> &counts) {
@@ -193,6 +197,10 @@ void validate_append(const Tensor &k, const Tensor &v, const Tensor &kc, const T
                       ": k and v must share a dtype and a device");
     TORCH_CHECK_VALUE(kc.size(1) == k.size(1), what, ": k has ", k.size(1), " heads, the cache ", kc.size(1));
     for (const Tensor *t : {&kc, &vc, &ks, &vs}) at::assert_no_internal_overlap(*t);
+    TORCH_CHECK_VALUE(!kc.is_same(vc) && !ks.is_same(vs) &&
+                          (kc.is_meta() || (kc.data_ptr() != vc.data_ptr() && ks.data_ptr() != vs.data_ptr())),
+                      what, ": keys and values must not share a cache");
+    on_gpu(what, k);
 }
 void validate_attention(const Tensor &q, const Tensor &kc, const Tensor &vc, const Tensor &ks, const Tensor &vs,
                         const Tensor &pages, const Tensor &lengths, const optional<Tensor> &counts, int64_t kernel_size) {
@@ -200,6 +208,7 @@ void validate_attention(const Tensor &q, const Tensor &kc, const Tensor &vc, con
     validate_cache(what, "q", q, kc, vc, ks, vs, pages, lengths, counts);
     TORCH_CHECK_VALUE(q.size(1) % kc.size(1) == 0, what, ": ", q.size(1), " heads are no multiple of the cache's ", kc.size(1));
     TORCH_CHECK_VALUE(kernel_size >= 0, what, ": kernel_size must be >= 1, or 0 for all tokens, got ", kernel_size);
+    on_gpu(what, q);
 }
 // the columns of a row of pages are neighbours
 Tensor page_rows(const Tensor &t) { return t.stride(1) == 1 || t.size(1) == 1 ? t : t.contiguous(); }
@@ -232,9 +241,9 @@ Tensor cache_attention(const Tensor &q_, const Tensor &kc, const Tensor &vc, con
     validate_attention(q_, kc, vc, ks, vs, pages_, lengths_, counts_, kernel_size);
     if (q_.is_meta()) return empty_rows(kernel_layout(q_));
     const c10::DeviceGuard guard(q_.device());
-    const Tensor q = aligned_rows(q_), pages = page_rows(pages_);
+    const Tensor rows = kernel_layout(q_), q = aligned_rows(rows), pages = page_rows(pages_);
     const Tensor lengths = lengths_.contiguous(), counts = counts_.has_value() ? counts_->contiguous() : Tensor();
-    Tensor o = aligned_rows(empty_rows(q));
+    const Tensor o = aligned_rows(empty_rows(rows));
     const int window = (int)std::min<int64_t>(kernel_size, 0x7fffffff);
     const int B = q.size(0), N = q.size(1), Nk = kc.size(1), T = q.size(2), D = q.size(3);
     const int page = kc.size(2), columns = pages.size(1);
@@ -257,7 +266,7 @@ void no_gradient(const char *what, std::initializer_list<const Tensor *> inputs)
 }
 void cache_append_autograd(const Tensor &k, const Tensor &v, const Tensor &kc, const Tensor &vc, const Tensor &ks,
                            const Tensor &vs, const Tensor &pages, const Tensor &lengths, const optional<Tensor> &counts) {
-    no_gradient("cache_append", {&k, &v, &ks, &vs});
+    no_gradient("cache_append", {&k, &v, &kc, &vc, &ks, &vs});
     {
         at::AutoDispatchBelowADInplaceOrView below;
         static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("enatten::cache_append", "").typed<decltype(cache_append)>();
@@ -269,7 +278,7 @@ void cache_append_autograd(const Tensor &k, const Tensor &v, const Tensor &kc, c
 Tensor cache_attention_autograd(const Tensor &q, const Tensor &kc, const Tensor &vc, const Tensor &ks, const Tensor &vs,
                                 const Tensor &pages, const Tensor &lengths, const optional<Tensor> &counts,
                                 int64_t kernel_size, double scale) {
-    no_gradient("cache_attention", {&q, &ks, &vs});
+    no_gradient("cache_attention", {&q, &kc, &vc, &ks, &vs});
     at::AutoDispatchBelowADInplaceOrView below;
     static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("enatten::cache_attention", "").typed<decltype(cache_attention)>();
     return op.call(q, kc, vc, ks, vs, pages, lengths, counts, kernel_size, scale);

@@ -87,6 +87,8 @@ def _rows(name, x, dtypes):
                          % (x.dtype, ", ".join(str(d).replace("torch.", "") for d in dtypes)))
     if x.numel() == 0:
         raise ValueError("empty tensors are not supported")
+    if max(x.shape) > 0x7fffffff or x.shape[1] > 1 << 20:
+        raise ValueError("tensor too large")
 
 
 # --- rotary ---
@@ -96,6 +98,8 @@ def _validate_rotary(q, k, positions, frequencies) -> None:
     if k is not None:
         if k.dim() != 4 or k.shape[1] < 1 or k.shape[::2] != q.shape[::2] or k.shape[3] != q.shape[3]:
             raise ValueError("q and k must differ in their heads only, got %s, %s" % (tuple(q.shape), tuple(k.shape)))
+        if k.shape[1] > 1 << 20:
+            raise ValueError("tensor too large")
         if k.dtype != q.dtype:
             raise ValueError("q and k must share a dtype")
         if k.device != q.device:
@@ -175,6 +179,8 @@ def rotary(q, k, positions, frequencies, interleaved=False, scale=1.0):
     _tensors(q=q, positions=positions, frequencies=frequencies)
     if k is not None:
         _tensors(k=k)
+    if torch.is_grad_enabled() and frequencies.requires_grad:
+        raise RuntimeError("frequencies have no gradient; call it on detached ones")
     call = _OPS[0] if NATIVE_BINDING else Rotary.apply
     out = call(q, k, positions, frequencies, bool(interleaved), float(scale), False)
     return out[0], out[1] if k is not None else None
@@ -201,6 +207,8 @@ def _validate_cache(name, x, k_cache, v_cache, k_scale, v_scale, pages, lengths,
             raise ValueError("k_scale and v_scale must be float32")
     if pages.dim() != 2 or pages.shape[0] != B or pages.shape[1] < 1 or pages.dtype != torch.int32:
         raise ValueError("pages must be int32 [B, columns], got %s %s" % (pages.dtype, list(pages.shape)))
+    if pages.shape[1] > 0x7fffffff or k_cache.shape[0] > 0x7fffffff or k_cache.shape[2] > 1024:
+        raise ValueError("too many pages, or more than 1024 tokens in one")
     for what, t in (("lengths", lengths), ("counts", counts)):
         if t is not None and (t.dim() != 1 or t.shape[0] != B or t.dtype != torch.int32):
             raise ValueError("%s must be int32 [B], got %s %s" % (what, t.dtype, list(t.shape)))
@@ -238,8 +246,10 @@ def _append_impl(k, v, k_cache, v_cache, k_scale, v_scale, pages, lengths, count
     for t in (k_cache, v_cache, k_scale, v_scale):
         if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
             raise RuntimeError("the cache must not share memory between its elements")
+    if k_cache.data_ptr() == v_cache.data_ptr() or k_scale.data_ptr() == v_scale.data_ptr():
+        raise ValueError("keys and values must not share a cache")
     _require_gpu(k, "cache_append")
-    _no_gradient("cache_append", k, v, k_scale, v_scale)
+    _no_gradient("cache_append", k, v, k_cache, v_cache, k_scale, v_scale)
     lib = _lib.load()
     k, v, pages = _kernel_layout(k), _kernel_layout(v), _page_rows(pages)
     lengths, counts = lengths.contiguous(), None if counts is None else counts.contiguous()
@@ -262,14 +272,15 @@ def _attention_impl(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, count
     if q.shape[1] % k_cache.shape[1]:
         raise ValueError("%d heads are no multiple of the cache's %d" % (q.shape[1], k_cache.shape[1]))
     _require_gpu(q, "cache_attention")
-    _no_gradient("cache_attention", q, k_scale, v_scale)
+    _no_gradient("cache_attention", q, k_cache, v_cache, k_scale, v_scale)
     lib = _lib.load()
-    q, pages = _aligned_rows(q), _page_rows(pages)
+    rows, pages = _kernel_layout(q), _page_rows(pages)
+    q = _aligned_rows(rows)
     lengths, counts = lengths.contiguous(), None if counts is None else counts.contiguous()
     B, N, T, D = q.shape
     heads, page, columns, window = k_cache.shape[1], k_cache.shape[2], pages.shape[1], min(kernel_size, 0x7fffffff)
     with torch.cuda.device(q.device):
-        o = _aligned_rows(_kernel_layout(torch.empty_like(q)))
+        o = _aligned_rows(_kernel_layout(torch.empty_like(rows)))
         need = lib.enatten_cache_attention_workspace_bytes(B, N, heads, T, D, page, columns, window, _DTYPES[q.dtype])
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         _check(lib.enatten_cache_attention(
@@ -289,8 +300,8 @@ def cache_append(k, v, k_cache, v_cache, k_scale, v_scale, pages, lengths, count
     ``k_cache, v_cache``  ``[pages, heads, page, d]``, int8 or float8_e4m3fn; d a multiple of 16 up to
         256, page a multiple of 16 up to 1024.  Strided views with unit stride on d, such as one
         layer of a larger pool, if strides and address are multiples of 16.
-    ``k_scale, v_scale``  float32 ``[pages, heads]``: a code stands for code * scale of its block
-        (page, head).
+    ``k_scale, v_scale``  float32 ``[pages, heads]``, not negative: a code stands for code * scale of
+        its block (page, head).
     ``pages``  int32 ``[B, columns]``: token j of sequence b is row j % page of page pages[b, j // page].
         A page that tokens are written to belongs to one sequence.
     ``lengths``  int32 ``[B]``: tokens of each sequence, the new ones included.
@@ -321,6 +332,11 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, kerne
     last ``kernel_size`` tokens up to and including its own, or all of them (None).  Logits are
     q.k * scale.  ``heads`` is a multiple of the cache's heads; head h reads head h // (heads / cache
     heads).  Rows from counts[b] on are 0.  float32, bfloat16 and float16.  No gradient.
+
+    The products are those of float16 terms, two each for float32, with sums and statistics in float32.
+    A call's work is cut by the lengths of all its sequences, so that another sequence's length may
+    change where a result is rounded; the same call gives the same bits.  A token whose logit is below
+    -6e14 counts for nothing.
     """
     _tensors(q=q, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, pages=pages,
              lengths=lengths)

@@ -319,7 +319,9 @@ int enatten_rotary(const void *q, const void *k, void *q_out, void *k_out, const
  * enatten_cache_attention writes NaN.  A page outside 0 .. num_pages - 1 is neither read nor written;
  * a query that sees a token on one gets NaN.
  * All codes are finite numbers: the two codes of E4M3 that are not (0x7f, 0xff) are never written, and
- * read as +-480 or NaN by the queries that see them.  What a block holds behind a sequence's last token is of no consequence.
+ * read as +-480 or NaN by the queries that see them.  What a block holds behind a sequence's last
+ * token is of no consequence.  At most 2^30 - 4096 tokens in a sequence's columns, and 2^30 rows
+ * (B * heads * T) in a call.
  *
  * enatten_cache_append writes the new tokens k, v [B, heads, T, D] (`dtype` F32, BF16 or F16; strides
  * (batch, head, position)).  Block by block, with M = 127 or 448:
@@ -339,12 +341,11 @@ int enatten_cache_append(const void *k, const void *v, void *k_cache, void *v_ca
 
 /*
  * Attention of the last tokens of each sequence over the cache.  q, o: [B, heads, T, D] of `dtype`
- * (F32, BF16 or F16), strides (batch, head, position), rows at multiples of 16 bytes; heads is a multiple
- * of heads_kv and head h
- * reads head h / (heads / heads_kv) of the cache.  Query t < counts[b] stands at position
+ * (F32, BF16 or F16), strides (batch, head, position), rows at multiples of 16 bytes; heads is a
+ * multiple of heads_kv and head h reads head h / (heads / heads_kv) of the cache.  Query t < counts[b] stands at position
  * p = lengths[b] - counts[b] + t and sees the tokens max(p - kernel_size + 1, 0) .. p, or all up to p
  * with kernel_size 0: the windows of enatten2d_fwd_window's causal axis.  Logits are q.k * scale.
- * o is 0 for t >= counts[b].
+ * o is 0 for t >= counts[b].  A token whose logit is below -6e14 counts for nothing.
  *   workspace  enatten_cache_attention_workspace_bytes() of this call's sizes, 16-byte aligned; may
  *              be NULL if that is 0.  Calls that may overlap need one each.
  */

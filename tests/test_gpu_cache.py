@@ -134,6 +134,17 @@ def _check(o, ref, bound, dtype, what):
     ([513, 400], [257, 1], 4, 1, 257, 64, 16, BF16, I8, None),
     ([200, 130], [129, 130], 6, 2, 130, 256, 32, F32, E4M3, 70),
     ([200, 130], [129, 130], 6, 2, 130, 112, 80, F32, I8, None),
+    ([900, 130, 200], None, 3, 1, 1, 256, 64, BF16, I8, None),       # up to 16 rows of more than 128 channels
+    ([900, 130, 200], None, 6, 2, 3, 256, 16, F16, I8, None),
+    ([900, 130, 200], None, 4, 2, 1, 192, 16, BF16, E4M3, 100),
+    ([900, 130, 200], None, 5, 1, 3, 240, 32, F32, I8, None),
+    ([900, 130, 200], None, 4, 4, 4, 144, 16, F32, E4M3, 77),
+    ([900, 130, 200], None, 12, 2, 3, 256, 16, BF16, E4M3, None),    # 18
+    ([900, 130, 200], None, 8, 2, 5, 160, 48, F32, I8, None),
+    ([900, 130, 200], None, 8, 1, 5, 128, 16, BF16, I8, None),       # 40 rows of 128
+    ([900, 130, 200], None, 8, 1, 6, 128, 16, F16, E4M3, 55),
+    ([900, 130, 200], None, 8, 1, 6, 112, 16, F32, I8, 55),
+    ([900, 130, 200], None, 8, 1, 5, 80, 16, F32, E4M3, None),
 ])
 def test_attention(lengths, counts, N, heads, T, d, page, dtype, cache_dtype, window):
     ensure_built()
