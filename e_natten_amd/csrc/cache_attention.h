@@ -132,6 +132,7 @@ __device__ __forceinline__ Share share_of(const AttnArgs &a, int item) {
 // in one line (heads, then sequences, then row tiles; a tile without steps counts as one, so that its
 // rows are written), cut into `parts` ranges.  A range takes what is left of a tile, whole tiles, and the
 // beginning of one; only tiles that are cut have parts to join, and every workgroup has the same work.
+constexpr int padded(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 constexpr int64_t item_floats(int rows, int D) { return (int64_t)rows * (D + 2); }  // maxima, sums, sums of values
 struct Ranges {
     int64_t line, each;  // steps of one cache head, of one range
@@ -180,7 +181,7 @@ __device__ __forceinline__ int tile_at(const AttnArgs &a, int64_t y, int &into) 
 // Workspace of the ranges: for each the number of the tile that it starts within, or -1; then two slots
 // each, for the tile that it starts within and for the one that it ends within.
 __device__ __forceinline__ float *slot_of(const AttnArgs &a, int slot) {
-    return a.ws + (a.parts + 3) / 4 * 4 + slot * item_floats(kWideRows, a.D);
+    return a.ws + (a.parts + 3) / 4 * 4 + slot * item_floats(kWideRows, padded(a.D));
 }
 
 // The workspace: first item and items of every entry, then for every (item, cache head) the maxima and
@@ -369,24 +370,25 @@ __device__ __forceinline__ void load_channels(const Rows &r, int64_t at, float (
         }
     }
 }
+template <int DT>
+__device__ __forceinline__ u32x2 narrow4(f32x4 x) {
+    u32x2 y;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        if constexpr (DT == ENATTEN_BF16) {
+            typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+            y[i] = __builtin_bit_cast(unsigned, bf16x2{(__bf16)x[2 * i], (__bf16)x[2 * i + 1]});
+        } else {
+            y[i] = __builtin_bit_cast(unsigned, f16x2{(_Float16)x[2 * i], (_Float16)x[2 * i + 1]});
+        }
+    }
+    return y;
+}
 // 4 channels of a row
 template <int DT>
 __device__ __forceinline__ void store_channels(const Rows &r, int64_t at, f32x4 x) {
-    if constexpr (DT == ENATTEN_F32) {
-        *reinterpret_cast<f32x4 *>(static_cast<float *>(const_cast<void *>(r.ptr)) + at) = x;
-    } else {
-        u32x2 y;
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            if constexpr (DT == ENATTEN_BF16) {
-                typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-                y[i] = __builtin_bit_cast(unsigned, bf16x2{(__bf16)x[2 * i], (__bf16)x[2 * i + 1]});
-            } else {
-                y[i] = __builtin_bit_cast(unsigned, f16x2{(_Float16)x[2 * i], (_Float16)x[2 * i + 1]});
-            }
-        }
-        *reinterpret_cast<u32x2 *>(static_cast<unsigned short *>(const_cast<void *>(r.ptr)) + at) = y;
-    }
+    if constexpr (DT == ENATTEN_F32) *reinterpret_cast<f32x4 *>(static_cast<float *>(const_cast<void *>(r.ptr)) + at) = x;
+    else *reinterpret_cast<u32x2 *>(static_cast<unsigned short *>(const_cast<void *>(r.ptr)) + at) = narrow4<DT>(x);
 }
 
 __device__ __forceinline__ float lane_float(float x, int l) {

@@ -494,7 +494,7 @@ Plan plan_of(int B, int heads, int heads_kv, int T, int D, int page, int columns
     if (window && window + (int64_t)p.rows < tokens) tokens = window + (int64_t)p.rows;
     p.parts = 0;
     p.items = entries;
-    const int target = 256 * (waves_of(D <= 64 ? 64 : D <= 128 ? 128 : 256, p.rows / 16, dtype == ENATTEN_F32 ? 2 : 1) > 1 ? 2 : 1);
+    const int target = 256 * (waves_of(padded(D), p.rows / 16, dtype == ENATTEN_F32 ? 2 : 1) > 1 ? 2 : 1);
     if (p.rows == kWideRows) {
         p.parts = 256;  // ranges: one workgroup per CU
     } else if (entries * heads_kv < target && tokens > kLeast) {
@@ -563,7 +563,7 @@ size_t enatten_cache_attention_workspace_bytes(int B, int heads, int heads_kv, i
         return 0;
     const Plan p = plan_of(B, heads, heads_kv, T, D, page, columns, kernel_size, dtype);
     if (!p.parts) return 0;
-    if (p.rows == kWideRows) return ((size_t)(p.parts + 3) / 4 * 4 + 2 * p.parts * item_floats(kWideRows, D)) * sizeof(float);
+    if (p.rows == kWideRows) return ((size_t)(p.parts + 3) / 4 * 4 + 2 * p.parts * item_floats(kWideRows, padded(D))) * sizeof(float);
     return (size_t)(head_floats((int64_t)B * p.row_tiles) + p.items * heads_kv * item_floats(p.rows, D)) * sizeof(float);
 }
 

@@ -399,34 +399,75 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
     }
 
     l = pair_sum(l);
+    __syncthreads();  // (the last step's operands are read: their place is for the rows now)
     {
     const AttnArgs &a = args_again();
     const float back = __builtin_amdgcn_exp2f(ref - kPTop + (E4M3 ? 8 : 0));
     const float poison = s.ok ? 0.f : __uint_as_float(0x7fc00000u);
     const float norm = (l == 0.f ? 0.f : 1.f / l) * back;
-    const int r = wave * 32 + n, row = row0 + n, t_row = row / a.group;
-    const bool live = t_row < s.count;
-    float *part = slot_of(a, slot);
-    if (row < a.T * a.group) {
-        if (parted && h == 0) {
-            part[r] = m;
-            part[kWideRows + r] = l;
+    const int row = row0 + n;
+    const bool here = row < a.T * a.group, live = here && row / a.group < s.count;
+    // 4 neighbouring channels, 4 mm + 128 i: words of one value row, blocks i of O, or for DP 64 rows 16 apart too
+    auto channels = [&](int i, int j) {
+        if constexpr (DP == 64) return f32x4{acc[0][j], acc[0][j + 8], acc[1][j], acc[1][j + 8]};
+        else return f32x4{acc[i * 4][j], acc[i * 4 + 1][j], acc[i * 4 + 2][j], acc[i * 4 + 3][j]};
+    };
+    constexpr int BIG = DP == 256 ? 2 : 1, JS = DP == 64 ? 8 : 16;
+    if (parted) {
+        // (lane by lane, as it lies in the registers)
+        float *part = slot_of(a, slot);
+        if (here && h == 0) {
+            part[wave * 32 + n] = m;
+            part[kWideRows + wave * 32 + n] = l;
         }
+        f32x4 *to = reinterpret_cast<f32x4 *>(part + 2 * kWideRows) + wave * (BIG * JS) * 64 + lane;
+        if (row0 < a.T * a.group) {
+#pragma unroll
+            for (int i = 0; i < BIG; i++)
+#pragma unroll
+                for (int j = 0; j < JS; j++) to[(i * JS + j) * 64] = channels(i, j) * back;
+        }
+    } else if constexpr (DT == ENATTEN_F32) {
+        const int t_row = row / a.group;
         const int64_t to = b * a.o.sb + (head * a.group + row - t_row * a.group) * a.o.sh + t_row * a.o.st;
-        const float f = parted ? back : live ? norm : 0.f;
-        // 4 neighbouring channels: words of one value row, blocks i of O, or for DP 64 rows 16 apart too
 #pragma unroll
-        for (int i = 0; i < OB; i += DP == 64 ? 2 : 4)
+        for (int i = 0; i < BIG; i++)
 #pragma unroll
-            for (int j = 0; j < (DP == 64 ? 8 : 16); j++) {
-                const int mm = j / 4 * 8 + h * 4 + j % 4;
-                f32x4 y;
-                if constexpr (DP == 64) y = f32x4{acc[0][j], acc[0][j + 8], acc[1][j], acc[1][j + 8]};
-                else y = f32x4{acc[i][j], acc[i + 1][j], acc[i + 2][j], acc[i + 3][j]};
-                const int d = 4 * mm + i / 4 * 128;
-                if (d >= a.D) continue;
-                if (parted) *reinterpret_cast<f32x4 *>(part + 2 * kWideRows + r * a.D + d) = y * f;
-                else store_channels<DT>(a.o, to + d, (live ? y * f : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
+            for (int j = 0; j < JS; j++) {
+                const int d = 4 * (j / 4 * 8 + h * 4 + j % 4) + i * 128;
+                if (here && d < a.D) store_channels<DT>(a.o, to + d, (live ? channels(i, j) * norm : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
+            }
+    } else {
+        // 64 channels at a time through LDS, so that a store takes whole lines of 8 rows and not pieces of
+        // 8 bytes of 32: a wave's place is 32 rows of 128 bytes, their runs of 16 bytes swapped by row
+        char *place = reinterpret_cast<char *>(&k_lds[0][0]) + wave * 4096;
+        const int cols = lane % 8;
+#pragma unroll
+        for (int i = 0; i < BIG; i++)
+#pragma unroll
+            for (int q = 0; q < JS / 8; q++) {
+                u32x2 y[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const f32x4 x = (live ? channels(i, q * 8 + j) * norm : f32x4{0.f, 0.f, 0.f, 0.f}) + poison;
+                    y[j] = narrow4<DT>(x);
+                }
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int mm = j / 4 * 8 + h * 4 + j % 4;
+                    *reinterpret_cast<u32x2 *>(place + n * 128 + ((mm / 2) ^ (n / 2 & 7)) * 16 + mm % 2 * 8) = y[j];
+                }
+                __builtin_amdgcn_wave_barrier();
+                const int d = i * 128 + q * 64 + cols * 8;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int r = k * 8 + lane / 8, to_row = row0 + r, t = to_row / a.group;
+                    const u32x4 x = *reinterpret_cast<const u32x4 *>(place + r * 128 + (cols ^ (r / 2 & 7)) * 16);
+                    if (to_row < a.T * a.group && d < a.D)
+                        *reinterpret_cast<u32x4 *>(static_cast<unsigned short *>(const_cast<void *>(a.o.ptr)) + b * a.o.sb +
+                                                   (head * a.group + to_row - t * a.group) * a.o.sh + t * a.o.st + d) = x;
+                }
             }
     }
     }
@@ -438,84 +479,83 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
 }
 
 // Tiles that ranges cut, joined: one workgroup per (start of a range, 16 rows), the one of the first
-// start within a tile for all its parts.  A wave takes a row at a time: 16 lanes over the channels, 4 in
-// 64 each, and every fourth part.
-template <int DT>
+// start within a tile for all its parts.  A wave takes every fourth part: 16 lanes over the rows, 4 over
+// neighbouring words of 4 channels.
+template <int DP, int DT>
 __global__ __launch_bounds__(256) void join_rows(AttnArgs a) {
-    constexpr int BLOCKS = kWideRows / 16;
-    const int range = blockIdx.x / BLOCKS, c = threadIdx.x % 16 * 4, g = threadIdx.x / 16 % 4;
+    constexpr int BLOCKS = kWideRows / 16, WORDS = DP / 16;
+    const int range = blockIdx.x / BLOCKS, n = threadIdx.x % 16, c = threadIdx.x / 16 % 4, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int *note = reinterpret_cast<const int *>(a.ws);
     const int tile = note[range];
     if (tile < 0 || note[range - 1] == tile) return;  // (the first range starts with a tile)
     const int entries = a.B * a.row_tiles, head = tile / entries, entry = tile - head * entries;
-    const int b = entry / a.row_tiles, row0 = (entry - b * a.row_tiles) * kWideRows;
+    const int b = entry / a.row_tiles, r = blockIdx.x % BLOCKS * 16 + n;
+    const int row = (entry - b * a.row_tiles) * kWideRows + r;
+    if (row - n >= a.T * a.group) return;  // (none of the 16)
     const int count = a.tb.counts ? a.tb.counts[b] : a.T;
     // the parts: the end of the range before, then the beginnings of the ranges that start within the tile
     int parts = 1;
     for (;; parts += 64) {
-        const int q = range + parts - 1 + (threadIdx.x & 63);
+        const int q = range + parts - 1 + lane;
         const unsigned long long others = __ballot(q >= a.parts || note[q] != tile);
         if (others) {
             parts += __ffsll(others) - 1;
             break;
         }
     }
-    for (int k = 0; k < 4; k++) {
-        const int r = blockIdx.x % BLOCKS * 16 + k * 4 + threadIdx.x / 64, row = row0 + r;
-        if (row >= a.T * a.group) return;
-        f32x4 y[4];
+    // rows behind the last one have no sums: they go along with its
+    const int from = min(r, a.T * a.group - 1 - (row - r));
+    auto part_at = [&](int q) { return slot_of(a, q ? 2 * (range + q - 1) : 2 * range - 1); };
+    float top = kFloor, sum = 0.f;
+    for (int q = wave; q < parts; q += 4) top = fmaxf(top, part_at(q)[from]);
+    f32x4 y[WORDS];
 #pragma unroll
-        for (int i = 0; i < 4; i++) y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        float top = kFloor, sum = 0.f;
-        constexpr int DEEP = 4;  // parts whose loads are under way at a time
-        for (int q0 = g; q0 < parts; q0 += 4 * DEEP) {
-            float m[DEEP], l[DEEP];
-            f32x4 x[DEEP][4];
+    for (int i = 0; i < WORDS; i++) y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int q = wave; q < parts; q += 4) {
+        const float *part = part_at(q);
+        const float f = __builtin_amdgcn_exp2f(part[from] - top);
+        sum += f * part[kWideRows + from];
+        const f32x4 *x = reinterpret_cast<const f32x4 *>(part + 2 * kWideRows) + from / 32 * (DP / 8) * 64 + from % 32;
+        // the word of channels 4 mm + 128 k .. lies at place 16 k + j of the lanes h
 #pragma unroll
-            for (int n = 0; n < DEEP; n++) {
-                const int q = q0 + 4 * n;
-                m[n] = kFloor;
-                l[n] = 0.f;
-#pragma unroll
-                for (int i = 0; i < 4; i++) x[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (q >= parts) continue;
-                const float *part = slot_of(a, q ? 2 * (range + q - 1) : 2 * range - 1);
-                m[n] = part[r];
-                l[n] = part[kWideRows + r];
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (c + 64 * i < a.D) x[n][i] = *reinterpret_cast<const f32x4 *>(part + 2 * kWideRows + r * a.D + c + 64 * i);
-            }
-            float most = top;
-#pragma unroll
-            for (int n = 0; n < DEEP; n++) most = fmaxf(most, m[n]);
-            const float old = __builtin_amdgcn_exp2f(top - most);
-            top = most;
-            sum *= old;
-#pragma unroll
-            for (int i = 0; i < 4; i++) y[i] *= old;
-#pragma unroll
-            for (int n = 0; n < DEEP; n++) {
-                const float f = __builtin_amdgcn_exp2f(m[n] - top);
-                sum += f * l[n];
-#pragma unroll
-                for (int i = 0; i < 4; i++) y[i] += f * x[n][i];
-            }
+        for (int i = 0; i < WORDS; i++) {
+            const int mm = i % 8 * 4 + c, place = i / 8 * 16 + mm / 8 * 4 + mm % 4, h = mm / 4 % 2;
+            y[i] += f * x[place * 64 + h * 32];
         }
-        const float most = row_max(top), f = __builtin_amdgcn_exp2f(top - most);
-        sum = row_sum(sum * f);
-        const int t = row / a.group;
-        const int64_t to = b * a.o.sb + (head * a.group + row - t * a.group) * a.o.sh + t * a.o.st;
-        const float norm = sum == 0.f || t >= count ? 0.f : 1.f / sum;
+    }
+    __shared__ __align__(16) f32x4 red[4][WORDS][64];
+    __shared__ float tops[4][16], sums[4][16];
+    if (c == 0) {
+        tops[wave][n] = top;
+        sums[wave][n] = sum;
+    }
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (c + 64 * i >= a.D) break;
-            f32x4 z;
+    for (int i = 0; i < WORDS; i++) red[wave][i][lane] = y[i];
+    __syncthreads();
+    top = kFloor;
 #pragma unroll
-            for (int j = 0; j < 4; j++) z[j] = row_sum(y[i][j] * f) * norm;
-            if (t >= count) z = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (g == 0) store_channels<DT>(a.o, to + c + 64 * i, z);
-        }
+    for (int v = 0; v < 4; v++) top = fmaxf(top, tops[v][n]);
+    float f[4];
+    sum = 0.f;
+#pragma unroll
+    for (int v = 0; v < 4; v++) {
+        f[v] = __builtin_amdgcn_exp2f(tops[v][n] - top);
+        sum += f[v] * sums[v][n];
+    }
+    if (row >= a.T * a.group) return;
+    const int t = row / a.group;
+    const int64_t to = b * a.o.sb + (head * a.group + row - t * a.group) * a.o.sh + t * a.o.st;
+    const float norm = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int k = 0; k < WORDS / 4; k++) {
+        const int i = k * 4 + wave, d = i * 16 + c * 4;
+        if (d >= a.D) break;
+        f32x4 z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int v = 0; v < 4; v++) z += f[v] * red[v][i][lane];
+        store_channels<DT>(a.o, to + d, t < count ? z * norm : f32x4{0.f, 0.f, 0.f, 0.f});
     }
 }
 
@@ -528,7 +568,7 @@ int launch(const char *fn, const AttnArgs &a, hipStream_t st) {
     const int rc = launched(fn);
     if (rc) return rc;
     ProfScope prof(ENATTEN_KERNEL_CACHE_JOIN, "join_rows", st);
-    join_rows<DT><<<a.parts * (kWideRows / 16), 256, 0, st>>>(a);
+    join_rows<DP, DT><<<a.parts * (kWideRows / 16), 256, 0, st>>>(a);
     return launched(fn);
 }
 template <int DP, bool E4M3>
