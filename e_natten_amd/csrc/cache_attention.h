@@ -36,10 +36,7 @@ typedef short s16x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFloor = -1e15f;  // the maximum of a row that has seen nothing: finite, below every logit
-// Tokens of a part at least, and of a range of steps on tiles of many rows: below, what a workgroup takes
-// to get going is more than what it brings (72 rows over 300 tokens: 18.8 us with 128, more with 512)
-constexpr int kLeast = 256;
-constexpr int kLeastWide = 128;
+constexpr int kLeast = 256;       // tokens of a part at least: what a workgroup takes to get going pays from there
 constexpr int kWideRows = 256;    // rows of those tiles
 constexpr int kTop = 14;          // rows of q are brought to 2^kTop .. 2 * 2^kTop
 constexpr int kPTop = 7;          // probabilities to 2^kPTop, and up to 2^kSlack times that where the
@@ -153,11 +150,14 @@ __device__ __forceinline__ Ranges ranges_of(const AttnArgs &a) {
         r.line += (unsigned)__builtin_amdgcn_readlane(running_sum(n), 63);
     }
     r.each = (r.line * a.heads_kv + a.parts - 1) / a.parts;
-    // The parts of a cut tile are 256 rows of sums, written and read: with a tile for every workgroup that
-    // costs more than up to 30% that some are longer than the mean (2048 tokens of two sequences of 16384 and
-    // 12288: 565 us whole, 576 cut)
-    r.whole = (int64_t)entries * a.heads_kv <= a.parts && !__any(10 * (int64_t)most > 13 * r.each);
-    if (r.each < kLeastWide / TOK) r.each = kLeastWide / TOK;
+    // The parts of cut tiles are their rows' sums in float32, written and read, which takes as long as some
+    // steps: at 128 channels about 2 for 64 tiles of 256 rows.  A tile for every workgroup pays where the
+    // longest is hardly longer than that beyond the mean.  2048 tokens each of 16384 and 12288 (256 tiles
+    // of 224 steps on average, 256 at most): 506 us cut, 570 whole; 256 tokens each of 8 sequences of 300
+    // (128 tiles of 5): 37 us cut, 27 whole; half as many tiles: 21 us cut, 24 whole.
+    const int64_t tiles = (int64_t)entries * a.heads_kv;
+    const int64_t steps = tiles * min(ROWS, a.T * a.group) * padded(a.D) >> 20;
+    r.whole = tiles <= a.parts && !__any(most > r.each + steps);
     return r;
 }
 // The row tile at step `y` of a head's line, and how far into it that is

@@ -33,8 +33,8 @@
 // every workgroup computes it for itself.  Short calls are bound by the two launches and one chain of
 // loads (lengths, pages, codes).
 //
-// Measured on MI355X, heads of 128 channels: 32 sequences of 4096 .. 16384 tokens, 8 heads, E4M3: 147 us
-// (4.7 TB/s of codes, a plain copy reaches 5.0); 16 + 4 heads, a sequence of 131072 tokens: 33 us; five
+// Measured on MI355X, heads of 128 channels: 32 sequences of 4096 .. 16384 tokens, 8 heads, E4M3: 142 us
+// (5.7 TB/s; reads alone reach 6.4); 16 + 4 heads, a sequence of 131072 tokens: 33 us; five
 // tokens each for 8 sequences of up to 8192: 21 us; a window of 1024 tokens, one sequence: 5.8 us.
 #include "cache_attention.h"
 
@@ -479,7 +479,7 @@ __global__ __launch_bounds__(256) void attend_join(AttnArgs a) {
 // Rows.  A wave holds q, the sums and the probabilities of all rows of its tile in registers, which
 // leaves room for 64 rows of 64 channels, 48 of 128 and 16 of 256 with two tiles of codes under way.
 // Beyond, tiles of 256 rows over codes that LDS holds as float16; 72 rows of 64 channels over 300 tokens
-// take 18.8 us there and took 33.2 in tiles of 32 here.  float32 rows of more than 128 channels have too
+// take 14.7 us there and took 33.2 in tiles of 32 here.  float32 rows of more than 128 channels have too
 // many registers for that and stay here.
 // Workgroups.  Two per CU where their registers leave room for two waves per SIMD, else one: with 48 rows
 // of 128 channels a second one per CU only waits.

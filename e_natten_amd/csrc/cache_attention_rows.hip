@@ -18,8 +18,8 @@
 // constant and not a selection of exponents.
 //
 // Measured on MI355X, 2048 tokens each of sequences of 16384 and 12288, 16 heads of 128 channels over 4
-// of an int8 cache: 567 us, 787 TFLOP/s; a product of two 8192 x 8192 matrices reaches 1181 in float16.
-// 64 channels: 349 us, 256 channels: 1229 us; 512 new tokens: 163 us, 128: 74 us.
+// of an int8 cache: 495 us, 900 TFLOP/s; a product of two 8192 x 8192 matrices reaches 1181 in float16.
+// 64 channels: 306 us, 256 channels: 1109 us; 512 new tokens: 151 us, 128: 62 us.
 #include "cache_attention.h"
 
 #include <type_traits>
