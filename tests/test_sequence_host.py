@@ -309,3 +309,18 @@ def test_workspace_sizes():
     assert need(T=40, N=16) == need(T=400, N=16) == 4 * (256 + 2 * 256 * 256 * 66)
     for bad in (dict(B=0), dict(N=3), dict(hk=0), dict(T=0), dict(D=0), dict(page=0), dict(cols=0), dict(win=-1)):
         assert need(**bad) == 0
+
+
+def test_attention_kernels_do_not_spill():
+    """A spilled operand of a matrix instruction came back incomplete where the compiler kept a part of it in
+    an accumulation register: kernels that use these must not spill (cache_attention.hip).  What the
+    compiler notes of every kernel is in the built library, its keys in alphabetical order."""
+    ensure_built()
+    import re
+    from e_natten_amd import _lib
+    text = open(_lib.LIB_PATH, "rb").read()
+    entry = re.compile(rb"\.symbol.{1,3}?(_ZN7enatten12_GLOBAL__N_1\d+(?:attend|attend_join)I\w+)\.kd"
+                       rb".{0,200}?\.vgpr_spill_count(.)", re.S)
+    spills = {m.group(1): m.group(2)[0] for m in entry.finditer(text)}
+    assert len(spills) > 40
+    assert not any(spills.values()), [k for k, n in spills.items() if n]
