@@ -336,3 +336,57 @@ def test_operators_agree_with_their_schemas():
     odd = torch.randn(2, 7, 4, 67, device="cuda", dtype=BF16).transpose(1, 2)[..., 1:65]
     for q in (x[:, :4], odd):
         torch.library.opcheck(ops.cache_attention.default, (q, *cache, n, None, 0, 1.0), test_utils=utils)
+
+
+def test_calls_on_two_streams_at_once():
+    ensure_built()
+    from e_natten_amd import cache_attention
+    cases = []
+    for T, length in ((1, 6000), (70, 3000)):
+        cache = Cache([length, length // 2], 2, 32, 128, E4M3, seed=T)
+        q = torch.randn((2, 8, T, 128), generator=torch.Generator().manual_seed(T)).to(BF16).cuda()
+        args = (q, *cache.on("cuda"), _ints([length, length // 2]), None, 0.1)
+        cases.append((args, cache_attention(*args), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    out = [[], []]
+    for _ in range(10):
+        for i, (args, _, stream) in enumerate(cases):
+            with torch.cuda.stream(stream):
+                out[i].append(cache_attention(*args))
+    torch.cuda.synchronize()
+    for (_, want, _), got in zip(cases, out):
+        assert all(torch.equal(o, want) for o in got)
+
+
+def test_compiled_steps():
+    """Traced as a whole, a training step and an answering step give the same bits."""
+    ensure_built()
+    import e_natten_amd as E
+    if not E.ops.NATIVE_BINDING:
+        pytest.skip("needs the native binding")
+    f, _ = E.rotary_frequencies(64, device="cuda")
+    p = torch.arange(7, device="cuda")
+    x = torch.randn(2, 7, 8, 64, device="cuda", dtype=BF16)
+
+    def train(x):
+        y = x.transpose(1, 2)
+        q, k = E.rotary(y[:, :4], y[:, 4:], p, f)
+        return E.natten1d(q, k, y[:, :4], 5, 0.125, is_causal=True)
+
+    def serve(x, kc, vc, ks, vs, pages, n):
+        y = x.transpose(1, 2)
+        q, k = E.rotary(y[:, :4], y[:, 4:6], p, f)
+        E.cache_append(k, y[:, 6:], kc, vc, ks, vs, pages, n)
+        return E.cache_attention(q, kc, vc, ks, vs, pages, n, None, 0.125)
+
+    a, b = (x.detach().requires_grad_(True) for _ in range(2))
+    o, want = torch.compile(train, backend="aot_eager", fullgraph=True)(a), train(b)
+    assert torch.equal(o, want)
+    assert torch.equal(torch.autograd.grad(o, a, want.detach())[0], torch.autograd.grad(want, b, want.detach())[0])
+    first, second = (list(Cache([100, 60], 2, 16, 64, I8).on("cuda")) for _ in range(2))
+    n = _ints([100, 60])
+    with torch.no_grad():
+        o = torch.compile(serve, backend="aot_eager", fullgraph=True)(x, *first, n)
+        assert torch.equal(o, serve(x, *second, n))
+    for s, t in zip(first, second):
+        assert torch.equal(s.nan_to_num(nan=-1.0), t.nan_to_num(nan=-1.0)) if s.dtype == F32 else torch.equal(s, t)
