@@ -21,6 +21,9 @@ void on_gpu(const char *what, const Tensor &t) {
     TORCH_CHECK(t.is_cuda() || t.is_meta(), what, ": tensors must be on the GPU; this build has no CPU path");
 }
 void *stream_now() { return c10::hip::getCurrentHIPStream().stream(); }
+// A tangent of forward mode.  A tensor can have one without requires_grad and in every grad mode: calls that
+// make no node look for it themselves.
+bool has_tangent(const Tensor &t) { return t._fw_grad(/*level=*/0).defined(); }
 
 // ---- rotary ----------------------------------------------------------------
 
@@ -132,6 +135,8 @@ struct RotaryFn : public torch::autograd::Function<RotaryFn> {
 };
 std::vector<Tensor> rotary_autograd(const Tensor &q, const optional<Tensor> &k, const Tensor &positions,
                                     const Tensor &frequencies, bool interleaved, double scale, bool inverse) {
+    TORCH_CHECK(!has_tangent(q) && !(k.has_value() && has_tangent(*k)) && !has_tangent(frequencies),
+                "rotary: there is no forward-mode derivative; gradients come by the backward pass");
     if (!at::GradMode::is_enabled() || !(q.requires_grad() || (k.has_value() && k->requires_grad()))) {
         at::AutoDispatchBelowADInplaceOrView below;  // (no node: inference)
         return call_turn(q, k, positions, frequencies, interleaved, scale, inverse);
@@ -260,9 +265,11 @@ Tensor cache_attention(const Tensor &q_, const Tensor &kc, const Tensor &vc, con
 
 // Codes are rounded: neither operator has a gradient, and a caller that would get none is told so.
 void no_gradient(const char *what, std::initializer_list<const Tensor *> inputs) {
-    if (!at::GradMode::is_enabled()) return;
+    const bool mode = at::GradMode::is_enabled();
     for (const Tensor *t : inputs)
-        TORCH_CHECK(!t->requires_grad(), what, ": a cache of 8 bits has no gradient; call it under torch.no_grad() or on detached tensors");
+        TORCH_CHECK(!(mode && t->requires_grad()) && !has_tangent(*t), what,
+                    ": a cache of 8 bits has no gradient; call it under torch.no_grad() or on detached tensors, which "
+                    "have no tangent");
 }
 void cache_append_autograd(const Tensor &k, const Tensor &v, const Tensor &kc, const Tensor &vc, const Tensor &ks,
                            const Tensor &vs, const Tensor &pages, const Tensor &lengths, const optional<Tensor> &counts) {

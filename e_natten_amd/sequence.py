@@ -21,6 +21,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import NATIVE_BINDING, _DTYPES, _check, _kernel_layout, _require_gpu, _stream_of
@@ -167,7 +168,8 @@ class Rotary(torch.autograd.Function):
 
 def rotary(q, k, positions, frequencies, interleaved=False, scale=1.0):
     """Rotary positions: ``(q', k')`` of ``q [B, heads, T, d]`` and ``k [B, heads_k, T, d]`` (or None,
-    which comes back as None).  Differentiable in q and k, any number of times.
+    which comes back as None).  Differentiable in q and k, any number of times, by the backward pass
+    (forward mode is refused).
 
     The first ``R = 2 len(frequencies)`` channels form pairs, ``(i, i + R / 2)``, or ``(2 i, 2 i + 1)``
     if ``interleaved``; the pair of the token at position p turns by the angle ``p * frequencies[i]``
@@ -218,9 +220,10 @@ def _validate_cache(name, x, k_cache, v_cache, k_scale, v_scale, pages, lengths,
 
 
 def _no_gradient(what, *inputs) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in inputs):
+    mode = torch.is_grad_enabled()
+    if any(mode and t.requires_grad or forward_ad.unpack_dual(t).tangent is not None for t in inputs):
         raise RuntimeError("%s: a cache of 8 bits has no gradient; call it under torch.no_grad() or on "
-                           "detached tensors" % what)
+                           "detached tensors, which have no tangent" % what)
 
 
 def _page_rows(t):

@@ -210,6 +210,51 @@ def test_nothing_of_a_cache_has_a_gradient():
                 getattr(E, name)(*args)
 
 
+def test_tangents_are_not_dropped():
+    """A dual tensor has its tangent without requires_grad, in every grad mode; none of the operators has a
+    derivative of forward mode, and a caller that would silently get zeros is told (tensors without data)."""
+    ensure_built()
+    import e_natten_amd as E
+    from torch.autograd import forward_ad
+    if not E.ops.NATIVE_BINDING:
+        pytest.skip("needs the native binding")
+    q, k, p, f = _rotary_args("meta")
+    calls = [(q, lambda x: E.rotary(x, k, p, f)), (q, lambda x: E.rotary(x, None, p, f)),
+             (k, lambda x: E.rotary(q, x, p, f)), (f, lambda x: E.rotary(q, k, p, x))]
+    for name, which in (("cache_attention", (0, 3, 4)), ("cache_append", (0, 1, 4, 5))):
+        args, _ = _cache_args(name, "meta")
+        for i in which:
+            calls.append((args[i], lambda x, name=name, args=args, i=i: getattr(E, name)(*args[:i], x, *args[i + 1:])))
+    for x, call in calls:
+        for mode in (torch.enable_grad, torch.no_grad):
+            with forward_ad.dual_level(), mode():
+                with pytest.raises(RuntimeError, match="forward-mode|no gradient"):
+                    call(forward_ad.make_dual(x, torch.ones_like(x)))
+                call(x)     # within the level, without a tangent
+            with mode(), pytest.raises(RuntimeError, match="forward-mode|no gradient"):
+                torch.func.jvp(lambda y: (call(y), y)[1], (x,), (torch.ones_like(x),))
+    with pytest.raises(RuntimeError):
+        torch.func.jacfwd(lambda y: E.rotary(y, None, p, f)[0].sum())(q)
+
+
+def test_tangents_are_not_dropped_through_ctypes(monkeypatch):
+    ensure_built()
+    from e_natten_amd import sequence as S
+    from torch.autograd import forward_ad
+    monkeypatch.setattr(S, "_rotary_impl", lambda q, k, *rest: [q * 2.0] if k is None else [q * 2.0, k * 2.0])
+    q, k, p, f = _rotary_args()
+    call = lambda q, k, f: S.Rotary.apply(q, k, p, f, False, 1.0, False)
+    for mode in (torch.enable_grad, torch.no_grad):
+        with forward_ad.dual_level(), mode():
+            dual = lambda x: forward_ad.make_dual(x, torch.ones_like(x))
+            for args in ((dual(q), k, f), (dual(q), None, f), (q, dual(k), f), (q, k, dual(f))):
+                with pytest.raises(RuntimeError):
+                    call(*args)
+                with pytest.raises(RuntimeError, match="no gradient"):
+                    S._no_gradient("cache_append", *(x for x in args if x is not None))
+            S._no_gradient("cache_append", q, k, f)
+
+
 def test_shapes_without_data():
     ensure_built()
     import e_natten_amd as E
