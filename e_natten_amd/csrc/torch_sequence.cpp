@@ -271,13 +271,25 @@ void no_gradient(const char *what, std::initializer_list<const Tensor *> inputs)
                     ": a cache of 8 bits has no gradient; call it under torch.no_grad() or on detached tensors, which "
                     "have no tangent");
 }
+using AppendSig = decltype(cache_append);
+void call_append(const Tensor &k, const Tensor &v, const Tensor &kc, const Tensor &vc, const Tensor &ks,
+                 const Tensor &vs, const Tensor &pages, const Tensor &lengths, const optional<Tensor> &counts) {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("enatten::cache_append", "").typed<AppendSig>();
+    op.call(k, v, kc, vc, ks, vs, pages, lengths, counts);
+}
 void cache_append_autograd(const Tensor &k, const Tensor &v, const Tensor &kc, const Tensor &vc, const Tensor &ks,
                            const Tensor &vs, const Tensor &pages, const Tensor &lengths, const optional<Tensor> &counts) {
     no_gradient("cache_append", {&k, &v, &kc, &vc, &ks, &vs});
+    at::AutoDispatchBelowAutograd below;
+    call_append(k, v, kc, vc, ks, vs, pages, lengths, counts);
+}
+// The version counters of what is written.  Ordinary tensors come here in inference mode too, where the
+// autograd key is left out: a graph made before may have saved them.
+void cache_append_in_place(const Tensor &k, const Tensor &v, const Tensor &kc, const Tensor &vc, const Tensor &ks,
+                           const Tensor &vs, const Tensor &pages, const Tensor &lengths, const optional<Tensor> &counts) {
     {
         at::AutoDispatchBelowADInplaceOrView below;
-        static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("enatten::cache_append", "").typed<decltype(cache_append)>();
-        op.call(k, v, kc, vc, ks, vs, pages, lengths, counts);
+        call_append(k, v, kc, vc, ks, vs, pages, lengths, counts);
     }
     for (const Tensor *t : {&kc, &vc, &ks, &vs})
         if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
@@ -315,4 +327,8 @@ TORCH_LIBRARY_IMPL(enatten, Autograd, m) {
     m.impl("rotary", &rotary_autograd);
     m.impl("cache_append", &cache_append_autograd);
     m.impl("cache_attention", &cache_attention_autograd);
+}
+
+TORCH_LIBRARY_IMPL(enatten, ADInplaceOrView, m) {
+    m.impl("cache_append", &cache_append_in_place);
 }

@@ -255,6 +255,33 @@ def test_tangents_are_not_dropped_through_ctypes(monkeypatch):
             S._no_gradient("cache_append", q, k, f)
 
 
+def test_append_counts_versions_in_every_mode():
+    """A graph that saved a cache or its scales notices an append under torch.inference_mode() too."""
+    ensure_built()
+    import e_natten_amd as E
+    if not E.ops.NATIVE_BINDING:
+        pytest.skip("needs the native binding")
+    x = torch.ones(6, 2, device="meta", requires_grad=True)
+    for mode in (torch.enable_grad, torch.no_grad, torch.inference_mode):
+        args, _ = _cache_args("cache_append", "meta")
+        written = args[2:6]
+        saved = x * args[4]
+        before = [t._version for t in written]
+        with mode():
+            E.cache_append(*args)
+        assert [t._version for t in written] == [n + 1 for n in before], mode
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            saved.sum().backward()
+    with torch.inference_mode():
+        args, _ = _cache_args("cache_append", "meta")   # inference tensors have no versions
+        E.cache_append(*args)
+    args, _ = _cache_args("cache_append", "meta")
+    with torch.inference_mode():
+        rows, _ = _cache_args("cache_append", "meta")
+        E.cache_append(*rows[:2], *args[2:])            # new tokens of that mode, a cache that is older
+    assert [t._version for t in args[2:6]] == [1] * 4
+
+
 def test_shapes_without_data():
     ensure_built()
     import e_natten_amd as E
