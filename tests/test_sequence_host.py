@@ -396,3 +396,47 @@ def test_attention_kernels_do_not_spill():
     spills = {m.group(1): m.group(2)[0] for m in entry.finditer(text)}
     assert len(spills) > 40
     assert not any(spills.values()), [k for k, n in spills.items() if n]
+
+
+def _registers():
+    """{kernel: (accumulation registers, spilled registers)} of the built library, as the compiler notes them:
+    maps with their keys in alphabetical order, .agpr_count first, numbers of up to two bytes."""
+    import re
+    from e_natten_amd import _lib
+
+    def number(b):
+        return b[0] if b[0] < 0x80 else b[1] if b[0] == 0xcc else int.from_bytes(b[1:3], "big")
+
+    found = {}
+    for part in open(_lib.LIB_PATH, "rb").read().split(b".agpr_count")[1:]:
+        name = re.search(rb"\.symbol.{1,3}?(_Z\w+)\.kd", part[:40000], re.S)
+        spilled = re.search(rb"\.vgpr_spill_count(.{3})", part[:40000], re.S)
+        if name and spilled and name.start() < spilled.start():
+            found[name.group(1).decode()] = number(part), number(spilled.group(1))
+    return found
+
+
+def test_kernels_that_spill_have_no_accumulation_registers():
+    """The other half of the rule above: attend_rows spills (50 to 53 registers above 128 channels, 2 in one
+    float32 build), which is sound as long as every spilled register goes to memory, that is as long as the
+    kernel has no accumulation registers.  Every instantiation of the four kernels has to be there."""
+    ensure_built()
+    import re
+    found = _registers()
+    ours = {kind: {n: v for n, v in found.items() if re.match(r"_ZN7enatten12_GLOBAL__N_1%d%sI" % (len(kind), kind), n)}
+            for kind in ("attend", "attend_join", "attend_rows", "join_rows")}
+    # 4 + 3 + 1 numbers of row tiles by head dim, 2 caches, 3 types; float32 above 128 channels has no wide tile
+    assert {kind: len(v) for kind, v in ours.items()} == {"attend": 48, "attend_join": 12, "attend_rows": 16, "join_rows": 8}
+    bad = {n: v for kind in ours.values() for n, v in kind.items() if v[0] and v[1]}
+    assert not bad, bad
+    assert not any(v[0] for v in ours["attend_rows"].values())
+
+
+def test_no_other_kernel_spills_beside_accumulation_registers():
+    """Three builds of the dQ pass with a bias at head_dim 128, 11x11 and 13x13 windows, do: what they spill are
+    single words and pairs, each back in ordinary registers before its use.  A further one has to be read first."""
+    ensure_built()
+    import re
+    beside = {n: v for n, v in _registers().items() if v[0] and v[1]}
+    known = re.compile(r"_ZN7enatten12_GLOBAL__N_112bwd_dq2_mfmaILb[01]ELi128ELi1[13]ELi4ELb0ELb0EEEv")
+    assert len(beside) <= 3 and all(known.match(n) for n in beside), beside
