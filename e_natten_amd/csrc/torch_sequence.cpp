@@ -8,6 +8,10 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <algorithm>
+#include <functional>
+#include <utility>
+
 #include "torch_shim.h"
 
 namespace {
@@ -193,6 +197,43 @@ void validate_cache(const char *what, const char *name, const Tensor &x, const T
     TORCH_CHECK_VALUE(x.size(0) <= 0x7fffffff && x.size(1) <= (1 << 20) && x.size(2) <= 0x7fffffff && x.size(3) <= 256,
                       what, ": head_dim must be a multiple of 16 up to 256, got ", x.size(3));
 }
+// Whether two tensors of the same shape share an element.  Exact where both are dense, and where they have the
+// same strides and these are nested (each longer than all that lies within it), as views of one pool have: the
+// distance of the addresses is then a whole number of each stride, with two choices at most.  Other views whose
+// ranges cross are let pass.
+using Axis = std::pair<int64_t, int64_t>;  // stride, size
+bool is_distance(int64_t distance, const Axis *axes, int n) {  // longest stride first
+    if (n == 0) return distance == 0;
+    int64_t inner = 0;
+    for (int i = 1; i < n; i++) inner += axes[i].first * (axes[i].second - 1);
+    const auto [stride, size] = axes[0];
+    if (stride <= inner) return false;
+    for (int64_t k = distance / stride - 1; k <= distance / stride + 1; k++)
+        if (std::abs(k) < size && std::abs(distance - k * stride) <= inner &&
+            is_distance(distance - k * stride, axes + 1, n - 1))
+            return true;
+    return false;
+}
+bool share_memory(const Tensor &a, const Tensor &b) {
+    const int64_t size = a.element_size();
+    const auto extent = [&](const Tensor &t) {
+        int64_t last = 0;
+        for (int64_t i = 0; i < t.dim(); i++) last += t.stride(i) * (t.size(i) - 1);
+        return (last + 1) * size;
+    };
+    const int64_t distance = static_cast<const char *>(b.data_ptr()) - static_cast<const char *>(a.data_ptr());
+    if (distance >= extent(a) || -distance >= extent(b)) return false;
+    if (a.is_non_overlapping_and_dense() && b.is_non_overlapping_and_dense()) return true;
+    Axis axes[4];
+    int n = 0;
+    for (int64_t i = 0; i < a.dim(); i++) {
+        if (a.size(i) == 1) continue;
+        if (a.stride(i) != b.stride(i)) return false;
+        axes[n++] = {a.stride(i), a.size(i)};
+    }
+    std::sort(axes, axes + n, std::greater<Axis>());
+    return distance % size == 0 && is_distance(distance / size, axes, n);
+}
 void validate_append(const Tensor &k, const Tensor &v, const Tensor &kc, const Tensor &vc, const Tensor &ks,
                      const Tensor &vs, const Tensor &pages, const Tensor &lengths, const optional<Tensor> &counts) {
     const char *what = "cache_append";
@@ -203,7 +244,7 @@ void validate_append(const Tensor &k, const Tensor &v, const Tensor &kc, const T
     TORCH_CHECK_VALUE(kc.size(1) == k.size(1), what, ": k has ", k.size(1), " heads, the cache ", kc.size(1));
     for (const Tensor *t : {&kc, &vc, &ks, &vs}) at::assert_no_internal_overlap(*t);
     TORCH_CHECK_VALUE(!kc.is_same(vc) && !ks.is_same(vs) &&
-                          (kc.is_meta() || (kc.data_ptr() != vc.data_ptr() && ks.data_ptr() != vs.data_ptr())),
+                          (kc.is_meta() || !(share_memory(kc, vc) || share_memory(ks, vs))),
                       what, ": keys and values must not share a cache");
     on_gpu(what, k);
 }

@@ -238,6 +238,37 @@ def _aligned_rows(t):
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def _is_distance(distance, axes):
+    """Whether a distance is a sum of whole numbers of the strides; axes: (stride, size), longest stride first."""
+    if not axes:
+        return distance == 0
+    (stride, size), rest = axes[0], axes[1:]
+    inner = sum(s * (n - 1) for s, n in rest)
+    if stride <= inner:
+        return False
+    near = distance // stride
+    return any(abs(k) < size and abs(distance - k * stride) <= inner and _is_distance(distance - k * stride, rest)
+               for k in (near, near + 1))
+
+
+def _share_memory(a, b):
+    """Whether two tensors of the same shape share an element.  Exact where both are dense, and where they have
+    the same strides and these are nested (each longer than all that lies within it), as views of one pool have:
+    the distance of the addresses is then a whole number of each stride, with two choices at most.  Other views
+    whose ranges cross are let pass."""
+    size = a.element_size()
+    extents = [(1 + sum(s * (n - 1) for s, n in zip(t.stride(), t.shape))) * size for t in (a, b)]
+    distance = b.data_ptr() - a.data_ptr()
+    if distance >= extents[0] or -distance >= extents[1]:
+        return False
+    if all(torch.ops.aten.is_non_overlapping_and_dense(t) for t in (a, b)):
+        return True
+    axes = [(s, r, n) for s, r, n in zip(a.stride(), b.stride(), a.shape) if n > 1]
+    if any(s != r for s, r, _ in axes):
+        return False
+    return distance % size == 0 and _is_distance(distance // size, sorted(((s, n) for s, _, n in axes), reverse=True))
+
+
 def _append_impl(k, v, k_cache, v_cache, k_scale, v_scale, pages, lengths, counts) -> None:
     _validate_cache("k", k, k_cache, v_cache, k_scale, v_scale, pages, lengths, counts)
     if v.shape != k.shape:
@@ -249,7 +280,7 @@ def _append_impl(k, v, k_cache, v_cache, k_scale, v_scale, pages, lengths, count
     for t in (k_cache, v_cache, k_scale, v_scale):
         if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
             raise RuntimeError("the cache must not share memory between its elements")
-    if k_cache.data_ptr() == v_cache.data_ptr() or k_scale.data_ptr() == v_scale.data_ptr():
+    if _share_memory(k_cache, v_cache) or _share_memory(k_scale, v_scale):
         raise ValueError("keys and values must not share a cache")
     _require_gpu(k, "cache_append")
     _no_gradient("cache_append", k, v, k_cache, v_cache, k_scale, v_scale)

@@ -175,6 +175,51 @@ def test_append_refuses(change, text):
             call(*args, **extra)
 
 
+def _pool(*shape, dtype=I8):
+    return torch.zeros(shape, dtype=dtype)
+
+
+_LAYERS = _pool(9, 3, 2, 16, 32)            # pages, layers, heads, tokens, channels
+_PAIRS = _pool(6, 2, 2, 16, 32)             # pages, keys and values, heads, ...
+_TOKENS = _pool(6, 16, 2, 2, 32)            # pages, tokens, keys and values, heads, ...
+_Z = _pool(6, 2, 2, dtype=F32)
+
+
+@pytest.mark.parametrize("shared,change", [
+    (True, dict(k_cache=_LAYERS[:6, 0], v_cache=_LAYERS[3:, 0])),              # some pages of both
+    (False, dict(k_cache=_LAYERS[:6, 0], v_cache=_LAYERS[3:, 1])),             # those of two layers
+    (True, dict(k_cache=_LAYERS[3:, 1], v_cache=_LAYERS[:6, 1])),
+    (True, dict(k_cache=_pool(9, 2, 16, 32)[:6], v_cache=None)),               # (v_cache: the same pool, from page 3)
+    (False, dict(k_cache=_PAIRS[:, 0], v_cache=_PAIRS[:, 1])),
+    (True, dict(k_cache=_pool(6, 3, 16, 32)[:, :2], v_cache=1)),               # (... from head 1)
+    (False, dict(k_cache=_TOKENS[:, :, 0].transpose(1, 2), v_cache=_TOKENS[:, :, 1].transpose(1, 2))),
+    (True, dict(k_cache=_TOKENS[:, :, 0].transpose(1, 2), v_cache=_TOKENS[:, :, 0].transpose(1, 2))),
+    (False, dict(k_cache=_pool(6, 2, 16, 64)[..., :32], v_cache=32)),          # (... from channel 32)
+    (True, dict(k_cache=_pool(6, 2, 16, 64)[..., :32], v_cache=16)),
+    (True, dict(k_scale=_Z[:, 0], v_scale=_Z[:, 0])),
+    (False, dict(k_scale=_Z[:, 0], v_scale=_Z[:, 1])),
+    (True, dict(k_scale=_Z.view(12, 2)[:6], v_scale=_Z.view(12, 2)[5:11])),
+    (False, dict(k_scale=_Z.view(12, 2)[:6], v_scale=_Z.view(12, 2)[6:])),
+    (False, dict(k_scale=_Z[..., 0], v_scale=_Z[..., 1])),
+])
+def test_append_refuses_keys_and_values_that_share_some_memory(shared, change):
+    """Not only the same tensor twice: any element in common; views that lie between each other are fine."""
+    ensure_built()
+    start = change.get("v_cache", 0)
+    if "v_cache" in change and not isinstance(start, torch.Tensor):
+        k = change["k_cache"]
+        offset = {None: 3 * k.stride(0), 1: k.stride(1)}.get(start, start)
+        change = dict(change, v_cache=k.as_strided(k.shape, k.stride(), offset))
+    k, v = (change.get(n) for n in (("k_cache", "v_cache") if "k_cache" in change else ("k_scale", "v_scale")))
+    places = [set((t.storage_offset() + sum((torch.arange(n) * s).view([-1] + [1] * (3 - i)) for i, (n, s) in enumerate(
+        zip((1,) * (4 - t.dim()) + tuple(t.shape), (0,) * (4 - t.dim()) + t.stride())))).flatten().tolist()) for t in (k, v)]
+    assert bool(places[0] & places[1]) == shared and k.untyped_storage().data_ptr() == v.untyped_storage().data_ptr()
+    args, _ = _cache_args("cache_append", **change)
+    for call in _impls("cache_append"):
+        with pytest.raises((ValueError, RuntimeError), match="must not share" if shared else "GPU"):
+            call(*args)
+
+
 def test_kernel_sizes_and_what_is_no_tensor():
     ensure_built()
     from e_natten_amd import cache_append, cache_attention
