@@ -100,7 +100,7 @@ __global__ __launch_bounds__(256, waves_of(DP, R, DT == ENATTEN_F32 ? 2 : 1)) vo
         hi_r[r] = s.start + tv + 1;
         lo_r[r] = a.window ? max(hi_r[r] - a.window, 0) : 0;
         const int64_t at = b * a.q.sb + (head * a.group + row - t * a.group) * a.q.sh + t * a.q.st;
-        float x[KC][16], top = 0.f, nan = 0.f;
+        float x[KC][16], top = 0.f, nan = a.scale * 0.f;
 #pragma unroll
         for (int c = 0; c < KC; c++) {
 #pragma unroll
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256, waves_of(DP, R, DT == ENATTEN_F32 ? 2 : 1)) vo
 #pragma unroll
             for (int j = 0; j < 16; j++) {
                 top = fmaxf(top, fabsf(x[c][j]));
-                nan += x[c][j] * 0.f;  // a value that is not finite makes its row NaN
+                nan += x[c][j] * 0.f;  // a value that is not finite makes its row NaN, a factor all rows
             }
         nan = row_sum(nan);
         top = row_max(top);

@@ -104,7 +104,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
     {
         const int64_t at = b * a.q.sb + (head * a.group + row - t_row * a.group) * a.q.sh + t_row * a.q.st;
         const float flip = a.scale < 0.f ? -1.f : 1.f;  // into q, so that units are not negative
-        float x[SD][8], top = 0.f, nan = 0.f;
+        float x[SD][8], top = 0.f, nan = a.scale * 0.f;
 #pragma unroll
         for (int c = 0; c < SD; c++) {
 #pragma unroll
@@ -116,13 +116,13 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 top = fmaxf(top, fabsf(x[c][j]));
-                nan += x[c][j] * 0.f;  // a value that is not finite makes its row NaN
+                nan += x[c][j] * 0.f;  // a value that is not finite makes its row NaN, a factor all rows
             }
         nan = pair_sum(nan);
         top = pair_max(top);
         const int up = kTop + 1 - (top > 0.f ? __builtin_amdgcn_frexp_expf(top) : 0);
         unit = __builtin_ldexpf(fabsf(a.scale) * kLog2e, -up + (E4M3 ? 8 : 0));
-        l = nan;  // (and stays NaN for a row of q that is not finite)
+        l = nan;  // (and stays NaN for a row of q or a factor that is not finite)
 #pragma unroll
         for (int c = 0; c < SD; c++)
 #pragma unroll

@@ -293,3 +293,18 @@ def test_extreme_scales(dtype):
         n = torch.tensor([500.0, 90.0]).view(2, 1, 1, 1)
         bound = bound + (n * top * 2.0 ** -31).repeat_interleave(2, 1)
         _check(o, ref, bound, dtype, "o, factor %g" % scale)
+
+
+@pytest.mark.parametrize("T,dtype,cache_dtype", [(1, BF16, I8), (1, F32, E4M3), (6, F16, E4M3), (40, BF16, I8),
+                                                 (90, BF16, E4M3), (90, F32, I8)])
+def test_a_factor_that_is_not_finite(T, dtype, cache_dtype):
+    """Logits are no numbers then: NaN for every row that a sequence has, whatever the tile; 0 behind."""
+    ensure_built()
+    from e_natten_amd import cache_attention
+    cache = Cache([150, 100], 2, 32, 64, cache_dtype, seed=T)
+    q = torch.randn((2, 4, T, 64), generator=torch.Generator().manual_seed(3)).to(dtype).cuda()
+    counts = [T, T // 2]
+    for scale in (float("nan"), float("inf"), float("-inf")):
+        o = cache_attention(q, *cache.on("cuda"), _ints([150, 100]), None, scale, _ints(counts))
+        assert torch.isnan(o[0]).all() and torch.isnan(o[1, :, :T // 2]).all(), scale
+        assert not o[1, :, T // 2:].any()
