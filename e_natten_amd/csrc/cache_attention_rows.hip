@@ -315,7 +315,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
                 if ((bad >> g & 1) && first < hi_r && first + 16 > hi_r - seen) l = __uint_as_float(0x7fc00000u);
             }
         }
-        const float unit_z = __builtin_amdgcn_exp2f(ref - kPTop);
+        const int unit_z = (int)ref - kPTop;
         float u[GR], top = kFloor;
 #pragma unroll
         for (int g = 0; g < GR; g++) {
@@ -355,7 +355,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) pf[0][j] = (_Float16)p[j];
                 // (at most 2^40, as the weight is at least 2^-40)
-                l = fmaf(part, fminf(z_lds[buffer][2][g] * unit_z, 0x1p40f), l);
+                l = fmaf(part, fminf(__builtin_ldexpf(z_lds[buffer][2][g], unit_z), 0x1p40f), l);
             } else {
                 l += part;
 #pragma unroll
@@ -402,9 +402,9 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
     __syncthreads();  // (the last step's operands are read: their place is for the rows now)
     {
     const AttnArgs &a = args_again();
-    const float back = __builtin_amdgcn_exp2f(ref - kPTop + (E4M3 ? 8 : 0));
+    const int back = (int)ref - kPTop + (E4M3 ? 8 : 0);
     const float poison = s.ok ? 0.f : __uint_as_float(0x7fc00000u);
-    const float norm = (l == 0.f ? 0.f : 1.f / l) * back;
+    const float norm = l == 0.f ? 0.f : 1.f / l;
     const int row = row0 + n;
     const bool here = row < a.T * a.group, live = here && row / a.group < s.count;
     // 4 neighbouring channels, 4 mm + 128 i: words of one value row, blocks i of O, or for DP 64 rows 16 apart too
@@ -425,7 +425,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
 #pragma unroll
             for (int i = 0; i < BIG; i++)
 #pragma unroll
-                for (int j = 0; j < JS; j++) to[(i * JS + j) * 64] = channels(i, j) * back;
+                for (int j = 0; j < JS; j++) to[(i * JS + j) * 64] = times_power(channels(i, j), back);
         }
     } else if constexpr (DT == ENATTEN_F32) {
         const int t_row = row / a.group;
@@ -435,7 +435,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
 #pragma unroll
             for (int j = 0; j < JS; j++) {
                 const int d = 4 * (j / 4 * 8 + h * 4 + j % 4) + i * 128;
-                if (here && d < a.D) store_channels<DT>(a.o, to + d, (live ? channels(i, j) * norm : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
+                if (here && d < a.D) store_channels<DT>(a.o, to + d, (live ? times_power(channels(i, j) * norm, back) : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
             }
     } else {
         // 64 channels at a time through LDS, so that a store takes whole lines of 8 rows and not pieces of
@@ -449,7 +449,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
                 u32x2 y[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const f32x4 x = (live ? channels(i, q * 8 + j) * norm : f32x4{0.f, 0.f, 0.f, 0.f}) + poison;
+                    const f32x4 x = (live ? times_power(channels(i, q * 8 + j) * norm, back) : f32x4{0.f, 0.f, 0.f, 0.f}) + poison;
                     y[j] = narrow4<DT>(x);
                 }
                 __builtin_amdgcn_wave_barrier();

@@ -308,3 +308,22 @@ def test_a_factor_that_is_not_finite(T, dtype, cache_dtype):
         o = cache_attention(q, *cache.on("cuda"), _ints([150, 100]), None, scale, _ints(counts))
         assert torch.isnan(o[0]).all() and torch.isnan(o[1, :, :T // 2]).all(), scale
         assert not o[1, :, T // 2:].any()
+
+
+@pytest.mark.parametrize("T,dtype,cache_dtype", [(1, BF16, I8), (1, F32, E4M3), (6, F32, I8), (90, BF16, I8),
+                                                 (90, F32, E4M3), (90, BF16, E4M3), (300, F32, I8)])
+def test_values_next_to_the_smallest(T, dtype, cache_dtype):
+    """Value scales from 2^-126, the smallest that cache_append writes, to 2^-119: nothing of them is lost on the
+    way.  Results under 2^-126 are whole multiples of 2^-149 (bfloat16: 2^-133), a rounding there is off by half
+    of that; so are the sums of up to 8 parts and of 4 waves each, in float32."""
+    ensure_built()
+    from e_natten_amd import cache_attention
+    lengths = [1500, 301]
+    cache = Cache(lengths, 2, 32, 64, cache_dtype, seed=T)
+    g = torch.Generator().manual_seed(7)
+    tiny = torch.exp2(-126 + 7 * torch.rand(cache.scales[1].shape, generator=g)).clamp(min=2.0 ** -126)
+    cache.scales[1] = torch.where(torch.isnan(cache.scales[1]), cache.scales[1], tiny)
+    q = torch.randn((2, 4, T, 64), generator=g).to(dtype)
+    o = cache_attention(q.cuda(), *cache.on("cuda"), _ints(lengths), None, 0.2)
+    ref, bound = attention_ref(q, cache, None, None, 0.2)
+    _check(o, ref, bound + 64 * 2.0 ** -150 + (2.0 ** -134 if dtype == BF16 else 0.0), dtype, "o")
