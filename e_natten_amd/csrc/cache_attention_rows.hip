@@ -295,9 +295,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
         }
 
         // lane's tokens: 32 i + 16 g + 8 (j / 4) + 4 h + j % 4 for its 8 values j of a group
-        float cap = INFINITY;
         if (!whole) {
-            if (token >= hi_r || token + TOK <= hi_r - seen) cap = kFloor;  // the row sees none of them
 #pragma unroll
             for (int i = 0; i < NB; i++)
 #pragma unroll
@@ -325,7 +323,6 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
             for (int j = 0; j < 8; j++) most = fmaxf(most, st[g / 2][g % 2 * 8 + j]);
             top = fmaxf(top, most * u[g]);
         }
-        top = fminf(top, cap);
         if (__any(top > m + kSlack)) {
             // (row by row: what other rows see changes nothing here)
             top = pair_max(top);
