@@ -317,10 +317,9 @@ __device__ __forceinline__ bool close(float lz) { return __builtin_amdgcn_readfi
 // What divides the factor out of a sum; 0 for NaN, which the sum of a row that sees such a group has
 // itself, and one that does not is 0.
 __device__ __forceinline__ float inverse_weight(float lz) { return lz == lz ? __builtin_amdgcn_exp2f(-lz) : 0.f; }
-// Four sums back from their weights, 2^e: a product with the power itself would lose what lies under 2^-126.
-__device__ __forceinline__ f32x4 times_power(f32x4 x, int e) {
-    return f32x4{__builtin_ldexpf(x[0], e), __builtin_ldexpf(x[1], e), __builtin_ldexpf(x[2], e), __builtin_ldexpf(x[3], e)};
-}
+// 2^e, also where that is a number under 2^-126 (for which exp2 gives 0): products with it are exact while the
+// result is not under 2^-126 itself.
+__device__ __forceinline__ float power_of_two(float e) { return __builtin_ldexpf(1.f, (int)e); }
 // sum of four float16 values in float32
 __device__ __forceinline__ float sum4(_Float16 a, _Float16 b, _Float16 c, _Float16 d, float more) {
     const f16x2 one = {(_Float16)1.f, (_Float16)1.f};

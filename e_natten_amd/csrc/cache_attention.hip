@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256, waves_of(DP, R, DT == ENATTEN_F32 ? 2 : 1)) vo
 #pragma unroll
             for (int j = 0; j < 16; j++) {
                 top = fmaxf(top, fabsf(x[c][j]));
-                nan += x[c][j] * 0.f;  // a value that is not finite makes its row NaN, a factor all rows
+                nan += x[c][j] * 0.f;  // a value that is not finite makes its row NaN, the factor all rows
             }
         nan = row_sum(nan);
         top = row_max(top);
@@ -351,7 +351,7 @@ __global__ __launch_bounds__(256, waves_of(DP, R, DT == ENATTEN_F32 ? 2 : 1)) vo
     const int rows = min(ROWS, a.T * a.group - row0);
     __shared__ __align__(16) float part_o[4][ROWS][DP + 4];
     __shared__ float part_m[4][ROWS], part_l[4][ROWS];
-    const int back = (int)ref - kPTop + (E4M3 ? 8 : 0);
+    const float back = power_of_two(ref - kPTop + (E4M3 ? 8 : 0));
 #pragma unroll
     for (int r = 0; r < R; r++) {
         const float sum = row_sum(l[r]);
@@ -366,7 +366,7 @@ __global__ __launch_bounds__(256, waves_of(DP, R, DT == ENATTEN_F32 ? 2 : 1)) vo
 #pragma unroll
             for (int c = 0; c < CW; c += 4)
                 *reinterpret_cast<f32x4 *>(&part_o[wave][row][(g4 * 4 + i) * CW + c]) =
-                    times_power(f32x4{acc[r][c][i], acc[r][c + 1][i], acc[r][c + 2][i], acc[r][c + 3][i]}, back);
+                    f32x4{acc[r][c][i], acc[r][c + 1][i], acc[r][c + 2][i], acc[r][c + 3][i]} * back;
     }
     __syncthreads();
     const float poison = s.ok ? 0.f : __uint_as_float(0x7fc00000u);

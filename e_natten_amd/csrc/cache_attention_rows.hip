@@ -104,7 +104,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
     {
         const int64_t at = b * a.q.sb + (head * a.group + row - t_row * a.group) * a.q.sh + t_row * a.q.st;
         const float flip = a.scale < 0.f ? -1.f : 1.f;  // into q, so that units are not negative
-        float x[SD][8], top = 0.f, nan = a.scale * 0.f;
+        float x[SD][8], top = 0.f, nan = 0.f;
 #pragma unroll
         for (int c = 0; c < SD; c++) {
 #pragma unroll
@@ -116,13 +116,13 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 top = fmaxf(top, fabsf(x[c][j]));
-                nan += x[c][j] * 0.f;  // a value that is not finite makes its row NaN, a factor all rows
+                nan += x[c][j] * 0.f;  // a value that is not finite makes its row NaN, the factor all rows
             }
         nan = pair_sum(nan);
         top = pair_max(top);
         const int up = kTop + 1 - (top > 0.f ? __builtin_amdgcn_frexp_expf(top) : 0);
         unit = __builtin_ldexpf(fabsf(a.scale) * kLog2e, -up + (E4M3 ? 8 : 0));
-        l = nan;  // (and stays NaN for a row of q or a factor that is not finite)
+        l = nan + a.scale * 0.f;  // (and stays NaN for a row of q or a factor that is not finite)
 #pragma unroll
         for (int c = 0; c < SD; c++)
 #pragma unroll
@@ -313,7 +313,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
                 if ((bad >> g & 1) && first < hi_r && first + 16 > hi_r - seen) l = __uint_as_float(0x7fc00000u);
             }
         }
-        const int unit_z = (int)ref - kPTop;
+        const float unit_z = power_of_two(ref - kPTop);
         float u[GR], top = kFloor;
 #pragma unroll
         for (int g = 0; g < GR; g++) {
@@ -352,7 +352,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) pf[0][j] = (_Float16)p[j];
                 // (at most 2^40, as the weight is at least 2^-40)
-                l = fmaf(part, fminf(__builtin_ldexpf(z_lds[buffer][2][g], unit_z), 0x1p40f), l);
+                l = fmaf(part, fminf(z_lds[buffer][2][g] * unit_z, 0x1p40f), l);
             } else {
                 l += part;
 #pragma unroll
@@ -399,7 +399,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
     __syncthreads();  // (the last step's operands are read: their place is for the rows now)
     {
     const AttnArgs &a = args_again();
-    const int back = (int)ref - kPTop + (E4M3 ? 8 : 0);
+    const float back = power_of_two(ref - kPTop + (E4M3 ? 8 : 0));
     const float poison = s.ok ? 0.f : __uint_as_float(0x7fc00000u);
     const float norm = l == 0.f ? 0.f : 1.f / l;
     const int row = row0 + n;
@@ -422,7 +422,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
 #pragma unroll
             for (int i = 0; i < BIG; i++)
 #pragma unroll
-                for (int j = 0; j < JS; j++) to[(i * JS + j) * 64] = times_power(channels(i, j), back);
+                for (int j = 0; j < JS; j++) to[(i * JS + j) * 64] = channels(i, j) * back;
         }
     } else if constexpr (DT == ENATTEN_F32) {
         const int t_row = row / a.group;
@@ -432,7 +432,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
 #pragma unroll
             for (int j = 0; j < JS; j++) {
                 const int d = 4 * (j / 4 * 8 + h * 4 + j % 4) + i * 128;
-                if (here && d < a.D) store_channels<DT>(a.o, to + d, (live ? times_power(channels(i, j) * norm, back) : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
+                if (here && d < a.D) store_channels<DT>(a.o, to + d, (live ? channels(i, j) * norm * back : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
             }
     } else {
         // 64 channels at a time through LDS, so that a store takes whole lines of 8 rows and not pieces of
@@ -446,7 +446,7 @@ __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
                 u32x2 y[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const f32x4 x = (live ? times_power(channels(i, q * 8 + j) * norm, back) : f32x4{0.f, 0.f, 0.f, 0.f}) + poison;
+                    const f32x4 x = (live ? channels(i, q * 8 + j) * norm * back : f32x4{0.f, 0.f, 0.f, 0.f}) + poison;
                     y[j] = narrow4<DT>(x);
                 }
                 __builtin_amdgcn_wave_barrier();
