@@ -327,3 +327,21 @@ def test_values_next_to_the_smallest(T, dtype, cache_dtype):
     o = cache_attention(q.cuda(), *cache.on("cuda"), _ints(lengths), None, 0.2)
     ref, bound = attention_ref(q, cache, None, None, 0.2)
     _check(o, ref, bound + 64 * 2.0 ** -150 + (2.0 ** -134 if dtype == BF16 else 0.0), dtype, "o")
+
+
+@pytest.mark.parametrize("N,heads,d,page,dtype,cache_dtype,window", [
+    (4, 2, 256, 32, BF16, I8, None), (4, 2, 256, 32, F16, E4M3, 40), (4, 4, 128, 64, F16, E4M3, None),
+    (6, 2, 64, 16, F32, I8, 90), (2, 2, 128, 48, F32, E4M3, None), (4, 2, 160, 16, F32, I8, None),
+])
+def test_whole_prompts_at_once(N, heads, d, page, dtype, cache_dtype, window):
+    """Nothing stands before the new tokens: the causal triangle alone, over several tiles of 256 rows (16 for
+    float32 above 128 channels) whose first ones see next to nothing; prompts of different lengths, one token."""
+    ensure_built()
+    from e_natten_amd import cache_attention
+    lengths = [600, 257, 1]
+    cache = Cache(lengths, heads, page, d, cache_dtype, seed=d + N)
+    q = (torch.randn((3, N, 600, d), generator=torch.Generator().manual_seed(4)) * 2).to(dtype)
+    o = cache_attention(q.cuda(), *cache.on("cuda"), _ints(lengths), window, d ** -0.5, _ints(lengths))
+    ref, bound = attention_ref(q, cache, lengths, window, d ** -0.5)
+    _check(o, ref, bound, dtype, "o")
+    assert not o[1, :, 257:].any() and not o[2, :, 1:].any()
