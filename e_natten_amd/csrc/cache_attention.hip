@@ -25,17 +25,22 @@
 // of the exponent: log2 of z'_j relative to the largest power of two among the z' so far, and the sums
 // are scaled down where that grows.  The sum of the probabilities is formed of the rounded ones, so that
 // a result stays a mean of values, but for groups whose z' is far below the largest, which float16 drops.
+// The sums are formed before their division, so that a value times 2^8 times the number of tokens has to stay
+// within float32.
 //
 // What bounds it.  One token of a sequence: every code is read once, two products of 16 rows cost a few
 // percent of the matrix cores: HBM.  Work is split along the tokens so that the chip is filled whatever
 // the number of sequences and heads; the parts leave their sums, maximum and output in the workspace and
 // a second launch joins them.  The split goes by the lengths of this call, which are on the device:
 // every workgroup computes it for itself.  Short calls are bound by the two launches and one chain of
-// loads (lengths, pages, codes).
+// loads (lengths, pages, codes), and several rows by what a workgroup takes to get going: five tokens each
+// for 8 sequences of up to 512 tokens, 16 + 2 heads of 64 channels, take 14 us, of which the join is 4.4, and
+// 22 us with 32 times as many codes.
 //
-// Measured on MI355X, heads of 128 channels: 32 sequences of 4096 .. 16384 tokens, 8 heads, E4M3: 142 us
-// (5.7 TB/s; reads alone reach 6.4); 16 + 4 heads, a sequence of 131072 tokens: 33 us; five
-// tokens each for 8 sequences of up to 8192: 21 us; a window of 1024 tokens, one sequence: 5.8 us.
+// Measured on MI355X, heads of 128 channels: 64 sequences of 4160 .. 8192 tokens, 32 + 8 heads, E4M3: 146 us
+// (809 MB, 5.5 TB/s; reads alone reach 6.4), 32 sequences of 8448 .. 16384: 175 us (4.7 TB/s); 32 + 4 heads, a
+// sequence of 131072 tokens, int8: 33 us as a graph, 37 as calls; 16 + 16 heads, one sequence: a window of 128
+// tokens 6 us, of 1024, which is split, 11 us.
 #include "cache_attention.h"
 
 #include <type_traits>
@@ -479,8 +484,9 @@ __global__ __launch_bounds__(256) void attend_join(AttnArgs a) {
 // Rows.  A wave holds q, the sums and the probabilities of all rows of its tile in registers, which
 // leaves room for 64 rows of 64 channels, 48 of 128 and 16 of 256 with two tiles of codes under way.
 // Beyond, tiles of 256 rows over codes that LDS holds as float16; 72 rows of 64 channels over 300 tokens
-// take 14.7 us there and took 33.2 in tiles of 32 here.  float32 rows of more than 128 channels have too
-// many registers for that and stay here.
+// (8 sequences, 2 heads of the cache) take 15 us there and took 33 in tiles of 32 here.  float32 rows of more than
+// 128 channels have too many registers for that and stay here, where every 16 rows read the cache anew: 512
+// tokens each of 16384 and 12288, 16 + 4 heads of 256 channels, take 783 us and 334 in bfloat16.
 // Workgroups.  Two per CU where their registers leave room for two waves per SIMD, else one: with 48 rows
 // of 128 channels a second one per CU only waits.
 Plan plan_of(int B, int heads, int heads_kv, int T, int D, int page, int columns, int window, int dtype) {

@@ -1,8 +1,9 @@
 // cache_attention with many rows per cache head (chunks of prompts): tiles of 256 rows.
 //
-// The mathematics is that of cache_attention.hip.  With this many rows the matrix cores bound the call,
-// so the codes are turned into float16 once for all rows: eight waves take 32 rows each, and go
-// together over steps of 8192 / DP tokens whose keys and values lie in LDS as the operands of
+// The mathematics is that of cache_attention.hip, but that the sum of the probabilities is formed before
+// they are rounded to float16: a result is a mean of values up to that rounding.  With this many rows the
+// matrix cores bound the call, so the codes are turned into float16 once for all rows: eight waves take 32
+// rows each, and go together over steps of 8192 / DP tokens whose keys and values lie in LDS as the operands of
 // v_mfma_f32_32x32x16_f16, in the order in which lanes read them.  Waves 0 to 3 turn keys, 4 to 7
 // values; codes come two steps ahead into registers and are turned into the other half of LDS while the
 // step's products run.
@@ -18,8 +19,10 @@
 // constant and not a selection of exponents.
 //
 // Measured on MI355X, 2048 tokens each of sequences of 16384 and 12288, 16 heads of 128 channels over 4
-// of an int8 cache: 495 us, 900 TFLOP/s; a product of two 8192 x 8192 matrices reaches 1181 in float16.
-// 64 channels: 306 us, 256 channels: 1109 us; 512 new tokens: 151 us, 128: 62 us.
+// of an int8 cache, bfloat16: 490 to 510 us by the card, 880 to 910 TFLOP/s; a product of two 8192 x 8192 matrices
+// reaches 1181 in float16.  64 channels: 327 us, where a logit takes as many vector instructions for half the
+// products; 256 channels: 1135 us, with 50 registers spilled; float32, in two terms: 64 channels 472 us, 128:
+// 825 us.  512 new tokens: 154 us, 128: 62 us; the first 8192 tokens of two prompts (8192 and 8192 long): 760 us.
 #include "cache_attention.h"
 
 #include <type_traits>

@@ -368,9 +368,14 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, kerne
     heads).  Rows from counts[b] on are 0.  float32, bfloat16 and float16.  No gradient.
 
     The products are those of float16 terms, two each for float32, with sums and statistics in float32.
-    A call's work is cut by the lengths of all its sequences, so that another sequence's length may
-    change where a result is rounded; the same call gives the same bits.  A token whose logit is below
-    -6e14 counts for nothing.
+    Weighted values are summed up before the division: one times 256 times the number of tokens has to
+    stay within float32.  A call's work is cut by the lengths of all its sequences, so that another
+    sequence's length may change where a result is rounded; the same call gives the same bits.  A token
+    whose logit is below -6e14 counts for nothing.  A ``scale`` that is not finite gives NaN.
+
+    A float8 cache that :func:`cache_append` wrote holds finite codes only.  The two codes that are no
+    numbers, written there by other means, read as +-480 or as NaN by the queries that see them, by the
+    sizes of the call; queries that do not see them never notice.
     """
     _tensors(q=q, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, pages=pages,
              lengths=lengths)

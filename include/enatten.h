@@ -345,7 +345,8 @@ int enatten_cache_append(const void *k, const void *v, void *k_cache, void *v_ca
  * multiple of heads_kv and head h reads head h / (heads / heads_kv) of the cache.  Query t < counts[b] stands at position
  * p = lengths[b] - counts[b] + t and sees the tokens max(p - kernel_size + 1, 0) .. p, or all up to p
  * with kernel_size 0: the windows of enatten2d_fwd_window's causal axis.  Logits are q.k * scale.
- * o is 0 for t >= counts[b].  A token whose logit is below -6e14 counts for nothing.
+ * o is 0 for t >= counts[b].  A token whose logit is below -6e14 counts for nothing; a scale that is not
+ * finite gives NaN.  A value times 2^8 times the number of tokens has to stay within float32.
  *   workspace  enatten_cache_attention_workspace_bytes() of this call's sizes, 16-byte aligned; may
  *              be NULL if that is 0.  Calls that may overlap need one each.
  */

@@ -462,9 +462,9 @@ def _registers():
 
 
 def test_kernels_that_spill_have_no_accumulation_registers():
-    """The other half of the rule above: attend_rows spills (50 to 53 registers above 128 channels, 2 in one
-    float32 build), which is sound as long as every spilled register goes to memory, that is as long as the
-    kernel has no accumulation registers.  Every instantiation of the four kernels has to be there."""
+    """The other half of the rule above: attend_rows spills above 128 channels (about 50 registers), which is
+    sound as long as every spilled register goes to memory, that is as long as the kernel has no accumulation
+    registers.  Every instantiation of the four kernels has to be there."""
     ensure_built()
     import re
     found = _registers()
