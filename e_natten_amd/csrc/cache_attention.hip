@@ -21,7 +21,8 @@
 //
 // Probabilities go into the second product as float16, at 2^7 for the running maximum.  That maximum is
 // let lag by up to 2^8, so that the sums are seldom rescaled; what is below 2^-21 of the largest (2^-29
-// with the lag) has fewer than 11 bits.  float32 takes two terms.  z'_j goes into them too, as a summand
+// with the lag) has fewer than 11 bits.  float32 takes two terms, 22 bits but no step under 2^-24, so that a
+// probability is off by up to 2^-32 of the largest however small it is.  z'_j goes into them too, as a summand
 // of the exponent: log2 of z'_j relative to the largest power of two among the z' so far, and the sums
 // are scaled down where that grows.  The sum of the probabilities is formed of the rounded ones, so that
 // a result stays a mean of values, but for groups whose z' is far below the largest, which float16 drops.
