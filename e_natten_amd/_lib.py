@@ -45,10 +45,17 @@ SIGNATURES = {
     "enatten1d_bwd": (_i, [_vp] * 10 + [_i] * 6 + [_sp] * 5 + [ctypes.c_float, _vp]),
     "enatten1d_bwd_into": (_i, [_vp] * 10 + [_i] * 6 + [_sp] * 6 + [ctypes.c_float, _vp]),
     "enatten_rotary": (_i, [_vp] * 6 + [_i] * 11 + [_sp] * 4 + [ctypes.c_int64, ctypes.c_double, _vp]),
+    "enatten_rotary_axes": (_i, [_vp] * 7 + [_i] * 12 + [_sp] * 4 + [ctypes.c_int64] * 2 + [ctypes.c_double, _vp]),
     "enatten_cache_append": (_i, [_vp] * 9 + [_i] * 9 + [_sp] * 6 + [ctypes.c_int64, _vp]),
     "enatten_cache_attention_workspace_bytes": (ctypes.c_size_t, [_i] * 9),
     "enatten_cache_attention": (_i, [_vp] * 10 + [_i] * 11 + [_sp] * 6
                                 + [ctypes.c_int64, ctypes.c_float, _vp]),
+    "enatten_cache_fork": (_i, [_vp] * 4 + [_i] * 4 + [ctypes.c_int64, _vp]),
+    "enatten_cache_reserve_workspace_bytes": (ctypes.c_size_t, [_i] * 3),
+    "enatten_cache_reserve": (_i, [_vp] * 3 + [_i] + [_vp] * 3 + [_i] * 4 + [ctypes.c_int64, _vp]),
+    "enatten_cache_copy": (_i, [_vp] * 5 + [_i] * 6 + [_sp] * 4 + [_vp]),
+    "enatten_cache_compact_workspace_bytes": (ctypes.c_size_t, [_i]),
+    "enatten_cache_compact": (_i, [_vp] * 4 + [_i] * 4 + [ctypes.c_int64, _vp]),
     "enatten_profile_enable": (_i, [_i]),
     "enatten_profile_read": (_i, [_i, ctypes.POINTER(_i), ctypes.POINTER(ctypes.c_double)]),
     "enatten_profile_read_overhead": (_i, [_i, ctypes.POINTER(ctypes.c_double)]),
@@ -92,6 +99,11 @@ def strides3(t) -> ctypes.Array:
 def strides2(t) -> ctypes.Array:
     """Element strides of the first two axes as int64_t[2]."""
     return (ctypes.c_int64 * 2)(*t.stride()[:2])
+
+
+def strides(t, axes: int) -> ctypes.Array:
+    """Element strides of the first axes as int64_t[axes]."""
+    return (ctypes.c_int64 * axes)(*t.stride()[:axes])
 
 
 def strides4(t) -> ctypes.Array:

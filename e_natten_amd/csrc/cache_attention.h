@@ -65,20 +65,6 @@ __device__ __forceinline__ Span span_of(const AttnArgs &a, int entry) {
 template <int TOK>
 __device__ __forceinline__ int steps_of(const Span &s) { return s.hi > s.lo ? (s.hi - (s.lo & -16) + TOK - 1) / TOK : 0; }
 
-// Sums over the lanes up to and including each.
-template <int CTRL, int ROW_MASK>
-__device__ __forceinline__ int plus_moved(int x) {
-    return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROW_MASK, 0xf, false);
-}
-__device__ __forceinline__ int running_sum(int x) {
-    x = plus_moved<0x111, 0xf>(x);  // row_shr:1, 2, 4, 8: within 16 lanes
-    x = plus_moved<0x112, 0xf>(x);
-    x = plus_moved<0x114, 0xf>(x);
-    x = plus_moved<0x118, 0xf>(x);
-    x = plus_moved<0x142, 0xa>(x);  // row_bcast:15: lane 15 into the next 16, lane 47 likewise
-    return plus_moved<0x143, 0xc>(x);  // row_bcast:31
-}
-
 // One workgroup's share: some steps of a row tile ("entry").  Entries are cut into items of at most
 // `chunk` steps, about as many items as the call's `parts`; all items are equally long but the last of
 // an entry.  Every wave finds its item from the lengths.

@@ -6,7 +6,8 @@
 // Every value is read and written once and takes three operations, so the kernel is bound by HBM.
 // Sines and cosines depend on the token and the pair alone: a workgroup takes a few tokens, forms
 // their R / 2 turns once into LDS and goes over the heads of both tensors with them.  Nothing is
-// kept between calls, and no table bounds the positions.
+// kept between calls, and no table bounds the positions.  With several axes (an image's rows and columns, a
+// video's time besides) p is the pair's own of a token's positions; an axis that is not there gives NaN.
 //
 // Measured on MI355X: 8 + 8 heads of 64 channels, 4 x 16384 tokens, bfloat16: 56 us where rows lie
 // [token, head] (4.8 TB/s, a plain copy of that size reaches 5.0), 46 us where they lie [head, token];
@@ -22,7 +23,9 @@ namespace {
 struct RotaryArgs {
     Rows x[2], y[2];  // q and k, in and out
     const void *positions, *frequencies;
-    int64_t positions_stride;
+    const int *axes;  // which of num_axes positions turns a pair; nullptr: there is one
+    int64_t positions_stride, axis_stride;
+    int num_axes;
     int heads[2];
     int B, T, D, R;
     bool wide_positions, wide_frequencies, head_first[2];
@@ -63,7 +66,12 @@ __global__ __launch_bounds__(256) void rotary_turn(RotaryArgs a) {
     const int t0 = tile * TOKENS, nt = min(TOKENS, a.T - t0), half = a.R / 2;
     for (int i = threadIdx.x; i < nt * half; i += 256) {
         const int t = i / half, f = i - t * half;
-        const int64_t at = b * a.positions_stride + t0 + t;
+        const int axis = a.axes ? a.axes[f] : 0;
+        if (a.axes && (unsigned)axis >= (unsigned)a.num_axes) {  // (an axis that is not there)
+            table[i] = Turn{(C)NAN, (C)NAN};
+            continue;
+        }
+        const int64_t at = axis * a.axis_stride + b * a.positions_stride + t0 + t;
         const double p = a.wide_positions ? (double)static_cast<const int64_t *>(a.positions)[at]
                                           : (double)static_cast<const int *>(a.positions)[at];
         const double w = a.wide_frequencies ? static_cast<const double *>(a.frequencies)[f]
@@ -194,15 +202,13 @@ int launch_type(const char *fn, RotaryArgs &a, bool interleaved, hipStream_t st)
 
 using namespace enatten;
 
-extern "C" {
-#pragma GCC visibility push(default)
-
-int enatten_rotary(const void *q, const void *k, void *q_out, void *k_out, const void *positions,
-                   const void *frequencies, int B, int heads_q, int heads_k, int T, int D, int R, int dtype,
-                   int positions_dtype, int frequencies_dtype, int interleaved, int inverse,
-                   const int64_t *q_strides, const int64_t *k_strides, const int64_t *q_out_strides,
-                   const int64_t *k_out_strides, int64_t positions_stride, double scale, void *stream) {
-    const char *fn = "enatten_rotary";
+// axes: nullptr for one position per token
+static int rotary_entry(const char *fn, const void *q, const void *k, void *q_out, void *k_out, const void *positions,
+                        const void *frequencies, const int *axes, int num_axes, int B, int heads_q, int heads_k, int T,
+                        int D, int R, int dtype, int positions_dtype, int frequencies_dtype, int interleaved,
+                        int inverse, const int64_t *q_strides, const int64_t *k_strides,
+                        const int64_t *q_out_strides, const int64_t *k_out_strides, int64_t positions_stride,
+                        int64_t axis_stride, double scale, void *stream) {
     if (dtype != ENATTEN_F32 && dtype != ENATTEN_BF16 && dtype != ENATTEN_F16 && dtype != ENATTEN_F64) {
         set_error("%s: unknown dtype code %d (expected ENATTEN_F32/BF16/F16/F64)", fn, dtype);
         return ENATTEN_EINVAL;
@@ -244,6 +250,9 @@ int enatten_rotary(const void *q, const void *k, void *q_out, void *k_out, const
     a.positions = positions;
     a.frequencies = frequencies;
     a.positions_stride = positions_stride;
+    a.axes = axes;
+    a.num_axes = num_axes;
+    a.axis_stride = axis_stride;
     a.wide_positions = positions_dtype == ENATTEN_I64;
     a.wide_frequencies = frequencies_dtype == ENATTEN_F64;
     a.B = B; a.T = T; a.D = D; a.R = R;
@@ -256,6 +265,35 @@ int enatten_rotary(const void *q, const void *k, void *q_out, void *k_out, const
         case ENATTEN_F16: return launch_type<_Float16>(fn, a, interleaved, st);
         default: return launch_type<double>(fn, a, interleaved, st);
     }
+}
+
+extern "C" {
+#pragma GCC visibility push(default)
+
+int enatten_rotary(const void *q, const void *k, void *q_out, void *k_out, const void *positions,
+                   const void *frequencies, int B, int heads_q, int heads_k, int T, int D, int R, int dtype,
+                   int positions_dtype, int frequencies_dtype, int interleaved, int inverse,
+                   const int64_t *q_strides, const int64_t *k_strides, const int64_t *q_out_strides,
+                   const int64_t *k_out_strides, int64_t positions_stride, double scale, void *stream) {
+    return rotary_entry("enatten_rotary", q, k, q_out, k_out, positions, frequencies, nullptr, 1, B, heads_q, heads_k, T,
+                        D, R, dtype, positions_dtype, frequencies_dtype, interleaved, inverse, q_strides, k_strides,
+                        q_out_strides, k_out_strides, positions_stride, 0, scale, stream);
+}
+
+int enatten_rotary_axes(const void *q, const void *k, void *q_out, void *k_out, const void *positions,
+                        const void *frequencies, const int *axes, int num_axes, int B, int heads_q, int heads_k, int T,
+                        int D, int R, int dtype, int positions_dtype, int frequencies_dtype, int interleaved,
+                        int inverse, const int64_t *q_strides, const int64_t *k_strides,
+                        const int64_t *q_out_strides, const int64_t *k_out_strides, int64_t positions_stride,
+                        int64_t axis_stride, double scale, void *stream) {
+    const char *fn = "enatten_rotary_axes";
+    if (!axes || num_axes < 1 || axis_stride < 0) {
+        set_error("%s: axes must not be NULL, there is one at least, and their stride is not negative", fn);
+        return ENATTEN_EINVAL;
+    }
+    return rotary_entry(fn, q, k, q_out, k_out, positions, frequencies, axes, num_axes, B, heads_q, heads_k, T, D, R,
+                        dtype, positions_dtype, frequencies_dtype, interleaved, inverse, q_strides, k_strides,
+                        q_out_strides, k_out_strides, positions_stride, axis_stride, scale, stream);
 }
 
 #pragma GCC visibility pop

@@ -37,6 +37,20 @@ __device__ __forceinline__ bool sequence_of(const Table &tb, int b, int &len, in
     return ok;
 }
 
+// Sums over the lanes up to and including each.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ int plus_moved(int x) {
+    return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROW_MASK, 0xf, false);
+}
+__device__ __forceinline__ int running_sum(int x) {
+    x = plus_moved<0x111, 0xf>(x);  // row_shr:1, 2, 4, 8: within 16 lanes
+    x = plus_moved<0x112, 0xf>(x);
+    x = plus_moved<0x114, 0xf>(x);
+    x = plus_moved<0x118, 0xf>(x);
+    x = plus_moved<0x142, 0xa>(x);  // row_bcast:15: lane 15 into the next 16, lane 47 likewise
+    return plus_moved<0x143, 0xc>(x);  // row_bcast:31
+}
+
 inline int set_rows(const char *fn, const char *name, const void *p, const int64_t *st, int heads, int T, int D,
                     Rows *out) {
     if (!p) {

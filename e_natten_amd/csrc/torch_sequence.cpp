@@ -1,10 +1,9 @@
 // Native torch binding of the operators of growing sequences: enatten::rotary (differentiable, any
 // number of times), enatten::cache_append and enatten::cache_attention.  Host code only; the checks and
-// error classes are those of the Python host side (sequence.py).
+// error classes are those of the Python host side (sequence.py).  Pages: torch_pages.cpp.
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
@@ -21,17 +20,10 @@ using c10::optional;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-void on_gpu(const char *what, const Tensor &t) {
-    TORCH_CHECK(t.is_cuda() || t.is_meta(), what, ": tensors must be on the GPU; this build has no CPU path");
-}
-void *stream_now() { return c10::hip::getCurrentHIPStream().stream(); }
-// A tangent of forward mode.  A tensor can have one without requires_grad and in every grad mode: calls that
-// make no node look for it themselves.
-bool has_tangent(const Tensor &t) { return t._fw_grad(/*level=*/0).defined(); }
-
 // ---- rotary ----------------------------------------------------------------
 
-void validate_rotary(const Tensor &q, const optional<Tensor> &k, const Tensor &positions, const Tensor &frequencies) {
+void validate_rotary(const Tensor &q, const optional<Tensor> &k, const Tensor &positions, const Tensor &frequencies,
+                     const optional<Tensor> &axes) {
     const char *what = "rotary";
     TORCH_CHECK_VALUE(q.dim() == 4, what, ": expected [B, heads, T, head_dim] tensors, got ", q.dim(), "-D q");
     TORCH_CHECK_VALUE(dtype_code(q) >= 0, what, ": dtype ", q.scalar_type(),
@@ -46,21 +38,28 @@ void validate_rotary(const Tensor &q, const optional<Tensor> &k, const Tensor &p
     }
     TORCH_CHECK_VALUE(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong, what,
                       ": positions must be int32 or int64, got ", positions.scalar_type());
-    TORCH_CHECK_VALUE((positions.dim() == 1 || (positions.dim() == 2 && (positions.size(0) == q.size(0) || positions.size(0) == 1))) &&
-                          positions.size(-1) == q.size(2),
-                      what, ": positions must have shape [T] or [B, T], got ", positions.sizes());
+    const int64_t lead = axes.has_value();  // (the axes come first)
+    TORCH_CHECK_VALUE((positions.dim() == lead + 1 || (positions.dim() == lead + 2 && (positions.size(lead) == q.size(0) ||
+                                                                                       positions.size(lead) == 1))) &&
+                          positions.size(-1) == q.size(2) && positions.size(0) > 0,
+                      what, ": positions must have shape [T] or [B, T]", lead ? " for every axis" : "", ", got ",
+                      positions.sizes());
     TORCH_CHECK_VALUE(frequencies.scalar_type() == at::kFloat || frequencies.scalar_type() == at::kDouble, what,
                       ": frequencies must be float32 or float64, got ", frequencies.scalar_type());
     TORCH_CHECK_VALUE(frequencies.dim() == 1 && frequencies.size(0) > 0 && 2 * frequencies.size(0) <= q.size(3), what,
                       ": frequencies must be one for every rotated pair, at most head_dim / 2, got ", frequencies.sizes());
+    TORCH_CHECK_VALUE(!axes.has_value() || (axes->scalar_type() == at::kInt && axes->sizes() == frequencies.sizes()), what,
+                      ": axes must be int32, one for every frequency, got ", axes.has_value() ? axes->sizes() : q.sizes());
     TORCH_CHECK_VALUE(q.size(0) <= 0x7fffffff && q.size(1) <= (1 << 20) && q.size(2) <= 0x7fffffff &&
-                          (!k.has_value() || k->size(1) <= (1 << 20)),
+                          (!k.has_value() || k->size(1) <= (1 << 20)) &&
+                          (!axes.has_value() || positions.size(0) <= 0x7fffffff),
                       what, ": tensor too large");
     TORCH_CHECK_VALUE(q.size(3) <= 1024, what, ": head_dim ", q.size(3), " exceeds the supported maximum of 1024");
     TORCH_CHECK(!at::GradMode::is_enabled() || !frequencies.requires_grad(), what,
                 ": frequencies have no gradient; call it on detached ones");
     TORCH_CHECK_VALUE(positions.device() == q.device() && frequencies.device() == q.device(), what,
                       ": positions and frequencies must be on the device of q");
+    TORCH_CHECK_VALUE(!axes.has_value() || axes->device() == q.device(), what, ": axes must be on the device of q");
     on_gpu(what, q);
 }
 
@@ -68,8 +67,9 @@ void validate_rotary(const Tensor &q, const optional<Tensor> &k, const Tensor &p
 Tensor empty_rows(const Tensor &x) { return kernel_layout(at::empty_like(x)); }
 
 std::vector<Tensor> rotary_turn(const Tensor &q_, const optional<Tensor> &k_, const Tensor &positions_,
-                                const Tensor &frequencies_, bool interleaved, double scale, bool inverse) {
-    validate_rotary(q_, k_, positions_, frequencies_);
+                                const Tensor &frequencies_, bool interleaved, double scale, bool inverse,
+                                const optional<Tensor> &axes_) {
+    validate_rotary(q_, k_, positions_, frequencies_, axes_);
     const bool two = k_.has_value();
     std::vector<Tensor> out;
     if (q_.is_meta()) {
@@ -83,28 +83,44 @@ std::vector<Tensor> rotary_turn(const Tensor &q_, const optional<Tensor> &k_, co
     const Tensor frequencies = frequencies_.contiguous();
     out.push_back(empty_rows(q));
     if (two) out.push_back(empty_rows(k));
-    check_rc(enatten_rotary(
-        q.data_ptr(), two ? k.data_ptr() : nullptr, out[0].data_ptr(), two ? out[1].data_ptr() : nullptr,
-        positions.data_ptr(), frequencies.data_ptr(), q.size(0), q.size(1), two ? k.size(1) : 0, q.size(2), q.size(3),
-        2 * frequencies.size(0), dtype_code(q), positions.scalar_type() == at::kInt ? ENATTEN_I32 : ENATTEN_I64,
-        frequencies.scalar_type() == at::kFloat ? ENATTEN_F32 : ENATTEN_F64, interleaved, inverse, q.strides().data(),
-        two ? k.strides().data() : nullptr, out[0].strides().data(), two ? out[1].strides().data() : nullptr,
-        positions.dim() == 2 && positions.size(0) > 1 ? positions.stride(0) : 0, scale, stream_now()));
+    const int64_t lead = axes_.has_value();
+    const int64_t positions_stride = positions.dim() == lead + 2 && positions.size(lead) > 1 ? positions.stride(lead) : 0;
+    const int code = dtype_code(q), positions_code = positions.scalar_type() == at::kInt ? ENATTEN_I32 : ENATTEN_I64;
+    const int frequencies_code = frequencies.scalar_type() == at::kFloat ? ENATTEN_F32 : ENATTEN_F64;
+    const void *k_in = two ? k.data_ptr() : nullptr;
+    void *k_out = two ? out[1].data_ptr() : nullptr;
+    const int64_t *k_strides = two ? k.strides().data() : nullptr, *k_out_strides = two ? out[1].strides().data() : nullptr;
+    const int64_t k_heads = two ? k.size(1) : 0;
+    if (axes_.has_value()) {
+        const Tensor axes = axes_->contiguous();
+        check_rc(enatten_rotary_axes(
+            q.data_ptr(), k_in, out[0].data_ptr(), k_out, positions.data_ptr(), frequencies.data_ptr(), axes.data_ptr<int>(),
+            positions.size(0), q.size(0), q.size(1), k_heads, q.size(2), q.size(3), 2 * frequencies.size(0), code,
+            positions_code, frequencies_code, interleaved, inverse, q.strides().data(), k_strides, out[0].strides().data(),
+            k_out_strides, positions_stride, positions.stride(0), scale, stream_now()));
+        return out;
+    }
+    check_rc(enatten_rotary(q.data_ptr(), k_in, out[0].data_ptr(), k_out, positions.data_ptr(), frequencies.data_ptr(),
+                            q.size(0), q.size(1), k_heads, q.size(2), q.size(3), 2 * frequencies.size(0), code,
+                            positions_code, frequencies_code, interleaved, inverse, q.strides().data(), k_strides,
+                            out[0].strides().data(), k_out_strides, positions_stride, scale, stream_now()));
     return out;
 }
 
 using RotarySig = std::vector<Tensor>(const Tensor &, const optional<Tensor> &, const Tensor &, const Tensor &, bool,
-                                      double, bool);
+                                      double, bool, const optional<Tensor> &);
 // (through the dispatcher: tracers see one operator)
 std::vector<Tensor> call_turn(const Tensor &q, const optional<Tensor> &k, const Tensor &positions,
-                              const Tensor &frequencies, bool interleaved, double scale, bool inverse) {
+                              const Tensor &frequencies, bool interleaved, double scale, bool inverse,
+                              const optional<Tensor> &axes) {
     static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("enatten::rotary_turn", "").typed<RotarySig>();
-    return op.call(q, k, positions, frequencies, interleaved, scale, inverse);
+    return op.call(q, k, positions, frequencies, interleaved, scale, inverse, axes);
 }
 std::vector<Tensor> call_rotary(const Tensor &q, const optional<Tensor> &k, const Tensor &positions,
-                                const Tensor &frequencies, bool interleaved, double scale, bool inverse) {
+                                const Tensor &frequencies, bool interleaved, double scale, bool inverse,
+                                const optional<Tensor> &axes) {
     static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("enatten::rotary", "").typed<RotarySig>();
-    return op.call(q, k, positions, frequencies, interleaved, scale, inverse);
+    return op.call(q, k, positions, frequencies, interleaved, scale, inverse, axes);
 }
 
 // The gradient is the turn the other way round of the upstream gradients: the same operator, so that it
@@ -112,14 +128,14 @@ std::vector<Tensor> call_rotary(const Tensor &q, const optional<Tensor> &k, cons
 struct RotaryFn : public torch::autograd::Function<RotaryFn> {
     static variable_list forward(AutogradContext *ctx, const Tensor &q, const optional<Tensor> &k,
                                  const Tensor &positions, const Tensor &frequencies, bool interleaved, double scale,
-                                 bool inverse) {
+                                 bool inverse, const optional<Tensor> &axes) {
         at::AutoDispatchBelowADInplaceOrView below;
-        ctx->save_for_backward({positions, frequencies});
+        ctx->save_for_backward({positions, frequencies, axes.has_value() ? *axes : Tensor()});
         ctx->saved_data["interleaved"] = interleaved;
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["inverse"] = inverse;
         ctx->set_materialize_grads(false);
-        return call_turn(q, k, positions, frequencies, interleaved, scale, inverse);
+        return call_turn(q, k, positions, frequencies, interleaved, scale, inverse, axes);
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         const variable_list s = ctx->get_saved_variables();
@@ -130,34 +146,33 @@ struct RotaryFn : public torch::autograd::Function<RotaryFn> {
         if (grads[0].defined() || two) {
             const Tensor &first = grads[0].defined() ? grads[0] : grads[1];
             const optional<Tensor> second = grads[0].defined() && two ? optional<Tensor>(grads[1]) : c10::nullopt;
-            const auto out = call_rotary(first, second, s[0], s[1], interleaved, scale, !inverse);
+            const optional<Tensor> axes = s[2].defined() ? optional<Tensor>(s[2]) : c10::nullopt;
+            const auto out = call_rotary(first, second, s[0], s[1], interleaved, scale, !inverse, axes);
             (grads[0].defined() ? dq : dk) = out[0];
             if (second.has_value()) dk = out[1];
         }
-        return {dq, dk, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        return {dq, dk, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
 std::vector<Tensor> rotary_autograd(const Tensor &q, const optional<Tensor> &k, const Tensor &positions,
-                                    const Tensor &frequencies, bool interleaved, double scale, bool inverse) {
+                                    const Tensor &frequencies, bool interleaved, double scale, bool inverse,
+                                    const optional<Tensor> &axes) {
     TORCH_CHECK(!has_tangent(q) && !(k.has_value() && has_tangent(*k)) && !has_tangent(frequencies),
                 "rotary: there is no forward-mode derivative; gradients come by the backward pass");
     if (!at::GradMode::is_enabled() || !(q.requires_grad() || (k.has_value() && k->requires_grad()))) {
         at::AutoDispatchBelowADInplaceOrView below;  // (no node: inference)
-        return call_turn(q, k, positions, frequencies, interleaved, scale, inverse);
+        return call_turn(q, k, positions, frequencies, interleaved, scale, inverse, axes);
     }
-    validate_rotary(q, k, positions, frequencies);
-    return RotaryFn::apply(q, k, positions, frequencies, interleaved, scale, inverse);
+    validate_rotary(q, k, positions, frequencies, axes);
+    return RotaryFn::apply(q, k, positions, frequencies, interleaved, scale, inverse, axes);
 }
 std::vector<Tensor> rotary_plain(const Tensor &q, const optional<Tensor> &k, const Tensor &positions,
-                                 const Tensor &frequencies, bool interleaved, double scale, bool inverse) {
-    return call_turn(q, k, positions, frequencies, interleaved, scale, inverse);
+                                 const Tensor &frequencies, bool interleaved, double scale, bool inverse,
+                                 const optional<Tensor> &axes) {
+    return call_turn(q, k, positions, frequencies, interleaved, scale, inverse, axes);
 }
 
 // ---- cache -----------------------------------------------------------------
-
-int cache_code(const Tensor &t) {
-    return t.scalar_type() == at::kChar ? ENATTEN_I8 : t.scalar_type() == at::kFloat8_e4m3fn ? ENATTEN_E4M3 : -1;
-}
 
 // x: q, or k of new tokens
 void validate_cache(const char *what, const char *name, const Tensor &x, const Tensor &kc, const Tensor &vc,
@@ -304,14 +319,6 @@ Tensor cache_attention(const Tensor &q_, const Tensor &kc, const Tensor &vc, con
     return o;
 }
 
-// Codes are rounded: neither operator has a gradient, and a caller that would get none is told so.
-void no_gradient(const char *what, std::initializer_list<const Tensor *> inputs) {
-    const bool mode = at::GradMode::is_enabled();
-    for (const Tensor *t : inputs)
-        TORCH_CHECK(!(mode && t->requires_grad()) && !has_tangent(*t), what,
-                    ": a cache of 8 bits has no gradient; call it under torch.no_grad() or on detached tensors, which "
-                    "have no tangent");
-}
 using AppendSig = decltype(cache_append);
 void call_append(const Tensor &k, const Tensor &v, const Tensor &kc, const Tensor &vc, const Tensor &ks,
                  const Tensor &vs, const Tensor &pages, const Tensor &lengths, const optional<Tensor> &counts) {
@@ -348,9 +355,9 @@ Tensor cache_attention_autograd(const Tensor &q, const Tensor &kc, const Tensor 
 
 TORCH_LIBRARY_FRAGMENT(enatten, m) {
     m.def("rotary_turn(Tensor q, Tensor? k, Tensor positions, Tensor frequencies, bool interleaved, float scale, "
-          "bool inverse) -> Tensor[]");
+          "bool inverse, Tensor? axes=None) -> Tensor[]");
     m.def("rotary(Tensor q, Tensor? k, Tensor positions, Tensor frequencies, bool interleaved, float scale, "
-          "bool inverse) -> Tensor[]");
+          "bool inverse, Tensor? axes=None) -> Tensor[]");
     m.def("cache_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scale, "
           "Tensor(d!) v_scale, Tensor pages, Tensor lengths, Tensor? counts) -> ()");
     m.def("cache_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor pages, "

@@ -2,6 +2,7 @@
 #pragma once
 
 #include <ATen/ATen.h>
+#include <c10/hip/HIPStream.h>
 
 #include "enatten.h"
 
@@ -21,6 +22,25 @@ inline int dtype_code(const at::Tensor &t) {
 // channel axis.
 inline at::Tensor kernel_layout(const at::Tensor &t) {
     return (t.stride(-1) != 1 && t.size(-1) != 1) ? t.contiguous() : t;
+}
+
+inline void on_gpu(const char *what, const at::Tensor &t) {
+    TORCH_CHECK(t.is_cuda() || t.is_meta(), what, ": tensors must be on the GPU; this build has no CPU path");
+}
+inline void *stream_now() { return c10::hip::getCurrentHIPStream().stream(); }
+// A tangent of forward mode.  A tensor can have one without requires_grad and in every grad mode: calls that
+// make no node look for it themselves.
+inline bool has_tangent(const at::Tensor &t) { return t._fw_grad(/*level=*/0).defined(); }
+// Codes are rounded: the operators of a cache have no gradient, and a caller that would get none is told so.
+inline void no_gradient(const char *what, std::initializer_list<const at::Tensor *> inputs) {
+    const bool mode = at::GradMode::is_enabled();
+    for (const at::Tensor *t : inputs)
+        TORCH_CHECK(!(mode && t->requires_grad()) && !has_tangent(*t), what,
+                    ": a cache of 8 bits has no gradient; call it under torch.no_grad() or on detached tensors, which "
+                    "have no tangent");
+}
+inline int cache_code(const at::Tensor &t) {
+    return t.scalar_type() == at::kChar ? ENATTEN_I8 : t.scalar_type() == at::kFloat8_e4m3fn ? ENATTEN_E4M3 : -1;
 }
 
 inline void check_rc(int rc) {

@@ -94,7 +94,7 @@ def _rows(name, x, dtypes):
 
 # --- rotary ---
 
-def _validate_rotary(q, k, positions, frequencies) -> None:
+def _validate_rotary(q, k, positions, frequencies, axes) -> None:
     _rows("q", q, _DTYPES)
     if k is not None:
         if k.dim() != 4 or k.shape[1] < 1 or k.shape[::2] != q.shape[::2] or k.shape[3] != q.shape[3]:
@@ -107,21 +107,29 @@ def _validate_rotary(q, k, positions, frequencies) -> None:
             raise ValueError("q and k must be on the same device")
     if positions.dtype not in (torch.int32, torch.int64):
         raise ValueError("positions must be int32 or int64, got %s" % positions.dtype)
-    if tuple(positions.shape) not in ((q.shape[2],), (1, q.shape[2]), (q.shape[0], q.shape[2])):
-        raise ValueError("positions must have shape [T] or [B, T], got %s" % (tuple(positions.shape),))
+    shape = tuple(positions.shape) if axes is None else tuple(positions.shape[1:])
+    if shape not in ((q.shape[2],), (1, q.shape[2]), (q.shape[0], q.shape[2])) or positions.shape[0] < 1:
+        raise ValueError("positions must have shape [T] or [B, T]%s, got %s"
+                         % ("" if axes is None else " for every axis", tuple(positions.shape)))
     if frequencies.dtype not in (torch.float32, torch.float64):
         raise ValueError("frequencies must be float32 or float64, got %s" % frequencies.dtype)
     if frequencies.dim() != 1 or not 0 < 2 * frequencies.shape[0] <= q.shape[3]:
         raise ValueError("frequencies must be one for every rotated pair, at most head_dim / 2, got %s"
                          % (tuple(frequencies.shape),))
+    if axes is not None and (axes.dtype != torch.int32 or axes.shape != frequencies.shape):
+        raise ValueError("axes must be int32, one for every frequency, got %s %s" % (axes.dtype, tuple(axes.shape)))
+    if axes is not None and positions.shape[0] > 0x7fffffff:
+        raise ValueError("tensor too large")
     if q.shape[3] > 1024:
         raise ValueError("head_dim %d exceeds the supported maximum of 1024" % q.shape[3])
     if positions.device != q.device or frequencies.device != q.device:
         raise ValueError("positions and frequencies must be on the device of q")
+    if axes is not None and axes.device != q.device:
+        raise ValueError("axes must be on the device of q")
 
 
-def _rotary_impl(q, k, positions, frequencies, interleaved: bool, scale: float, inverse: bool):
-    _validate_rotary(q, k, positions, frequencies)
+def _rotary_impl(q, k, positions, frequencies, interleaved: bool, scale: float, inverse: bool, axes=None):
+    _validate_rotary(q, k, positions, frequencies, axes)
     _require_gpu(q, "rotary")
     lib = _lib.load()
     xs = [_kernel_layout(t) for t in ((q,) if k is None else (q, k))]
@@ -132,15 +140,20 @@ def _rotary_impl(q, k, positions, frequencies, interleaved: bool, scale: float, 
         ys = [_kernel_layout(torch.empty_like(x)) for x in xs]
         x2, y2 = (xs[1], ys[1]) if k is not None else (None, None)
         B, N, T, D = q.shape
-        _check(lib.enatten_rotary(
-            xs[0].data_ptr(), x2 if x2 is None else x2.data_ptr(), ys[0].data_ptr(),
-            y2 if y2 is None else y2.data_ptr(), positions.data_ptr(), frequencies.data_ptr(), B, N,
-            0 if k is None else k.shape[1], T, D, 2 * frequencies.shape[0], _DTYPES[q.dtype],
-            _lib.I32 if positions.dtype == torch.int32 else _lib.I64, _DTYPES[frequencies.dtype],
-            int(interleaved), int(inverse), _lib.strides3(xs[0]), None if x2 is None else _lib.strides3(x2),
-            _lib.strides3(ys[0]), None if y2 is None else _lib.strides3(y2),
-            positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0, float(scale),
-            _stream_of(q)))
+        each = positions if axes is None else positions[0]
+        data = (xs[0].data_ptr(), x2 if x2 is None else x2.data_ptr(), ys[0].data_ptr(),
+                y2 if y2 is None else y2.data_ptr(), positions.data_ptr(), frequencies.data_ptr())
+        sizes = (B, N, 0 if k is None else k.shape[1], T, D, 2 * frequencies.shape[0], _DTYPES[q.dtype],
+                 _lib.I32 if positions.dtype == torch.int32 else _lib.I64, _DTYPES[frequencies.dtype],
+                 int(interleaved), int(inverse), _lib.strides3(xs[0]), None if x2 is None else _lib.strides3(x2),
+                 _lib.strides3(ys[0]), None if y2 is None else _lib.strides3(y2),
+                 each.stride(0) if each.dim() == 2 and each.shape[0] > 1 else 0)
+        if axes is None:
+            _check(lib.enatten_rotary(*data, *sizes, float(scale), _stream_of(q)))
+        else:
+            axes = axes.contiguous()
+            _check(lib.enatten_rotary_axes(*data, axes.data_ptr(), positions.shape[0], *sizes, positions.stride(0),
+                                           float(scale), _stream_of(q)))
     return ys
 
 
@@ -148,11 +161,11 @@ class Rotary(torch.autograd.Function):
     """(q, k) -> (q', k') with k None or a tensor; the gradient is the turn the other way round."""
 
     @staticmethod
-    def forward(ctx, q, k, positions, frequencies, interleaved, scale, inverse):
-        ctx.save_for_backward(positions, frequencies)
+    def forward(ctx, q, k, positions, frequencies, interleaved, scale, inverse, axes=None):
+        ctx.save_for_backward(positions, frequencies, axes)
         ctx.args = (interleaved, scale, inverse)
         ctx.set_materialize_grads(False)
-        return tuple(_rotary_impl(q, k, positions, frequencies, interleaved, scale, inverse))
+        return tuple(_rotary_impl(q, k, positions, frequencies, interleaved, scale, inverse, axes))
 
     @staticmethod
     def backward(ctx, *grads):
@@ -160,13 +173,46 @@ class Rotary(torch.autograd.Function):
         there = [g for g in grads if g is not None]
         out = iter(())
         if there:
-            out = iter(Rotary.apply(there[0], there[1] if len(there) > 1 else None, *ctx.saved_tensors,
-                                    interleaved, scale, not inverse))
+            positions, frequencies, axes = ctx.saved_tensors
+            out = iter(Rotary.apply(there[0], there[1] if len(there) > 1 else None, positions, frequencies,
+                                    interleaved, scale, not inverse, axes))
         dq, dk = (next(out) if i < len(grads) and grads[i] is not None else None for i in range(2))
-        return dq, dk, None, None, None, None, None
+        return dq, dk, None, None, None, None, None, None
 
 
-def rotary(q, k, positions, frequencies, interleaved=False, scale=1.0):
+def rotary_axes(rotary_dim, axes, order="blocks", device=None):
+    """Which of a token's ``axes`` positions turns each of the ``rotary_dim / 2`` pairs, for :func:`rotary`.
+
+    ``axes``  how many there are, or a list with the number of pairs of each.  With a number the pairs are
+              shared out evenly, the first axes taking one more where that leaves a rest.
+    ``order``  ``"blocks"``: the pairs of an axis are neighbours, in the order of the axes; ``"cyclic"``: the
+              axes take turns, 0, 1, ..., 0, 1, ..., and one whose pairs are used up is passed over.
+    """
+    if not isinstance(rotary_dim, int) or isinstance(rotary_dim, bool):
+        raise TypeError("rotary_dim must be an int")
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be even and >= 2, got %d" % rotary_dim)
+    if order not in ("blocks", "cyclic"):
+        raise ValueError("order must be 'blocks' or 'cyclic', got %r" % (order,))
+    pairs = rotary_dim // 2
+    if isinstance(axes, int) and not isinstance(axes, bool):
+        if axes < 1:
+            raise ValueError("there must be one axis at least, got %d" % axes)
+        sizes = [pairs // axes + (a < pairs % axes) for a in range(axes)]
+    else:
+        sizes = list(axes)
+        if any(not isinstance(n, int) or isinstance(n, bool) for n in sizes):
+            raise TypeError("axes must be an int, or the number of pairs of each axis")
+    if not sizes or min(sizes) < 0 or sum(sizes) != pairs:
+        raise ValueError("the axes' pairs must add up to %d, got %r" % (pairs, sizes))
+    if order == "blocks":
+        which = [a for a, n in enumerate(sizes) for _ in range(n)]
+    else:
+        which = [a for i in range(max(sizes)) for a, n in enumerate(sizes) if i < n]
+    return torch.tensor(which, dtype=torch.int32, device=device)
+
+
+def rotary(q, k, positions, frequencies, interleaved=False, scale=1.0, axes=None):
     """Rotary positions: ``(q', k')`` of ``q [B, heads, T, d]`` and ``k [B, heads_k, T, d]`` (or None,
     which comes back as None).  Differentiable in q and k, any number of times, by the backward pass
     (forward mode is refused).
@@ -177,6 +223,13 @@ def rotary(q, k, positions, frequencies, interleaved=False, scale=1.0):
     ``[T]`` or ``[B, T]``, of any sign and size: angles are formed in double.  ``frequencies`` are
     float32 or float64, on the tensors' device (:func:`rotary_frequencies`); neither has a gradient.
     float32, bfloat16, float16 and float64; computed in float32 (float64 in double), rounded once.
+
+    Tokens with several positions, as pixels of an image (row, column) or a video (time, row, column):
+    ``axes``, int32, names for every pair the position that turns it (:func:`rotary_axes`), and
+    ``positions`` are ``[axes, T]`` or ``[axes, B, T]``.  A pair whose axis is not there becomes NaN.
+    Then q and k may also be images as :func:`natten2d` takes them, ``[B, heads, H, W, d]``, with
+    positions ``[axes, H, W]`` or ``[axes, B, H, W]``; ones whose rows do not follow each other at an
+    even distance are copied first.
     """
     _tensors(q=q, positions=positions, frequencies=frequencies)
     if k is not None:
@@ -184,7 +237,22 @@ def rotary(q, k, positions, frequencies, interleaved=False, scale=1.0):
     if torch.is_grad_enabled() and frequencies.requires_grad:
         raise RuntimeError("frequencies have no gradient; call it on detached ones")
     call = _OPS[0] if NATIVE_BINDING else Rotary.apply
-    out = call(q, k, positions, frequencies, bool(interleaved), float(scale), False)
+    if axes is None:
+        out = call(q, k, positions, frequencies, bool(interleaved), float(scale), False)
+        return out[0], out[1] if k is not None else None
+    _tensors(axes=axes)
+    image = q.shape[2:4] if q.dim() == 5 else None
+    if image is not None:
+        if k is not None and (k.dim() != 5 or k.shape[2:4] != image):
+            raise ValueError("q and k must differ in their heads only, got %s, %s" % (tuple(q.shape), tuple(k.shape)))
+        if positions.dim() < 3 or positions.shape[-2:] != image:
+            raise ValueError("positions must have shape [H, W] or [B, H, W] for every axis, got %s"
+                             % (tuple(positions.shape),))
+        q, positions = q.flatten(2, 3), positions.flatten(-2, -1)
+        k = None if k is None else k.flatten(2, 3)
+    out = call(q, k, positions, frequencies, bool(interleaved), float(scale), False, axes)
+    if image is not None:
+        out = [x.unflatten(2, image) for x in out]
     return out[0], out[1] if k is not None else None
 
 

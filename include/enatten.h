@@ -302,6 +302,19 @@ int enatten_rotary(const void *q, const void *k, void *q_out, void *k_out, const
                    int dtype, int positions_dtype, int frequencies_dtype, int interleaved, int inverse,
                    const int64_t *q_strides, const int64_t *k_strides, const int64_t *q_out_strides,
                    const int64_t *k_out_strides, int64_t positions_stride, double scale, void *stream);
+/*
+ * The same for tokens that have several positions, as the pixels of an image or a video do:
+ *   positions  [num_axes, T] or [num_axes, B, T], axis_stride elements between the axes
+ *   axes       [R / 2], 0 .. num_axes - 1: which position turns a pair.  A pair with any other number
+ *              becomes NaN.
+ */
+int enatten_rotary_axes(const void *q, const void *k, void *q_out, void *k_out, const void *positions,
+                        const void *frequencies, const int *axes, int num_axes, int B, int heads_q,
+                        int heads_k, int T, int D, int R, int dtype, int positions_dtype,
+                        int frequencies_dtype, int interleaved, int inverse, const int64_t *q_strides,
+                        const int64_t *k_strides, const int64_t *q_out_strides,
+                        const int64_t *k_out_strides, int64_t positions_stride, int64_t axis_stride,
+                        double scale, void *stream);
 
 /*
  * A cache of 8 bits for sequences that grow, in pages of `page` tokens:
@@ -363,6 +376,51 @@ int enatten_cache_attention(const void *q, const void *k_cache, const void *v_ca
                             int64_t pages_stride, float scale, void *stream);
 
 /*
+ * Pages that sequences share, leave and get.  Beside the table and the lengths:
+ *   holders    int32 [num_pages]: how many entries of the table name each page; 0: free
+ * An entry of the table outside 0 .. num_pages - 1 is no page (-1 is written).  All of a row counts, also
+ * entries behind its last token.  What the calls write depends on their arguments alone: pages are given
+ * out from the lowest free one on, to rows and columns in their order.  At most 8192 rows, and 2^30
+ * entries.
+ *
+ * enatten_cache_fork: row b becomes what row parents[b] was: the pages of its lengths[parents[b]] tokens,
+ * which both hold then, and its length.  -1 leaves it empty; its own number, or any other, as it is.
+ */
+int enatten_cache_fork(int *pages, int *lengths, int *holders, const int *parents, int B, int columns,
+                       int num_pages, int page, int64_t pages_stride, void *stream);
+/*
+ * enatten_cache_reserve: a page of its own for every place of the last counts[b] of lengths[b] tokens of
+ * row b (counts NULL: `count` each).  Entries that are no page get a free one.  A first page that holds
+ * older tokens too and that others hold is left to them and replaced; if all its holders leave it in this
+ * call, the last row keeps it.  copies [B, 3] is (page left, page got, older tokens) for a row that has
+ * to be copied so, else (-1, -1, 0).  Where no free page is left the entry becomes -1, and one that should
+ * hold older tokens but is no page stays none.  Rows whose numbers do not fit together are left out.
+ *   workspace  enatten_cache_reserve_workspace_bytes(), 16-byte aligned; calls that may overlap need one each
+ */
+size_t enatten_cache_reserve_workspace_bytes(int B, int columns, int num_pages);
+int enatten_cache_reserve(int *pages, const int *lengths, const int *counts, int count, int *holders,
+                          int *copies, void *workspace, int B, int columns, int num_pages, int page,
+                          int64_t pages_stride, void *stream);
+/*
+ * enatten_cache_copy: for each of n (source, target, tokens) the codes of the first `tokens` tokens of
+ * every head, and the scales, of page `source` into page `target`, in `layers` layers.  Pages outside the
+ * cache, and a target that is its source, are passed over; a page must not be the target of two, nor
+ * target and source.  Strides (layer, page, head, token) and (layer, page, head), multiples of 16 for codes.
+ */
+int enatten_cache_copy(void *k_cache, void *v_cache, float *k_scale, float *v_scale, const int *copies,
+                       int n, int layers, int heads, int D, int num_pages, int page,
+                       const int64_t *k_cache_strides, const int64_t *v_cache_strides,
+                       const int64_t *k_scale_strides, const int64_t *v_scale_strides, void *stream);
+/*
+ * enatten_cache_compact: the held pages to the low end of the pool.  With n of them, those from n on move
+ * to the free ones below n, both in their order; the table and holders follow.  copies
+ * [max(num_pages / 2, 1), 3]: (source, target, page) for each move, then (-1, -1, 0).
+ */
+size_t enatten_cache_compact_workspace_bytes(int num_pages);
+int enatten_cache_compact(int *pages, int *holders, int *copies, void *workspace, int B, int columns,
+                          int num_pages, int page, int64_t pages_stride, void *stream);
+
+/*
  * Per-kernel timing aid for benchmarks (no counterpart in the reference, whose
  * bench.py:28,59 times whole calls with triton.testing.do_bench).  While
  * enabled, kernels this library launches are bracketed by HIP events on the
@@ -379,7 +437,8 @@ int enatten_cache_attention(const void *q, const void *k_cache, const void *v_ca
  */
 enum { ENATTEN_KERNEL_FWD = 0, ENATTEN_KERNEL_BWD_DQ = 1, ENATTEN_KERNEL_BWD_DKDV = 2,
        ENATTEN_KERNEL_BWD_FUSED = 3, ENATTEN_KERNEL_ROTARY = 4, ENATTEN_KERNEL_CACHE_APPEND = 5,
-       ENATTEN_KERNEL_CACHE_ATTENTION = 6, ENATTEN_KERNEL_CACHE_JOIN = 7, ENATTEN_KERNEL_COUNT = 8 };
+       ENATTEN_KERNEL_CACHE_ATTENTION = 6, ENATTEN_KERNEL_CACHE_JOIN = 7, ENATTEN_KERNEL_CACHE_PAGES = 8,
+       ENATTEN_KERNEL_CACHE_COPY = 9, ENATTEN_KERNEL_COUNT = 10 };
 int enatten_profile_enable(int on);
 int enatten_profile_read(int kernel, int *launches, double *total_ms);
 /* What the brackets themselves added to total_ms: after each timed launch's closing
