@@ -50,6 +50,9 @@ SIGNATURES = {
     "enatten_cache_attention_workspace_bytes": (ctypes.c_size_t, [_i] * 9),
     "enatten_cache_attention": (_i, [_vp] * 10 + [_i] * 11 + [_sp] * 6
                                 + [ctypes.c_int64, ctypes.c_float, _vp]),
+    "enatten_cache_attention_shared_workspace_bytes": (ctypes.c_size_t, [_i] * 10),
+    "enatten_cache_attention_shared": (_i, [_vp] * 9 + [_i] + [_vp] * 2 + [_i] * 11 + [_sp] * 6
+                                       + [ctypes.c_int64, ctypes.c_float, _vp]),
     "enatten_cache_fork": (_i, [_vp] * 4 + [_i] * 4 + [ctypes.c_int64, _vp]),
     "enatten_cache_reserve_workspace_bytes": (ctypes.c_size_t, [_i] * 3),
     "enatten_cache_reserve": (_i, [_vp] * 3 + [_i] + [_vp] * 3 + [_i] * 4 + [ctypes.c_int64, _vp]),

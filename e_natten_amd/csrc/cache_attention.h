@@ -1,6 +1,8 @@
 // What the kernels of cache_attention share: the split of a call's work, and codes to float16.
 #pragma once
 
+#include <type_traits>
+
 #include "sequence_common.h"
 
 namespace enatten {
@@ -16,6 +18,17 @@ struct AttnArgs {
     float scale;
     float *ws;       // (part_of)
 };
+
+// Sequences in runs that share their first tokens: two passes over the same kernels.  In the first an entry is a
+// run, its rows are those of all its sequences and its tokens the shared ones; what they come to goes to `canon`.
+// In the second an entry is a sequence with the tokens behind, and that is joined in.  A type of its own, so that
+// the other kernels' arguments stay what they are.
+struct SharedArgs : AttnArgs {
+    const int *shared;  // [runs], tokens
+    int runs, size;     // sequences of a run
+    float *canon;       // rows (b, head, t): their sums of D values each, then the maxima, then the sums
+};
+template <int PASS> struct PassArgs : SharedArgs {};
 
 // How a call is cut, from its sizes alone (the lengths are on the device).
 struct Plan {
@@ -48,7 +61,7 @@ struct Span {
     bool ok;
 };
 template <int ROWS>
-__device__ __forceinline__ Span span_of(const AttnArgs &a, int entry) {
+__device__ __forceinline__ Span plain_span(const AttnArgs &a, int entry) {
     Span s;
     const int b = entry / a.row_tiles, tile = entry - b * a.row_tiles;
     s.ok = sequence_of(a.tb, b, s.len, s.count);
@@ -60,6 +73,52 @@ __device__ __forceinline__ Span span_of(const AttnArgs &a, int entry) {
         s.hi = s.start + last + 1;
     }
     return s;
+}
+template <class Args> constexpr bool kShared = std::is_base_of_v<SharedArgs, Args>;
+template <class Args> constexpr bool kFirstPass = std::is_same_v<Args, PassArgs<1>>;
+template <class Args> constexpr bool kSecondPass = std::is_same_v<Args, PassArgs<2>>;
+// (sequences or runs) x row tiles, and the rows that one of these has per cache head
+template <class Args>
+__device__ __forceinline__ int entries_of(const Args &a) {
+    if constexpr (kFirstPass<Args>) return a.runs * a.row_tiles;
+    else return a.B * a.row_tiles;
+}
+template <class Args>
+__device__ __forceinline__ int rows_of(const Args &a) {
+    if constexpr (kFirstPass<Args>) return a.T * a.group * a.size;
+    else return a.T * a.group;
+}
+// How many tokens run r shares: whole pages.
+__device__ __forceinline__ int shared_end(const SharedArgs &a, int r) {
+    const int n = min(a.shared[r], a.tb.columns * a.tb.page);
+    return n > 0 ? n / a.tb.page * a.tb.page : 0;
+}
+// ... and how many of them sequence b reads with its run: all, or none if its new tokens start before that end.
+__device__ __forceinline__ int shared_by(const SharedArgs &a, int b, const Span &s) {
+    const int end = shared_end(a, b / a.size);
+    return s.ok && s.count > 0 && s.start >= end ? end : 0;
+}
+template <int ROWS, class Args>
+__device__ __forceinline__ Span span_of(const Args &a, int entry) {
+    if constexpr (kFirstPass<Args>) {
+        const int r = entry / a.row_tiles;
+        Span s{0, 0, 0, 0, shared_end(a, r), true};
+        if (a.window && s.hi) {  // from the first token on that any row sees
+            int least = s.hi;
+            for (int i = 0; i < a.size; i++) {
+                int len, count;
+                if (sequence_of(a.tb, r * a.size + i, len, count) && count > 0 && len - count >= s.hi)
+                    least = min(least, max(len - count + 1 - a.window, 0));
+            }
+            s.lo = least;
+        }
+        return s;
+    } else {
+        Span s = plain_span<ROWS>(a, entry);
+        if constexpr (kSecondPass<Args>)
+            if (s.hi > s.lo) s.lo = max(s.lo, shared_by(a, entry / a.row_tiles, s));
+        return s;
+    }
 }
 // steps of TOK tokens, from the group of 16 that holds the first one on
 template <int TOK>
@@ -73,11 +132,11 @@ struct Share {
     int step0, step1, item;
 };
 // WAVES: how many waves share the steps of an item (each takes whole ones).
-template <int ROWS, int TOK, int WAVES>
-__device__ __forceinline__ Share share_of(const AttnArgs &a, int item) {
+template <int ROWS, int TOK, int WAVES, class Args>
+__device__ __forceinline__ Share share_of(const Args &a, int item) {
     Share w;
     w.item = item;
-    const int entries = a.B * a.row_tiles, lane = threadIdx.x & 63;
+    const int entries = entries_of(a), lane = threadIdx.x & 63;
     auto steps_at = [&](int e) { return e < entries ? steps_of<TOK>(span_of<ROWS>(a, e)) : 0; };
     float total = 0.f;
     int steps = 0;
@@ -121,13 +180,13 @@ struct Ranges {
     int64_t line, each;  // steps of one cache head, of one range
     bool whole;          // no more tiles than ranges, and nearly as long as those: a tile each, none cut
 };
-template <int ROWS, int TOK>
-__device__ __forceinline__ int counted_steps(const AttnArgs &a, int e) {
-    return e < a.B * a.row_tiles ? max(1, steps_of<TOK>(span_of<ROWS>(a, e))) : 0;
+template <int ROWS, int TOK, class Args>
+__device__ __forceinline__ int counted_steps(const Args &a, int e) {
+    return e < entries_of(a) ? max(1, steps_of<TOK>(span_of<ROWS>(a, e))) : 0;
 }
-template <int ROWS, int TOK>
-__device__ __forceinline__ Ranges ranges_of(const AttnArgs &a) {
-    const int entries = a.B * a.row_tiles, lane = threadIdx.x & 63;
+template <int ROWS, int TOK, class Args>
+__device__ __forceinline__ Ranges ranges_of(const Args &a) {
+    const int entries = entries_of(a), lane = threadIdx.x & 63;
     Ranges r{0, 0, false};
     int most = 0;
     for (int e0 = 0; e0 < entries; e0 += 64) {
@@ -142,14 +201,14 @@ __device__ __forceinline__ Ranges ranges_of(const AttnArgs &a) {
     // of 224 steps on average, 256 at most): 506 us cut, 570 whole; 256 tokens each of 8 sequences of 300
     // (128 tiles of 5): 37 us cut, 27 whole; half as many tiles: 21 us cut, 24 whole.
     const int64_t tiles = (int64_t)entries * a.heads_kv;
-    const int64_t steps = tiles * min(ROWS, a.T * a.group) * padded(a.D) >> 20;
+    const int64_t steps = tiles * min(ROWS, rows_of(a)) * padded(a.D) >> 20;
     r.whole = tiles <= a.parts && !__any(most > r.each + steps);
     return r;
 }
 // The row tile at step `y` of a head's line, and how far into it that is
-template <int ROWS, int TOK>
-__device__ __forceinline__ int tile_at(const AttnArgs &a, int64_t y, int &into) {
-    const int entries = a.B * a.row_tiles, lane = threadIdx.x & 63;
+template <int ROWS, int TOK, class Args>
+__device__ __forceinline__ int tile_at(const Args &a, int64_t y, int &into) {
+    const int entries = entries_of(a), lane = threadIdx.x & 63;
     for (int e0 = 0; e0 < entries; e0 += 64) {
         const unsigned n = counted_steps<ROWS, TOK>(a, e0 + lane), upto = running_sum(n);
         const unsigned all = __builtin_amdgcn_readlane(upto, 63);
@@ -173,8 +232,9 @@ __device__ __forceinline__ float *slot_of(const AttnArgs &a, int slot) {
 // The workspace: first item and items of every entry, then for every (item, cache head) the maxima and
 // sums of its rows and rows x D sums of values.
 __host__ __device__ inline int64_t head_floats(int64_t entries) { return (2 * entries + 3) / 4 * 4; }
-__device__ __forceinline__ float *part_of(const AttnArgs &a, int rows, int item, int head) {
-    return a.ws + head_floats((int64_t)a.B * a.row_tiles) + ((int64_t)item * a.heads_kv + head) * item_floats(rows, a.D);
+template <class Args>
+__device__ __forceinline__ float *part_of(const Args &a, int rows, int item, int head) {
+    return a.ws + head_floats((int64_t)entries_of(a)) + ((int64_t)item * a.heads_kv + head) * item_floats(rows, a.D);
 }
 // (for the launch that joins the parts)
 __device__ __forceinline__ void note_share(const AttnArgs &a, const Share &w, int head) {
@@ -380,6 +440,56 @@ __device__ __forceinline__ void store_channels(const Rows &r, int64_t at, f32x4 
     else *reinterpret_cast<u32x2 *>(static_cast<unsigned short *>(const_cast<void *>(r.ptr)) + at) = narrow4<DT>(x);
 }
 
+// A row of an entry: sequence, new token, query head.
+struct Place {
+    int b, t, head;
+};
+template <class Args>
+__device__ __forceinline__ Place place_of(const Args &a, int which, int head, int row) {  // which: sequence or run
+    Place p{which, row / a.group, 0};
+    p.head = head * a.group + row - p.t * a.group;
+    if constexpr (kFirstPass<Args>) {
+        const int i = p.t / a.T;
+        p.b = which * a.size + i;
+        p.t -= i * a.T;
+    }
+    return p;
+}
+__device__ __forceinline__ int64_t offset_of(const Rows &r, const Place &p) { return p.b * r.sb + p.head * r.sh + p.t * r.st; }
+
+// What a run's rows come to over the shared tokens, for the second pass: sums of values (4 channels from d on), and
+// by whoever has `first`, the maximum and the sum.
+__device__ __forceinline__ int64_t canon_row(const SharedArgs &a, const Place &p) {
+    return ((int64_t)p.b * a.heads + p.head) * a.T + p.t;
+}
+__device__ __forceinline__ void put_canon(const SharedArgs &a, const Place &p, int d, bool first, float top, float sum, f32x4 y) {
+    const int64_t row = canon_row(a, p), rows = (int64_t)a.B * a.heads * a.T;
+    *reinterpret_cast<f32x4 *>(a.canon + row * a.D + d) = y;
+    if (first) {
+        a.canon[rows * a.D + row] = top;
+        a.canon[rows * (a.D + 1) + row] = sum;
+    }
+}
+// The factors of a row's own part and of that one, both for the same maximum; the row's sum becomes that of both.
+struct Joined {
+    float mine, other;
+    const float *y;  // nullptr: nothing to join
+};
+__device__ __forceinline__ Joined join_canon(const SharedArgs &a, const Place &p, bool shares, float top, float &sum) {
+    Joined j{1.f, 0.f, nullptr};
+    if (!shares) return j;
+    const int64_t row = canon_row(a, p), rows = (int64_t)a.B * a.heads * a.T;
+    const float m = a.canon[rows * a.D + row], l = a.canon[rows * (a.D + 1) + row], most = fmaxf(top, m);
+    j.mine = __builtin_amdgcn_exp2f(top - most);
+    j.other = __builtin_amdgcn_exp2f(m - most);
+    j.y = a.canon + row * a.D;
+    sum = j.mine * sum + j.other * l;
+    return j;
+}
+__device__ __forceinline__ f32x4 joined(const Joined &j, int d, f32x4 y) {
+    return j.y ? j.mine * y + j.other * *reinterpret_cast<const f32x4 *>(j.y + d) : y;
+}
+
 __device__ __forceinline__ float lane_float(float x, int l) {
     return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), l));
 }
@@ -392,5 +502,19 @@ __device__ __forceinline__ int64_t lane_offset(int64_t x, int l) {
 
 // Tiles of kWideRows rows (cache_attention_rows.hip), a.parts ranges
 int launch_attend_rows(const char *fn, const AttnArgs &a, bool e4m3, hipStream_t st);
+int launch_rows_first(const char *fn, const SharedArgs &a, bool e4m3, hipStream_t st);
+int launch_rows_second(const char *fn, const SharedArgs &a, bool e4m3, hipStream_t st);
+// The same and the kernels of cache_attention.hip in the two passes (cache_attention_first.hip, _second.hip)
+Plan plan_of(int B, int heads, int heads_kv, int T, int D, int page, int columns, int window, int dtype);
+size_t workspace_bytes(const Plan &p, int B, int heads_kv, int D);  // B: sequences, or runs
+// The arguments that all calls have, checked, but for row_tiles, parts and ws
+int set_attention(const char *fn, const void *q, const void *k_cache, const void *v_cache, const float *k_scale,
+                  const float *v_scale, const int *pages, const int *lengths, const int *counts, void *o, int B, int heads,
+                  int heads_kv, int T, int D, int num_pages, int page, int columns, int kernel_size, int dtype,
+                  int cache_dtype, const int64_t *q_strides, const int64_t *o_strides, const int64_t *k_cache_strides,
+                  const int64_t *v_cache_strides, const int64_t *k_scale_strides, const int64_t *v_scale_strides,
+                  int64_t pages_stride, float scale, AttnArgs *a);
+int launch_first(const char *fn, const SharedArgs &a, const Plan &p, bool e4m3, hipStream_t st);
+int launch_second(const char *fn, const SharedArgs &a, const Plan &p, bool e4m3, hipStream_t st);
 
 }  // namespace enatten

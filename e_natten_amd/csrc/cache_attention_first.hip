@@ -1,0 +1,10 @@
+// The first pass of cache_attention over runs of sequences that share their first tokens: up to 64 rows.
+#include "cache_attention_passes.h"
+
+namespace enatten {
+
+int launch_first(const char *fn, const SharedArgs &a, const Plan &p, bool e4m3, hipStream_t st) {
+    return launch_pass<1>(fn, a, p, e4m3, st);
+}
+
+}  // namespace enatten

@@ -264,11 +264,19 @@ void validate_append(const Tensor &k, const Tensor &v, const Tensor &kc, const T
     on_gpu(what, k);
 }
 void validate_attention(const Tensor &q, const Tensor &kc, const Tensor &vc, const Tensor &ks, const Tensor &vs,
-                        const Tensor &pages, const Tensor &lengths, const optional<Tensor> &counts, int64_t kernel_size) {
+                        const Tensor &pages, const Tensor &lengths, const optional<Tensor> &counts, int64_t kernel_size,
+                        const optional<Tensor> &shared) {
     const char *what = "cache_attention";
     validate_cache(what, "q", q, kc, vc, ks, vs, pages, lengths, counts);
     TORCH_CHECK_VALUE(q.size(1) % kc.size(1) == 0, what, ": ", q.size(1), " heads are no multiple of the cache's ", kc.size(1));
     TORCH_CHECK_VALUE(kernel_size >= 0, what, ": kernel_size must be >= 1, or 0 for all tokens, got ", kernel_size);
+    if (shared.has_value()) {
+        TORCH_CHECK_VALUE(shared->dim() == 1 && shared->scalar_type() == at::kInt && shared->size(0) > 0 &&
+                              q.size(0) % shared->size(0) == 0,
+                          what, ": shared must be int32 [runs], runs a divisor of ", q.size(0), " sequences, got ",
+                          shared->scalar_type(), " ", shared->sizes());
+        TORCH_CHECK_VALUE(shared->device() == q.device(), what, ": all tensors must be on the same device");
+    }
     on_gpu(what, q);
 }
 // the columns of a row of pages are neighbours
@@ -298,8 +306,8 @@ void cache_append(const Tensor &k_, const Tensor &v_, const Tensor &kc, const Te
 }
 Tensor cache_attention(const Tensor &q_, const Tensor &kc, const Tensor &vc, const Tensor &ks, const Tensor &vs,
                        const Tensor &pages_, const Tensor &lengths_, const optional<Tensor> &counts_,
-                       int64_t kernel_size, double scale) {
-    validate_attention(q_, kc, vc, ks, vs, pages_, lengths_, counts_, kernel_size);
+                       int64_t kernel_size, double scale, const optional<Tensor> &shared_) {
+    validate_attention(q_, kc, vc, ks, vs, pages_, lengths_, counts_, kernel_size, shared_);
     if (q_.is_meta()) return empty_rows(kernel_layout(q_));
     const c10::DeviceGuard guard(q_.device());
     const Tensor rows = kernel_layout(q_), q = aligned_rows(rows), pages = page_rows(pages_);
@@ -308,8 +316,20 @@ Tensor cache_attention(const Tensor &q_, const Tensor &kc, const Tensor &vc, con
     const int window = (int)std::min<int64_t>(kernel_size, 0x7fffffff);
     const int B = q.size(0), N = q.size(1), Nk = kc.size(1), T = q.size(2), D = q.size(3);
     const int page = kc.size(2), columns = pages.size(1);
-    const size_t need = enatten_cache_attention_workspace_bytes(B, N, Nk, T, D, page, columns, window, dtype_code(q));
+    const Tensor shared = shared_.has_value() ? shared_->contiguous() : Tensor();
+    const int runs = shared.defined() ? shared.size(0) : 0;
+    const size_t need = runs ? enatten_cache_attention_shared_workspace_bytes(B, N, Nk, T, D, page, columns, window, dtype_code(q), runs)
+                             : enatten_cache_attention_workspace_bytes(B, N, Nk, T, D, page, columns, window, dtype_code(q));
     const Tensor ws = need ? at::empty({(int64_t)need}, q.options().dtype(at::kByte)) : Tensor();
+    if (runs) {
+        check_rc(enatten_cache_attention_shared(
+            q.data_ptr(), kc.data_ptr(), vc.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(), pages.data_ptr<int>(),
+            lengths.data_ptr<int>(), counts.defined() ? counts.data_ptr<int>() : nullptr, shared.data_ptr<int>(), runs,
+            o.data_ptr(), need ? ws.data_ptr() : nullptr, B, N, Nk, T, D, kc.size(0), page, columns, window, dtype_code(q),
+            cache_code(kc), q.strides().data(), o.strides().data(), kc.strides().data(), vc.strides().data(),
+            ks.strides().data(), vs.strides().data(), pages.stride(0), (float)scale, stream_now()));
+        return o;
+    }
     check_rc(enatten_cache_attention(
         q.data_ptr(), kc.data_ptr(), vc.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(), pages.data_ptr<int>(),
         lengths.data_ptr<int>(), counts.defined() ? counts.data_ptr<int>() : nullptr, o.data_ptr(),
@@ -344,11 +364,11 @@ void cache_append_in_place(const Tensor &k, const Tensor &v, const Tensor &kc, c
 }
 Tensor cache_attention_autograd(const Tensor &q, const Tensor &kc, const Tensor &vc, const Tensor &ks, const Tensor &vs,
                                 const Tensor &pages, const Tensor &lengths, const optional<Tensor> &counts,
-                                int64_t kernel_size, double scale) {
+                                int64_t kernel_size, double scale, const optional<Tensor> &shared) {
     no_gradient("cache_attention", {&q, &kc, &vc, &ks, &vs});
     at::AutoDispatchBelowADInplaceOrView below;
     static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("enatten::cache_attention", "").typed<decltype(cache_attention)>();
-    return op.call(q, kc, vc, ks, vs, pages, lengths, counts, kernel_size, scale);
+    return op.call(q, kc, vc, ks, vs, pages, lengths, counts, kernel_size, scale, shared);
 }
 
 }  // namespace
@@ -361,7 +381,7 @@ TORCH_LIBRARY_FRAGMENT(enatten, m) {
     m.def("cache_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scale, "
           "Tensor(d!) v_scale, Tensor pages, Tensor lengths, Tensor? counts) -> ()");
     m.def("cache_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor pages, "
-          "Tensor lengths, Tensor? counts, int kernel_size, float scale) -> Tensor");
+          "Tensor lengths, Tensor? counts, int kernel_size, float scale, Tensor? shared=None) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(enatten, CompositeExplicitAutograd, m) {

@@ -369,10 +369,17 @@ def _append_impl(k, v, k_cache, v_cache, k_scale, v_scale, pages, lengths, count
             torch.autograd.graph.increment_version(t)
 
 
-def _attention_impl(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, counts, kernel_size: int, scale: float):
+def _attention_impl(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, counts, kernel_size: int, scale: float,
+                    shared=None):
     _validate_cache("q", q, k_cache, v_cache, k_scale, v_scale, pages, lengths, counts)
     if q.shape[1] % k_cache.shape[1]:
         raise ValueError("%d heads are no multiple of the cache's %d" % (q.shape[1], k_cache.shape[1]))
+    if shared is not None:
+        if shared.dim() != 1 or shared.dtype != torch.int32 or shared.shape[0] < 1 or q.shape[0] % shared.shape[0]:
+            raise ValueError("shared must be int32 [runs], runs a divisor of %d sequences, got %s %s"
+                             % (q.shape[0], shared.dtype, list(shared.shape)))
+        if shared.device != q.device:
+            raise ValueError("all tensors must be on the same device")
     _require_gpu(q, "cache_attention")
     _no_gradient("cache_attention", q, k_cache, v_cache, k_scale, v_scale)
     lib = _lib.load()
@@ -383,15 +390,21 @@ def _attention_impl(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, count
     heads, page, columns, window = k_cache.shape[1], k_cache.shape[2], pages.shape[1], min(kernel_size, 0x7fffffff)
     with torch.cuda.device(q.device):
         o = _aligned_rows(_kernel_layout(torch.empty_like(rows)))
-        need = lib.enatten_cache_attention_workspace_bytes(B, N, heads, T, D, page, columns, window, _DTYPES[q.dtype])
+        sizes = (B, N, heads, T, D, page, columns, window, _DTYPES[q.dtype])
+        need = (lib.enatten_cache_attention_workspace_bytes(*sizes) if shared is None
+                else lib.enatten_cache_attention_shared_workspace_bytes(*sizes, shared.shape[0]))
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        _check(lib.enatten_cache_attention(
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-            pages.data_ptr(), lengths.data_ptr(), None if counts is None else counts.data_ptr(), o.data_ptr(),
-            ws.data_ptr() if need else None, B, N, heads, T, D, k_cache.shape[0], page, columns, window,
-            _DTYPES[q.dtype], _CACHE_DTYPES[k_cache.dtype], _lib.strides3(q), _lib.strides3(o),
-            _lib.strides3(k_cache), _lib.strides3(v_cache), _lib.strides2(k_scale), _lib.strides2(v_scale),
-            pages.stride(0), float(scale), _stream_of(q)))
+        data = (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                pages.data_ptr(), lengths.data_ptr(), None if counts is None else counts.data_ptr())
+        rest = (o.data_ptr(), ws.data_ptr() if need else None, B, N, heads, T, D, k_cache.shape[0], page, columns, window,
+                _DTYPES[q.dtype], _CACHE_DTYPES[k_cache.dtype], _lib.strides3(q), _lib.strides3(o),
+                _lib.strides3(k_cache), _lib.strides3(v_cache), _lib.strides2(k_scale), _lib.strides2(v_scale),
+                pages.stride(0), float(scale), _stream_of(q))
+        if shared is None:
+            _check(lib.enatten_cache_attention(*data, *rest))
+        else:
+            shared = shared.contiguous()
+            _check(lib.enatten_cache_attention_shared(*data, shared.data_ptr(), shared.shape[0], *rest))
     return o
 
 
@@ -425,7 +438,7 @@ def cache_append(k, v, k_cache, v_cache, k_scale, v_scale, pages, lengths, count
 
 
 def cache_attention(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, kernel_size=None, scale=1.0,
-                    counts=None):
+                    counts=None, shared=None):
     """Attention of the last tokens of each sequence over its cache: ``q [B, heads, T, d] -> o`` of the
     same shape, what ``natten1d(..., is_causal=True)`` gives for these tokens of a whole sequence.
 
@@ -444,11 +457,19 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, kerne
     A float8 cache that :func:`cache_append` wrote holds finite codes only.  The two codes that are no
     numbers, written there by other means, read as +-480 or as NaN by the queries that see them, by the
     sizes of the call; queries that do not see them never notice.
+
+    ``shared``, int32 ``[runs]``, is for sequences that continue one prompt: they come in that many runs of
+    neighbours, B / runs each, and those of run r have their first ``shared[r]`` tokens on the same pages
+    (:func:`cache_fork`).  These are read once for all rows of the run; whole pages of them count.  A sequence
+    whose new tokens start before their end is computed by itself, and numbers below 1 share nothing, so
+    that the result is the same but for its rounding.
     """
     _tensors(q=q, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, pages=pages,
              lengths=lengths)
     if counts is not None:
         _tensors(counts=counts)
+    if shared is not None:
+        _tensors(shared=shared)
     if kernel_size is None:
         kernel_size = 0
     elif not isinstance(kernel_size, int) or isinstance(kernel_size, bool):
@@ -456,4 +477,6 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, kerne
     elif kernel_size < 1:
         raise ValueError("kernel_size must be >= 1, got %d" % kernel_size)
     call = _OPS[2] if NATIVE_BINDING else _attention_impl
-    return call(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, counts, kernel_size, float(scale))
+    if shared is None:
+        return call(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, counts, kernel_size, float(scale))
+    return call(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, counts, kernel_size, float(scale), shared)

@@ -376,6 +376,27 @@ int enatten_cache_attention(const void *q, const void *k_cache, const void *v_ca
                             int64_t pages_stride, float scale, void *stream);
 
 /*
+ * The same for sequences that continue one prompt: the B sequences are `runs` runs of B / runs
+ * neighbours each, and the sequences of run r have the same first shared[r] tokens, on the same pages
+ * (int32 [runs], on the device; whole pages count, the rest of a page is each sequence's own).  These
+ * tokens are read once for all rows of the run.  A sequence whose new tokens start before that end is
+ * computed by itself, and a number below 1 shares nothing: results are enatten_cache_attention's but
+ * for where they are rounded.  The pages are those of the run's first sequence that shares them.
+ */
+size_t enatten_cache_attention_shared_workspace_bytes(int B, int heads, int heads_kv, int T, int D,
+                                                      int page, int columns, int kernel_size, int dtype,
+                                                      int runs);
+int enatten_cache_attention_shared(const void *q, const void *k_cache, const void *v_cache,
+                                   const float *k_scale, const float *v_scale, const int *pages,
+                                   const int *lengths, const int *counts, const int *shared, int runs,
+                                   void *o, void *workspace, int B, int heads, int heads_kv, int T, int D,
+                                   int num_pages, int page, int columns, int kernel_size, int dtype,
+                                   int cache_dtype, const int64_t *q_strides, const int64_t *o_strides,
+                                   const int64_t *k_cache_strides, const int64_t *v_cache_strides,
+                                   const int64_t *k_scale_strides, const int64_t *v_scale_strides,
+                                   int64_t pages_stride, float scale, void *stream);
+
+/*
  * Pages that sequences share, leave and get.  Beside the table and the lengths:
  *   holders    int32 [num_pages]: how many entries of the table name each page; 0: free
  * An entry of the table outside 0 .. num_pages - 1 is no page (-1 is written).  All of a row counts, also

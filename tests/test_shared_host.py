@@ -1,0 +1,87 @@
+"""Host side of cache_attention over runs that share their first tokens, without a GPU: what the entry points
+refuse, workspaces, and the built kernels' registers."""
+import ctypes
+import re
+
+import pytest
+import torch
+
+from _util import ensure_built
+
+BF16, F32, I8, I32 = torch.bfloat16, torch.float32, torch.int8, torch.int32
+
+
+def _z(*shape, dtype=I32):
+    return torch.zeros(shape, dtype=dtype)
+
+
+def _args(**change):
+    a = dict(q=_z(6, 4, 1, 32, dtype=BF16), k=_z(8, 2, 16, 32, dtype=I8), v=_z(8, 2, 16, 32, dtype=I8),
+             ks=_z(8, 2, dtype=F32), vs=_z(8, 2, dtype=F32), pages=_z(6, 3), lengths=_z(6), counts=None, shared=_z(2))
+    a.update(change)
+    return a
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(shared=_z(4)), "divisor of 6"), (dict(shared=_z(0)), "divisor"), (dict(shared=_z(12)), "divisor"),
+    (dict(shared=_z(2, 1)), "shared must be"), (dict(shared=_z(2, dtype=torch.int64)), "int32"), (dict(shared=_z(2, dtype=F32)), "int32"),
+    (dict(shared=torch.zeros(2, dtype=I32, device="meta")), "same device"), (dict(lengths=_z(5)), "lengths"), (dict(), "GPU"),
+])
+def test_shared_refuses(change, text):
+    ensure_built()
+    import e_natten_amd as E
+    from e_natten_amd import sequence as S
+    a = _args(**change)
+    front = (a["q"], a["k"], a["v"], a["ks"], a["vs"], a["pages"], a["lengths"])
+    for call in (lambda: E.cache_attention(*front, None, 1.0, a["counts"], a["shared"]),
+                 lambda: S._attention_impl(*front, a["counts"], 0, 1.0, a["shared"])):
+        with pytest.raises((ValueError, RuntimeError), match=text):
+            call()
+
+
+def test_shared_is_a_tensor_and_has_shapes_without_data():
+    ensure_built()
+    import e_natten_amd as E
+    a = _args()
+    front = [a["q"], a["k"], a["v"], a["ks"], a["vs"], a["pages"], a["lengths"]]
+    for bad in (3, [0, 0], 1.5):
+        with pytest.raises(TypeError, match="tensor"):
+            E.cache_attention(*front, None, 1.0, None, bad)
+    if E.ops.NATIVE_BINDING:
+        o = E.cache_attention(*(x.to("meta") for x in front), None, 1.0, None, a["shared"].to("meta"))
+        assert o.shape == a["q"].shape and o.dtype == BF16
+
+
+def test_c_shared_validates_before_launch():
+    ensure_built()
+    from e_natten_amd import _lib
+    lib = _lib.load()
+    at, none = ctypes.c_void_p(16), None
+
+    def call(shared=at, runs=2, B=6, heads=4, ws=at, o=at, D=32, lengths=at):
+        return lib.enatten_cache_attention_shared(at, at, at, at, at, at, lengths, none, shared, runs, o, ws, B, heads, 2, 1, D,
+                                                  8, 16, 3, 0, _lib.BF16, _lib.I8, none, none, none, none, none, none, 3, 1.0, none)
+
+    for bad in (dict(shared=none), dict(runs=0), dict(runs=-1), dict(runs=4), dict(runs=12), dict(ws=none),
+                dict(ws=ctypes.c_void_p(8)), dict(heads=3), dict(o=none), dict(D=24), dict(lengths=none), dict(B=0)):
+        assert call(**bad) == 1 and "enatten_cache_attention_shared" in lib.enatten_last_error().decode(), bad
+    need = lambda B=6, runs=2, T=1, cols=3, heads=4: lib.enatten_cache_attention_shared_workspace_bytes(
+        B, heads, 2, T, 32, 16, cols, 0, _lib.BF16, runs)
+    rows = lambda B, T: (B * 4 * T * 34 + 3) // 4 * 16   # sums of values, maximum and sum of every row
+    assert need() >= rows(6, 1) and need(T=3) >= rows(6, 3) and need(cols=4096) > need()
+    for bad in (dict(B=0), dict(runs=0), dict(runs=4), dict(T=0), dict(cols=0), dict(heads=3), dict(T=1 << 28)):
+        assert need(**bad) == 0
+
+
+def test_kernels_do_not_spill_beside_accumulation_registers():
+    """As those for sequences by themselves: a spilled operand of a matrix instruction is sound only where every
+    spilled register goes to memory, that is in kernels without accumulation registers.  Every instantiation of
+    the two passes has to be there."""
+    ensure_built()
+    from test_sequence_host import _registers
+    found = _registers()
+    ours = {kind: {n: v for n, v in found.items() if re.match(r"_ZN7enatten12_GLOBAL__N_1%d%sI" % (len(kind), kind), n)}
+            for kind in ("run_attend", "run_join", "run_rows", "run_join_rows")}
+    assert {kind: len(v) for kind, v in ours.items()} == {"run_attend": 96, "run_join": 24, "run_rows": 32, "run_join_rows": 16}
+    for kind, kernels in ours.items():
+        assert not {n: v for n, v in kernels.items() if v[1] and (v[0] or kind != "run_rows")}
