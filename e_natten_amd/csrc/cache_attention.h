@@ -470,24 +470,18 @@ __device__ __forceinline__ void put_canon(const SharedArgs &a, const Place &p, i
         a.canon[rows * (a.D + 1) + row] = sum;
     }
 }
-// The factors of a row's own part and of that one, both for the same maximum; the row's sum becomes that of both.
-struct Joined {
-    float mine, other;
-    const float *y;  // nullptr: nothing to join
-};
-__device__ __forceinline__ Joined join_canon(const SharedArgs &a, const Place &p, bool shares, float top, float &sum) {
-    Joined j{1.f, 0.f, nullptr};
-    if (!shares) return j;
-    const int64_t row = canon_row(a, p), rows = (int64_t)a.B * a.heads * a.T;
+// A row's own part and that one joined: the factors of both for the larger maximum; the row's sum becomes that of
+// both.  (Numbers by themselves and no struct: what the compiler keeps of one in an array goes through LDS, and
+// finding its place there takes a load from the queue's packet, in host memory, which cost 12 us.)
+__device__ __forceinline__ void join_canon(const SharedArgs &a, int64_t row, float top, float &sum, float &mine, float &other) {
+    const int64_t rows = (int64_t)a.B * a.heads * a.T;
     const float m = a.canon[rows * a.D + row], l = a.canon[rows * (a.D + 1) + row], most = fmaxf(top, m);
-    j.mine = __builtin_amdgcn_exp2f(top - most);
-    j.other = __builtin_amdgcn_exp2f(m - most);
-    j.y = a.canon + row * a.D;
-    sum = j.mine * sum + j.other * l;
-    return j;
+    mine = __builtin_amdgcn_exp2f(top - most);
+    other = __builtin_amdgcn_exp2f(m - most);
+    sum = mine * sum + other * l;
 }
-__device__ __forceinline__ f32x4 joined(const Joined &j, int d, f32x4 y) {
-    return j.y ? j.mine * y + j.other * *reinterpret_cast<const f32x4 *>(j.y + d) : y;
+__device__ __forceinline__ f32x4 canon_values(const SharedArgs &a, int64_t row, int d) {
+    return *reinterpret_cast<const f32x4 *>(a.canon + row * a.D + d);
 }
 
 __device__ __forceinline__ float lane_float(float x, int l) {

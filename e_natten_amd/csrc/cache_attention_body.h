@@ -398,9 +398,12 @@ __device__ __forceinline__ void attend_body(const Args &a) {
         const Place where = place_of(a, which, head, row0 + r);
         const int64_t at = offset_of(a.o, where);
         const bool live = where.t < s.count;
-        Joined j{};
-        if constexpr (kSecondPass<Args>)
-            if (w.items <= 1) j = join_canon(a, where, joins > 0 && live, top, all);
+        float mine = 1.f, other = 0.f;
+        bool joined = false;
+        if constexpr (kSecondPass<Args>) {
+            joined = joins > 0 && live && w.items <= 1;
+            if (joined) join_canon(a, canon_row(a, where), top, all, mine, other);
+        }
         const float norm = all == 0.f || !live ? 0.f : 1.f / all;
 #pragma unroll
         for (int c = 0; c < DP; c += 64) {
@@ -416,7 +419,8 @@ __device__ __forceinline__ void attend_body(const Args &a) {
             if constexpr (kFirstPass<Args>) {
                 put_canon(a, where, d, d == 0, top, all, y);
             } else {
-                if constexpr (kSecondPass<Args>) y = joined(j, d, y);
+                if constexpr (kSecondPass<Args>)
+                    if (joined) y = mine * y + other * canon_values(a, canon_row(a, where), d);
                 store_channels<DT>(a.o, at + d, (live ? y * norm : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
             }
         }
@@ -494,7 +498,11 @@ __device__ __forceinline__ void join_body(const Args &a) {
         }
         if constexpr (kSecondPass<Args>) {
             const Span s = plain_span<ROWS>(a, entry);
-            y = joined(join_canon(a, where, shared_by(a, which, s) > 0 && where.t < s.count, top, sum), c * 4, y);
+            if (shared_by(a, which, s) > 0 && where.t < s.count) {
+                float mine, other;
+                join_canon(a, canon_row(a, where), top, sum, mine, other);
+                y = mine * y + other * canon_values(a, canon_row(a, where), c * 4);
+            }
         }
         const int count = a.tb.counts ? a.tb.counts[which] : a.T;
         const float norm = sum == 0.f ? 0.f : 1.f / sum;

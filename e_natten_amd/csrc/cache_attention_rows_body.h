@@ -410,11 +410,12 @@ __device__ __forceinline__ void rows_body(const Args &args) {
     const float poison = s.ok ? 0.f : __uint_as_float(0x7fc00000u);
     const int row = row0 + n, all_rows = rows_of(a);
     const bool here = row < all_rows, live = here && row / a.group < s.count;
-    Joined other{};
-    Place where{};
-    if constexpr (kShared<Args>) {
-        where = place_of(a, which, head, min(row, all_rows - 1));
-        if (kSecondPass<Args> && !parted) other = join_canon(a, where, joins > 0 && live, m, l);
+    const Place where = place_of(a, which, head, min(row, all_rows - 1));
+    float mine = 1.f, other = 0.f;
+    bool joined = false;
+    if constexpr (kSecondPass<Args>) {
+        joined = joins > 0 && live && !parted;
+        if (joined) join_canon(a, canon_row(a, where), m, l, mine, other);
     }
     const float norm = l == 0.f ? 0.f : 1.f / l;
     // 4 neighbouring channels, 4 mm + 128 i: words of one value row, blocks i of O, or for DP 64 rows 16 apart too
@@ -424,8 +425,13 @@ __device__ __forceinline__ void rows_body(const Args &args) {
     };
     // a row's 4 channels from d on, divided; in the second pass with what the shared tokens come to
     auto with_back = [&](int i, int j, int d) {
-        if constexpr (kSecondPass<Args>) return joined(other, min(d, a.D - 4), channels(i, j) * back) * norm;
-        else return channels(i, j) * norm * back;
+        if constexpr (kSecondPass<Args>) {
+            f32x4 y = channels(i, j) * back;
+            if (joined) y = mine * y + other * canon_values(a, canon_row(a, where), min(d, a.D - 4));
+            return y * norm;
+        } else {
+            return channels(i, j) * norm * back;
+        }
     };
     constexpr int BIG = DP == 256 ? 2 : 1, JS = DP == 64 ? 8 : 16;
     if (parted) {
@@ -571,9 +577,12 @@ __device__ __forceinline__ void join_rows_body(const Args &a) {
     if (row >= all_rows) return;
     const Place where = place_of(a, which, head, row);
     const int64_t to = offset_of(a.o, where);
-    Joined other{};
-    if constexpr (kSecondPass<Args>)
-        other = join_canon(a, where, shared_by(a, which, plain_span<kWideRows>(a, entry)) > 0 && where.t < count, top, sum);
+    float mine = 1.f, other = 0.f;
+    bool joined = false;
+    if constexpr (kSecondPass<Args>) {
+        joined = shared_by(a, which, plain_span<kWideRows>(a, entry)) > 0 && where.t < count;
+        if (joined) join_canon(a, canon_row(a, where), top, sum, mine, other);
+    }
     const float norm = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int k = 0; k < WORDS / 4; k++) {
@@ -585,7 +594,8 @@ __device__ __forceinline__ void join_rows_body(const Args &a) {
         if constexpr (kFirstPass<Args>) {
             put_canon(a, where, d, d == 0, top, sum, z);
         } else {
-            if constexpr (kSecondPass<Args>) z = joined(other, d, z);
+            if constexpr (kSecondPass<Args>)
+                if (joined) z = mine * z + other * canon_values(a, canon_row(a, where), d);
             store_channels<DT>(a.o, to + d, where.t < count ? z * norm : f32x4{0.f, 0.f, 0.f, 0.f});
         }
     }
