@@ -21,8 +21,8 @@ SOURCES = ["na2d_mfma.hip", "na2d_mfma_narrow.hip", "na2d_mfma_dilated.hip", "na
            "enatten_capi.hip", "enatten_prof.cpp", "na2d_simt.hip",
            "na2d_f64.hip", "na2d_mfma_fused.hip", "na2d_mfma_onepass.hip", "na2d_mfma_f32.hip", "na1d_mfma.hip",
            "na1d_mfma_narrow.hip", "na1d_band_mfma.hip", "rotary.hip", "cache_append.hip",
-           "cache_attention.hip", "cache_attention_rows.hip", "cache_attention_first.hip",
-           "cache_attention_second.hip", "cache_attention_shared_rows.hip", "cache_attention_shared.hip", "cache_pages.hip"]
+           "cache_attention.hip", "cache_attention_rows.hip", "cache_attention_shared.hip",
+           "cache_attention_shared_rows.hip", "cache_pages.hip"]
 TORCH_SOURCES = ["torch_shim.cpp", "torch_sequence.cpp", "torch_pages.cpp"]
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden",

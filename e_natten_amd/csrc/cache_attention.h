@@ -19,14 +19,18 @@ struct AttnArgs {
     float *ws;       // (part_of)
 };
 
-// Sequences in runs that share their first tokens: two passes over the same kernels.  In the first an entry is a
-// run, its rows are those of all its sequences and its tokens the shared ones; what they come to goes to `canon`.
-// In the second an entry is a sequence with the tokens behind, and that is joined in.  A type of its own, so that
-// the other kernels' arguments stay what they are.
+// Sequences in runs that share their first tokens (cache_attention_shared.hip).  The first part of the work: an entry
+// is a run, its rows are those of all its sequences, its tokens the shared ones; the second: an entry is a
+// sequence with the tokens behind.  Types of their own, so that the other kernels' arguments stay what they are.
 struct SharedArgs : AttnArgs {
-    const int *shared;  // [runs], tokens
-    int runs, size;     // sequences of a run
-    float *canon;       // rows (b, head, t): their sums of D values each, then the maxima, then the sums
+    const int *shared;   // [runs], tokens
+    int runs, size;      // sequences of a run
+    // of the first part: what row_tiles, parts and ws are of the second; the items of its tiles of 16 rows, which
+    // come before the second part's in one launch (0: it has tiles of more rows and a launch of its own)
+    int first_tiles, first_parts, first_items, first_rows;
+    float *first_ws;
+    float *canon;        // what the first part comes to, joined: rows (b, head, t), their sums of D values, then
+                         // their maxima, then their sums; where the second part has tiles of kWideRows rows
 };
 template <int PASS> struct PassArgs : SharedArgs {};
 
@@ -75,18 +79,32 @@ __device__ __forceinline__ Span plain_span(const AttnArgs &a, int entry) {
     return s;
 }
 template <class Args> constexpr bool kShared = std::is_base_of_v<SharedArgs, Args>;
-template <class Args> constexpr bool kFirstPass = std::is_same_v<Args, PassArgs<1>>;
-template <class Args> constexpr bool kSecondPass = std::is_same_v<Args, PassArgs<2>>;
-// (sequences or runs) x row tiles, and the rows that one of these has per cache head
+// (sequences or runs) x row tiles, and the rows that one of these has per cache head.  `first` wherever it stands: of
+// the first part of a call with shared tokens.
 template <class Args>
-__device__ __forceinline__ int entries_of(const Args &a) {
-    if constexpr (kFirstPass<Args>) return a.runs * a.row_tiles;
+__device__ __forceinline__ int tiles_of(const Args &a, bool first) {
+    if constexpr (kShared<Args>) return first ? a.first_tiles : a.row_tiles;
+    else return a.row_tiles;
+}
+template <class Args>
+__device__ __forceinline__ int entries_of(const Args &a, bool first) {
+    if constexpr (kShared<Args>) return first ? a.runs * a.first_tiles : a.B * a.row_tiles;
     else return a.B * a.row_tiles;
 }
 template <class Args>
-__device__ __forceinline__ int rows_of(const Args &a) {
-    if constexpr (kFirstPass<Args>) return a.T * a.group * a.size;
+__device__ __forceinline__ int rows_of(const Args &a, bool first) {
+    if constexpr (kShared<Args>) return a.T * a.group * (first ? a.size : 1);
     else return a.T * a.group;
+}
+template <class Args>
+__device__ __forceinline__ int parts_of(const Args &a, bool first) {
+    if constexpr (kShared<Args>) return first ? a.first_parts : a.parts;
+    else return a.parts;
+}
+template <class Args>
+__device__ __forceinline__ float *ws_of(const Args &a, bool first) {
+    if constexpr (kShared<Args>) return first ? a.first_ws : a.ws;
+    else return a.ws;
 }
 // How many tokens run r shares: whole pages.
 __device__ __forceinline__ int shared_end(const SharedArgs &a, int r) {
@@ -99,25 +117,27 @@ __device__ __forceinline__ int shared_by(const SharedArgs &a, int b, const Span 
     return s.ok && s.count > 0 && s.start >= end ? end : 0;
 }
 template <int ROWS, class Args>
-__device__ __forceinline__ Span span_of(const Args &a, int entry) {
-    if constexpr (kFirstPass<Args>) {
-        const int r = entry / a.row_tiles;
-        Span s{0, 0, 0, 0, shared_end(a, r), true};
-        if (a.window && s.hi) {  // from the first token on that any row sees
-            int least = s.hi;
-            for (int i = 0; i < a.size; i++) {
-                int len, count;
-                if (sequence_of(a.tb, r * a.size + i, len, count) && count > 0 && len - count >= s.hi)
-                    least = min(least, max(len - count + 1 - a.window, 0));
+__device__ __forceinline__ Span span_of(const Args &a, int entry, bool first) {
+    if constexpr (kShared<Args>) {
+        if (first) {
+            const int r = entry / a.first_tiles;
+            Span s{0, 0, 0, 0, shared_end(a, r), true};
+            if (a.window && s.hi) {  // from the first token on that any row sees
+                int least = s.hi;
+                for (int i = 0; i < a.size; i++) {
+                    int len, count;
+                    if (sequence_of(a.tb, r * a.size + i, len, count) && count > 0 && len - count >= s.hi)
+                        least = min(least, max(len - count + 1 - a.window, 0));
+                }
+                s.lo = least;
             }
-            s.lo = least;
+            return s;
         }
+        Span s = plain_span<ROWS>(a, entry);
+        if (s.hi > s.lo) s.lo = max(s.lo, shared_by(a, entry / a.row_tiles, s));
         return s;
     } else {
-        Span s = plain_span<ROWS>(a, entry);
-        if constexpr (kSecondPass<Args>)
-            if (s.hi > s.lo) s.lo = max(s.lo, shared_by(a, entry / a.row_tiles, s));
-        return s;
+        return plain_span<ROWS>(a, entry);
     }
 }
 // steps of TOK tokens, from the group of 16 that holds the first one on
@@ -133,11 +153,11 @@ struct Share {
 };
 // WAVES: how many waves share the steps of an item (each takes whole ones).
 template <int ROWS, int TOK, int WAVES, class Args>
-__device__ __forceinline__ Share share_of(const Args &a, int item) {
+__device__ __forceinline__ Share share_of(const Args &a, int item, bool first) {
     Share w;
     w.item = item;
-    const int entries = entries_of(a), lane = threadIdx.x & 63;
-    auto steps_at = [&](int e) { return e < entries ? steps_of<TOK>(span_of<ROWS>(a, e)) : 0; };
+    const int entries = entries_of(a, first), lane = threadIdx.x & 63;
+    auto steps_at = [&](int e) { return e < entries ? steps_of<TOK>(span_of<ROWS>(a, e, first)) : 0; };
     float total = 0.f;
     int steps = 0;
     for (int e0 = 0; e0 < entries; e0 += 64) {
@@ -145,7 +165,7 @@ __device__ __forceinline__ Share share_of(const Args &a, int item) {
         total += (float)(unsigned)__builtin_amdgcn_readlane(running_sum(steps), 63);
     }
     // (a little more than the quotient: the items are at most `parts` and one for every entry)
-    const int each = (int)(total * 1.00001f / a.parts) + 1;
+    const int each = (int)(total * 1.00001f / parts_of(a, first)) + 1;
     const int chunk = max(kLeast / TOK, each + WAVES - 1) / WAVES * WAVES;
     int before = 0;
     for (int e0 = 0; e0 < entries; e0 += 64) {
@@ -181,36 +201,41 @@ struct Ranges {
     bool whole;          // no more tiles than ranges, and nearly as long as those: a tile each, none cut
 };
 template <int ROWS, int TOK, class Args>
-__device__ __forceinline__ int counted_steps(const Args &a, int e) {
-    return e < entries_of(a) ? max(1, steps_of<TOK>(span_of<ROWS>(a, e))) : 0;
+__device__ __forceinline__ int counted_steps(const Args &a, int e, bool first) {
+    return e < entries_of(a, first) ? max(1, steps_of<TOK>(span_of<ROWS>(a, e, first))) : 0;
 }
 template <int ROWS, int TOK, class Args>
-__device__ __forceinline__ Ranges ranges_of(const Args &a) {
-    const int entries = entries_of(a), lane = threadIdx.x & 63;
+__device__ __forceinline__ Ranges ranges_of(const Args &a, bool first) {
+    const int entries = entries_of(a, first), lane = threadIdx.x & 63;
     Ranges r{0, 0, false};
     int most = 0;
     for (int e0 = 0; e0 < entries; e0 += 64) {
-        const int n = counted_steps<ROWS, TOK>(a, e0 + lane);
+        const int n = counted_steps<ROWS, TOK>(a, e0 + lane, first);
         most = max(most, n);
         r.line += (unsigned)__builtin_amdgcn_readlane(running_sum(n), 63);
     }
-    r.each = (r.line * a.heads_kv + a.parts - 1) / a.parts;
+    const int parts = parts_of(a, first);
+    r.each = (r.line * a.heads_kv + parts - 1) / parts;
+    if (first) {  // all tiles leave parts; ranges of 128 tokens at least
+        r.each = max(r.each, (int64_t)(128 / TOK));
+        return r;
+    }
     // The parts of cut tiles are their rows' sums in float32, written and read, which takes as long as some
     // steps: at 128 channels about 2 for 64 tiles of 256 rows.  A tile for every workgroup pays where the
     // longest is hardly longer than that beyond the mean.  2048 tokens each of 16384 and 12288 (256 tiles
     // of 224 steps on average, 256 at most): 506 us cut, 570 whole; 256 tokens each of 8 sequences of 300
     // (128 tiles of 5): 37 us cut, 27 whole; half as many tiles: 21 us cut, 24 whole.
     const int64_t tiles = (int64_t)entries * a.heads_kv;
-    const int64_t steps = tiles * min(ROWS, rows_of(a)) * padded(a.D) >> 20;
+    const int64_t steps = tiles * min(ROWS, rows_of(a, first)) * padded(a.D) >> 20;
     r.whole = tiles <= a.parts && !__any(most > r.each + steps);
     return r;
 }
 // The row tile at step `y` of a head's line, and how far into it that is
 template <int ROWS, int TOK, class Args>
-__device__ __forceinline__ int tile_at(const Args &a, int64_t y, int &into) {
-    const int entries = entries_of(a), lane = threadIdx.x & 63;
+__device__ __forceinline__ int tile_at(const Args &a, int64_t y, int &into, bool first) {
+    const int entries = entries_of(a, first), lane = threadIdx.x & 63;
     for (int e0 = 0; e0 < entries; e0 += 64) {
-        const unsigned n = counted_steps<ROWS, TOK>(a, e0 + lane), upto = running_sum(n);
+        const unsigned n = counted_steps<ROWS, TOK>(a, e0 + lane, first), upto = running_sum(n);
         const unsigned all = __builtin_amdgcn_readlane(upto, 63);
         if (y < all) {
             const unsigned long long who = __ballot((unsigned)y < upto);
@@ -233,13 +258,14 @@ __device__ __forceinline__ float *slot_of(const AttnArgs &a, int slot) {
 // sums of its rows and rows x D sums of values.
 __host__ __device__ inline int64_t head_floats(int64_t entries) { return (2 * entries + 3) / 4 * 4; }
 template <class Args>
-__device__ __forceinline__ float *part_of(const Args &a, int rows, int item, int head) {
-    return a.ws + head_floats((int64_t)entries_of(a)) + ((int64_t)item * a.heads_kv + head) * item_floats(rows, a.D);
+__device__ __forceinline__ float *part_of(const Args &a, int rows, int item, int head, bool first) {
+    return ws_of(a, first) + head_floats((int64_t)entries_of(a, first)) + ((int64_t)item * a.heads_kv + head) * item_floats(rows, a.D);
 }
 // (for the launch that joins the parts)
-__device__ __forceinline__ void note_share(const AttnArgs &a, const Share &w, int head) {
+template <class Args>
+__device__ __forceinline__ void note_share(const Args &a, const Share &w, int head, bool first) {
     if (w.item == w.first && head == 0 && threadIdx.x == 0) {
-        int *note = reinterpret_cast<int *>(a.ws) + 2 * w.entry;
+        int *note = reinterpret_cast<int *>(ws_of(a, first)) + 2 * w.entry;
         note[0] = w.first;
         note[1] = w.items;
     }
@@ -445,27 +471,35 @@ struct Place {
     int b, t, head;
 };
 template <class Args>
-__device__ __forceinline__ Place place_of(const Args &a, int which, int head, int row) {  // which: sequence or run
+__device__ __forceinline__ Place place_of(const Args &a, int which, int head, int row, bool first) {  // which: sequence or run
     Place p{which, row / a.group, 0};
     p.head = head * a.group + row - p.t * a.group;
-    if constexpr (kFirstPass<Args>) {
-        const int i = p.t / a.T;
-        p.b = which * a.size + i;
-        p.t -= i * a.T;
+    if constexpr (kShared<Args>) {
+        if (first) {
+            const int i = p.t / a.T;
+            p.b = which * a.size + i;
+            p.t -= i * a.T;
+        }
     }
     return p;
 }
 __device__ __forceinline__ int64_t offset_of(const Rows &r, const Place &p) { return p.b * r.sb + p.head * r.sh + p.t * r.st; }
 
-// What a run's rows come to over the shared tokens, for the second pass: sums of values (4 channels from d on), and
-// by whoever has `first`, the maximum and the sum.
+// Parts of the first part's tiles of many rows.  Tiles and ranges that have one in common follow each other like steps
+// of a staircase, so that (range + tile) is a place of its own for each such pair.  Before the places for every tile
+// its first and its last range; a place has the maxima of its rows, their sums, and the sums of values in the order of
+// the registers.
+__device__ __forceinline__ float *stair_of(const SharedArgs &a, int64_t place) {
+    const int64_t tiles = (int64_t)a.runs * a.first_tiles * a.heads_kv;
+    return a.first_ws + (2 * tiles + 3) / 4 * 4 + place * item_floats(a.first_rows, padded(a.D));
+}
 __device__ __forceinline__ int64_t canon_row(const SharedArgs &a, const Place &p) {
     return ((int64_t)p.b * a.heads + p.head) * a.T + p.t;
 }
-__device__ __forceinline__ void put_canon(const SharedArgs &a, const Place &p, int d, bool first, float top, float sum, f32x4 y) {
-    const int64_t row = canon_row(a, p), rows = (int64_t)a.B * a.heads * a.T;
+__device__ __forceinline__ void put_canon(const SharedArgs &a, int64_t row, int d, float top, float sum, f32x4 y) {
+    const int64_t rows = (int64_t)a.B * a.heads * a.T;
     *reinterpret_cast<f32x4 *>(a.canon + row * a.D + d) = y;
-    if (first) {
+    if (d == 0) {
         a.canon[rows * a.D + row] = top;
         a.canon[rows * (a.D + 1) + row] = sum;
     }
@@ -496,9 +530,12 @@ __device__ __forceinline__ int64_t lane_offset(int64_t x, int l) {
 
 // Tiles of kWideRows rows (cache_attention_rows.hip), a.parts ranges
 int launch_attend_rows(const char *fn, const AttnArgs &a, bool e4m3, hipStream_t st);
-int launch_rows_first(const char *fn, const SharedArgs &a, bool e4m3, hipStream_t st);
-int launch_rows_second(const char *fn, const SharedArgs &a, bool e4m3, hipStream_t st);
-// The same and the kernels of cache_attention.hip in the two passes (cache_attention_first.hip, _second.hip)
+// Tiles of 128 or kWideRows rows of the first part, of kWideRows of the second, and the joins behind them
+// (cache_attention_shared_rows.hip)
+int launch_first_rows(const char *fn, const SharedArgs &a, int rows, bool e4m3, hipStream_t st);
+int launch_first_join(const char *fn, const SharedArgs &a, int rows, hipStream_t st);  // into canon
+int launch_last_join(const char *fn, const SharedArgs &a, int rows, int second_rows, hipStream_t st);
+int launch_second_rows(const char *fn, const SharedArgs &a, bool e4m3, hipStream_t st);
 Plan plan_of(int B, int heads, int heads_kv, int T, int D, int page, int columns, int window, int dtype);
 size_t workspace_bytes(const Plan &p, int B, int heads_kv, int D);  // B: sequences, or runs
 // The arguments that all calls have, checked, but for row_tiles, parts and ws
@@ -508,7 +545,5 @@ int set_attention(const char *fn, const void *q, const void *k_cache, const void
                   int cache_dtype, const int64_t *q_strides, const int64_t *o_strides, const int64_t *k_cache_strides,
                   const int64_t *v_cache_strides, const int64_t *k_scale_strides, const int64_t *v_scale_strides,
                   int64_t pages_stride, float scale, AttnArgs *a);
-int launch_first(const char *fn, const SharedArgs &a, const Plan &p, bool e4m3, hipStream_t st);
-int launch_second(const char *fn, const SharedArgs &a, const Plan &p, bool e4m3, hipStream_t st);
 
 }  // namespace enatten

@@ -20,8 +20,7 @@ __device__ __forceinline__ int reader_of(const SharedArgs &a, int r, int end) {
     return -1;
 }
 // The first shared token that a row sees.
-template <class Args>
-__device__ __forceinline__ int shared_lo(const Args &a, const Place &p, int end) {
+__device__ __forceinline__ int shared_lo(const SharedArgs &a, const Place &p, int end) {
     int len, count;
     if (!a.window || !sequence_of(a.tb, p.b, len, count) || p.t >= count || len - count < end) return 0;
     return min(max(len - count + p.t + 1 - a.window, 0), end);
@@ -58,30 +57,40 @@ __device__ __forceinline__ void attend_body(const Args &a) {
 
     // which row tile, and which of its steps
     const int head = blockIdx.x % a.heads_kv;
+    int item = blockIdx.x / a.heads_kv;
+    bool first = false;
+    if constexpr (kShared<Args> && R == 1) {
+        first = item < a.first_items;
+        if (!first) item -= a.first_items;
+    }
+    const int parts = parts_of(a, first);
     Share w;
-    if (a.parts) {
-        w = share_of<ROWS, TOK, 4>(a, blockIdx.x / a.heads_kv);
+    if (parts) {
+        w = share_of<ROWS, TOK, 4>(a, item, first);
         if (w.entry < 0) return;
-        note_share(a, w, head);
+        note_share(a, w, head, first);
     } else {
-        w.entry = blockIdx.x / a.heads_kv;
+        w.entry = w.item = item;
         w.items = 1;
     }
     const int entry = w.entry;
-    const Span s = span_of<ROWS>(a, entry);
-    if (!a.parts) {
+    const Span s = span_of<ROWS>(a, entry, first);
+    if (!parts) {
         w.step0 = 0;
         w.step1 = steps_of<TOK>(s);
     }
-    const int which = entry / a.row_tiles, row0 = (entry - which * a.row_tiles) * ROWS;
-    int b = which, all_rows = a.T * a.group, joins = 0;  // joins: shared tokens, whose part the second pass joins in
+    const int which = entry / tiles_of(a, first), row0 = (entry - which * tiles_of(a, first)) * ROWS;
+    int b = which, joins = 0;  // joins: shared tokens, which are not the second part's
+    const int all_rows = rows_of(a, first);
     int step0 = w.step0, step1 = w.step1;
-    if constexpr (kFirstPass<Args>) {
-        all_rows = rows_of(a);
-        b = reader_of(a, which, s.hi);
-        if (b < 0) b = which * a.size, step0 = step1 = 0;  // (nobody reads them)
+    if constexpr (kShared<Args>) {
+        if (first) {
+            b = reader_of(a, which, s.hi);
+            if (b < 0) b = which * a.size, step0 = step1 = 0;  // (nobody reads them)
+        } else {
+            joins = shared_by(a, which, s);
+        }
     }
-    if constexpr (kSecondPass<Args>) joins = shared_by(a, which, s);
     const int base = s.lo & -16;
 
     // q: lane (row n16, g4) has channels 64 c + 16 g4 .. + 15
@@ -93,16 +102,17 @@ __device__ __forceinline__ void attend_body(const Args &a) {
 #pragma unroll
     for (int r = 0; r < R; r++) {
         const int row = min(row0 + r * 16 + n16, all_rows - 1);
-        const Place where = place_of(a, which, head, row);
-        if constexpr (kFirstPass<Args>) {
-            hi_r[r] = s.hi;  // (rows of a sequence that does not share them come to what nobody reads)
-            lo_r[r] = shared_lo(a, where, s.hi);
-            if (a.window) most_lo = max(most_lo, lo_r[r]);
-        } else {
-            const int tv = min(where.t, max(s.count - 1, 0));
-            hi_r[r] = s.start + tv + 1;
-            lo_r[r] = a.window ? max(hi_r[r] - a.window, 0) : 0;
-            if constexpr (kSecondPass<Args>) lo_r[r] = max(lo_r[r], joins);
+        const Place where = place_of(a, which, head, row, first);
+        const int tv = min(where.t, max(s.count - 1, 0));
+        hi_r[r] = s.start + tv + 1;
+        lo_r[r] = a.window ? max(hi_r[r] - a.window, 0) : 0;
+        if constexpr (kShared<Args>) {
+            lo_r[r] = max(lo_r[r], joins);
+            if (first) {
+                hi_r[r] = s.hi;  // (rows of a sequence that does not share them come to what nobody reads)
+                lo_r[r] = shared_lo(a, where, s.hi);
+                if (a.window) most_lo = max(most_lo, lo_r[r]);
+            }
         }
         const int64_t at = offset_of(a.q, where);
         float x[KC][16], top = 0.f, nan = a.scale * 0.f;
@@ -146,10 +156,12 @@ __device__ __forceinline__ void attend_body(const Args &a) {
     // between these all rows see every token
     int all_lo = a.window ? max(s.start + min((row0 + ROWS - 1) / a.group, s.count - 1) + 1 - a.window, 0) : 0;
     int all_hi = s.start + row0 / a.group + 1;
-    if constexpr (kSecondPass<Args>) all_lo = max(all_lo, joins);
-    if constexpr (kFirstPass<Args>) {
-        all_lo = a.window ? wave_max(most_lo) : 0;
-        all_hi = s.hi;
+    if constexpr (kShared<Args>) {
+        all_lo = max(all_lo, joins);
+        if (first) {
+            all_lo = a.window ? wave_max(most_lo) : 0;
+            all_hi = s.hi;
+        }
     }
 
     f32x4 acc[R][CW];
@@ -380,7 +392,8 @@ __device__ __forceinline__ void attend_body(const Args &a) {
     }
     __syncthreads();
     const float poison = s.ok ? 0.f : __uint_as_float(0x7fc00000u);
-    float *part = part_of(a, ROWS, w.item, head);
+    const bool leaves = kShared<Args> || w.items > 1;  // its part, for another launch
+    float *part = part_of(a, ROWS, w.item, head, first);
     const int mc = threadIdx.x & 15;  // of the channels, 4 in 64
     for (int r = threadIdx.x >> 4; r < rows; r += 16) {
         float top = part_m[0][r], f[4], all = 0.f;
@@ -391,19 +404,13 @@ __device__ __forceinline__ void attend_body(const Args &a) {
             f[v] = __builtin_amdgcn_exp2f(part_m[v][r] - top);
             all += f[v] * part_l[v][r];
         }
-        if (w.items > 1 && mc == 0) {
+        if (leaves && mc == 0) {
             part[r] = top;
             part[ROWS + r] = all;
         }
-        const Place where = place_of(a, which, head, row0 + r);
+        const Place where = place_of(a, which, head, row0 + r, first);
         const int64_t at = offset_of(a.o, where);
         const bool live = where.t < s.count;
-        float mine = 1.f, other = 0.f;
-        bool joined = false;
-        if constexpr (kSecondPass<Args>) {
-            joined = joins > 0 && live && w.items <= 1;
-            if (joined) join_canon(a, canon_row(a, where), top, all, mine, other);
-        }
         const float norm = all == 0.f || !live ? 0.f : 1.f / all;
 #pragma unroll
         for (int c = 0; c < DP; c += 64) {
@@ -412,25 +419,16 @@ __device__ __forceinline__ void attend_body(const Args &a) {
             f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int v = 0; v < 4; v++) y += f[v] * *reinterpret_cast<const f32x4 *>(&part_o[v][r][d]);
-            if (w.items > 1) {
-                *reinterpret_cast<f32x4 *>(part + 2 * ROWS + r * a.D + d) = y;
-                continue;
-            }
-            if constexpr (kFirstPass<Args>) {
-                put_canon(a, where, d, d == 0, top, all, y);
-            } else {
-                if constexpr (kSecondPass<Args>)
-                    if (joined) y = mine * y + other * canon_values(a, canon_row(a, where), d);
-                store_channels<DT>(a.o, at + d, (live ? y * norm : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
-            }
+            if (leaves) *reinterpret_cast<f32x4 *>(part + 2 * ROWS + r * a.D + d) = y;
+            else store_channels<DT>(a.o, at + d, (live ? y * norm : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
         }
     }
 }
 
 // The parts of a row joined: one workgroup per (row tile, cache head, row).
-template <int ROWS, int DT, class Args>
-__device__ __forceinline__ void join_body(const Args &a) {
-    const int all_rows = rows_of(a), per = min(ROWS, all_rows);
+template <int ROWS, int DT>
+__device__ __forceinline__ void join_body(const AttnArgs &a) {
+    const int all_rows = a.T * a.group, per = min(ROWS, all_rows);
     int block = blockIdx.x;
     const int r = block % per;
     block /= per;
@@ -439,7 +437,7 @@ __device__ __forceinline__ void join_body(const Args &a) {
     const int first = note[0], items = note[1];
     const int which = entry / a.row_tiles, row = (entry - which * a.row_tiles) * ROWS + r;
     if (items == 1 || row >= all_rows) return;
-    const float *ws = part_of(a, ROWS, first, head);
+    const float *ws = part_of(a, ROWS, first, head, false);
     const int64_t stride = a.heads_kv * item_floats(ROWS, a.D);
 
     // lanes over the channels, 4 each, and the remaining factor of 256 over the items, each with the
@@ -491,19 +489,7 @@ __device__ __forceinline__ void join_body(const Args &a) {
             sum += f * sums[i * lanes];
             y += f * *reinterpret_cast<const f32x4 *>(red[i * lanes + c]);
         }
-        const Place where = place_of(a, which, head, row);
-        if constexpr (kFirstPass<Args>) {
-            put_canon(a, where, c * 4, c == 0, top, sum, y);
-            return;
-        }
-        if constexpr (kSecondPass<Args>) {
-            const Span s = plain_span<ROWS>(a, entry);
-            if (shared_by(a, which, s) > 0 && where.t < s.count) {
-                float mine, other;
-                join_canon(a, canon_row(a, where), top, sum, mine, other);
-                y = mine * y + other * canon_values(a, canon_row(a, where), c * 4);
-            }
-        }
+        const Place where = place_of(a, which, head, row, false);
         const int count = a.tb.counts ? a.tb.counts[which] : a.T;
         const float norm = sum == 0.f ? 0.f : 1.f / sum;
         store_channels<DT>(a.o, offset_of(a.o, where) + c * 4, where.t < count ? y * norm : f32x4{0.f, 0.f, 0.f, 0.f});

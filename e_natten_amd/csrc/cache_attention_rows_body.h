@@ -20,10 +20,13 @@ __device__ __forceinline__ const Args &args_again() {
 }
 
 // DP: head_dim rounded up to 64, 128 or 256; DT: type of q and o, float32 in two float16 terms of q and p.
-template <int DP, bool E4M3, int DT, class Args>
+// WAVES: 8, or 4 for tiles of half as many rows and steps of half as many tokens.
+template <int DP, bool E4M3, int DT, int WAVES, class Args>
 __device__ __forceinline__ void rows_body(const Args &args) {
+    constexpr bool FIRST = std::is_same_v<Args, PassArgs<1>>, SECOND = std::is_same_v<Args, PassArgs<2>>;
+    constexpr int ROWS = 32 * WAVES, HALF = WAVES / 2;
     constexpr int TERMS = DT == ENATTEN_F32 ? 2 : 1;
-    constexpr int TOK = 8192 / DP;    // tokens of a step: 128, 64, 32
+    constexpr int TOK = 1024 * WAVES / DP;  // tokens of a step: 128, 64, 32
     constexpr int NB = TOK / 32;      // blocks of 32 of them
     constexpr int GR = TOK / 16;      // groups of 16, each within a page
     constexpr int SD = DP / 16;       // products along head_dim of S
@@ -33,26 +36,26 @@ __device__ __forceinline__ void rows_body(const Args &args) {
     // operands of one step: K [NB][SD][64 lanes][8], V [OB][TOK / 16][64 lanes][8]; eight lanes that turn
     // one or two tokens write to as many operands of K, which therefore start 1 or 2 lanes apart in the banks
     constexpr int PART = 64 + (CH < 8 ? 8 / CH : 1);
-    __shared__ f16x8 k_lds[2][NB * SD * PART], v_lds[2][1024];
+    __shared__ f16x8 k_lds[2][NB * SD * PART], v_lds[2][TOK * DP / 8];
     __shared__ float z_lds[2][3][GR];  // of the step's groups: key scales, value scales (log2), their inverses
     __shared__ int z_bad[2][2];        // ... and which of either are not finite (0 in their place)
     // Rows of q stay in registers, at head dims above 128 all but the last operands, for which there are
     // none left: those a lane puts into LDS and reads again.
     constexpr int KEPT = DP == 256 ? 10 : SD;
-    __shared__ f16x8 q_lds[8 * 64 * (SD - KEPT) + 1];
+    __shared__ f16x8 q_lds[WAVES * 64 * (SD - KEPT) + 1];
     const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (branches on it are the wave's)
 
     // The workgroup's range of steps.  Blocks 8 apart share an XCD and its L2: they get neighbouring ranges,
     // which read the same keys and values where they belong to the same head.
     const Args &a = args;
-    const int range = blockIdx.x % 8 * (a.parts / 8) + blockIdx.x / 8;
-    const Ranges line = ranges_of<kWideRows, TOK>(a);
+    const int range = blockIdx.x % 8 * (parts_of(a, FIRST) / 8) + blockIdx.x / 8;
+    const Ranges line = ranges_of<ROWS, TOK>(a, FIRST);
     const int heads = a.heads_kv;
     int64_t end = min((range + 1) * line.each, line.line * heads);
     int64_t at_step = range * line.each;
-    const int entries = entries_of(a), all_rows = rows_of(a);
-    int *note = reinterpret_cast<int *>(a.ws) + range;
+    const int entries = entries_of(a, FIRST), all_rows = rows_of(a, FIRST);
+    int *note = reinterpret_cast<int *>(ws_of(a, FIRST)) + range;
     int head, entry, into = 0;
     if (line.whole) {  // a tile each
         head = range / entries;
@@ -61,39 +64,46 @@ __device__ __forceinline__ void rows_body(const Args &args) {
         end = min(end, (int64_t)1);
     } else {
         head = (int)(at_step / line.line);
-        entry = at_step < end ? tile_at<kWideRows, TOK>(a, at_step - head * line.line, into) : 0;
+        entry = at_step < end ? tile_at<ROWS, TOK>(a, at_step - head * line.line, into, FIRST) : 0;
     }
-    if (threadIdx.x == 0) *note = into ? head * entries + entry : -1;
+    if (!FIRST && threadIdx.x == 0) *note = into ? head * entries + entry : -1;
 
     for (; at_step < end; into = 0) {
     const Args &a = args_again<Args>();
-    const Span s = span_of<kWideRows>(a, entry);
+    const Span s = span_of<ROWS>(a, entry, FIRST);
     const int total = steps_of<TOK>(s), counted = max(1, total), step0 = into;
     int step1 = line.whole ? total : min(total, (int)min((int64_t)counted, step0 + (end - at_step)));
-    const bool parted = !line.whole && (into || step0 + (end - at_step) < counted);
+    const bool parted = FIRST || (!line.whole && (into || step0 + (end - at_step) < counted));
     const int slot = into ? 2 * range : 2 * range + 1;
+    if constexpr (FIRST) {
+        if (into == 0 && threadIdx.x == 0) {  // (for the launch that joins the parts)
+            int *ranges = reinterpret_cast<int *>(a.first_ws) + 2 * (head * entries + entry);
+            ranges[0] = range;
+            ranges[1] = (int)((at_step + counted - 1) / line.each);
+        }
+    }
     at_step += counted - into;
-    const int which = entry / a.row_tiles, row0 = (entry - which * a.row_tiles) * kWideRows + wave * 32;
+    const int which = entry / tiles_of(a, FIRST), row0 = (entry - which * tiles_of(a, FIRST)) * ROWS + wave * 32;
     const int base = s.lo & -16;
-    int b = which, joins = 0;  // joins: shared tokens, whose part the second pass joins in
-    if constexpr (kFirstPass<Args>) {
+    int b = which, joins = 0;  // joins: shared tokens, which are not the second part's
+    if constexpr (FIRST) {
         b = reader_of(a, which, s.hi);
         if (b < 0) b = which * a.size, step1 = step0;  // (nobody reads them)
     }
-    if constexpr (kSecondPass<Args>) joins = shared_by(a, which, s);
+    if constexpr (SECOND) joins = shared_by(a, which, s);
 
     // the lane's row; q: lane (n, h) has channels 16 c + 8 h .. + 7
-    const Place where = place_of(a, which, head, min(row0 + n, all_rows - 1));
-    const bool live = row0 + n < all_rows && (kFirstPass<Args> || where.t < s.count);
+    const Place where = place_of(a, which, head, min(row0 + n, all_rows - 1), FIRST);
+    const bool live = row0 + n < all_rows && (FIRST || where.t < s.count);
     int hi_r = live ? s.start + where.t + 1 : 0, seen = a.window ? a.window : hi_r;  // tokens hi_r - seen .. hi_r - 1
     int most_lo = 0;
-    if constexpr (kFirstPass<Args>) {  // (rows of a sequence that does not share them come to what nobody reads)
+    if constexpr (FIRST) {  // (rows of a sequence that does not share them come to what nobody reads)
         const int first = shared_lo(a, where, s.hi);
         if (live) most_lo = first;
         hi_r = live ? s.hi : 0;
         seen = hi_r - first;
     }
-    if constexpr (kSecondPass<Args>) seen = min(seen, hi_r - joins);
+    if constexpr (SECOND) seen = min(seen, hi_r - joins);
     f16x8 qf[KEPT][TERMS], *q_rest = &q_lds[threadIdx.x];
     float unit, l;
     {
@@ -142,7 +152,7 @@ __device__ __forceinline__ void rows_body(const Args &args) {
 #pragma unroll
             for (int t = 0; t < TERMS; t++) {
                 if (c < KEPT) qf[c][t] = w[t];
-                else q_rest[(c - KEPT) * 512] = w[t];
+                else q_rest[(c - KEPT) * (64 * WAVES)] = w[t];
             }
         }
     }
@@ -152,8 +162,8 @@ __device__ __forceinline__ void rows_body(const Args &args) {
     int some_lo = any_row && a.window ? max(s.start + t_first + 1 - a.window, 0) : 0;
     int some_hi = any_row ? s.start + t_last + 1 : 0;
     int all_lo = a.window ? max(s.start + t_last + 1 - a.window, 0) : 0, all_hi = s.start + t_first + 1;
-    if constexpr (kSecondPass<Args>) all_lo = max(all_lo, joins);
-    if constexpr (kFirstPass<Args>) {
+    if constexpr (SECOND) all_lo = max(all_lo, joins);
+    if constexpr (FIRST) {
         some_lo = 0;
         some_hi = row0 < all_rows ? s.hi : 0;
         all_lo = a.window ? wave_max(most_lo) : 0;
@@ -172,7 +182,7 @@ __device__ __forceinline__ void rows_body(const Args &args) {
     int filled = -64;
     int64_t at = 0;
     float z_at = 0.f;  // of keys, or log2 of values (for float32 the scale itself)
-    const bool for_v = wave >= 4;
+    const bool for_v = wave >= HALF;
     auto fill = [&](int group) {
         const Args &a = args_again<Args>();
         filled = group;
@@ -196,10 +206,10 @@ __device__ __forceinline__ void rows_body(const Args &args) {
     };
     // What a thread brings: of keys two runs of 16 codes, of values a word of 4 channels of 8 tokens.
     unsigned raw[8];
-    float raw_z = 0.f;  // lanes 0 .. GR - 1 of wave 0: key scales of the step's groups, of wave 4: value scales
+    float raw_z = 0.f;  // lanes 0 .. GR - 1 of wave 0: key scales of the step's groups, of wave HALF: value scales
     // (offsets within a group of 16 tokens; a wave's 64 runs of keys lie in one group, its 64 words of
     // values too, but for DP 64, where each half of the wave has its own)
-    const int run = (wave & 3) * (64 * 4 / DP) + lane / QUADS, quad = lane % QUADS;  // runs of 8 tokens
+    const int run = wave % HALF * (64 * 4 / DP) + lane / QUADS, quad = lane % QUADS;  // runs of 8 tokens
     const unsigned within = for_v ? run % 2 * 4 * (unsigned)a.v.st + min(quad * 4, a.D - 4)
                                   : (wave * (128 / CH) + lane / CH) % 16 * (unsigned)a.k.st + min(lane % CH * 16, a.D - 16);
     auto fetch = [&](int step) {
@@ -217,8 +227,8 @@ __device__ __forceinline__ void rows_body(const Args &args) {
                 for (int i = 0; i < 4; i++) raw[j * 4 + i] = x[i];
             }
         } else {
-            int64_t off = lane_offset(at, here + (wave & 3) * (64 * 4 / DP) / 2);
-            if constexpr (DP == 64) off = lane < 32 ? off : lane_offset(at, here + (wave & 3) * 2 + 1);
+            int64_t off = lane_offset(at, here + wave % HALF * (64 * 4 / DP) / 2);
+            if constexpr (DP == 64) off = lane < 32 ? off : lane_offset(at, here + wave % HALF * 2 + 1);
             const char *from = static_cast<const char *>(a.v.codes) + off;
 #pragma unroll
             for (int j = 0; j < 8; j++)
@@ -244,7 +254,7 @@ __device__ __forceinline__ void rows_body(const Args &args) {
                 v_lds[buffer][(block * (TOK / 16) + run / 2) * 64 + run % 2 * 32 + mm] = v[i];
             }
         }
-        if ((wave & 3) == 0) {
+        if (wave % HALF == 0) {
             const bool finite = for_v && TERMS == 1 ? raw_z < INFINITY : fabsf(raw_z) < INFINITY;
             const float z = finite ? raw_z : for_v && TERMS == 1 ? -INFINITY : 0.f;
             if (lane < GR) {
@@ -256,10 +266,10 @@ __device__ __forceinline__ void rows_body(const Args &args) {
         }
     };
     // (the workgroup's first and last rows, for the shorter way of turning E4M3)
-    const int wg_row = row0 - wave * 32, wg_last = min((wg_row + kWideRows - 1) / a.group, s.count - 1);
+    const int wg_row = row0 - wave * 32, wg_last = min((wg_row + ROWS - 1) / a.group, s.count - 1);
     int wg_lo = a.window ? max(s.start + wg_last + 1 - a.window, 0) : 0, wg_hi = s.start + wg_row / a.group + 1;
-    if constexpr (kSecondPass<Args>) wg_lo = max(wg_lo, joins);
-    if constexpr (kFirstPass<Args>) {
+    if constexpr (SECOND) wg_lo = max(wg_lo, joins);
+    if constexpr (FIRST) {
         wg_lo = a.window ? s.hi : 0;
         wg_hi = s.hi;
     }
@@ -297,7 +307,7 @@ __device__ __forceinline__ void rows_body(const Args &args) {
                 const f16x8 kf = kp[(i * SD + c) * PART];
 #pragma unroll
                 for (int t = TERMS - 1; t >= 0; t--)
-                    st[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, c < KEPT ? qf[c][t] : q_rest[(c - KEPT) * 512], st[i], 0, 0, 0);
+                    st[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, c < KEPT ? qf[c][t] : q_rest[(c - KEPT) * (64 * WAVES)], st[i], 0, 0, 0);
             }
         }
 
@@ -408,12 +418,12 @@ __device__ __forceinline__ void rows_body(const Args &args) {
     const Args &a = args_again<Args>();
     const float back = power_of_two(ref - kPTop + (E4M3 ? 8 : 0));
     const float poison = s.ok ? 0.f : __uint_as_float(0x7fc00000u);
-    const int row = row0 + n, all_rows = rows_of(a);
+    const int row = row0 + n, all_rows = rows_of(a, FIRST);
     const bool here = row < all_rows, live = here && row / a.group < s.count;
-    const Place where = place_of(a, which, head, min(row, all_rows - 1));
+    const Place where = place_of(a, which, head, min(row, all_rows - 1), FIRST);
     float mine = 1.f, other = 0.f;
     bool joined = false;
-    if constexpr (kSecondPass<Args>) {
+    if constexpr (SECOND) {
         joined = joins > 0 && live && !parted;
         if (joined) join_canon(a, canon_row(a, where), m, l, mine, other);
     }
@@ -425,7 +435,7 @@ __device__ __forceinline__ void rows_body(const Args &args) {
     };
     // a row's 4 channels from d on, divided; in the second pass with what the shared tokens come to
     auto with_back = [&](int i, int j, int d) {
-        if constexpr (kSecondPass<Args>) {
+        if constexpr (SECOND) {
             f32x4 y = channels(i, j) * back;
             if (joined) y = mine * y + other * canon_values(a, canon_row(a, where), min(d, a.D - 4));
             return y * norm;
@@ -436,26 +446,25 @@ __device__ __forceinline__ void rows_body(const Args &args) {
     constexpr int BIG = DP == 256 ? 2 : 1, JS = DP == 64 ? 8 : 16;
     if (parted) {
         // (lane by lane, as it lies in the registers)
-        float *part = slot_of(a, slot);
+        float *part;
+        int rows = kWideRows;
+        if constexpr (FIRST) {
+            part = stair_of(a, (int64_t)range + head * entries_of(a, FIRST) + entry);
+            rows = a.first_rows;
+        } else {
+            part = slot_of(a, slot);
+        }
         if (here && h == 0) {
             part[wave * 32 + n] = m;
-            part[kWideRows + wave * 32 + n] = l;
+            part[rows + wave * 32 + n] = l;
         }
-        f32x4 *to = reinterpret_cast<f32x4 *>(part + 2 * kWideRows) + wave * (BIG * JS) * 64 + lane;
+        f32x4 *to = reinterpret_cast<f32x4 *>(part + 2 * rows) + wave * (BIG * JS) * 64 + lane;
         if (row0 < all_rows) {
 #pragma unroll
             for (int i = 0; i < BIG; i++)
 #pragma unroll
                 for (int j = 0; j < JS; j++) to[(i * JS + j) * 64] = channels(i, j) * back;
         }
-    } else if constexpr (kFirstPass<Args>) {
-#pragma unroll
-        for (int i = 0; i < BIG; i++)
-#pragma unroll
-            for (int j = 0; j < JS; j++) {
-                const int d = 4 * (j / 4 * 8 + h * 4 + j % 4) + i * 128;
-                if (here && d < a.D) put_canon(a, where, d, d == 0, m, l, channels(i, j) * back);
-            }
     } else if constexpr (DT == ENATTEN_F32) {
         const int t_row = row / a.group;
         const int64_t to = b * a.o.sb + (head * a.group + row - t_row * a.group) * a.o.sh + t_row * a.o.st;
@@ -513,17 +522,18 @@ __device__ __forceinline__ void rows_body(const Args &args) {
 // neighbouring words of 4 channels.
 template <int DP, int DT, class Args>
 __device__ __forceinline__ void join_rows_body(const Args &a) {
+    constexpr bool SECOND = std::is_same_v<Args, PassArgs<2>>;
     constexpr int BLOCKS = kWideRows / 16, WORDS = DP / 16;
     const int range = blockIdx.x / BLOCKS, n = threadIdx.x % 16, c = threadIdx.x / 16 % 4, lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int *note = reinterpret_cast<const int *>(a.ws);
     const int tile = note[range];
     if (tile < 0 || note[range - 1] == tile) return;  // (the first range starts with a tile)
-    const int entries = entries_of(a), all_rows = rows_of(a), head = tile / entries, entry = tile - head * entries;
+    const int entries = entries_of(a, false), all_rows = rows_of(a, false), head = tile / entries, entry = tile - head * entries;
     const int which = entry / a.row_tiles, r = blockIdx.x % BLOCKS * 16 + n;
     const int row = (entry - which * a.row_tiles) * kWideRows + r;
     if (row - n >= all_rows) return;  // (none of the 16)
-    const int count = kFirstPass<Args> ? 0 : a.tb.counts ? a.tb.counts[which] : a.T;
+    const int count = a.tb.counts ? a.tb.counts[which] : a.T;
     // the parts: the end of the range before, then the beginnings of the ranges that start within the tile
     int parts = 1;
     for (;; parts += 64) {
@@ -575,11 +585,11 @@ __device__ __forceinline__ void join_rows_body(const Args &a) {
         sum += f[v] * sums[v][n];
     }
     if (row >= all_rows) return;
-    const Place where = place_of(a, which, head, row);
+    const Place where = place_of(a, which, head, row, false);
     const int64_t to = offset_of(a.o, where);
     float mine = 1.f, other = 0.f;
     bool joined = false;
-    if constexpr (kSecondPass<Args>) {
+    if constexpr (SECOND) {
         joined = shared_by(a, which, plain_span<kWideRows>(a, entry)) > 0 && where.t < count;
         if (joined) join_canon(a, canon_row(a, where), top, sum, mine, other);
     }
@@ -591,13 +601,9 @@ __device__ __forceinline__ void join_rows_body(const Args &a) {
         f32x4 z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int v = 0; v < 4; v++) z += f[v] * red[v][i][lane];
-        if constexpr (kFirstPass<Args>) {
-            put_canon(a, where, d, d == 0, top, sum, z);
-        } else {
-            if constexpr (kSecondPass<Args>)
-                if (joined) z = mine * z + other * canon_values(a, canon_row(a, where), d);
-            store_channels<DT>(a.o, to + d, where.t < count ? z * norm : f32x4{0.f, 0.f, 0.f, 0.f});
-        }
+        if constexpr (SECOND)
+            if (joined) z = mine * z + other * canon_values(a, canon_row(a, where), d);
+        store_channels<DT>(a.o, to + d, where.t < count ? z * norm : f32x4{0.f, 0.f, 0.f, 0.f});
     }
 }
 

@@ -4,30 +4,144 @@
 //
 // with maximum m, sum l and sums of values y over a sequence's own tokens, and m', l', y' over those that it
 // shares with its run.  The latter are a product of their own with as many rows as the whole run has, so that
-// the shared codes are read once for all of them and, from 49 rows on (65 of up to 64 channels), turned into
-// float16 once.  Both are the kernels of cache_attention.hip over other rows and tokens: a first pass whose
-// entries are runs leaves m', l' and y' in the workspace, a second one goes over the tokens behind and joins
-// them in where it writes.
-#include "cache_attention.h"
+// the shared codes are read once for all of them.  Both parts of the work are the kernels of cache_attention.hip and
+// cache_attention_rows.hip over other rows and tokens, and leave what they come to in the workspace; the last
+// launch joins it.
+//
+// Up to 16 rows in a run both parts are tiles of 16 rows and one launch.  Beyond, the first part has tiles of
+// 128 or 256 rows over codes that LDS holds as float16, in a launch of its own, also where only some of a
+// tile's rows are there: its waves without rows turn codes, and two workgroups per CU hide each other's waits.
+#include "cache_attention_body.h"
 
 namespace enatten {
 namespace {
 
-// Both passes' plans, and where their workspaces lie: what the runs' rows come to, then what either pass needs.
+template <int DP, int R, bool E4M3, int DT>
+__global__ __launch_bounds__(256, waves_of(DP, R, DT == ENATTEN_F32 ? 2 : 1)) void run_attend(SharedArgs a) {
+    attend_body<DP, R, E4M3, DT>(a);
+}
+
+// The parts of both halves of the work joined, where both have tiles of 16 rows: one workgroup per row.  Lanes over
+// the channels, 4 each, and the remaining factor of 256 over the parts.
+template <int DT>
+__global__ __launch_bounds__(256) void run_join_tiles(SharedArgs a) {
+    int block = blockIdx.x;
+    const int head = block % a.heads, hk = head / a.group, g = head - hk * a.group;
+    block /= a.heads;
+    const int t = block % a.T, b = block / a.T, which = b / a.size;
+    int len, count;
+    const bool ok = sequence_of(a.tb, b, len, count), shares = ok && count > 0 && len - count >= shared_end(a, which);
+    // (a part that is not cut is the item of its entry's number)
+    const int row = ((b - which * a.size) * a.T + t) * a.group + g, own = t * a.group + g;
+    const int entry = which * a.first_tiles + row / 16, own_entry = b * a.row_tiles + own / 16;
+    const int *note = reinterpret_cast<const int *>(a.first_ws) + 2 * entry, *own_note = reinterpret_cast<const int *>(a.ws) + 2 * own_entry;
+    const int first = a.first_parts ? note[0] : entry, items = shares ? a.first_parts ? note[1] : 1 : 0;
+    const int own_first = a.parts ? own_note[0] : own_entry, all = items + (a.parts ? own_note[1] : 1);
+
+    __shared__ __align__(16) float red[256][4];
+    __shared__ float tops[256], sums[256];
+    const int lanes = a.D / 4, groups = 256 / lanes, c = threadIdx.x % lanes, k = threadIdx.x / lanes;
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f, top = kFloor;
+    if (k < groups) {
+#pragma unroll 4
+        for (int i = k; i < all; i += groups) {
+            const bool of_run = i < items;
+            const int r = (of_run ? row : own) % 16;
+            const float *p = of_run ? part_of(a, 16, first + i, hk, true) : part_of(a, 16, own_first + i - items, hk, false);
+            const float m = p[r], most = fmaxf(top, m), f = __builtin_amdgcn_exp2f(top - most), h = __builtin_amdgcn_exp2f(m - most);
+            y = f * y + h * *reinterpret_cast<const f32x4 *>(p + 32 + r * a.D + c * 4);
+            sum = f * sum + h * p[16 + r];
+            top = most;
+        }
+    }
+    tops[threadIdx.x] = top;
+    sums[threadIdx.x] = sum;
+    *reinterpret_cast<f32x4 *>(red[threadIdx.x]) = y;
+    __syncthreads();
+    if (k != 0) return;
+    for (int i = 1; i < groups; i++) top = fmaxf(top, tops[i * lanes]);
+    sum = 0.f;
+    y = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < groups; i++) {
+        const float f = __builtin_amdgcn_exp2f(tops[i * lanes] - top);
+        sum += f * sums[i * lanes];
+        y += f * *reinterpret_cast<const f32x4 *>(red[i * lanes + c]);
+    }
+    const float norm = sum == 0.f ? 0.f : 1.f / sum, poison = ok ? 0.f : __uint_as_float(0x7fc00000u);
+    store_channels<DT>(a.o, b * a.o.sb + head * a.o.sh + t * a.o.st + c * 4, (t < count ? y * norm : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
+}
+
+// How a call is cut: both parts' plans, and where their workspaces lie (in floats).
 struct SharedPlan {
     Plan first, second;
-    int64_t canon;  // floats
-    size_t bytes;
+    int first_rows;  // of a place of the first part's workspace
+    bool many, second_many;  // tiles of more than 64 rows
+    int64_t second_at, canon_at, floats;
 };
 SharedPlan shared_plan(int B, int heads, int heads_kv, int T, int D, int page, int columns, int window, int dtype, int runs) {
     SharedPlan p;
     const int size = B / runs;
-    p.first = plan_of(runs, heads, heads_kv, T * size, D, page, columns, window, dtype);
+    const int64_t rows = (int64_t)T * size * (heads / heads_kv);
     p.second = plan_of(B, heads, heads_kv, T, D, page, columns, window, dtype);
-    p.canon = ((int64_t)B * heads * T * (D + 2) + 3) / 4 * 4;
-    const size_t a = workspace_bytes(p.first, runs, heads_kv, D), b = workspace_bytes(p.second, B, heads_kv, D);
-    p.bytes = p.canon * sizeof(float) + (a > b ? a : b);
+    p.second_many = p.second.rows == kWideRows;
+    p.many = rows > 16 && !(D > 128 && dtype == ENATTEN_F32);
+    int64_t floats;
+    if (p.many) {
+        p.first.rows = D <= 128 && rows <= 128 ? 128 : kWideRows;
+        p.first.row_tiles = (int)((rows + p.first.rows - 1) / p.first.rows);
+        p.first.parts = p.first.rows == 128 ? 512 : 256;
+        p.first.items = 0;
+        p.first_rows = rows < p.first.rows ? (int)(rows + 31) / 32 * 32 : p.first.rows;
+        const int64_t tiles = (int64_t)runs * p.first.row_tiles * heads_kv;
+        floats = (2 * tiles + 3) / 4 * 4 + (tiles + p.first.parts) * item_floats(p.first_rows, padded(D));
+    } else {
+        p.first = plan_of(runs, heads, heads_kv, T * size, D, page, columns, window, dtype);
+        p.first_rows = 16;
+        floats = head_floats((int64_t)runs * p.first.row_tiles) + p.first.items * heads_kv * item_floats(16, D);
+    }
+    p.second_at = floats;
+    if (p.second_many) {
+        floats += workspace_bytes(p.second, B, heads_kv, D) / sizeof(float);
+        p.canon_at = floats;
+        floats += ((int64_t)B * heads * T * (D + 2) + 3) / 4 * 4;
+    } else {
+        floats += head_floats((int64_t)B * p.second.row_tiles) + p.second.items * heads_kv * item_floats(p.second.rows, D);
+        p.canon_at = 0;
+    }
+    p.floats = floats;
     return p;
+}
+
+template <int DP, int R, bool E4M3>
+int launch_type(const char *fn, const SharedArgs &a, int64_t items, hipStream_t st) {
+    const int blocks = (int)(items * a.heads_kv);
+    ProfScope prof(ENATTEN_KERNEL_CACHE_ATTENTION, "run_attend", st);
+    if (a.dtype == ENATTEN_BF16) run_attend<DP, R, E4M3, ENATTEN_BF16><<<blocks, 256, 0, st>>>(a);
+    else if (a.dtype == ENATTEN_F32) run_attend<DP, R, E4M3, ENATTEN_F32><<<blocks, 256, 0, st>>>(a);
+    else run_attend<DP, R, E4M3, ENATTEN_F16><<<blocks, 256, 0, st>>>(a);
+    return launched(fn);
+}
+template <int DP, bool E4M3>
+int launch_tiles(const char *fn, const SharedArgs &a, int rows, int64_t items, hipStream_t st) {
+    if (items * a.heads_kv > 0xffffff) {  // (2^32 threads)
+        set_error("%s: too many row tiles", fn);
+        return ENATTEN_EUNSUPPORTED;
+    }
+    if (rows == 16) return launch_type<DP, 1, E4M3>(fn, a, items, st);
+    if constexpr (DP <= 128) {
+        if (rows == 32) return launch_type<DP, 2, E4M3>(fn, a, items, st);
+        if (rows == 48) return launch_type<DP, 3, E4M3>(fn, a, items, st);
+    }
+    if constexpr (DP == 64)
+        if (rows == 64) return launch_type<DP, 4, E4M3>(fn, a, items, st);
+    set_error("%s: no tile of %d rows of %d channels", fn, rows, a.D);
+    return ENATTEN_EUNSUPPORTED;
+}
+int launch_attend(const char *fn, const SharedArgs &a, int rows, int64_t items, bool e, hipStream_t st) {
+    if (a.D <= 64) return e ? launch_tiles<64, true>(fn, a, rows, items, st) : launch_tiles<64, false>(fn, a, rows, items, st);
+    if (a.D <= 128) return e ? launch_tiles<128, true>(fn, a, rows, items, st) : launch_tiles<128, false>(fn, a, rows, items, st);
+    return e ? launch_tiles<256, true>(fn, a, rows, items, st) : launch_tiles<256, false>(fn, a, rows, items, st);
 }
 
 }  // namespace
@@ -43,7 +157,7 @@ size_t enatten_cache_attention_shared_workspace_bytes(int B, int heads, int head
     if (B < 1 || heads < 1 || heads_kv < 1 || heads % heads_kv || T < 1 || D < 1 || page < 1 || columns < 1 ||
         kernel_size < 0 || runs < 1 || B % runs || (int64_t)B * heads * T > (1 << 30))
         return 0;
-    return shared_plan(B, heads, heads_kv, T, D, page, columns, kernel_size, dtype, runs).bytes;
+    return shared_plan(B, heads, heads_kv, T, D, page, columns, kernel_size, dtype, runs).floats * sizeof(float);
 }
 
 int enatten_cache_attention_shared(const void *q, const void *k_cache, const void *v_cache, const float *k_scale,
@@ -72,16 +186,30 @@ int enatten_cache_attention_shared(const void *q, const void *k_cache, const voi
     a.shared = shared;
     a.runs = runs;
     a.size = B / runs;
-    a.canon = static_cast<float *>(workspace);
-    a.ws = a.canon + p.canon;
-    const hipStream_t st = static_cast<hipStream_t>(stream);
-    const bool e = cache_dtype == ENATTEN_E4M3;
-    a.row_tiles = p.first.row_tiles;
-    a.parts = p.first.parts;
-    if ((rc = launch_first(fn, a, p.first, e, st))) return rc;
+    a.first_ws = static_cast<float *>(workspace);
+    a.ws = a.first_ws + p.second_at;
+    a.canon = a.first_ws + p.canon_at;
+    a.first_tiles = p.first.row_tiles;
+    a.first_parts = p.first.parts;
+    a.first_rows = p.first_rows;
+    a.first_items = p.many ? 0 : (int)p.first.items;
     a.row_tiles = p.second.row_tiles;
     a.parts = p.second.parts;
-    return launch_second(fn, a, p.second, e, st);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const bool e = cache_dtype == ENATTEN_E4M3;
+    if (p.many && (rc = launch_first_rows(fn, a, p.first.rows, e, st))) return rc;
+    if (p.second_many) {
+        if ((rc = launch_first_join(fn, a, p.first.rows, st))) return rc;
+        return launch_second_rows(fn, a, e, st);
+    }
+    if ((rc = launch_attend(fn, a, p.second.rows, a.first_items + p.second.items, e, st))) return rc;
+    if (p.many) return launch_last_join(fn, a, p.first.rows, p.second.rows, st);
+    ProfScope prof(ENATTEN_KERNEL_CACHE_JOIN, "run_join_tiles", st);
+    const int blocks = B * heads * T;
+    if (dtype == ENATTEN_BF16) run_join_tiles<ENATTEN_BF16><<<blocks, 256, 0, st>>>(a);
+    else if (dtype == ENATTEN_F32) run_join_tiles<ENATTEN_F32><<<blocks, 256, 0, st>>>(a);
+    else run_join_tiles<ENATTEN_F16><<<blocks, 256, 0, st>>>(a);
+    return launched(fn);
 }
 
 #pragma GCC visibility pop

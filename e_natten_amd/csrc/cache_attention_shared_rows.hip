@@ -1,55 +1,180 @@
-// The tiles of 256 rows of cache_attention_rows.hip for runs that share their first tokens
-// (cache_attention_shared.hip).
+// cache_attention of runs that share their first tokens (cache_attention_shared.hip): tiles of many rows, and
+// the joins behind them.  The kernel is that of cache_attention_rows.hip.
 #include "cache_attention_rows_body.h"
 
 namespace enatten {
 namespace {
 
-template <int PASS, int DP, bool E4M3, int DT>
-__global__ __launch_bounds__(512, 2) void run_rows(PassArgs<PASS> args) {
-    rows_body<DP, E4M3, DT>(args);
+template <int PASS, int DP, bool E4M3, int DT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void run_rows(PassArgs<PASS> args) {
+    rows_body<DP, E4M3, DT, WAVES>(args);
 }
-template <int PASS, int DP, int DT>
-__global__ __launch_bounds__(256) void run_join_rows(PassArgs<PASS> a) {
+template <int DP, int DT>
+__global__ __launch_bounds__(256) void run_join_rows(PassArgs<2> a) {
     join_rows_body<DP, DT>(a);
 }
 
-template <int PASS, int DP, bool E4M3, int DT>
-int launch(const char *fn, const PassArgs<PASS> &a, hipStream_t st) {
+// The parts of the first part's tiles joined, and (but for CANON, which leaves that to the second part's own tiles of
+// many rows) with the second part's.  One workgroup per (tile, 16 rows, 32 channels): few tiles have many parts.  A
+// wave takes every fourth part: 16 lanes over the rows, 4 over neighbouring words of 4 channels.
+template <int DP, int DT, bool CANON>
+__global__ __launch_bounds__(256) void run_join(SharedArgs a, int tile_rows, int second_rows) {
+    constexpr int WORDS = 2, SPLIT = DP / 32;
+    const int n = threadIdx.x % 16, c = threadIdx.x / 16 % 4, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int block = blockIdx.x;
+    const int split = block % SPLIT;
+    block /= SPLIT;
+    const int groups = a.first_rows / 16, r = block % groups * 16 + n, tile = block / groups;
+    const int entries = entries_of(a, true), all_rows = rows_of(a, true), head = tile / entries, entry = tile - head * entries;
+    const int which = entry / a.first_tiles, row = (entry - which * a.first_tiles) * tile_rows + r;
+    if (row - n >= all_rows || split * 32 >= a.D) return;
+    const int *ranges = reinterpret_cast<const int *>(a.first_ws) + 2 * tile;
+    const int first = ranges[0], parts = ranges[1] - first + 1;
+    // rows behind the last one have no sums: they go along with its
+    const int from = min(r, all_rows - 1 - (row - r));
+    auto part_at = [&](int q) { return stair_of(a, (int64_t)first + q + tile); };
+    float top = kFloor, sum = 0.f;
+    for (int q = wave; q < parts; q += 4) top = fmaxf(top, part_at(q)[from]);
+    f32x4 y[WORDS];
+#pragma unroll
+    for (int i = 0; i < WORDS; i++) y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int q = wave; q < parts; q += 4) {
+        const float *part = part_at(q);
+        const float f = __builtin_amdgcn_exp2f(part[from] - top);
+        sum += f * part[a.first_rows + from];
+        const f32x4 *x = reinterpret_cast<const f32x4 *>(part + 2 * a.first_rows) + from / 32 * (DP / 8) * 64 + from % 32;
+        // the word of channels 4 mm + 128 k.. lies at place 16 k + j of the lanes h
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) {
+            const int word = split * WORDS + i, mm = word % 8 * 4 + c, place = word / 8 * 16 + mm / 8 * 4 + mm % 4, h = mm / 4 % 2;
+            y[i] += f * x[place * 64 + h * 32];
+        }
+    }
+    __shared__ __align__(16) f32x4 red[4][WORDS][64];
+    __shared__ float tops[4][16], sums[4][16];
+    if (c == 0) {
+        tops[wave][n] = top;
+        sums[wave][n] = sum;
+    }
+#pragma unroll
+    for (int i = 0; i < WORDS; i++) red[wave][i][lane] = y[i];
+    __syncthreads();
+    const int d = (split * WORDS + wave) * 16 + c * 4;
+    if (wave >= WORDS || row >= all_rows || d >= a.D) return;
+    top = kFloor;
+#pragma unroll
+    for (int v = 0; v < 4; v++) top = fmaxf(top, tops[v][n]);
+    sum = 0.f;
+    f32x4 z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < 4; v++) {
+        const float f = __builtin_amdgcn_exp2f(tops[v][n] - top);
+        sum += f * sums[v][n];
+        z += f * red[v][wave][lane];
+    }
+    const Place where = place_of(a, which, head, row, true);
+    if constexpr (CANON) {
+        put_canon(a, canon_row(a, where), d, top, sum, z);
+    } else {
+        int len, count;
+        const bool ok = sequence_of(a.tb, where.b, len, count);
+        if (!(ok && count > 0 && len - count >= shared_end(a, which))) {  // (it does not share them)
+            top = kFloor;
+            sum = 0.f;
+            z = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        const int own = where.t * a.group + where.head - head * a.group, own_entry = where.b * a.row_tiles + own / second_rows;
+        const int own_row = own % second_rows;
+        const int *note = reinterpret_cast<const int *>(a.ws) + 2 * own_entry;
+        const int own_first = a.parts ? note[0] : own_entry, items = a.parts ? note[1] : 1;
+        for (int i = 0; i < items; i++) {
+            const float *p = part_of(a, second_rows, own_first + i, head, false);
+            const float m = p[own_row], most = fmaxf(top, m), f = __builtin_amdgcn_exp2f(top - most), g = __builtin_amdgcn_exp2f(m - most);
+            z = f * z + g * *reinterpret_cast<const f32x4 *>(p + 2 * second_rows + own_row * a.D + d);
+            sum = f * sum + g * p[second_rows + own_row];
+            top = most;
+        }
+        const float norm = sum == 0.f ? 0.f : 1.f / sum, poison = ok ? 0.f : __uint_as_float(0x7fc00000u);
+        store_channels<DT>(a.o, offset_of(a.o, where) + d, (where.t < count ? z * norm : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
+    }
+}
+
+template <int PASS>
+PassArgs<PASS> pass_args(const SharedArgs &s) {
+    PassArgs<PASS> a;
+    static_cast<SharedArgs &>(a) = s;
+    return a;
+}
+
+template <int DP, bool E4M3, int DT>
+int first_rows(const char *fn, const SharedArgs &a, int rows, hipStream_t st) {
+    ProfScope prof(ENATTEN_KERNEL_CACHE_ATTENTION, "run_rows", st);
+    if constexpr (DP <= 128) {
+        if (rows == 128) {
+            run_rows<1, DP, E4M3, DT, 4><<<a.first_parts, 256, 0, st>>>(pass_args<1>(a));
+            return launched(fn);
+        }
+    }
+    run_rows<1, DP, E4M3, DT, 8><<<a.first_parts, 512, 0, st>>>(pass_args<1>(a));
+    return launched(fn);
+}
+template <int DP, bool E4M3, int DT>
+int second_rows(const char *fn, const SharedArgs &a, hipStream_t st) {
     {
         ProfScope prof(ENATTEN_KERNEL_CACHE_ATTENTION, "run_rows", st);
-        run_rows<PASS, DP, E4M3, DT><<<a.parts, 512, 0, st>>>(a);
+        run_rows<2, DP, E4M3, DT, 8><<<a.parts, 512, 0, st>>>(pass_args<2>(a));
     }
     const int rc = launched(fn);
     if (rc) return rc;
     ProfScope prof(ENATTEN_KERNEL_CACHE_JOIN, "run_join_rows", st);
-    run_join_rows<PASS, DP, DT><<<a.parts * (kWideRows / 16), 256, 0, st>>>(a);
+    run_join_rows<DP, DT><<<a.parts * (kWideRows / 16), 256, 0, st>>>(pass_args<2>(a));
     return launched(fn);
 }
-template <int PASS, int DP, bool E4M3>
-int launch_type(const char *fn, const PassArgs<PASS> &a, hipStream_t st) {
-    if (a.dtype == ENATTEN_BF16) return launch<PASS, DP, E4M3, ENATTEN_BF16>(fn, a, st);
-    if constexpr (DP <= 128)
-        if (a.dtype == ENATTEN_F32) return launch<PASS, DP, E4M3, ENATTEN_F32>(fn, a, st);
-    return launch<PASS, DP, E4M3, ENATTEN_F16>(fn, a, st);
-}
-template <int PASS, bool E4M3>
-int launch_dim(const char *fn, const PassArgs<PASS> &a, hipStream_t st) {
-    if (a.D <= 64) return launch_type<PASS, 64, E4M3>(fn, a, st);
-    if (a.D <= 128) return launch_type<PASS, 128, E4M3>(fn, a, st);
-    return launch_type<PASS, 256, E4M3>(fn, a, st);
+template <int DP, int DT, bool CANON>
+int join(const char *fn, const SharedArgs &a, int rows, int second, hipStream_t st) {
+    const int64_t blocks = (int64_t)a.runs * a.first_tiles * a.heads_kv * (a.first_rows / 16) * (DP / 32);
+    if (blocks > 0xffffff) {  // (2^32 threads)
+        set_error("%s: too many rows", fn);
+        return ENATTEN_EUNSUPPORTED;
+    }
+    ProfScope prof(ENATTEN_KERNEL_CACHE_JOIN, "run_join", st);
+    run_join<DP, DT, CANON><<<(int)blocks, 256, 0, st>>>(a, rows, second);
+    return launched(fn);
 }
 
-template <int PASS>
-int launch_pass(const char *fn, const SharedArgs &s, bool e4m3, hipStream_t st) {
-    PassArgs<PASS> a;
-    static_cast<SharedArgs &>(a) = s;
-    return e4m3 ? launch_dim<PASS, true>(fn, a, st) : launch_dim<PASS, false>(fn, a, st);
+// f(head dim, whether E4M3, type) with constants; float32 above 128 channels has no such tiles
+template <int V> using Const = std::integral_constant<int, V>;
+template <int DP, class F>
+int by_type(const SharedArgs &a, F f) {
+    if (a.dtype == ENATTEN_BF16) return f(Const<DP>{}, Const<ENATTEN_BF16>{});
+    if constexpr (DP <= 128)
+        if (a.dtype == ENATTEN_F32) return f(Const<DP>{}, Const<ENATTEN_F32>{});
+    return f(Const<DP>{}, Const<ENATTEN_F16>{});
+}
+template <class F>
+int by_dim(const SharedArgs &a, F f) {
+    return a.D <= 64 ? by_type<64>(a, f) : a.D <= 128 ? by_type<128>(a, f) : by_type<256>(a, f);
 }
 
 }  // namespace
 
-int launch_rows_first(const char *fn, const SharedArgs &a, bool e4m3, hipStream_t st) { return launch_pass<1>(fn, a, e4m3, st); }
-int launch_rows_second(const char *fn, const SharedArgs &a, bool e4m3, hipStream_t st) { return launch_pass<2>(fn, a, e4m3, st); }
+int launch_first_rows(const char *fn, const SharedArgs &a, int rows, bool e4m3, hipStream_t st) {
+    return by_dim(a, [&](auto dp, auto dt) {
+        return e4m3 ? first_rows<dp.value, true, dt.value>(fn, a, rows, st) : first_rows<dp.value, false, dt.value>(fn, a, rows, st);
+    });
+}
+int launch_second_rows(const char *fn, const SharedArgs &a, bool e4m3, hipStream_t st) {
+    return by_dim(a, [&](auto dp, auto dt) {
+        return e4m3 ? second_rows<dp.value, true, dt.value>(fn, a, st) : second_rows<dp.value, false, dt.value>(fn, a, st);
+    });
+}
+int launch_first_join(const char *fn, const SharedArgs &a, int rows, hipStream_t st) {
+    return by_dim(a, [&](auto dp, auto) { return join<dp.value, ENATTEN_F32, true>(fn, a, rows, 16, st); });
+}
+int launch_last_join(const char *fn, const SharedArgs &a, int rows, int second, hipStream_t st) {
+    return by_dim(a, [&](auto dp, auto dt) { return join<dp.value, dt.value, false>(fn, a, rows, second, st); });
+}
 
 }  // namespace enatten
