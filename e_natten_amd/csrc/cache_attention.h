@@ -25,8 +25,8 @@ struct AttnArgs {
 struct SharedArgs : AttnArgs {
     const int *shared;   // [runs], tokens
     int runs, size;      // sequences of a run
-    // of the first part: what row_tiles, parts and ws are of the second; the items of its tiles of 16 rows, which
-    // come before the second part's in one launch (0: it has tiles of more rows and a launch of its own)
+    // of the first part: what row_tiles, parts and ws are of the second; the items of a launch that are its own, which
+    // come before the second part's; rows of a place of its workspace
     int first_tiles, first_parts, first_items, first_rows;
     float *first_ws;
     float *canon;        // what the first part comes to, joined: rows (b, head, t), their sums of D values, then
@@ -166,7 +166,19 @@ __device__ __forceinline__ Share share_of(const Args &a, int item, bool first) {
     }
     // (a little more than the quotient: the items are at most `parts` and one for every entry)
     const int each = (int)(total * 1.00001f / parts_of(a, first)) + 1;
-    const int chunk = max(kLeast / TOK, each + WAVES - 1) / WAVES * WAVES;
+    int chunk = max(kLeast / TOK, each + WAVES - 1) / WAVES * WAVES;
+    if constexpr (kShared<Args>) {
+        if (first) {  // no more items than parts: all of them start at once
+            if (entries > 64) chunk = (max(kLeast / TOK, (int)(total * 1.00001f / (parts_of(a, first) - entries)) + 1) + WAVES - 1) / WAVES * WAVES;
+            else
+                for (;;) {
+                    const int n = lane < entries ? max(1, (steps + chunk - 1) / chunk) : 0;
+                    const int all = __builtin_amdgcn_readlane(running_sum(n), 63);
+                    if (all <= parts_of(a, first)) break;
+                    chunk = max(chunk + WAVES, (int)((int64_t)chunk * all / parts_of(a, first)) / WAVES * WAVES);
+                }
+        }
+    }
     int before = 0;
     for (int e0 = 0; e0 < entries; e0 += 64) {
         const int e = e0 + lane;
@@ -530,11 +542,11 @@ __device__ __forceinline__ int64_t lane_offset(int64_t x, int l) {
 
 // Tiles of kWideRows rows (cache_attention_rows.hip), a.parts ranges
 int launch_attend_rows(const char *fn, const AttnArgs &a, bool e4m3, hipStream_t st);
-// Tiles of 128 or kWideRows rows of the first part, of kWideRows of the second, and the joins behind them
-// (cache_attention_shared_rows.hip)
-int launch_first_rows(const char *fn, const SharedArgs &a, int rows, bool e4m3, hipStream_t st);
-int launch_first_join(const char *fn, const SharedArgs &a, int rows, hipStream_t st);  // into canon
-int launch_last_join(const char *fn, const SharedArgs &a, int rows, int second_rows, hipStream_t st);
+// Tiles of many rows of either part, and the joins behind them (cache_attention_shared_rows.hip)
+int rows_of_first(int D);
+int launch_first_rows(const char *fn, const SharedArgs &a, bool e4m3, hipStream_t st);
+int launch_first_join(const char *fn, const SharedArgs &a, hipStream_t st);  // into canon
+int launch_last_join(const char *fn, const SharedArgs &a, int second_rows, hipStream_t st);
 int launch_second_rows(const char *fn, const SharedArgs &a, bool e4m3, hipStream_t st);
 Plan plan_of(int B, int heads, int heads_kv, int T, int D, int page, int columns, int window, int dtype);
 size_t workspace_bytes(const Plan &p, int B, int heads_kv, int D);  // B: sequences, or runs

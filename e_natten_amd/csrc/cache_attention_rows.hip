@@ -30,7 +30,7 @@ namespace {
 
 template <int DP, bool E4M3, int DT>
 __global__ __launch_bounds__(512, 2) void attend_rows(AttnArgs args) {
-    rows_body<DP, E4M3, DT, 8>(args);
+    rows_body<DP, E4M3, DT, 1, 1>(args);
 }
 template <int DP, int DT>
 __global__ __launch_bounds__(256) void join_rows(AttnArgs a) {

@@ -20,15 +20,18 @@ __device__ __forceinline__ const Args &args_again() {
 }
 
 // DP: head_dim rounded up to 64, 128 or 256; DT: type of q and o, float32 in two float16 terms of q and p.
-// WAVES: 8, or 4 for tiles of half as many rows and steps of half as many tokens.
-template <int DP, bool E4M3, int DT, int WAVES, class Args>
+// TG: groups of the eight waves that share their rows and take some of a step's tokens each; their sums meet in LDS at
+// the end of a tile (the first part of a call with shared tokens).  M: how many times as many tokens a step has.
+template <int DP, bool E4M3, int DT, int TG, int M, class Args>
 __device__ __forceinline__ void rows_body(const Args &args) {
     constexpr bool FIRST = std::is_same_v<Args, PassArgs<1>>, SECOND = std::is_same_v<Args, PassArgs<2>>;
-    constexpr int ROWS = 32 * WAVES, HALF = WAVES / 2;
+    constexpr int RB = 8 / TG, ROWS = 32 * RB;  // blocks of 32 rows
+    static_assert(TG == 1 || FIRST, "only parts are joined");
     constexpr int TERMS = DT == ENATTEN_F32 ? 2 : 1;
-    constexpr int TOK = 1024 * WAVES / DP;  // tokens of a step: 128, 64, 32
+    constexpr int TOK = 8192 * M / DP;  // tokens of a step: 128, 64, 32, or twice as many
     constexpr int NB = TOK / 32;      // blocks of 32 of them
     constexpr int GR = TOK / 16;      // groups of 16, each within a page
+    constexpr int NBW = NB / TG, GRW = GR / TG;  // those of a wave
     constexpr int SD = DP / 16;       // products along head_dim of S
     constexpr int OB = DP / 32;       // blocks of 32 channels of O
     constexpr int CH = DP / 16;       // loads of 16 codes per token
@@ -42,9 +45,10 @@ __device__ __forceinline__ void rows_body(const Args &args) {
     // Rows of q stay in registers, at head dims above 128 all but the last operands, for which there are
     // none left: those a lane puts into LDS and reads again.
     constexpr int KEPT = DP == 256 ? 10 : SD;
-    __shared__ f16x8 q_lds[WAVES * 64 * (SD - KEPT) + 1];
+    __shared__ f16x8 q_lds[8 * 64 * (SD - KEPT) + 1];
     const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (branches on it are the wave's)
+    const int rb = TG == 1 ? wave : wave % RB, tg = TG == 1 ? 0 : wave / RB;
 
     // The workgroup's range of steps.  Blocks 8 apart share an XCD and its L2: they get neighbouring ranges,
     // which read the same keys and values where they belong to the same head.
@@ -83,7 +87,7 @@ __device__ __forceinline__ void rows_body(const Args &args) {
         }
     }
     at_step += counted - into;
-    const int which = entry / tiles_of(a, FIRST), row0 = (entry - which * tiles_of(a, FIRST)) * ROWS + wave * 32;
+    const int which = entry / tiles_of(a, FIRST), row0 = (entry - which * tiles_of(a, FIRST)) * ROWS + rb * 32;
     const int base = s.lo & -16;
     int b = which, joins = 0;  // joins: shared tokens, which are not the second part's
     if constexpr (FIRST) {
@@ -152,7 +156,7 @@ __device__ __forceinline__ void rows_body(const Args &args) {
 #pragma unroll
             for (int t = 0; t < TERMS; t++) {
                 if (c < KEPT) qf[c][t] = w[t];
-                else q_rest[(c - KEPT) * (64 * WAVES)] = w[t];
+                else q_rest[(c - KEPT) * 512] = w[t];
             }
         }
     }
@@ -182,7 +186,7 @@ __device__ __forceinline__ void rows_body(const Args &args) {
     int filled = -64;
     int64_t at = 0;
     float z_at = 0.f;  // of keys, or log2 of values (for float32 the scale itself)
-    const bool for_v = wave >= HALF;
+    const bool for_v = wave >= 4;
     auto fill = [&](int group) {
         const Args &a = args_again<Args>();
         filled = group;
@@ -204,14 +208,14 @@ __device__ __forceinline__ void rows_body(const Args &args) {
             }
         }
     };
-    // What a thread brings: of keys two runs of 16 codes, of values a word of 4 channels of 8 tokens.
-    unsigned raw[8];
-    float raw_z = 0.f;  // lanes 0 .. GR - 1 of wave 0: key scales of the step's groups, of wave HALF: value scales
+    // What a thread brings, M times: of keys two runs of 16 codes, of values a word of 4 channels of 8 tokens.
+    unsigned raw[M][8];
+    float raw_z = 0.f;  // lanes 0 .. GR - 1 of wave 0: key scales of the step's groups, of wave 4: value scales
     // (offsets within a group of 16 tokens; a wave's 64 runs of keys lie in one group, its 64 words of
     // values too, but for DP 64, where each half of the wave has its own)
-    const int run = wave % HALF * (64 * 4 / DP) + lane / QUADS, quad = lane % QUADS;  // runs of 8 tokens
+    const int run = (wave & 3) * (64 * 4 / DP) * M + lane / QUADS, quad = lane % QUADS;  // (the first) run of 8 tokens
     const unsigned within = for_v ? run % 2 * 4 * (unsigned)a.v.st + min(quad * 4, a.D - 4)
-                                  : (wave * (128 / CH) + lane / CH) % 16 * (unsigned)a.k.st + min(lane % CH * 16, a.D - 16);
+                                  : (wave * (128 / CH) * M + lane / CH) % 16 * (unsigned)a.k.st + min(lane % CH * 16, a.D - 16);
     auto fetch = [&](int step) {
         const int group = step * GR;
         if (group >= filled + 64) fill(group);
@@ -219,42 +223,51 @@ __device__ __forceinline__ void rows_body(const Args &args) {
         raw_z = __shfl(z_at, here + (lane & (GR - 1)), 64);
         if (!for_v) {
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
+            for (int j = 0; j < 2 * M; j++) {
                 const char *from = static_cast<const char *>(a.k.codes) +
-                                   lane_offset(at, here + (wave * (128 / CH) + j * (64 / CH)) / 16);
-                const u32x4 x = *reinterpret_cast<const u32x4 *>(from + (DP == 64 ? 0 : j * (64 / CH)) * a.k.st + within);
+                                   lane_offset(at, here + (wave * (128 / CH) * M + j * (64 / CH)) / 16);
+                const u32x4 x = *reinterpret_cast<const u32x4 *>(from + (DP == 64 ? 0 : j % 2 * (64 / CH)) * a.k.st + within);
 #pragma unroll
-                for (int i = 0; i < 4; i++) raw[j * 4 + i] = x[i];
+                for (int i = 0; i < 4; i++) raw[j / 2][j % 2 * 4 + i] = x[i];
             }
         } else {
-            int64_t off = lane_offset(at, here + wave % HALF * (64 * 4 / DP) / 2);
-            if constexpr (DP == 64) off = lane < 32 ? off : lane_offset(at, here + wave % HALF * 2 + 1);
-            const char *from = static_cast<const char *>(a.v.codes) + off;
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                raw[j] = *reinterpret_cast<const unsigned *>(from + (j % 4 + j / 4 * 8) * a.v.st + within);
+            for (int k = 0; k < M; k++) {
+                const int first = ((wave & 3) * M + k) * (64 * 4 / DP) / 2;  // group
+                int64_t off = lane_offset(at, here + first);
+                if constexpr (DP == 64) off = lane < 32 ? off : lane_offset(at, here + first + 1);
+                const char *from = static_cast<const char *>(a.v.codes) + off;
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    raw[k][j] = *reinterpret_cast<const unsigned *>(from + (j % 4 + j / 4 * 8) * a.v.st + within);
+            }
         }
     };
     auto put_as = [&](auto seen, int buffer) {
         constexpr bool SEEN = decltype(seen)::value;
         if (!for_v) {
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int token = wave * (128 / CH) + j * (64 / CH) + lane / CH, c = lane % CH;
+            for (int j = 0; j < 2 * M; j++) {
+                const int token = wave * (128 / CH) * M + j * (64 / CH) + lane / CH, c = lane % CH;
+                const unsigned *x = raw[j / 2] + j % 2 * 4;
                 f16x8 *to = &k_lds[buffer][(token / 32 * SD + c) * PART + token % 32];
-                to[0] = widen_row<E4M3, SEEN>(raw[j * 4], raw[j * 4 + 1]);
-                to[32] = widen_row<E4M3, SEEN>(raw[j * 4 + 2], raw[j * 4 + 3]);
+                to[0] = widen_row<E4M3, SEEN>(x[0], x[1]);
+                to[32] = widen_row<E4M3, SEEN>(x[2], x[3]);
             }
         } else {
-            f16x8 v[4];
-            widen_columns<E4M3, SEEN>(raw, v);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int block = DP == 64 ? i / 2 : i + quad / 32 * 4, mm = DP == 64 ? (i & 1) * 16 + quad : quad & 31;
-                v_lds[buffer][(block * (TOK / 16) + run / 2) * 64 + run % 2 * 32 + mm] = v[i];
+            for (int k = 0; k < M; k++) {
+                f16x8 v[4];
+                widen_columns<E4M3, SEEN>(raw[k], v);
+                const int r = run + k * (64 * 4 / DP);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int block = DP == 64 ? i / 2 : i + quad / 32 * 4, mm = DP == 64 ? (i & 1) * 16 + quad : quad & 31;
+                    v_lds[buffer][(block * (TOK / 16) + r / 2) * 64 + r % 2 * 32 + mm] = v[i];
+                }
             }
         }
-        if (wave % HALF == 0) {
+        if ((wave & 3) == 0) {
             const bool finite = for_v && TERMS == 1 ? raw_z < INFINITY : fabsf(raw_z) < INFINITY;
             const float z = finite ? raw_z : for_v && TERMS == 1 ? -INFINITY : 0.f;
             if (lane < GR) {
@@ -266,7 +279,7 @@ __device__ __forceinline__ void rows_body(const Args &args) {
         }
     };
     // (the workgroup's first and last rows, for the shorter way of turning E4M3)
-    const int wg_row = row0 - wave * 32, wg_last = min((wg_row + ROWS - 1) / a.group, s.count - 1);
+    const int wg_row = row0 - rb * 32, wg_last = min((wg_row + ROWS - 1) / a.group, s.count - 1);
     int wg_lo = a.window ? max(s.start + wg_last + 1 - a.window, 0) : 0, wg_hi = s.start + wg_row / a.group + 1;
     if constexpr (SECOND) wg_lo = max(wg_lo, joins);
     if constexpr (FIRST) {
@@ -283,38 +296,38 @@ __device__ __forceinline__ void rows_body(const Args &args) {
     // are at least 1e-20, so that they end below -1e18 and their exponentials are 0 whatever the maximum
     // (kFloor at least), and a unit of 0 asks for nothing special.
     auto work = [&](bool whole, int token, int buffer) {
-        float kz[GR], lz[GR], most_z = -INFINITY;
+        float kz[GRW], lz[GRW], most_z = -INFINITY;
 #pragma unroll
-        for (int g = 0; g < GR; g++) {
-            kz[g] = z_lds[buffer][0][g];
-            lz[g] = z_lds[buffer][1][g];
+        for (int g = 0; g < GRW; g++) {
+            kz[g] = z_lds[buffer][0][tg * GRW + g];
+            lz[g] = z_lds[buffer][1][tg * GRW + g];
             most_z = fmaxf(most_z, lz[g]);
         }
         float scale = grow(ref, TERMS == 1 ? most_z : __builtin_amdgcn_logf(most_z));
 #pragma unroll
-        for (int g = 0; g < GR; g++) lz[g] = TERMS == 1 ? log_weight(lz[g], ref) : plain_weight(lz[g], ref);
+        for (int g = 0; g < GRW; g++) lz[g] = TERMS == 1 ? log_weight(lz[g], ref) : plain_weight(lz[g], ref);
 
-        f32x16 st[NB];
+        f32x16 st[NBW];
 #pragma unroll
-        for (int i = 0; i < NB; i++)
+        for (int i = 0; i < NBW; i++)
 #pragma unroll
             for (int j = 0; j < 16; j++) st[i][j] = 0.f;
-        const f16x8 *kp = &k_lds[buffer][lane];
+        const f16x8 *kp = &k_lds[buffer][lane + tg * (NBW * SD * PART)];
 #pragma unroll
         for (int c = 0; c < SD; c++) {
 #pragma unroll
-            for (int i = 0; i < NB; i++) {
+            for (int i = 0; i < NBW; i++) {
                 const f16x8 kf = kp[(i * SD + c) * PART];
 #pragma unroll
                 for (int t = TERMS - 1; t >= 0; t--)
-                    st[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, c < KEPT ? qf[c][t] : q_rest[(c - KEPT) * (64 * WAVES)], st[i], 0, 0, 0);
+                    st[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, c < KEPT ? qf[c][t] : q_rest[(c - KEPT) * 512], st[i], 0, 0, 0);
             }
         }
 
         // lane's tokens: 32 i + 16 g + 8 (j / 4) + 4 h + j % 4 for its 8 values j of a group
         if (!whole) {
 #pragma unroll
-            for (int i = 0; i < NB; i++)
+            for (int i = 0; i < NBW; i++)
 #pragma unroll
                 for (int j = 0; j < 16; j++) {
                     const int tk = token + i * 32 + j / 4 * 8 + h * 4 + j % 4;
@@ -325,15 +338,15 @@ __device__ __forceinline__ void rows_body(const Args &args) {
         const int bad = __builtin_amdgcn_readfirstlane(z_bad[buffer][0] | z_bad[buffer][1]);
         if (bad) {
 #pragma unroll
-            for (int g = 0; g < GR; g++) {
+            for (int g = 0; g < GRW; g++) {
                 const int first = token + g * 16;
-                if ((bad >> g & 1) && first < hi_r && first + 16 > hi_r - seen) l = __uint_as_float(0x7fc00000u);
+                if ((bad >> (tg * GRW + g) & 1) && first < hi_r && first + 16 > hi_r - seen) l = __uint_as_float(0x7fc00000u);
             }
         }
         const float unit_z = power_of_two(ref - kPTop);
-        float u[GR], top = kFloor;
+        float u[GRW], top = kFloor;
 #pragma unroll
-        for (int g = 0; g < GR; g++) {
+        for (int g = 0; g < GRW; g++) {
             u[g] = fmaxf(unit * kz[g], 1e-20f);
             float most = -3e38f;  // (a constant to start from: else the compiler makes values canonical)
 #pragma unroll
@@ -354,9 +367,9 @@ __device__ __forceinline__ void rows_body(const Args &args) {
             for (int i = 0; i < OB; i++) acc[i] *= scale;
         }
         // group by group, so that the exponentials of one go beside the products of another
-        const f16x8 *vp = &v_lds[buffer][lane];
+        const f16x8 *vp = &v_lds[buffer][lane + tg * (GRW * 64)];
 #pragma unroll
-        for (int g = 0; g < GR; g++) {
+        for (int g = 0; g < GRW; g++) {
             const float shift = (TERMS == 1 ? lz[g] : 0.f) - m;
             f16x8 pf[TERMS];
             float p[8];
@@ -369,7 +382,7 @@ __device__ __forceinline__ void rows_body(const Args &args) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) pf[0][j] = (_Float16)p[j];
                 // (at most 2^40, as the weight is at least 2^-40)
-                l = fmaf(part, fminf(z_lds[buffer][2][g] * unit_z, 0x1p40f), l);
+                l = fmaf(part, fminf(z_lds[buffer][2][tg * GRW + g] * unit_z, 0x1p40f), l);
             } else {
                 l += part;
 #pragma unroll
@@ -407,9 +420,9 @@ __device__ __forceinline__ void rows_body(const Args &args) {
             put(buffer ^ 1, step + 1);
             if (step + 2 < step1) fetch(step + 2);
         }
-        const int token = base + step * TOK;
-        if (token >= some_hi || token + TOK <= some_lo) continue;
-        work(token >= all_lo && token + TOK <= all_hi, token, buffer);
+        const int token = base + step * TOK + tg * (NBW * 32);
+        if (token >= some_hi || token + NBW * 32 <= some_lo) continue;
+        work(token >= all_lo && token + NBW * 32 <= all_hi, token, buffer);
     }
 
     l = pair_sum(l);
@@ -454,12 +467,49 @@ __device__ __forceinline__ void rows_body(const Args &args) {
         } else {
             part = slot_of(a, slot);
         }
-        if (here && h == 0) {
-            part[wave * 32 + n] = m;
-            part[rows + wave * 32 + n] = l;
-        }
-        f32x4 *to = reinterpret_cast<f32x4 *>(part + 2 * rows) + wave * (BIG * JS) * 64 + lane;
-        if (row0 < all_rows) {
+        f32x4 *to = reinterpret_cast<f32x4 *>(part + 2 * rows) + rb * (BIG * JS) * 64 + lane;
+        if constexpr (TG > 1) {
+            // the waves with the same rows: all sums into LDS, then each wave joins some of the words
+            constexpr int WORDS = BIG * JS, MINE = WORDS / TG;
+            static_assert(sizeof(k_lds) >= 4 * WORDS * 1024 && sizeof(v_lds) >= 4 * WORDS * 1024, "room for eight waves' sums");
+            __shared__ float wave_m[8][32], wave_l[8][32];
+            auto place = [&](int w) { return reinterpret_cast<f32x4 *>(w < 4 ? &k_lds[0][0] : &v_lds[0][0]) + (w & 3) * WORDS * 64 + lane; };
+            f32x4 *out = place(wave);
+#pragma unroll
+            for (int i = 0; i < BIG; i++)
+#pragma unroll
+                for (int j = 0; j < JS; j++) out[(i * JS + j) * 64] = channels(i, j) * back;
+            if (h == 0) {
+                wave_m[wave][n] = m;
+                wave_l[wave][n] = l;
+            }
+            __syncthreads();
+            float f[TG], sum = 0.f, top = kFloor;
+#pragma unroll
+            for (int t = 0; t < TG; t++) top = fmaxf(top, wave_m[t * RB + rb][n]);
+#pragma unroll
+            for (int t = 0; t < TG; t++) {
+                f[t] = __builtin_amdgcn_exp2f(wave_m[t * RB + rb][n] - top);
+                sum += f[t] * wave_l[t * RB + rb][n];
+            }
+            if (tg == 0 && here && h == 0) {
+                part[rb * 32 + n] = top;
+                part[rows + rb * 32 + n] = sum;
+            }
+            if (row0 < all_rows) {
+#pragma unroll
+                for (int w = 0; w < MINE; w++) {
+                    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int t = 0; t < TG; t++) y += f[t] * place(t * RB + rb)[(tg * MINE + w) * 64];
+                    to[(tg * MINE + w) * 64] = y;
+                }
+            }
+        } else if (row0 < all_rows) {
+            if (here && h == 0) {
+                part[rb * 32 + n] = m;
+                part[rows + rb * 32 + n] = l;
+            }
 #pragma unroll
             for (int i = 0; i < BIG; i++)
 #pragma unroll

@@ -8,9 +8,9 @@
 // cache_attention_rows.hip over other rows and tokens, and leave what they come to in the workspace; the last
 // launch joins it.
 //
-// Up to 16 rows in a run both parts are tiles of 16 rows and one launch.  Beyond, the first part has tiles of
-// 128 or 256 rows over codes that LDS holds as float16, in a launch of its own, also where only some of a
-// tile's rows are there: its waves without rows turn codes, and two workgroups per CU hide each other's waits.
+// The first part has tiles of up to 48 rows (64 of up to 64 channels, 16 above 128) as the second has, cut so that all of
+// its workgroups start at once, and in the same launch where both have tiles of as many rows.  Beyond, tiles of
+// 64 rows (256 above 128 channels) over codes that LDS holds as float16.
 #include "cache_attention_body.h"
 
 namespace enatten {
@@ -21,10 +21,10 @@ __global__ __launch_bounds__(256, waves_of(DP, R, DT == ENATTEN_F32 ? 2 : 1)) vo
     attend_body<DP, R, E4M3, DT>(a);
 }
 
-// The parts of both halves of the work joined, where both have tiles of 16 rows: one workgroup per row.  Lanes over
+// The parts of both halves of the work joined, where neither has tiles of many rows: one workgroup per row.  Lanes over
 // the channels, 4 each, and the remaining factor of 256 over the parts.
 template <int DT>
-__global__ __launch_bounds__(256) void run_join_tiles(SharedArgs a) {
+__global__ __launch_bounds__(256) void run_join_tiles(SharedArgs a, int first_rows, int second_rows) {
     int block = blockIdx.x;
     const int head = block % a.heads, hk = head / a.group, g = head - hk * a.group;
     block /= a.heads;
@@ -33,7 +33,7 @@ __global__ __launch_bounds__(256) void run_join_tiles(SharedArgs a) {
     const bool ok = sequence_of(a.tb, b, len, count), shares = ok && count > 0 && len - count >= shared_end(a, which);
     // (a part that is not cut is the item of its entry's number)
     const int row = ((b - which * a.size) * a.T + t) * a.group + g, own = t * a.group + g;
-    const int entry = which * a.first_tiles + row / 16, own_entry = b * a.row_tiles + own / 16;
+    const int entry = which * a.first_tiles + row / first_rows, own_entry = b * a.row_tiles + own / second_rows;
     const int *note = reinterpret_cast<const int *>(a.first_ws) + 2 * entry, *own_note = reinterpret_cast<const int *>(a.ws) + 2 * own_entry;
     const int first = a.first_parts ? note[0] : entry, items = shares ? a.first_parts ? note[1] : 1 : 0;
     const int own_first = a.parts ? own_note[0] : own_entry, all = items + (a.parts ? own_note[1] : 1);
@@ -47,11 +47,11 @@ __global__ __launch_bounds__(256) void run_join_tiles(SharedArgs a) {
 #pragma unroll 4
         for (int i = k; i < all; i += groups) {
             const bool of_run = i < items;
-            const int r = (of_run ? row : own) % 16;
-            const float *p = of_run ? part_of(a, 16, first + i, hk, true) : part_of(a, 16, own_first + i - items, hk, false);
+            const int rows = of_run ? first_rows : second_rows, r = (of_run ? row : own) % rows;
+            const float *p = part_of(a, rows, of_run ? first + i : own_first + i - items, hk, of_run);
             const float m = p[r], most = fmaxf(top, m), f = __builtin_amdgcn_exp2f(top - most), h = __builtin_amdgcn_exp2f(m - most);
-            y = f * y + h * *reinterpret_cast<const f32x4 *>(p + 32 + r * a.D + c * 4);
-            sum = f * sum + h * p[16 + r];
+            y = f * y + h * *reinterpret_cast<const f32x4 *>(p + 2 * rows + r * a.D + c * 4);
+            sum = f * sum + h * p[rows + r];
             top = most;
         }
     }
@@ -85,20 +85,25 @@ SharedPlan shared_plan(int B, int heads, int heads_kv, int T, int D, int page, i
     const int64_t rows = (int64_t)T * size * (heads / heads_kv);
     p.second = plan_of(B, heads, heads_kv, T, D, page, columns, window, dtype);
     p.second_many = p.second.rows == kWideRows;
-    p.many = rows > 16 && !(D > 128 && dtype == ENATTEN_F32);
+    p.first = plan_of(runs, heads, heads_kv, T * size, D, page, columns, window, dtype);
+    p.many = p.first.rows == kWideRows;
     int64_t floats;
     if (p.many) {
-        p.first.rows = D <= 128 && rows <= 128 ? 128 : kWideRows;
+        p.first.rows = rows_of_first(D);
         p.first.row_tiles = (int)((rows + p.first.rows - 1) / p.first.rows);
-        p.first.parts = p.first.rows == 128 ? 512 : 256;
+        p.first.parts = 256;  // ranges: one workgroup per CU
         p.first.items = 0;
         p.first_rows = rows < p.first.rows ? (int)(rows + 31) / 32 * 32 : p.first.rows;
         const int64_t tiles = (int64_t)runs * p.first.row_tiles * heads_kv;
         floats = (2 * tiles + 3) / 4 * 4 + (tiles + p.first.parts) * item_floats(p.first_rows, padded(D));
     } else {
-        p.first = plan_of(runs, heads, heads_kv, T * size, D, page, columns, window, dtype);
-        p.first_rows = 16;
-        floats = head_floats((int64_t)runs * p.first.row_tiles) + p.first.items * heads_kv * item_floats(16, D);
+        const int64_t entries = (int64_t)runs * p.first.row_tiles;
+        const int slots = 256 * (waves_of(padded(D), p.first.rows / 16, dtype == ENATTEN_F32 ? 2 : 1) > 1 ? 2 : 1) / heads_kv;
+        const int64_t useful = entries * (((int64_t)columns * page + 16 + kLeast - 1) / kLeast);
+        p.first.parts = slots > entries && useful > entries ? (int)(slots < useful ? slots : useful) : 0;
+        p.first.items = p.first.parts ? p.first.parts : entries;
+        p.first_rows = p.first.rows;
+        floats = head_floats(entries) + p.first.items * heads_kv * item_floats(p.first.rows, D);
     }
     p.second_at = floats;
     if (p.second_many) {
@@ -192,23 +197,29 @@ int enatten_cache_attention_shared(const void *q, const void *k_cache, const voi
     a.first_tiles = p.first.row_tiles;
     a.first_parts = p.first.parts;
     a.first_rows = p.first_rows;
-    a.first_items = p.many ? 0 : (int)p.first.items;
     a.row_tiles = p.second.row_tiles;
     a.parts = p.second.parts;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const bool e = cache_dtype == ENATTEN_E4M3;
-    if (p.many && (rc = launch_first_rows(fn, a, p.first.rows, e, st))) return rc;
+    if (p.many && (rc = launch_first_rows(fn, a, e, st))) return rc;
     if (p.second_many) {
-        if ((rc = launch_first_join(fn, a, p.first.rows, st))) return rc;
+        if ((rc = launch_first_join(fn, a, st))) return rc;
         return launch_second_rows(fn, a, e, st);
     }
+    if (!p.many) {
+        a.first_items = (int)p.first.items;
+        if (p.first.rows != p.second.rows) {
+            if ((rc = launch_attend(fn, a, p.first.rows, a.first_items, e, st))) return rc;
+            a.first_items = 0;
+        }
+    }
     if ((rc = launch_attend(fn, a, p.second.rows, a.first_items + p.second.items, e, st))) return rc;
-    if (p.many) return launch_last_join(fn, a, p.first.rows, p.second.rows, st);
+    if (p.many) return launch_last_join(fn, a, p.second.rows, st);
     ProfScope prof(ENATTEN_KERNEL_CACHE_JOIN, "run_join_tiles", st);
     const int blocks = B * heads * T;
-    if (dtype == ENATTEN_BF16) run_join_tiles<ENATTEN_BF16><<<blocks, 256, 0, st>>>(a);
-    else if (dtype == ENATTEN_F32) run_join_tiles<ENATTEN_F32><<<blocks, 256, 0, st>>>(a);
-    else run_join_tiles<ENATTEN_F16><<<blocks, 256, 0, st>>>(a);
+    if (dtype == ENATTEN_BF16) run_join_tiles<ENATTEN_BF16><<<blocks, 256, 0, st>>>(a, p.first.rows, p.second.rows);
+    else if (dtype == ENATTEN_F32) run_join_tiles<ENATTEN_F32><<<blocks, 256, 0, st>>>(a, p.first.rows, p.second.rows);
+    else run_join_tiles<ENATTEN_F16><<<blocks, 256, 0, st>>>(a, p.first.rows, p.second.rows);
     return launched(fn);
 }
 
