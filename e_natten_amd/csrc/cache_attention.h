@@ -543,10 +543,9 @@ __device__ __forceinline__ int64_t lane_offset(int64_t x, int l) {
 // Tiles of kWideRows rows (cache_attention_rows.hip), a.parts ranges
 int launch_attend_rows(const char *fn, const AttnArgs &a, bool e4m3, hipStream_t st);
 // Tiles of many rows of either part, and the joins behind them (cache_attention_shared_rows.hip)
-int rows_of_first(int D);
-int launch_first_rows(const char *fn, const SharedArgs &a, bool e4m3, hipStream_t st);
-int launch_first_join(const char *fn, const SharedArgs &a, hipStream_t st);  // into canon
-int launch_last_join(const char *fn, const SharedArgs &a, int second_rows, hipStream_t st);
+int launch_first_rows(const char *fn, const SharedArgs &a, int rows, bool e4m3, hipStream_t st);
+int launch_first_join(const char *fn, const SharedArgs &a, int rows, hipStream_t st);  // into canon
+int launch_last_join(const char *fn, const SharedArgs &a, int rows, int second_rows, hipStream_t st);
 int launch_second_rows(const char *fn, const SharedArgs &a, bool e4m3, hipStream_t st);
 Plan plan_of(int B, int heads, int heads_kv, int T, int D, int page, int columns, int window, int dtype);
 size_t workspace_bytes(const Plan &p, int B, int heads_kv, int D);  // B: sequences, or runs

@@ -110,7 +110,7 @@ __device__ __forceinline__ void rows_body(const Args &args) {
     if constexpr (SECOND) seen = min(seen, hi_r - joins);
     f16x8 qf[KEPT][TERMS], *q_rest = &q_lds[threadIdx.x];
     float unit, l;
-    {
+    auto take_q = [&] {
         const int64_t at = offset_of(a.q, where);
         const float flip = a.scale < 0.f ? -1.f : 1.f;  // into q, so that units are not negative
         float x[SD][8], top = 0.f, nan = 0.f;
@@ -159,7 +159,8 @@ __device__ __forceinline__ void rows_body(const Args &args) {
                 else q_rest[(c - KEPT) * 512] = w[t];
             }
         }
-    }
+    };
+    if constexpr (!FIRST) take_q();
     // tokens that any, and that all rows of the wave see
     const int t_first = min(row0, all_rows - 1) / a.group, t_last = min(min(row0 + 31, all_rows - 1) / a.group, s.count - 1);
     const bool any_row = row0 < all_rows && t_first < s.count;
@@ -243,6 +244,10 @@ __device__ __forceinline__ void rows_body(const Args &args) {
             }
         }
     };
+    if constexpr (FIRST) {
+        if (step0 < step1) fetch(step0);  // (under way while the rows of q come)
+        take_q();
+    }
     auto put_as = [&](auto seen, int buffer) {
         constexpr bool SEEN = decltype(seen)::value;
         if (!for_v) {
@@ -409,7 +414,7 @@ __device__ __forceinline__ void rows_body(const Args &args) {
 
     __syncthreads();  // (the last tile's operands are read)
     if (step0 < step1) {
-        fetch(step0);
+        if constexpr (!FIRST) fetch(step0);
         put(0, step0);
         if (step0 + 1 < step1) fetch(step0 + 1);
     }

@@ -89,7 +89,7 @@ SharedPlan shared_plan(int B, int heads, int heads_kv, int T, int D, int page, i
     p.many = p.first.rows == kWideRows;
     int64_t floats;
     if (p.many) {
-        p.first.rows = rows_of_first(D);
+        p.first.rows = D > 128 ? kWideRows : rows <= 64 ? 64 : 128;
         p.first.row_tiles = (int)((rows + p.first.rows - 1) / p.first.rows);
         p.first.parts = 256;  // ranges: one workgroup per CU
         p.first.items = 0;
@@ -201,9 +201,9 @@ int enatten_cache_attention_shared(const void *q, const void *k_cache, const voi
     a.parts = p.second.parts;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const bool e = cache_dtype == ENATTEN_E4M3;
-    if (p.many && (rc = launch_first_rows(fn, a, e, st))) return rc;
+    if (p.many && (rc = launch_first_rows(fn, a, p.first.rows, e, st))) return rc;
     if (p.second_many) {
-        if ((rc = launch_first_join(fn, a, st))) return rc;
+        if ((rc = launch_first_join(fn, a, p.first.rows, st))) return rc;
         return launch_second_rows(fn, a, e, st);
     }
     if (!p.many) {
@@ -214,7 +214,7 @@ int enatten_cache_attention_shared(const void *q, const void *k_cache, const voi
         }
     }
     if ((rc = launch_attend(fn, a, p.second.rows, a.first_items + p.second.items, e, st))) return rc;
-    if (p.many) return launch_last_join(fn, a, p.second.rows, st);
+    if (p.many) return launch_last_join(fn, a, p.first.rows, p.second.rows, st);
     ProfScope prof(ENATTEN_KERNEL_CACHE_JOIN, "run_join_tiles", st);
     const int blocks = B * heads * T;
     if (dtype == ENATTEN_BF16) run_join_tiles<ENATTEN_BF16><<<blocks, 256, 0, st>>>(a, p.first.rows, p.second.rows);

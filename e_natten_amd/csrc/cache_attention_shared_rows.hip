@@ -5,12 +5,10 @@
 namespace enatten {
 namespace {
 
-// The first part: tiles of 64 rows, steps of 128 tokens (256 of up to 64 channels) that four groups of waves share;
-// above 128 channels, where LDS has no room for such steps, and in the second part tiles of 256 rows.
-constexpr int first_groups(int DP) { return DP <= 128 ? 4 : 1; }
-template <int PASS, int DP, bool E4M3, int DT>
+// The first part: tiles of 64 or 128 rows, steps of 128 tokens (256 of up to 64 channels) that four or two groups of
+// waves share; above 128 channels, where LDS has no room for such steps, and in the second part tiles of 256 rows.
+template <int PASS, int DP, bool E4M3, int DT, int TG>
 __global__ __launch_bounds__(512, 2) void run_rows(PassArgs<PASS> args) {
-    constexpr int TG = PASS == 1 ? first_groups(DP) : 1;
     rows_body<DP, E4M3, DT, TG, TG == 1 ? 1 : 2>(args);
 }
 template <int DP, int DT>
@@ -113,16 +111,21 @@ PassArgs<PASS> pass_args(const SharedArgs &s) {
 }
 
 template <int DP, bool E4M3, int DT>
-int first_rows(const char *fn, const SharedArgs &a, hipStream_t st) {
+int first_rows(const char *fn, const SharedArgs &a, int rows, hipStream_t st) {
     ProfScope prof(ENATTEN_KERNEL_CACHE_ATTENTION, "run_rows", st);
-    run_rows<1, DP, E4M3, DT><<<a.first_parts, 512, 0, st>>>(pass_args<1>(a));
+    if constexpr (DP <= 128) {
+        if (rows == 64) run_rows<1, DP, E4M3, DT, 4><<<a.first_parts, 512, 0, st>>>(pass_args<1>(a));
+        else run_rows<1, DP, E4M3, DT, 2><<<a.first_parts, 512, 0, st>>>(pass_args<1>(a));
+    } else {
+        run_rows<1, DP, E4M3, DT, 1><<<a.first_parts, 512, 0, st>>>(pass_args<1>(a));
+    }
     return launched(fn);
 }
 template <int DP, bool E4M3, int DT>
 int second_rows(const char *fn, const SharedArgs &a, hipStream_t st) {
     {
         ProfScope prof(ENATTEN_KERNEL_CACHE_ATTENTION, "run_rows", st);
-        run_rows<2, DP, E4M3, DT><<<a.parts, 512, 0, st>>>(pass_args<2>(a));
+        run_rows<2, DP, E4M3, DT, 1><<<a.parts, 512, 0, st>>>(pass_args<2>(a));
     }
     const int rc = launched(fn);
     if (rc) return rc;
@@ -158,10 +161,9 @@ int by_dim(const SharedArgs &a, F f) {
 
 }  // namespace
 
-int rows_of_first(int D) { return 256 / first_groups(padded(D)); }
-int launch_first_rows(const char *fn, const SharedArgs &a, bool e4m3, hipStream_t st) {
+int launch_first_rows(const char *fn, const SharedArgs &a, int rows, bool e4m3, hipStream_t st) {
     return by_dim(a, [&](auto dp, auto dt) {
-        return e4m3 ? first_rows<dp.value, true, dt.value>(fn, a, st) : first_rows<dp.value, false, dt.value>(fn, a, st);
+        return e4m3 ? first_rows<dp.value, true, dt.value>(fn, a, rows, st) : first_rows<dp.value, false, dt.value>(fn, a, rows, st);
     });
 }
 int launch_second_rows(const char *fn, const SharedArgs &a, bool e4m3, hipStream_t st) {
@@ -169,11 +171,11 @@ int launch_second_rows(const char *fn, const SharedArgs &a, bool e4m3, hipStream
         return e4m3 ? second_rows<dp.value, true, dt.value>(fn, a, st) : second_rows<dp.value, false, dt.value>(fn, a, st);
     });
 }
-int launch_first_join(const char *fn, const SharedArgs &a, hipStream_t st) {
-    return by_dim(a, [&](auto dp, auto) { return join<dp.value, ENATTEN_F32, true>(fn, a, rows_of_first(a.D), 16, st); });
+int launch_first_join(const char *fn, const SharedArgs &a, int rows, hipStream_t st) {
+    return by_dim(a, [&](auto dp, auto) { return join<dp.value, ENATTEN_F32, true>(fn, a, rows, 16, st); });
 }
-int launch_last_join(const char *fn, const SharedArgs &a, int second, hipStream_t st) {
-    return by_dim(a, [&](auto dp, auto dt) { return join<dp.value, dt.value, false>(fn, a, rows_of_first(a.D), second, st); });
+int launch_last_join(const char *fn, const SharedArgs &a, int rows, int second, hipStream_t st) {
+    return by_dim(a, [&](auto dp, auto dt) { return join<dp.value, dt.value, false>(fn, a, rows, second, st); });
 }
 
 }  // namespace enatten
