@@ -13,8 +13,10 @@ namespace {
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kMostRows = 8192;  // of the table: 64 KB of LDS hold two numbers of each
+constexpr int kMostRows = 4096;  // of the table: 64 KB of LDS hold four numbers of each
 
+// Loads that some lanes do not need are made by all, of a place that is there: behind a branch each of them is waited
+// for before the next one.
 struct PageTable {
     int *pages;
     int64_t stride;
@@ -22,6 +24,21 @@ struct PageTable {
     __device__ int &at(int b, int column) const { return pages[b * stride + column]; }
     __device__ bool is_page(int e) const { return (unsigned)e < (unsigned)num_pages; }
 };
+
+// 16 neighbouring numbers from p on; what lies behind the last one is any of them
+__device__ __forceinline__ void load16(const int *from, int64_t p, int64_t total, int (&h)[16]) {
+    if ((uintptr_t)from % 16 == 0 && p + 16 <= total) {
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+            const i32x4 x = *reinterpret_cast<const i32x4 *>(from + p + j);
+#pragma unroll
+            for (int k = 0; k < 4; k++) h[j + k] = x[k];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; j++) h[j] = from[min(p + j, total - 1)];
+    }
+}
 
 // Sum of x over the workgroup's threads up to and including each, and over all.  part: one number for every wave.
 template <int THREADS>
@@ -52,45 +69,55 @@ struct ForkArgs {
     bool with_lengths;  // one workgroup for the whole table: the lengths too
 };
 __device__ __forceinline__ bool moves(int parent, int b, int B) { return parent >= -1 && parent < B && parent != b; }
-__device__ __forceinline__ int length_after(const ForkArgs &a, int b) {
-    const int p = a.parents[b];
-    return !moves(p, b, a.t.B) ? a.lengths[b] : p < 0 ? 0 : a.lengths[p];
-}
 
-// Some columns of all rows: read as they are into LDS, written anew from there.
-__global__ __launch_bounds__(256) void fork_rows(ForkArgs a) {
-    extern __shared__ int was[];  // [B][w], then the lengths
+// Some columns of all rows: read as they are into LDS, written anew from there.  Parents and the lengths that they
+// have are read once, beside the entries: 128 rows of 10 columns took 6.5 us with loads in front of every entry.
+__global__ __launch_bounds__(1024) void fork_rows(ForkArgs a) {
+    extern __shared__ int was[];  // [B][w]; per row its parent (-2: stays), its new tokens and their columns
+    const int threads = blockDim.x;
     const int c0 = blockIdx.x * a.width, w = min(a.width, a.t.columns - c0), all = a.t.B * w;
-    for (int i = threadIdx.x; i < all; i += 256) {
-        const int b = i / w;
-        was[i] = a.t.at(b, c0 + i - b * w);
-    }
-    int *tokens = was + a.t.B * a.width;
-    if (a.with_lengths)
-        for (int b = threadIdx.x; b < a.t.B; b += 256) tokens[b] = length_after(a, b);
-    __syncthreads();
-    for (int i = threadIdx.x; i < all; i += 256) {
-        const int b = i / w, column = c0 + i - b * w, p = a.parents[b];
-        if (!moves(p, b, a.t.B)) continue;
-        int e = -1;
-        if (p >= 0) {
-            const int64_t used = ((int64_t)a.lengths[p] + a.t.page - 1) / a.t.page;
-            if (column < used) e = was[p * w + column - c0];
+    int *parent = was + a.t.B * a.width, *tokens = parent + a.t.B, *used = tokens + a.t.B;
+    constexpr int DEEP = 4;
+    for (int i0 = threadIdx.x; i0 < all; i0 += threads * DEEP) {
+        int e[DEEP];
+#pragma unroll
+        for (int k = 0; k < DEEP; k++) {
+            const int i = min(i0 + k * threads, all - 1), b = i / w;
+            e[k] = a.t.at(b, c0 + i - b * w);
         }
-        const int old = was[i];
+#pragma unroll
+        for (int k = 0; k < DEEP; k++) was[min(i0 + k * threads, all - 1)] = e[k];
+    }
+    for (int b = threadIdx.x; b < a.t.B; b += threads) {
+        const int p = a.parents[b];
+        const bool moved = moves(p, b, a.t.B);
+        const int len = moved && p >= 0 ? a.lengths[p] : 0;
+        parent[b] = moved ? p : -2;
+        tokens[b] = len;
+        used[b] = (int)(((int64_t)len + a.t.page - 1) / a.t.page);
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int i = threadIdx.x; i < all; i += threads) {
+        const int b = i / w, c = i - b * w, p = parent[b];
+        if (p == -2) continue;
+        const int old = was[i], e = p >= 0 && c0 + c < used[b] ? was[p * w + c] : -1;
         if (e == old) continue;
-        a.t.at(b, column) = e;
+        a.t.at(b, c0 + c) = e;
         if (a.t.is_page(old)) atomicAdd(a.holders + old, -1);
         if (a.t.is_page(e)) atomicAdd(a.holders + e, 1);
     }
     if (!a.with_lengths) return;
-    __syncthreads();
-    for (int b = threadIdx.x; b < a.t.B; b += 256) a.lengths[b] = tokens[b];
+    for (int b = threadIdx.x; b < a.t.B; b += threads)
+        if (parent[b] != -2) a.lengths[b] = tokens[b];
 }
 // The lengths by a launch of their own, where several workgroups read them.
 __global__ __launch_bounds__(1024) void fork_lengths(ForkArgs a) {
     extern __shared__ int tokens[];
-    for (int b = threadIdx.x; b < a.t.B; b += 1024) tokens[b] = length_after(a, b);
+    for (int b = threadIdx.x; b < a.t.B; b += 1024) {
+        const int p = a.parents[b];
+        tokens[b] = !moves(p, b, a.t.B) ? a.lengths[b] : p < 0 ? 0 : a.lengths[p];
+    }
     __syncthreads();
     for (int b = threadIdx.x; b < a.t.B; b += 1024) a.lengths[b] = tokens[b];
 }
@@ -100,7 +127,7 @@ __global__ __launch_bounds__(1024) void fork_lengths(ForkArgs a) {
 struct ReserveArgs {
     PageTable t;
     const int *lengths, *counts;
-    int *holders, *copies, *keeper, *list;  // workspace: [num_pages], [B * columns]
+    int *holders, *copies, *keeper;  // keeper: workspace [num_pages]
     int count;
 };
 // The columns that a row's new tokens go to.
@@ -118,137 +145,268 @@ __device__ __forceinline__ Need need_of(const ReserveArgs &a, int b) {
     }
     return n;
 }
+__device__ __forceinline__ void put_copy(const ReserveArgs &a, int b, int from, int to, int tokens) {
+    a.copies[3 * b] = from;
+    a.copies[3 * b + 1] = to;
+    a.copies[3 * b + 2] = tokens;
+}
 // Stores and atomics of this wave are done: other waves see them in memory behind the next barrier.
 __device__ __forceinline__ void settle() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 __device__ __forceinline__ int load_now(const int *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
-// One workgroup.  Which rows leave a first page to others; the entries that want a page, in order; then the
-// free pages in theirs, each to the entry of its rank.
-__global__ __launch_bounds__(1024) void reserve_pages(ReserveArgs a) {
-    extern __shared__ int lds[];
-    __shared__ int part[16];
-    int *offset = lds;                                                     // [B + 1]: columns of the rows before
-    unsigned *common = reinterpret_cast<unsigned *>(lds + a.t.B + 1);      // a bit for each row: its first page
-    const int words = (a.t.B + 31) / 32;                                   // holds older tokens, and others hold it
-    unsigned *keeps = common + words;                                      // ... and it keeps it
-    const int tid = threadIdx.x;
-    auto bit = [](const unsigned *set, int b) { return (set[b / 32] >> (b % 32) & 1u) != 0; };
-    for (int i = tid; i < 2 * words; i += 1024) common[i] = 0;
-    __syncthreads();
-    bool any = false;
-    int upto = 0;
-    for (int b0 = 0; b0 < a.t.B; b0 += 1024) {
-        const int b = b0 + tid;
-        Need n{0, 0, 0};
-        if (b < a.t.B) {
-            n = need_of(a, b);
-            a.copies[3 * b] = a.copies[3 * b + 1] = -1;
-            a.copies[3 * b + 2] = 0;
-            if (n.columns && n.older) {
-                const int e = a.t.at(b, n.first);
-                if (a.t.is_page(e) && a.holders[e] > 1) {
-                    any = true;
-                    a.keeper[e] = -1;
-                    atomicOr(common + b / 32, 1u << (b % 32));
-                }
-            }
-        }
-        int total;
-        const int sum = block_sum<1024>(n.columns, part, total);
-        if (b < a.t.B) offset[b] = upto + sum - n.columns;
-        upto += total;
-    }
-    if (tid == 0) offset[a.t.B] = upto;
-    // If all holders of a page write to it, the last of them keeps it.
-    settle();
-    if (__syncthreads_or(any)) {
-        for (int b = tid; b < a.t.B; b += 1024) {
-            if (!bit(common, b)) continue;
-            const int e = a.t.at(b, need_of(a, b).first);
-            atomicMax(a.keeper + e, b);
-            atomicAdd(a.holders + e, -1);
-        }
-        settle();
-        __syncthreads();
-        for (int b = tid; b < a.t.B; b += 1024) {
-            if (!bit(common, b)) continue;
-            const int e = a.t.at(b, need_of(a, b).first);
-            if (load_now(a.holders + e) == 0 && load_now(a.keeper + e) == b) atomicOr(keeps + b / 32, 1u << (b % 32));
-        }
-        __syncthreads();
-        for (int b = tid; b < a.t.B; b += 1024)
-            if (bit(keeps, b)) atomicAdd(a.holders + a.t.at(b, need_of(a, b).first), 1);
-        settle();
-        __syncthreads();
-    }
-    auto leaves = [&](int b) { return bit(common, b) && !bit(keeps, b); };
-
-    int wanted = 0;
-    for (int i0 = 0; i0 < upto; i0 += 1024) {
-        const int i = i0 + tid;
-        int entry = -1;
-        if (i < upto) {
-            int lo = 0, hi = a.t.B;  // offset[lo] <= i < offset[hi]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) / 2;
-                if (offset[mid] <= i) lo = mid;
-                else hi = mid;
-            }
-            const Need n = need_of(a, lo);
-            const int column = n.first + i - offset[lo];
-            const bool begun = n.older && column == n.first;
-            if (begun ? leaves(lo) : !a.t.is_page(a.t.at(lo, column))) entry = lo * a.t.columns + column;
-        }
-        int total;
-        const int sum = block_sum<1024>(entry >= 0, part, total);
-        if (entry >= 0) a.list[wanted + sum - 1] = entry;
-        wanted += total;
-    }
-    settle();
-    __syncthreads();  // (the list is read by other threads)
-    if (wanted == 0) return;
-
-    auto give = [&](int rank, int page) {
-        const int entry = a.list[rank], b = entry / a.t.columns, column = entry - b * a.t.columns;
-        int &at = a.t.at(b, column);
-        if (page >= 0) {
-            a.holders[page] = 1;
-            const Need n = need_of(a, b);
-            if (n.older && column == n.first) {
-                a.copies[3 * b] = at;
-                a.copies[3 * b + 1] = page;
-                a.copies[3 * b + 2] = n.older;
-            }
-        }
-        at = page;
-    };
+// The first `wanted` free pages in order: put(rank, page).  Returns how many there are of them.
+template <class F>
+__device__ __forceinline__ int free_pages(const ReserveArgs &a, int wanted, int *part, F put) {
     constexpr int EACH = 16;  // pages of a thread
-    const bool aligned = (uintptr_t)a.holders % 16 == 0;
-    int given = 0;
-    for (int64_t p0 = 0; p0 < a.t.num_pages && given < wanted; p0 += 1024 * EACH) {
-        const int64_t p = p0 + tid * EACH;
+    auto look = [&](int64_t p0) {
+        const int64_t p = p0 + threadIdx.x * EACH;
         unsigned free = 0;
-        if (aligned && p + EACH <= a.t.num_pages) {
+        if (p < a.t.num_pages) {
+            int h[EACH];
+            load16(a.holders, p, a.t.num_pages, h);
 #pragma unroll
-            for (int j = 0; j < EACH; j += 4) {
-                const i32x4 h = *reinterpret_cast<const i32x4 *>(a.holders + p + j);
-#pragma unroll
-                for (int k = 0; k < 4; k++) free |= h[k] == 0 ? 1u << (j + k) : 0u;
-            }
-        } else {
-            for (int j = 0; j < EACH; j++)
-                if (p + j < a.t.num_pages && a.holders[p + j] == 0) free |= 1u << j;
+            for (int j = 0; j < EACH; j++) free |= p + j < a.t.num_pages && h[j] == 0 ? 1u << j : 0u;
         }
+        return free;
+    };
+    int given = 0;
+    unsigned next = look(0);
+    for (int64_t p0 = 0; p0 < a.t.num_pages && given < wanted; p0 += 1024 * EACH) {
+        unsigned free = next;
+        next = look(p0 + 1024 * EACH);  // (under way beside the sum)
         int total;
         int rank = given + block_sum<1024>(__popc(free), part, total) - __popc(free);
-        while (free && rank < wanted) {
-            const int j = __ffs(free) - 1;
-            free &= free - 1;
-            give(rank++, (int)p + j);
+        if (free && rank < wanted) {
+#pragma unroll
+            for (int j = 0; j < EACH; j++) {
+                if ((free >> j & 1) && rank < wanted) put(rank, (int)p0 + (int)threadIdx.x * EACH + j);
+                rank += free >> j & 1;
+            }
         }
         given += total;
     }
-    for (int rank = given + tid; rank < wanted; rank += 1024) give(rank, -1);
+    return min(given, wanted);
+}
+
+constexpr int kShortRows = 1024, kShortColumns = 4;
+
+// Up to 1024 rows, a thread each.  A row whose first page e holds older tokens and is held by others too (held > 1)
+// leaves it to them; if all its holders would, the last of them keeps it.  page_of: a number for every row.
+__device__ __forceinline__ bool leaves_page(const ReserveArgs &a, int e, int held, int *page_of) {
+    const int b = threadIdx.x;
+    const bool common = held > 1;
+    page_of[b] = common ? e : -1;
+    if (!__syncthreads_or(common) || !common) return false;
+    int writers = 0, last = 0;
+#pragma unroll 16
+    for (int i = 0; i < a.t.B; i++) {
+        const bool same = page_of[i] == e;
+        writers += same;
+        last = same ? i : last;
+    }
+    if (last == b) a.holders[e] = held - writers + (writers == held);
+    return !(writers == held && last == b);
+}
+
+// Up to 1024 rows that need four columns each at most, as single tokens do.  False if they are not.
+__device__ __forceinline__ bool reserve_short(const ReserveArgs &a, int *part, int *page_of, int *fresh) {
+    const int b = threadIdx.x;
+    Need n{0, 0, 0};
+    if (a.t.B > kShortRows) return false;
+    int e[kShortColumns];
+    if (b < a.t.B) n = need_of(a, b);
+#pragma unroll
+    for (int i = 0; i < kShortColumns; i++) e[i] = a.t.at(min(b, a.t.B - 1), n.first + min(i, max(n.columns - 1, 0)));
+    if (__syncthreads_or(n.columns > kShortColumns)) return false;
+    const bool leaves = leaves_page(a, e[0], n.older && a.t.is_page(e[0]) ? a.holders[e[0]] : 0, page_of);
+    unsigned wants = leaves ? 1u : 0u;
+#pragma unroll
+    for (int i = 0; i < kShortColumns; i++)
+        if (i < n.columns && !(i == 0 && n.older) && !a.t.is_page(e[i])) wants |= 1u << i;
+    int wanted;
+    int rank = block_sum<1024>(__popc(wants), part, wanted) - __popc(wants);
+    int given = 0;
+    if (wanted) {
+        given = free_pages(a, wanted, part, [&](int r, int page) { fresh[r] = page; });
+        __syncthreads();
+    }
+    if (b >= a.t.B) return true;
+    int to = -1;
+#pragma unroll
+    for (int i = 0; i < kShortColumns; i++) {
+        if (!(wants >> i & 1)) continue;
+        const int page = rank < given ? fresh[rank] : -1;
+        rank++;
+        a.t.at(b, n.first + i) = page;
+        if (page >= 0) a.holders[page] = 1;
+        if (i == 0 && leaves) to = page;
+    }
+    put_copy(a, b, to >= 0 ? e[0] : -1, to, to >= 0 ? n.older : 0);
+    return true;
+}
+
+// Columns c0 .. c0 + 64 N - 1 of a row that a wave goes over, from n.first on: those that want a page, a bit per lane
+// for each 64; `old` is what the lane's entries are.
+template <int N>
+__device__ __forceinline__ void wants_of(const ReserveArgs &a, int b, const Need &n, bool leaves, int c0, int (&old)[N],
+                                         unsigned long long (&who)[N]) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        const int c = c0 + j * 64 + lane;
+        old[j] = a.t.at(b, n.first + min(c, n.columns - 1));
+    }
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        const int c = c0 + j * 64 + lane;
+        who[j] = __ballot(c < n.columns && (c == 0 && n.older ? leaves : !a.t.is_page(old[j])));
+    }
+}
+
+// One workgroup.  But for short calls: which rows leave a first page to others; how many pages each row wants, by a
+// thread where it has up to four columns, else by a wave; the free pages in their order; and each to the entry of
+// its rank.  (With a thread for every entry the one CU was bound by instructions: 8000 entries took 14 us.)
+__global__ __launch_bounds__(1024) void reserve_pages(ReserveArgs a) {
+    extern __shared__ int lds[];
+    __shared__ int part[16], page_of[kShortRows], fresh_short[kShortRows * kShortColumns], long_rows;
+    if (reserve_short(a, part, page_of, fresh_short)) return;
+    int *count = lds, *row_of = lds + a.t.B;  // [B] each: pages that a row wants, then of the rows before; the long rows
+    unsigned *left = reinterpret_cast<unsigned *>(lds + 2 * a.t.B), *common = left + (a.t.B + 31) / 32;  // a bit for each row
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    auto bit = [](const unsigned *set, int b) { return (set[b / 32] >> (b % 32) & 1u) != 0; };
+    auto mark = [](unsigned *set, int b) { atomicOr(set + b / 32, 1u << (b % 32)); };
+    for (int i = tid; i < 2 * ((a.t.B + 31) / 32); i += 1024) left[i] = 0;
+    if (tid == 0) long_rows = 0;
+    __syncthreads();
+
+    // first pages that hold older tokens and that others hold
+    auto first_page = [&](int b, const Need &n) {
+        const int e = n.older ? a.t.at(b, n.first) : -1;
+        return a.t.is_page(e) && a.holders[e] > 1 ? e : -1;
+    };
+    if (a.t.B <= kShortRows) {
+        const int e = tid < a.t.B ? first_page(tid, need_of(a, tid)) : -1;
+        if (leaves_page(a, e, e >= 0 ? a.holders[e] : 0, page_of)) mark(left, tid);
+    } else {
+        bool any = false;
+        for (int b = tid; b < a.t.B; b += 1024) {
+            const int e = first_page(b, need_of(a, b));
+            if (e < 0) continue;
+            any = true;
+            a.keeper[e] = -1;
+            mark(common, b);
+        }
+        settle();
+        if (__syncthreads_or(any)) {
+            for (int b = tid; b < a.t.B; b += 1024) {
+                if (!bit(common, b)) continue;
+                const int e = a.t.at(b, need_of(a, b).first);
+                atomicMax(a.keeper + e, b);
+                atomicAdd(a.holders + e, -1);
+            }
+            settle();
+            __syncthreads();
+            for (int b = tid; b < a.t.B; b += 1024) {
+                if (!bit(common, b)) continue;
+                const int e = a.t.at(b, need_of(a, b).first);
+                if (load_now(a.holders + e) != 0 || load_now(a.keeper + e) != b) mark(left, b);
+            }
+            __syncthreads();
+            for (int b = tid; b < a.t.B; b += 1024)
+                if (bit(common, b) && !bit(left, b)) atomicAdd(a.holders + a.t.at(b, need_of(a, b).first), 1);
+            settle();
+        }
+    }
+    __syncthreads();
+
+    constexpr int N = 8;  // (4: 1.5 us more in a call of 32 rows with 256 columns each)
+    for (int b = tid; b < a.t.B; b += 1024) {
+        const Need n = need_of(a, b);
+        if (n.columns > kShortColumns) {
+            row_of[atomicAdd(&long_rows, 1)] = b;
+            continue;
+        }
+        const bool leaves = bit(left, b);
+        int wants = 0;
+        for (int c = 0; c < n.columns; c++) wants += c == 0 && n.older ? leaves : !a.t.is_page(a.t.at(b, n.first + c));
+        count[b] = wants;
+        put_copy(a, b, -1, -1, 0);
+    }
+    __syncthreads();
+    for (int i = wave; i < long_rows; i += 16) {
+        const int b = __builtin_amdgcn_readfirstlane(row_of[i]);
+        const Need n = need_of(a, b);
+        const bool leaves = bit(left, b);
+        int wants = 0;
+        for (int c0 = 0; c0 < n.columns; c0 += 64 * N) {
+            int old[N];
+            unsigned long long who[N];
+            wants_of(a, b, n, leaves, c0, old, who);
+#pragma unroll
+            for (int j = 0; j < N; j++) wants += __popcll(who[j]);
+        }
+        if (lane == 0) {
+            count[b] = wants;
+            put_copy(a, b, -1, -1, 0);
+        }
+    }
+    settle();
+    __syncthreads();
+    int wanted = 0;
+    for (int b0 = 0; b0 < a.t.B; b0 += 1024) {
+        const int b = b0 + tid, mine = b < a.t.B ? count[b] : 0;
+        int total;
+        const int sum = block_sum<1024>(mine, part, total);
+        if (b < a.t.B) count[b] = wanted + sum - mine;
+        wanted += total;
+    }
+    if (wanted == 0) return;
+    // (the places of `keeper` are free again: pages in the order in which they are given out)
+    int *fresh = a.keeper;
+    const int given = free_pages(a, wanted, part, [&](int r, int page) { fresh[r] = page; });
+    settle();
+    __syncthreads();
+
+    auto fresh_at = [&](int rank) {
+        const int page = fresh[min(rank, max(given - 1, 0))];
+        return rank < given ? page : -1;
+    };
+    auto give = [&](int b, const Need &n, int c, int old, int page) {
+        a.t.at(b, n.first + c) = page;
+        if (page < 0) return;
+        a.holders[page] = 1;
+        if (c == 0 && n.older) put_copy(a, b, old, page, n.older);
+    };
+    for (int b = tid; b < a.t.B; b += 1024) {
+        const Need n = need_of(a, b);
+        if (n.columns > kShortColumns) continue;
+        const bool leaves = bit(left, b);
+        int rank = count[b];
+        for (int c = 0; c < n.columns; c++) {
+            const int old = a.t.at(b, n.first + c);
+            if (c == 0 && n.older ? leaves : !a.t.is_page(old)) give(b, n, c, old, fresh_at(rank++));
+        }
+    }
+    for (int i = wave; i < long_rows; i += 16) {
+        const int b = __builtin_amdgcn_readfirstlane(row_of[i]);
+        const Need n = need_of(a, b);
+        const bool leaves = bit(left, b);
+        int rank = count[b];
+        for (int c0 = 0; c0 < n.columns; c0 += 64 * N) {
+            int old[N];
+            unsigned long long who[N];
+            wants_of(a, b, n, leaves, c0, old, who);
+            int page[N];
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                page[j] = fresh_at(rank + __popcll(who[j] & ((1ull << lane) - 1)));
+                rank += __popcll(who[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < N; j++)
+                if (who[j] >> lane & 1) give(b, n, c0 + j * 64 + lane, old[j], page[j]);
+        }
+    }
 }
 
 // ---- copies of pages ----------------------------------------------------------
@@ -265,11 +423,13 @@ struct CopyArgs {
     int n, layers, heads, D, num_pages, page, split;
 };
 
-// A unit is 16 codes of a token.  A workgroup takes pages `gridDim.x` apart, of each a share of its blocks
-// (key or value, layer, head); 64 entries of the list are looked at together, as most may be empty.
+// A workgroup takes pages `gridDim.x` apart, of each a share of its blocks (key or value, layer, head); 64 lines
+// of the list are looked at together, as most may be empty.  A wave goes over its part of these block by block in
+// chunks of 64 units of 16 codes, four of them under way; where that is comes by counting, since divisions for every
+// unit took as long as the copy.
 __global__ __launch_bounds__(256) void copy_pages(CopyArgs a) {
-    constexpr int DEEP = 4;  // units whose loads are under way at a time
-    const int lane = threadIdx.x & 63, blocks = 2 * a.layers * a.heads;
+    constexpr int DEEP = 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), blocks = 2 * a.layers * a.heads;
     const int per = (blocks + a.split - 1) / a.split, first = blockIdx.y * per, mine = min(per, blocks - first);
     if (mine <= 0) return;
     const int wide = a.D / 16;
@@ -286,28 +446,45 @@ __global__ __launch_bounds__(256) void copy_pages(CopyArgs a) {
         for (unsigned long long who = __ballot(there); who; who &= who - 1) {
             const int l = __ffsll(who) - 1;
             const int64_t from = __builtin_amdgcn_readlane(source, l), to = __builtin_amdgcn_readlane(target, l);
-            const unsigned units = __builtin_amdgcn_readlane(tokens, l) * wide;
+            const int units = __builtin_amdgcn_readlane(tokens, l) * wide, chunks = (units + 63) / 64;
             for (int k = threadIdx.x; k < mine; k += 256) {
                 const int block = first + k, which = block & 1, head = block / 2 % a.heads, layer = block / 2 / a.heads;
                 const PoolView &c = a.c[which];
                 float *z = c.scales + layer * c.zl + head * c.zh;
                 z[to * c.zp] = z[from * c.zp];
             }
-            const int64_t all = (int64_t)mine * units;
-            for (int64_t u0 = threadIdx.x; u0 < all; u0 += 256 * DEEP) {
+            const int all = mine * chunks, share = (all + 3) / 4;  // (at most 2^16 blocks of 2^8 chunks)
+            int at = wave * share;
+            const int end = min(at + share, all);
+            int block = first + at / chunks, chunk = at % chunks, head = block / 2 % a.heads, layer = block / 2 / a.heads;
+            while (at < end) {
                 u32x4 x[DEEP];
                 char *put[DEEP];
 #pragma unroll
                 for (int k = 0; k < DEEP; k++) {
-                    const int64_t u = u0 + k * 256;
                     put[k] = nullptr;
-                    if (u < all) {
-                        const unsigned nth = (unsigned)u / units, unit = (unsigned)u - nth * units, row = unit / wide;
-                        const int block = first + nth, which = block & 1, head = block / 2 % a.heads, layer = block / 2 / a.heads;
-                        const PoolView &c = a.c[which];
-                        char *at = c.codes + layer * c.sl + head * c.sh + row * c.st + (unit - row * wide) * 16;
-                        put[k] = at + to * c.sp;
-                        x[k] = *reinterpret_cast<const u32x4 *>(at + from * c.sp);
+                    if (at < end) {
+                        const PoolView &c = a.c[block & 1];
+                        const int unit = chunk * 64 + lane;
+                        if (unit < units) {
+                            char *p = c.codes + layer * c.sl + head * c.sh;
+                            if (c.st == a.D) {
+                                p += unit * 16;
+                            } else {
+                                const int row = (unsigned)unit / (unsigned)wide;
+                                p += row * c.st + (unit - row * wide) * 16;
+                            }
+                            put[k] = p + to * c.sp;
+                            x[k] = *reinterpret_cast<const u32x4 *>(p + from * c.sp);
+                        }
+                        at++;
+                        if (++chunk == chunks) {
+                            chunk = 0;
+                            if (++block % 2 == 0 && ++head == a.heads) {
+                                head = 0;
+                                layer++;
+                            }
+                        }
                     }
                 }
 #pragma unroll
@@ -330,10 +507,12 @@ struct CompactArgs {
 // 8 neighbouring pages of slab `slab`: a bit for each one that is held and lies below `end`.
 __device__ __forceinline__ unsigned held_of(const CompactArgs &a, int slab, int64_t end) {
     unsigned held = 0;
+    int h[8];
     const int64_t p = (int64_t)slab * kSlab + threadIdx.x * 8;
 #pragma unroll
-    for (int j = 0; j < 8; j++)
-        if (p + j < end && a.holders[p + j] != 0) held |= 1u << j;
+    for (int j = 0; j < 8; j++) h[j] = a.holders[min(p + j, (int64_t)a.t.num_pages - 1)];
+#pragma unroll
+    for (int j = 0; j < 8; j++) held |= p + j < end && h[j] != 0 ? 1u << j : 0u;
     return held;
 }
 __global__ __launch_bounds__(256) void count_held(CompactArgs a) {
@@ -402,6 +581,73 @@ __global__ __launch_bounds__(256) void move_pages(CompactArgs a) {
     }
 }
 
+// Pools of up to kSmallPool pages and tables of about as many entries: all of it in one workgroup.
+constexpr int kSmallPool = 16384;
+__global__ __launch_bounds__(1024) void compact_small(CompactArgs a) {
+    constexpr int EACH = kSmallPool / 1024;
+    __shared__ int part[16];
+    __shared__ unsigned short target[kSmallPool / 2], place[kSmallPool];  // of the k-th move; where a page goes
+    const int p0 = threadIdx.x * EACH, total_pages = a.t.num_pages;
+    int h[EACH];
+    unsigned held = 0;
+    load16(a.holders, p0, total_pages, h);
+#pragma unroll
+    for (int j = 0; j < EACH; j++) held |= p0 + j < total_pages && h[j] != 0 ? 1u << j : 0u;
+    int n, below;
+    int rank = block_sum<1024>(__popc(held), part, n) - __popc(held);
+    // held pages below n
+    const unsigned low = p0 >= n ? 0u : n - p0 >= EACH ? (1u << EACH) - 1 : (1u << (n - p0)) - 1;
+    block_sum<1024>(__popc(held & low), part, below);
+    const int moved = n - below;
+    int before = rank;
+#pragma unroll
+    for (int j = 0; j < EACH; j++) {
+        const int p = p0 + j;
+        if (p < n && !(held >> j & 1)) target[p - before] = (unsigned short)p;
+        before += held >> j & 1;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < EACH; j++) {
+        const int p = p0 + j;
+        if (p >= total_pages) continue;
+        int to = p;
+        if ((held >> j & 1) && p >= n) {
+            const int k = rank - below;
+            to = target[k];
+            a.holders[to] = h[j];
+            a.holders[p] = 0;
+            a.copies[3 * k] = p;
+            a.copies[3 * k + 1] = to;
+            a.copies[3 * k + 2] = a.t.page;
+        }
+        place[p] = (unsigned short)to;
+        rank += held >> j & 1;
+    }
+    __syncthreads();
+    for (int r = moved + threadIdx.x; r < a.most; r += 1024) {
+        a.copies[3 * r] = a.copies[3 * r + 1] = -1;
+        a.copies[3 * r + 2] = 0;
+    }
+    const int all = a.t.B * a.t.columns;
+    constexpr int DEEP = 4;
+    for (int i0 = threadIdx.x; i0 < all; i0 += 1024 * DEEP) {
+        int *at[DEEP], was[DEEP];
+#pragma unroll
+        for (int k = 0; k < DEEP; k++) {
+            const int i = min(i0 + k * 1024, all - 1), b = i / a.t.columns;
+            at[k] = &a.t.at(b, i - b * a.t.columns);
+            was[k] = *at[k];
+        }
+#pragma unroll
+        for (int k = 0; k < DEEP; k++) {
+            if (i0 + k * 1024 >= all || !a.t.is_page(was[k])) continue;
+            const int to = place[was[k]];
+            if (to != was[k]) *at[k] = to;
+        }
+    }
+}
+
 int set_table(const char *fn, int *pages, int B, int columns, int num_pages, int page, int64_t stride, PageTable *t) {
     if (!pages) {
         set_error("%s: pages is NULL", fn);
@@ -420,7 +666,7 @@ int set_table(const char *fn, int *pages, int B, int columns, int num_pages, int
         return ENATTEN_EINVAL;
     }
     if (B > kMostRows || (int64_t)B * columns > 1 << 30 || (int64_t)columns * page > (1 << 30) - 4096) {
-        set_error("%s: more than 8192 rows, 2^30 entries, or 2^30 tokens in a row's pages", fn);
+        set_error("%s: more than 4096 rows, 2^30 entries, or 2^30 tokens in a row's pages", fn);
         return ENATTEN_EUNSUPPORTED;
     }
     *t = PageTable{pages, B > 1 ? stride : 0, B, columns, num_pages, page};
@@ -452,17 +698,17 @@ int enatten_cache_fork(int *pages, int *lengths, int *holders, const int *parent
     a.lengths = lengths;
     a.holders = holders;
     a.parents = parents;
-    // About 8 entries per thread, whole lines of the table where 64 KB of LDS hold that many of all rows
-    int width = 2048 / B > 16 ? 2048 / B : 16;
-    if (width > 2 * kMostRows / B - 1) width = 2 * kMostRows / B - 1;
+    // About 4 entries per thread, whole lines of the table where 64 KB of LDS hold that many of all rows
+    int width = 4096 / B > 16 ? 4096 / B : 16;
+    if (width > 4 * kMostRows / B - 3) width = 4 * kMostRows / B - 3;
     if (width > columns) width = columns;
     a.width = width;
     a.with_lengths = width == columns;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const size_t lds = ((size_t)B * width + (a.with_lengths ? B : 0)) * sizeof(int);
+    const size_t lds = (size_t)B * (width + 3) * sizeof(int);
     {
         ProfScope prof(ENATTEN_KERNEL_CACHE_PAGES, "fork_rows", st);
-        fork_rows<<<(columns + width - 1) / width, 256, lds, st>>>(a);
+        fork_rows<<<(columns + width - 1) / width, (int64_t)B * width <= 512 ? 256 : 1024, lds, st>>>(a);
     }
     const int rc = launched(fn);
     if (rc || a.with_lengths) return rc;
@@ -473,7 +719,7 @@ int enatten_cache_fork(int *pages, int *lengths, int *holders, const int *parent
 
 size_t enatten_cache_reserve_workspace_bytes(int B, int columns, int num_pages) {
     if (B < 1 || columns < 1 || num_pages < 1) return 0;
-    return ((size_t)num_pages + (size_t)B * columns) * sizeof(int);
+    return (size_t)num_pages * sizeof(int);
 }
 
 int enatten_cache_reserve(int *pages, const int *lengths, const int *counts, int count, int *holders, int *copies,
@@ -490,10 +736,9 @@ int enatten_cache_reserve(int *pages, const int *lengths, const int *counts, int
     a.holders = holders;
     a.copies = copies;
     a.keeper = static_cast<int *>(workspace);
-    a.list = a.keeper + num_pages;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     ProfScope prof(ENATTEN_KERNEL_CACHE_PAGES, "reserve_pages", st);
-    reserve_pages<<<1, 1024, (B + 1 + 2 * ((B + 31) / 32)) * sizeof(int), st>>>(a);
+    reserve_pages<<<1, 1024, (2 * B + 2 * ((B + 31) / 32)) * sizeof(int), st>>>(a);
     return launched(fn);
 }
 
@@ -548,12 +793,11 @@ int enatten_cache_copy(void *k_cache, void *v_cache, float *k_scale, float *v_sc
     if (!copies) return missing(fn);
     a.copies = copies;
     a.n = n; a.layers = layers; a.heads = heads; a.D = D; a.num_pages = num_pages; a.page = page;
-    // Shares of a page of 16 KB or so, up to some thousand workgroups in all
-    const int64_t blocks = (int64_t)2 * layers * heads, bytes = blocks * page * D;
+    // About two thousand workgroups, which all start at once, of one share of a page's blocks each
+    const int64_t blocks = (int64_t)2 * layers * heads;
     const int x = n < 1024 ? n : 1024;
-    int64_t split = (bytes + 16383) / 16384;
+    int64_t split = (2048 + x - 1) / x;
     if (split > blocks) split = blocks;
-    if (split > 8192 / x) split = 8192 / x;
     a.split = (int)split;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     ProfScope prof(ENATTEN_KERNEL_CACHE_COPY, "copy_pages", st);
@@ -580,6 +824,11 @@ int enatten_cache_compact(int *pages, int *holders, int *copies, void *workspace
     a.place = static_cast<int *>(workspace);
     a.counts = a.place + num_pages;
     const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (num_pages <= kSmallPool && (int64_t)B * columns <= kSmallPool) {
+        ProfScope prof(ENATTEN_KERNEL_CACHE_PAGES, "compact_small", st);
+        compact_small<<<1, 1024, 0, st>>>(a);
+        return launched(fn);
+    }
     ProfScope prof(ENATTEN_KERNEL_CACHE_PAGES, "compact_pages", st);
     count_held<<<a.slabs, 256, 0, st>>>(a);
     if (int rc = launched(fn)) return rc;

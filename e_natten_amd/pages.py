@@ -163,7 +163,7 @@ def cache_fork(pages, lengths, holders, parents, page) -> None:
         pages of its tokens, which both hold then; -1 leaves the row empty.  Its own number, and any
         outside -1 .. B - 1, leaves the row as it is, pages behind its last token included.
 
-    Pages that no entry names any more are free.  At most 8192 rows.  Values at the front that several rows
+    Pages that no entry names any more are free.  At most 4096 rows.  Values at the front that several rows
     share may be read by all of them; before a row writes into one, :func:`cache_reserve` gives it its own.
     """
     _tensors(pages=pages, lengths=lengths, holders=holders, parents=parents)
@@ -185,7 +185,7 @@ def cache_reserve(pages, lengths, holders, page, counts=1):
 
     Where no page is free the entry becomes -1: :func:`cache_append` leaves its tokens out and
     :func:`cache_attention` gives NaN.  An entry that older tokens belong to and that is no page stays none.
-    Rows whose numbers do not fit together are left out.  At most 8192 rows.
+    Rows whose numbers do not fit together are left out.  At most 4096 rows.
     """
     _tensors(pages=pages, lengths=lengths, holders=holders)
     count = 0
@@ -217,7 +217,7 @@ def cache_compact(pages, holders, page):
 
     With n held pages, those from n on move to the free ones below n, both in their order, after which
     the pages from n on are free.  ``copies`` has (source, target, page) for each move, then (-1, -1, 0).  A page
-    that a program holds by ``holders`` alone moves too: it finds it in ``copies``.  At most 8192 rows.
+    that a program holds by ``holders`` alone moves too: it finds it in ``copies``.  At most 4096 rows.
     """
     _tensors(pages=pages, holders=holders)
     call = _OPS["cache_compact"] if NATIVE_BINDING else _compact_impl

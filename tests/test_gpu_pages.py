@@ -24,7 +24,7 @@ def _table(pages, layout):
 _SIZES = [
     # rows, columns, tokens of a page, free pages besides
     (1, 1, 16, 0), (2, 1, 16, 3), (4, 6, 16, 40), (5, 67, 64, 9), (32, 9, 48, 100), (70, 33, 128, 500),
-    (300, 5, 16, 700), (1100, 3, 64, 900), (9, 1000, 16, 3000), (8192, 1, 16, 50), (2100, 12, 32, 20),
+    (300, 5, 16, 700), (1100, 3, 64, 900), (9, 1000, 16, 3000), (4096, 1, 16, 50), (2100, 12, 32, 20),
 ]
 
 

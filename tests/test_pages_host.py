@@ -271,7 +271,7 @@ def test_c_pages_validate_before_launch():
         for bad in (dict(pages=none), dict(holders=none), dict(B=0), dict(columns=0), dict(total=0), dict(page=8),
                     dict(page=2048), dict(stride=2), dict(stride=-3)):
             assert call(**bad) == 1 and "enatten_cache" in _text(lib), (call, bad)
-        for bad in (dict(B=8193), dict(columns=1 << 30, stride=1 << 30), dict(columns=1 << 27, stride=1 << 27)):
+        for bad in (dict(B=4097), dict(columns=1 << 30, stride=1 << 30), dict(columns=1 << 27, stride=1 << 27)):
             assert call(**bad) not in (0, 1), (call, bad)
     for bad in (dict(lengths=none), dict(parents=none)):
         assert fork(**bad) == 1
@@ -279,7 +279,7 @@ def test_c_pages_validate_before_launch():
                        (compact, (dict(copies=none), dict(ws=none), dict(ws=ctypes.c_void_p(20))))):
         for bad in bads:
             assert call(**bad) == 1, (call, bad)
-    assert lib.enatten_cache_reserve_workspace_bytes(2, 3, 4) == 4 * (4 + 6)
+    assert lib.enatten_cache_reserve_workspace_bytes(2, 3, 4) == 4 * 4
     assert lib.enatten_cache_compact_workspace_bytes(4096) == 4 * (4096 + 2)
     assert lib.enatten_cache_compact_workspace_bytes(2 ** 31 - 1) == 4 * (2 ** 31 - 1 + 2 ** 20)
     for bad in ((0, 3, 4), (2, 0, 4), (2, 3, 0)):
