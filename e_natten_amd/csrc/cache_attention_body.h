@@ -59,7 +59,7 @@ __device__ __forceinline__ void attend_body(const Args &a) {
     const int head = blockIdx.x % a.heads_kv;
     int item = blockIdx.x / a.heads_kv;
     bool first = false;
-    if constexpr (kShared<Args>) {
+    if constexpr (kShared<Args> && R == 1) {
         first = item < a.first_items;
         if (!first) item -= a.first_items;
     }

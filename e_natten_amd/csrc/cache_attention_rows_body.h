@@ -21,7 +21,8 @@ __device__ __forceinline__ const Args &args_again() {
 
 // DP: head_dim rounded up to 64, 128 or 256; DT: type of q and o, float32 in two float16 terms of q and p.
 // TG: groups of the eight waves that share their rows and take some of a step's tokens each; their sums meet in LDS at
-// the end of a tile (the first part of a call with shared tokens).  M: how many times as many tokens a step has.
+// the end of a tile (the first part of a call with shared tokens).  M: how many times as many tokens a step has.  With
+// eight groups of 32 tokens a step's operands fill LDS and the next one's are put there when all have read them.
 template <int DP, bool E4M3, int DT, int TG, int M, class Args>
 __device__ __forceinline__ void rows_body(const Args &args) {
     constexpr bool FIRST = std::is_same_v<Args, PassArgs<1>>, SECOND = std::is_same_v<Args, PassArgs<2>>;
@@ -32,6 +33,7 @@ __device__ __forceinline__ void rows_body(const Args &args) {
     constexpr int NB = TOK / 32;      // blocks of 32 of them
     constexpr int GR = TOK / 16;      // groups of 16, each within a page
     constexpr int NBW = NB / TG, GRW = GR / TG;  // those of a wave
+    constexpr int BUFFERS = M == 4 ? 1 : 2;
     constexpr int SD = DP / 16;       // products along head_dim of S
     constexpr int OB = DP / 32;       // blocks of 32 channels of O
     constexpr int CH = DP / 16;       // loads of 16 codes per token
@@ -39,7 +41,7 @@ __device__ __forceinline__ void rows_body(const Args &args) {
     // operands of one step: K [NB][SD][64 lanes][8], V [OB][TOK / 16][64 lanes][8]; eight lanes that turn
     // one or two tokens write to as many operands of K, which therefore start 1 or 2 lanes apart in the banks
     constexpr int PART = 64 + (CH < 8 ? 8 / CH : 1);
-    __shared__ f16x8 k_lds[2][NB * SD * PART], v_lds[2][TOK * DP / 8];
+    __shared__ f16x8 k_lds[BUFFERS][NB * SD * PART], v_lds[BUFFERS][TOK * DP / 8];
     __shared__ float z_lds[2][3][GR];  // of the step's groups: key scales, value scales (log2), their inverses
     __shared__ int z_bad[2][2];        // ... and which of either are not finite (0 in their place)
     // Rows of q stay in registers, at head dims above 128 all but the last operands, for which there are
@@ -419,9 +421,14 @@ __device__ __forceinline__ void rows_body(const Args &args) {
         if (step0 + 1 < step1) fetch(step0 + 1);
     }
     for (int step = step0; step < step1; step++) {
-        const int buffer = (step - step0) & 1;
+        const int buffer = BUFFERS == 1 ? 0 : (step - step0) & 1;
+        if (BUFFERS == 1 && step > step0) {
+            __syncthreads();  // (the step before is read)
+            put(0, step);
+            if (step + 1 < step1) fetch(step + 1);
+        }
         __syncthreads();
-        if (step + 1 < step1) {
+        if (BUFFERS == 2 && step + 1 < step1) {
             put(buffer ^ 1, step + 1);
             if (step + 2 < step1) fetch(step + 2);
         }

@@ -8,9 +8,9 @@
 // cache_attention_rows.hip over other rows and tokens, and leave what they come to in the workspace; the last
 // launch joins it.
 //
-// The first part has tiles of up to 48 rows (64 of up to 64 channels, 16 above 128) as the second has, cut so that all of
-// its workgroups start at once, and in the same launch where both have tiles of as many rows.  Beyond, tiles of
-// 64 rows (256 above 128 channels) over codes that LDS holds as float16.
+// Up to 16 rows in a run both parts have tiles of 16 rows and are one launch, the first part cut so that all of its
+// workgroups start at once.  Beyond, it has tiles of 32, 64 or 128 rows (256 above 128 channels) over codes that LDS
+// holds as float16, and a launch of its own.
 #include "cache_attention_body.h"
 
 namespace enatten {
@@ -21,22 +21,25 @@ __global__ __launch_bounds__(256, waves_of(DP, R, DT == ENATTEN_F32 ? 2 : 1)) vo
     attend_body<DP, R, E4M3, DT>(a);
 }
 
-// The parts of both halves of the work joined, where neither has tiles of many rows: one workgroup per row.  Lanes over
+// The parts of both halves of the work joined, where both have tiles of 16 rows: one workgroup per row.  Lanes over
 // the channels, 4 each, and the remaining factor of 256 over the parts.
 template <int DT>
-__global__ __launch_bounds__(256) void run_join_tiles(SharedArgs a, int first_rows, int second_rows) {
+__global__ __launch_bounds__(256) void run_join_tiles(SharedArgs a) {
     int block = blockIdx.x;
     const int head = block % a.heads, hk = head / a.group, g = head - hk * a.group;
     block /= a.heads;
     const int t = block % a.T, b = block / a.T, which = b / a.size;
-    int len, count;
-    const bool ok = sequence_of(a.tb, b, len, count), shares = ok && count > 0 && len - count >= shared_end(a, which);
     // (a part that is not cut is the item of its entry's number)
     const int row = ((b - which * a.size) * a.T + t) * a.group + g, own = t * a.group + g;
-    const int entry = which * a.first_tiles + row / first_rows, own_entry = b * a.row_tiles + own / second_rows;
+    const int entry = which * a.first_tiles + row / 16, own_entry = b * a.row_tiles + own / 16;
     const int *note = reinterpret_cast<const int *>(a.first_ws) + 2 * entry, *own_note = reinterpret_cast<const int *>(a.ws) + 2 * own_entry;
-    const int first = a.first_parts ? note[0] : entry, items = shares ? a.first_parts ? note[1] : 1 : 0;
-    const int own_first = a.parts ? own_note[0] : own_entry, all = items + (a.parts ? own_note[1] : 1);
+    int first = entry, items = 1, own_first = own_entry, own_items = 1;
+    if (a.first_parts) first = note[0], items = note[1];
+    if (a.parts) own_first = own_note[0], own_items = own_note[1];
+    int len, count;
+    const bool ok = sequence_of(a.tb, b, len, count);
+    if (!(ok && count > 0 && len - count >= shared_end(a, which))) items = 0;  // (it does not share them)
+    const int all = items + own_items;
 
     __shared__ __align__(16) float red[256][4];
     __shared__ float tops[256], sums[256];
@@ -47,11 +50,11 @@ __global__ __launch_bounds__(256) void run_join_tiles(SharedArgs a, int first_ro
 #pragma unroll 4
         for (int i = k; i < all; i += groups) {
             const bool of_run = i < items;
-            const int rows = of_run ? first_rows : second_rows, r = (of_run ? row : own) % rows;
-            const float *p = part_of(a, rows, of_run ? first + i : own_first + i - items, hk, of_run);
+            const int r = (of_run ? row : own) % 16;
+            const float *p = part_of(a, 16, of_run ? first + i : own_first + i - items, hk, of_run);
             const float m = p[r], most = fmaxf(top, m), f = __builtin_amdgcn_exp2f(top - most), h = __builtin_amdgcn_exp2f(m - most);
-            y = f * y + h * *reinterpret_cast<const f32x4 *>(p + 2 * rows + r * a.D + c * 4);
-            sum = f * sum + h * p[rows + r];
+            y = f * y + h * *reinterpret_cast<const f32x4 *>(p + 32 + r * a.D + c * 4);
+            sum = f * sum + h * p[16 + r];
             top = most;
         }
     }
@@ -86,10 +89,10 @@ SharedPlan shared_plan(int B, int heads, int heads_kv, int T, int D, int page, i
     p.second = plan_of(B, heads, heads_kv, T, D, page, columns, window, dtype);
     p.second_many = p.second.rows == kWideRows;
     p.first = plan_of(runs, heads, heads_kv, T * size, D, page, columns, window, dtype);
-    p.many = p.first.rows == kWideRows;
+    p.many = p.first.rows > 16;
     int64_t floats;
     if (p.many) {
-        p.first.rows = D > 128 ? kWideRows : rows <= 64 ? 64 : 128;
+        p.first.rows = D > 128 ? kWideRows : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
         p.first.row_tiles = (int)((rows + p.first.rows - 1) / p.first.rows);
         p.first.parts = 256;  // ranges: one workgroup per CU
         p.first.items = 0;
@@ -206,20 +209,14 @@ int enatten_cache_attention_shared(const void *q, const void *k_cache, const voi
         if ((rc = launch_first_join(fn, a, p.first.rows, st))) return rc;
         return launch_second_rows(fn, a, e, st);
     }
-    if (!p.many) {
-        a.first_items = (int)p.first.items;
-        if (p.first.rows != p.second.rows) {
-            if ((rc = launch_attend(fn, a, p.first.rows, a.first_items, e, st))) return rc;
-            a.first_items = 0;
-        }
-    }
+    a.first_items = p.many ? 0 : (int)p.first.items;
     if ((rc = launch_attend(fn, a, p.second.rows, a.first_items + p.second.items, e, st))) return rc;
     if (p.many) return launch_last_join(fn, a, p.first.rows, p.second.rows, st);
     ProfScope prof(ENATTEN_KERNEL_CACHE_JOIN, "run_join_tiles", st);
     const int blocks = B * heads * T;
-    if (dtype == ENATTEN_BF16) run_join_tiles<ENATTEN_BF16><<<blocks, 256, 0, st>>>(a, p.first.rows, p.second.rows);
-    else if (dtype == ENATTEN_F32) run_join_tiles<ENATTEN_F32><<<blocks, 256, 0, st>>>(a, p.first.rows, p.second.rows);
-    else run_join_tiles<ENATTEN_F16><<<blocks, 256, 0, st>>>(a, p.first.rows, p.second.rows);
+    if (dtype == ENATTEN_BF16) run_join_tiles<ENATTEN_BF16><<<blocks, 256, 0, st>>>(a);
+    else if (dtype == ENATTEN_F32) run_join_tiles<ENATTEN_F32><<<blocks, 256, 0, st>>>(a);
+    else run_join_tiles<ENATTEN_F16><<<blocks, 256, 0, st>>>(a);
     return launched(fn);
 }
 

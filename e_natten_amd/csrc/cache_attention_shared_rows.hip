@@ -5,11 +5,12 @@
 namespace enatten {
 namespace {
 
-// The first part: tiles of 64 or 128 rows, steps of 128 tokens (256 of up to 64 channels) that four or two groups of
-// waves share; above 128 channels, where LDS has no room for such steps, and in the second part tiles of 256 rows.
+// The first part: tiles of 32, 64 or 128 rows, steps of 128 tokens (256 for 32 rows, and of up to 64 channels) that
+// eight, four or two groups of waves share; above 128 channels, where LDS has no room for such steps, and in the second
+// part tiles of 256 rows.
 template <int PASS, int DP, bool E4M3, int DT, int TG>
 __global__ __launch_bounds__(512, 2) void run_rows(PassArgs<PASS> args) {
-    rows_body<DP, E4M3, DT, TG, TG == 1 ? 1 : 2>(args);
+    rows_body<DP, E4M3, DT, TG, TG == 1 ? 1 : TG == 8 && DP == 128 ? 4 : 2>(args);
 }
 template <int DP, int DT>
 __global__ __launch_bounds__(256) void run_join_rows(PassArgs<2> a) {
@@ -114,7 +115,8 @@ template <int DP, bool E4M3, int DT>
 int first_rows(const char *fn, const SharedArgs &a, int rows, hipStream_t st) {
     ProfScope prof(ENATTEN_KERNEL_CACHE_ATTENTION, "run_rows", st);
     if constexpr (DP <= 128) {
-        if (rows == 64) run_rows<1, DP, E4M3, DT, 4><<<a.first_parts, 512, 0, st>>>(pass_args<1>(a));
+        if (rows == 32) run_rows<1, DP, E4M3, DT, 8><<<a.first_parts, 512, 0, st>>>(pass_args<1>(a));
+        else if (rows == 64) run_rows<1, DP, E4M3, DT, 4><<<a.first_parts, 512, 0, st>>>(pass_args<1>(a));
         else run_rows<1, DP, E4M3, DT, 2><<<a.first_parts, 512, 0, st>>>(pass_args<1>(a));
     } else {
         run_rows<1, DP, E4M3, DT, 1><<<a.first_parts, 512, 0, st>>>(pass_args<1>(a));
