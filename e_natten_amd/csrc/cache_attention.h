@@ -29,10 +29,7 @@ struct SharedArgs : AttnArgs {
     // come before the second part's; rows of a place of its workspace
     int first_tiles, first_parts, first_items, first_rows;
     float *first_ws;
-    float *canon;        // what the first part comes to, joined: rows (b, head, t), their sums of D values, then
-                         // their maxima, then their sums; where the second part has tiles of kWideRows rows
 };
-template <int PASS> struct PassArgs : SharedArgs {};
 
 // How a call is cut, from its sizes alone (the lengths are on the device).
 struct Plan {
@@ -78,7 +75,7 @@ __device__ __forceinline__ Span plain_span(const AttnArgs &a, int entry) {
     }
     return s;
 }
-template <class Args> constexpr bool kShared = std::is_base_of_v<SharedArgs, Args>;
+template <class Args> constexpr bool kShared = std::is_same_v<SharedArgs, Args>;
 // (sequences or runs) x row tiles, and the rows that one of these has per cache head.  `first` wherever it stands: of
 // the first part of a call with shared tokens.
 template <class Args>
@@ -505,30 +502,6 @@ __device__ __forceinline__ float *stair_of(const SharedArgs &a, int64_t place) {
     const int64_t tiles = (int64_t)a.runs * a.first_tiles * a.heads_kv;
     return a.first_ws + (2 * tiles + 3) / 4 * 4 + place * item_floats(a.first_rows, padded(a.D));
 }
-__device__ __forceinline__ int64_t canon_row(const SharedArgs &a, const Place &p) {
-    return ((int64_t)p.b * a.heads + p.head) * a.T + p.t;
-}
-__device__ __forceinline__ void put_canon(const SharedArgs &a, int64_t row, int d, float top, float sum, f32x4 y) {
-    const int64_t rows = (int64_t)a.B * a.heads * a.T;
-    *reinterpret_cast<f32x4 *>(a.canon + row * a.D + d) = y;
-    if (d == 0) {
-        a.canon[rows * a.D + row] = top;
-        a.canon[rows * (a.D + 1) + row] = sum;
-    }
-}
-// A row's own part and that one joined: the factors of both for the larger maximum; the row's sum becomes that of
-// both.  (Numbers by themselves and no struct: what the compiler keeps of one in an array goes through LDS, and
-// finding its place there takes a load from the queue's packet, in host memory, which cost 12 us.)
-__device__ __forceinline__ void join_canon(const SharedArgs &a, int64_t row, float top, float &sum, float &mine, float &other) {
-    const int64_t rows = (int64_t)a.B * a.heads * a.T;
-    const float m = a.canon[rows * a.D + row], l = a.canon[rows * (a.D + 1) + row], most = fmaxf(top, m);
-    mine = __builtin_amdgcn_exp2f(top - most);
-    other = __builtin_amdgcn_exp2f(m - most);
-    sum = mine * sum + other * l;
-}
-__device__ __forceinline__ f32x4 canon_values(const SharedArgs &a, int64_t row, int d) {
-    return *reinterpret_cast<const f32x4 *>(a.canon + row * a.D + d);
-}
 
 __device__ __forceinline__ float lane_float(float x, int l) {
     return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), l));
@@ -542,11 +515,11 @@ __device__ __forceinline__ int64_t lane_offset(int64_t x, int l) {
 
 // Tiles of kWideRows rows (cache_attention_rows.hip), a.parts ranges
 int launch_attend_rows(const char *fn, const AttnArgs &a, bool e4m3, hipStream_t st);
-// Tiles of many rows of either part, and the joins behind them (cache_attention_shared_rows.hip)
+// Tiles of many rows of the first part, and the join behind both (cache_attention_shared_rows.hip)
 int launch_first_rows(const char *fn, const SharedArgs &a, int rows, bool e4m3, hipStream_t st);
-int launch_first_join(const char *fn, const SharedArgs &a, int rows, hipStream_t st);  // into canon
 int launch_last_join(const char *fn, const SharedArgs &a, int rows, int second_rows, hipStream_t st);
-int launch_second_rows(const char *fn, const SharedArgs &a, bool e4m3, hipStream_t st);
+// A call without shared tokens, its arguments checked
+int launch_plain(const char *fn, AttnArgs a, const Plan &p, void *workspace, bool e4m3, hipStream_t st);
 Plan plan_of(int B, int heads, int heads_kv, int T, int D, int page, int columns, int window, int dtype);
 size_t workspace_bytes(const Plan &p, int B, int heads_kv, int D);  // B: sequences, or runs
 // The arguments that all calls have, checked, but for row_tiles, parts and ws

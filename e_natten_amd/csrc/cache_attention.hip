@@ -180,6 +180,20 @@ int launch_rows(const char *fn, const AttnArgs &a, const Plan &p, hipStream_t st
 }
 
 }  // namespace
+
+int launch_plain(const char *fn, AttnArgs a, const Plan &p, void *workspace, bool e, hipStream_t st) {
+    if (p.parts && (!workspace || (uintptr_t)workspace % 16)) {
+        set_error("%s: workspace is NULL or not 16-byte aligned", fn);
+        return ENATTEN_EINVAL;
+    }
+    a.row_tiles = p.row_tiles;
+    a.parts = p.parts;
+    a.ws = static_cast<float *>(workspace);
+    if (a.D <= 64) return e ? launch_rows<64, true>(fn, a, p, st) : launch_rows<64, false>(fn, a, p, st);
+    if (a.D <= 128) return e ? launch_rows<128, true>(fn, a, p, st) : launch_rows<128, false>(fn, a, p, st);
+    return e ? launch_rows<256, true>(fn, a, p, st) : launch_rows<256, false>(fn, a, p, st);
+}
+
 }  // namespace enatten
 
 using namespace enatten;
@@ -208,19 +222,8 @@ int enatten_cache_attention(const void *q, const void *k_cache, const void *v_ca
                                  D, num_pages, page, columns, kernel_size, dtype, cache_dtype, q_strides, o_strides,
                                  k_cache_strides, v_cache_strides, k_scale_strides, v_scale_strides, pages_stride, scale, &a);
     if (rc) return rc;
-    const Plan p = plan_of(B, heads, heads_kv, T, D, page, columns, kernel_size, dtype);
-    if (p.parts && (!workspace || (uintptr_t)workspace % 16)) {
-        set_error("%s: workspace is NULL or not 16-byte aligned", fn);
-        return ENATTEN_EINVAL;
-    }
-    a.row_tiles = p.row_tiles;
-    a.parts = p.parts;
-    a.ws = static_cast<float *>(workspace);
-    const hipStream_t st = static_cast<hipStream_t>(stream);
-    const bool e = cache_dtype == ENATTEN_E4M3;
-    if (D <= 64) return e ? launch_rows<64, true>(fn, a, p, st) : launch_rows<64, false>(fn, a, p, st);
-    if (D <= 128) return e ? launch_rows<128, true>(fn, a, p, st) : launch_rows<128, false>(fn, a, p, st);
-    return e ? launch_rows<256, true>(fn, a, p, st) : launch_rows<256, false>(fn, a, p, st);
+    return launch_plain(fn, a, plan_of(B, heads, heads_kv, T, D, page, columns, kernel_size, dtype), workspace,
+                        cache_dtype == ENATTEN_E4M3, static_cast<hipStream_t>(stream));
 }
 
 #pragma GCC visibility pop

@@ -25,7 +25,7 @@ __device__ __forceinline__ const Args &args_again() {
 // eight groups of 32 tokens a step's operands fill LDS and the next one's are put there when all have read them.
 template <int DP, bool E4M3, int DT, int TG, int M, class Args>
 __device__ __forceinline__ void rows_body(const Args &args) {
-    constexpr bool FIRST = std::is_same_v<Args, PassArgs<1>>, SECOND = std::is_same_v<Args, PassArgs<2>>;
+    constexpr bool FIRST = kShared<Args>;
     constexpr int RB = 8 / TG, ROWS = 32 * RB;  // blocks of 32 rows
     static_assert(TG == 1 || FIRST, "only parts are joined");
     constexpr int TERMS = DT == ENATTEN_F32 ? 2 : 1;
@@ -91,12 +91,11 @@ __device__ __forceinline__ void rows_body(const Args &args) {
     at_step += counted - into;
     const int which = entry / tiles_of(a, FIRST), row0 = (entry - which * tiles_of(a, FIRST)) * ROWS + rb * 32;
     const int base = s.lo & -16;
-    int b = which, joins = 0;  // joins: shared tokens, which are not the second part's
+    int b = which;
     if constexpr (FIRST) {
         b = reader_of(a, which, s.hi);
         if (b < 0) b = which * a.size, step1 = step0;  // (nobody reads them)
     }
-    if constexpr (SECOND) joins = shared_by(a, which, s);
 
     // the lane's row; q: lane (n, h) has channels 16 c + 8 h .. + 7
     const Place where = place_of(a, which, head, min(row0 + n, all_rows - 1), FIRST);
@@ -109,7 +108,6 @@ __device__ __forceinline__ void rows_body(const Args &args) {
         hi_r = live ? s.hi : 0;
         seen = hi_r - first;
     }
-    if constexpr (SECOND) seen = min(seen, hi_r - joins);
     f16x8 qf[KEPT][TERMS], *q_rest = &q_lds[threadIdx.x];
     float unit, l;
     auto take_q = [&] {
@@ -169,7 +167,6 @@ __device__ __forceinline__ void rows_body(const Args &args) {
     int some_lo = any_row && a.window ? max(s.start + t_first + 1 - a.window, 0) : 0;
     int some_hi = any_row ? s.start + t_last + 1 : 0;
     int all_lo = a.window ? max(s.start + t_last + 1 - a.window, 0) : 0, all_hi = s.start + t_first + 1;
-    if constexpr (SECOND) all_lo = max(all_lo, joins);
     if constexpr (FIRST) {
         some_lo = 0;
         some_hi = row0 < all_rows ? s.hi : 0;
@@ -288,7 +285,6 @@ __device__ __forceinline__ void rows_body(const Args &args) {
     // (the workgroup's first and last rows, for the shorter way of turning E4M3)
     const int wg_row = row0 - rb * 32, wg_last = min((wg_row + ROWS - 1) / a.group, s.count - 1);
     int wg_lo = a.window ? max(s.start + wg_last + 1 - a.window, 0) : 0, wg_hi = s.start + wg_row / a.group + 1;
-    if constexpr (SECOND) wg_lo = max(wg_lo, joins);
     if constexpr (FIRST) {
         wg_lo = a.window ? s.hi : 0;
         wg_hi = s.hi;
@@ -445,28 +441,11 @@ __device__ __forceinline__ void rows_body(const Args &args) {
     const float poison = s.ok ? 0.f : __uint_as_float(0x7fc00000u);
     const int row = row0 + n, all_rows = rows_of(a, FIRST);
     const bool here = row < all_rows, live = here && row / a.group < s.count;
-    const Place where = place_of(a, which, head, min(row, all_rows - 1), FIRST);
-    float mine = 1.f, other = 0.f;
-    bool joined = false;
-    if constexpr (SECOND) {
-        joined = joins > 0 && live && !parted;
-        if (joined) join_canon(a, canon_row(a, where), m, l, mine, other);
-    }
     const float norm = l == 0.f ? 0.f : 1.f / l;
     // 4 neighbouring channels, 4 mm + 128 i: words of one value row, blocks i of O, or for DP 64 rows 16 apart too
     auto channels = [&](int i, int j) {
         if constexpr (DP == 64) return f32x4{acc[0][j], acc[0][j + 8], acc[1][j], acc[1][j + 8]};
         else return f32x4{acc[i * 4][j], acc[i * 4 + 1][j], acc[i * 4 + 2][j], acc[i * 4 + 3][j]};
-    };
-    // a row's 4 channels from d on, divided; in the second pass with what the shared tokens come to
-    auto with_back = [&](int i, int j, int d) {
-        if constexpr (SECOND) {
-            f32x4 y = channels(i, j) * back;
-            if (joined) y = mine * y + other * canon_values(a, canon_row(a, where), min(d, a.D - 4));
-            return y * norm;
-        } else {
-            return channels(i, j) * norm * back;
-        }
     };
     constexpr int BIG = DP == 256 ? 2 : 1, JS = DP == 64 ? 8 : 16;
     if (parted) {
@@ -535,7 +514,7 @@ __device__ __forceinline__ void rows_body(const Args &args) {
 #pragma unroll
             for (int j = 0; j < JS; j++) {
                 const int d = 4 * (j / 4 * 8 + h * 4 + j % 4) + i * 128;
-                if (here && d < a.D) store_channels<DT>(a.o, to + d, (live ? with_back(i, j, d) : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
+                if (here && d < a.D) store_channels<DT>(a.o, to + d, (live ? channels(i, j) * norm * back : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
             }
     } else {
         // 64 channels at a time through LDS, so that a store takes whole lines of 8 rows and not pieces of
@@ -549,8 +528,7 @@ __device__ __forceinline__ void rows_body(const Args &args) {
                 u32x2 y[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const int d = 4 * ((q * 8 + j) / 4 * 8 + h * 4 + j % 4) + i * 128;
-                    const f32x4 x = (live ? with_back(i, q * 8 + j, d) : f32x4{0.f, 0.f, 0.f, 0.f}) + poison;
+                    const f32x4 x = (live ? channels(i, q * 8 + j) * norm * back : f32x4{0.f, 0.f, 0.f, 0.f}) + poison;
                     y[j] = narrow4<DT>(x);
                 }
                 __builtin_amdgcn_wave_barrier();
@@ -582,9 +560,8 @@ __device__ __forceinline__ void rows_body(const Args &args) {
 // Tiles that ranges cut, joined: one workgroup per (start of a range, 16 rows), the one of the first
 // start within a tile for all its parts.  A wave takes every fourth part: 16 lanes over the rows, 4 over
 // neighbouring words of 4 channels.
-template <int DP, int DT, class Args>
-__device__ __forceinline__ void join_rows_body(const Args &a) {
-    constexpr bool SECOND = std::is_same_v<Args, PassArgs<2>>;
+template <int DP, int DT>
+__device__ __forceinline__ void join_rows_body(const AttnArgs &a) {
     constexpr int BLOCKS = kWideRows / 16, WORDS = DP / 16;
     const int range = blockIdx.x / BLOCKS, n = threadIdx.x % 16, c = threadIdx.x / 16 % 4, lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -649,12 +626,6 @@ __device__ __forceinline__ void join_rows_body(const Args &a) {
     if (row >= all_rows) return;
     const Place where = place_of(a, which, head, row, false);
     const int64_t to = offset_of(a.o, where);
-    float mine = 1.f, other = 0.f;
-    bool joined = false;
-    if constexpr (SECOND) {
-        joined = shared_by(a, which, plain_span<kWideRows>(a, entry)) > 0 && where.t < count;
-        if (joined) join_canon(a, canon_row(a, where), top, sum, mine, other);
-    }
     const float norm = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int k = 0; k < WORDS / 4; k++) {
@@ -663,8 +634,6 @@ __device__ __forceinline__ void join_rows_body(const Args &a) {
         f32x4 z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int v = 0; v < 4; v++) z += f[v] * red[v][i][lane];
-        if constexpr (SECOND)
-            if (joined) z = mine * z + other * canon_values(a, canon_row(a, where), d);
         store_channels<DT>(a.o, to + d, where.t < count ? z * norm : f32x4{0.f, 0.f, 0.f, 0.f});
     }
 }

@@ -75,22 +75,32 @@ __global__ __launch_bounds__(256) void run_join_tiles(SharedArgs a) {
     store_channels<DT>(a.o, b * a.o.sb + head * a.o.sh + t * a.o.st + c * 4, (t < count ? y * norm : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
 }
 
-// How a call is cut: both parts' plans, and where their workspaces lie (in floats).
+// How a call is cut: both parts' plans, and where their workspaces lie (in floats).  Or not at all: the codes that
+// all sequences could have, read by each for itself, take about as long as what the launches cost in addition.
+// Measured, shared and by themselves, by those bytes.  One launch and the join, 16 rows: 7 MB 9.5 and 6.5 us, 13 MB 11.7
+// and 10.7, 38 MB 11.7 and 14.9, 139 MB 13.7 and 24.1.  Tiles of many rows, 32: 17 MB 25.5 and 13.1, 91 MB 31 and 28,
+// 288 MB 41 and 55; 48: 69 MB 27 and 20, 221 MB 32 and 36; 64 of 64 channels: 46 MB 23.5 and 17.4, 145 MB 28 and 31;
+// 256: 79 MB 26 and 12, 288 MB 29 and 30.  Sequences that have tiles of 256 rows each are bound by the matrix cores, whose
+// work is the same: 64 new tokens of 64 sequences behind 8192 take 412 and 328 us.
+constexpr int64_t kTilesFrom = 16 << 20, kRowsFrom = 160 << 20;
 struct SharedPlan {
     Plan first, second;
-    int first_rows;  // of a place of the first part's workspace
-    bool many, second_many;  // tiles of more than 64 rows
-    int64_t second_at, canon_at, floats;
+    bool shares;
+    bool many;       // the first part has tiles of many rows
+    int first_rows;  // of a place of its workspace
+    int64_t second_at, floats;
 };
 SharedPlan shared_plan(int B, int heads, int heads_kv, int T, int D, int page, int columns, int window, int dtype, int runs) {
     SharedPlan p;
     const int size = B / runs;
     const int64_t rows = (int64_t)T * size * (heads / heads_kv);
     p.second = plan_of(B, heads, heads_kv, T, D, page, columns, window, dtype);
-    p.second_many = p.second.rows == kWideRows;
     p.first = plan_of(runs, heads, heads_kv, T * size, D, page, columns, window, dtype);
     p.many = p.first.rows > 16;
-    int64_t floats;
+    int64_t tokens = (int64_t)columns * page;
+    if (window && window + (int64_t)T < tokens) tokens = window + (int64_t)T;
+    p.shares = p.second.rows != kWideRows && 2 * D * tokens * heads_kv * B >= (p.many ? kRowsFrom : kTilesFrom);
+    if (!p.shares) return p;
     if (p.many) {
         p.first.rows = D > 128 ? kWideRows : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
         p.first.row_tiles = (int)((rows + p.first.rows - 1) / p.first.rows);
@@ -98,26 +108,17 @@ SharedPlan shared_plan(int B, int heads, int heads_kv, int T, int D, int page, i
         p.first.items = 0;
         p.first_rows = rows < p.first.rows ? (int)(rows + 31) / 32 * 32 : p.first.rows;
         const int64_t tiles = (int64_t)runs * p.first.row_tiles * heads_kv;
-        floats = (2 * tiles + 3) / 4 * 4 + (tiles + p.first.parts) * item_floats(p.first_rows, padded(D));
+        p.second_at = (2 * tiles + 3) / 4 * 4 + (tiles + p.first.parts) * item_floats(p.first_rows, padded(D));
     } else {
         const int64_t entries = (int64_t)runs * p.first.row_tiles;
-        const int slots = 256 * (waves_of(padded(D), p.first.rows / 16, dtype == ENATTEN_F32 ? 2 : 1) > 1 ? 2 : 1) / heads_kv;
+        const int slots = 256 * (waves_of(padded(D), 1, dtype == ENATTEN_F32 ? 2 : 1) > 1 ? 2 : 1) / heads_kv;
         const int64_t useful = entries * (((int64_t)columns * page + 16 + kLeast - 1) / kLeast);
         p.first.parts = slots > entries && useful > entries ? (int)(slots < useful ? slots : useful) : 0;
         p.first.items = p.first.parts ? p.first.parts : entries;
-        p.first_rows = p.first.rows;
-        floats = head_floats(entries) + p.first.items * heads_kv * item_floats(p.first.rows, D);
+        p.first_rows = 16;
+        p.second_at = head_floats(entries) + p.first.items * heads_kv * item_floats(16, D);
     }
-    p.second_at = floats;
-    if (p.second_many) {
-        floats += workspace_bytes(p.second, B, heads_kv, D) / sizeof(float);
-        p.canon_at = floats;
-        floats += ((int64_t)B * heads * T * (D + 2) + 3) / 4 * 4;
-    } else {
-        floats += head_floats((int64_t)B * p.second.row_tiles) + p.second.items * heads_kv * item_floats(p.second.rows, D);
-        p.canon_at = 0;
-    }
-    p.floats = floats;
+    p.floats = p.second_at + head_floats((int64_t)B * p.second.row_tiles) + p.second.items * heads_kv * item_floats(p.second.rows, D);
     return p;
 }
 
@@ -165,7 +166,8 @@ size_t enatten_cache_attention_shared_workspace_bytes(int B, int heads, int head
     if (B < 1 || heads < 1 || heads_kv < 1 || heads % heads_kv || T < 1 || D < 1 || page < 1 || columns < 1 ||
         kernel_size < 0 || runs < 1 || B % runs || (int64_t)B * heads * T > (1 << 30))
         return 0;
-    return shared_plan(B, heads, heads_kv, T, D, page, columns, kernel_size, dtype, runs).floats * sizeof(float);
+    const SharedPlan p = shared_plan(B, heads, heads_kv, T, D, page, columns, kernel_size, dtype, runs);
+    return p.shares ? p.floats * sizeof(float) : workspace_bytes(p.second, B, heads_kv, D);
 }
 
 int enatten_cache_attention_shared(const void *q, const void *k_cache, const void *v_cache, const float *k_scale,
@@ -187,6 +189,9 @@ int enatten_cache_attention_shared(const void *q, const void *k_cache, const voi
         return ENATTEN_EINVAL;
     }
     const SharedPlan p = shared_plan(B, heads, heads_kv, T, D, page, columns, kernel_size, dtype, runs);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const bool e = cache_dtype == ENATTEN_E4M3;
+    if (!p.shares) return launch_plain(fn, a, p.second, workspace, e, st);
     if (!workspace || (uintptr_t)workspace % 16) {
         set_error("%s: workspace is NULL or not 16-byte aligned", fn);
         return ENATTEN_EINVAL;
@@ -196,19 +201,12 @@ int enatten_cache_attention_shared(const void *q, const void *k_cache, const voi
     a.size = B / runs;
     a.first_ws = static_cast<float *>(workspace);
     a.ws = a.first_ws + p.second_at;
-    a.canon = a.first_ws + p.canon_at;
     a.first_tiles = p.first.row_tiles;
     a.first_parts = p.first.parts;
     a.first_rows = p.first_rows;
     a.row_tiles = p.second.row_tiles;
     a.parts = p.second.parts;
-    const hipStream_t st = static_cast<hipStream_t>(stream);
-    const bool e = cache_dtype == ENATTEN_E4M3;
     if (p.many && (rc = launch_first_rows(fn, a, p.first.rows, e, st))) return rc;
-    if (p.second_many) {
-        if ((rc = launch_first_join(fn, a, p.first.rows, st))) return rc;
-        return launch_second_rows(fn, a, e, st);
-    }
     a.first_items = p.many ? 0 : (int)p.first.items;
     if ((rc = launch_attend(fn, a, p.second.rows, a.first_items + p.second.items, e, st))) return rc;
     if (p.many) return launch_last_join(fn, a, p.first.rows, p.second.rows, st);

@@ -5,22 +5,16 @@
 namespace enatten {
 namespace {
 
-// The first part: tiles of 32, 64 or 128 rows, steps of 128 tokens (256 for 32 rows, and of up to 64 channels) that
-// eight, four or two groups of waves share; above 128 channels, where LDS has no room for such steps, and in the second
-// part tiles of 256 rows.
-template <int PASS, int DP, bool E4M3, int DT, int TG>
-__global__ __launch_bounds__(512, 2) void run_rows(PassArgs<PASS> args) {
+// Tiles of 32, 64 or 128 rows, steps of 128 tokens (256 for 32 rows, and of up to 64 channels) that eight, four or two
+// groups of waves share; above 128 channels, where LDS has no room for such steps, tiles of 256 rows.
+template <int DP, bool E4M3, int DT, int TG>
+__global__ __launch_bounds__(512, 2) void run_rows(SharedArgs args) {
     rows_body<DP, E4M3, DT, TG, TG == 1 ? 1 : TG == 8 && DP == 128 ? 4 : 2>(args);
 }
-template <int DP, int DT>
-__global__ __launch_bounds__(256) void run_join_rows(PassArgs<2> a) {
-    join_rows_body<DP, DT>(a);
-}
 
-// The parts of the first part's tiles joined, and (but for CANON, which leaves that to the second part's own tiles of
-// many rows) with the second part's.  One workgroup per (tile, 16 rows, 32 channels): few tiles have many parts.  A
+// The parts of the first part's tiles joined, and with the second part's.  One workgroup per (tile, 16 rows, 32 channels): few tiles have many parts.  A
 // wave takes every fourth part: 16 lanes over the rows, 4 over neighbouring words of 4 channels.
-template <int DP, int DT, bool CANON>
+template <int DP, int DT>
 __global__ __launch_bounds__(256) void run_join(SharedArgs a, int tile_rows, int second_rows) {
     constexpr int WORDS = 2, SPLIT = DP / 32;
     const int n = threadIdx.x % 16, c = threadIdx.x / 16 % 4, lane = threadIdx.x & 63;
@@ -78,9 +72,7 @@ __global__ __launch_bounds__(256) void run_join(SharedArgs a, int tile_rows, int
         z += f * red[v][wave][lane];
     }
     const Place where = place_of(a, which, head, row, true);
-    if constexpr (CANON) {
-        put_canon(a, canon_row(a, where), d, top, sum, z);
-    } else {
+    {
         int len, count;
         const bool ok = sequence_of(a.tb, where.b, len, count);
         if (!(ok && count > 0 && len - count >= shared_end(a, which))) {  // (it does not share them)
@@ -104,38 +96,19 @@ __global__ __launch_bounds__(256) void run_join(SharedArgs a, int tile_rows, int
     }
 }
 
-template <int PASS>
-PassArgs<PASS> pass_args(const SharedArgs &s) {
-    PassArgs<PASS> a;
-    static_cast<SharedArgs &>(a) = s;
-    return a;
-}
-
 template <int DP, bool E4M3, int DT>
 int first_rows(const char *fn, const SharedArgs &a, int rows, hipStream_t st) {
     ProfScope prof(ENATTEN_KERNEL_CACHE_ATTENTION, "run_rows", st);
     if constexpr (DP <= 128) {
-        if (rows == 32) run_rows<1, DP, E4M3, DT, 8><<<a.first_parts, 512, 0, st>>>(pass_args<1>(a));
-        else if (rows == 64) run_rows<1, DP, E4M3, DT, 4><<<a.first_parts, 512, 0, st>>>(pass_args<1>(a));
-        else run_rows<1, DP, E4M3, DT, 2><<<a.first_parts, 512, 0, st>>>(pass_args<1>(a));
+        if (rows == 32) run_rows<DP, E4M3, DT, 8><<<a.first_parts, 512, 0, st>>>(a);
+        else if (rows == 64) run_rows<DP, E4M3, DT, 4><<<a.first_parts, 512, 0, st>>>(a);
+        else run_rows<DP, E4M3, DT, 2><<<a.first_parts, 512, 0, st>>>(a);
     } else {
-        run_rows<1, DP, E4M3, DT, 1><<<a.first_parts, 512, 0, st>>>(pass_args<1>(a));
+        run_rows<DP, E4M3, DT, 1><<<a.first_parts, 512, 0, st>>>(a);
     }
     return launched(fn);
 }
-template <int DP, bool E4M3, int DT>
-int second_rows(const char *fn, const SharedArgs &a, hipStream_t st) {
-    {
-        ProfScope prof(ENATTEN_KERNEL_CACHE_ATTENTION, "run_rows", st);
-        run_rows<2, DP, E4M3, DT, 1><<<a.parts, 512, 0, st>>>(pass_args<2>(a));
-    }
-    const int rc = launched(fn);
-    if (rc) return rc;
-    ProfScope prof(ENATTEN_KERNEL_CACHE_JOIN, "run_join_rows", st);
-    run_join_rows<DP, DT><<<a.parts * (kWideRows / 16), 256, 0, st>>>(pass_args<2>(a));
-    return launched(fn);
-}
-template <int DP, int DT, bool CANON>
+template <int DP, int DT>
 int join(const char *fn, const SharedArgs &a, int rows, int second, hipStream_t st) {
     const int64_t blocks = (int64_t)a.runs * a.first_tiles * a.heads_kv * (a.first_rows / 16) * (DP / 32);
     if (blocks > 0xffffff) {  // (2^32 threads)
@@ -143,7 +116,7 @@ int join(const char *fn, const SharedArgs &a, int rows, int second, hipStream_t 
         return ENATTEN_EUNSUPPORTED;
     }
     ProfScope prof(ENATTEN_KERNEL_CACHE_JOIN, "run_join", st);
-    run_join<DP, DT, CANON><<<(int)blocks, 256, 0, st>>>(a, rows, second);
+    run_join<DP, DT><<<(int)blocks, 256, 0, st>>>(a, rows, second);
     return launched(fn);
 }
 
@@ -168,16 +141,8 @@ int launch_first_rows(const char *fn, const SharedArgs &a, int rows, bool e4m3, 
         return e4m3 ? first_rows<dp.value, true, dt.value>(fn, a, rows, st) : first_rows<dp.value, false, dt.value>(fn, a, rows, st);
     });
 }
-int launch_second_rows(const char *fn, const SharedArgs &a, bool e4m3, hipStream_t st) {
-    return by_dim(a, [&](auto dp, auto dt) {
-        return e4m3 ? second_rows<dp.value, true, dt.value>(fn, a, st) : second_rows<dp.value, false, dt.value>(fn, a, st);
-    });
-}
-int launch_first_join(const char *fn, const SharedArgs &a, int rows, hipStream_t st) {
-    return by_dim(a, [&](auto dp, auto) { return join<dp.value, ENATTEN_F32, true>(fn, a, rows, 16, st); });
-}
 int launch_last_join(const char *fn, const SharedArgs &a, int rows, int second, hipStream_t st) {
-    return by_dim(a, [&](auto dp, auto dt) { return join<dp.value, dt.value, false>(fn, a, rows, second, st); });
+    return by_dim(a, [&](auto dp, auto dt) { return join<dp.value, dt.value>(fn, a, rows, second, st); });
 }
 
 }  // namespace enatten

@@ -28,6 +28,21 @@ def _share(cache, runs, shared):
     return cache
 
 
+def _columns(B, heads, page, d, rows):
+    """A table so wide that its sequences could have the codes from which on a run's tokens are read together: 16 MB
+    with up to 16 rows, else 160."""
+    return ((16 if rows <= 16 else 160) << 20) // (2 * d * page * heads * B) + 2
+
+
+def _shares(q, cache, runs, window=0):
+    """Whether a call's sizes make it one (else each sequence reads for itself): its workspace is another."""
+    from e_natten_amd import _lib
+    lib = ensure_built()
+    sizes = (*q.shape[:2], cache.heads, *q.shape[2:], cache.page, cache.pages.shape[1], window or 0,
+             {BF16: _lib.BF16, F16: _lib.F16, F32: _lib.F32}[q.dtype])
+    return lib.enatten_cache_attention_shared_workspace_bytes(*sizes, runs) != lib.enatten_cache_attention_workspace_bytes(*sizes)
+
+
 def _check(o, ref, bound, dtype, what):
     off = (o.detach().cpu().double() - ref).abs()
     limit = bound + half_step(dtype) * (ref.abs() + bound)
@@ -72,14 +87,20 @@ _CASES = [
     ([900, 910, 930], None, 1, [768], 8, 2, 1, 256, 64, BF16, I8, None),
     ([900 + i for i in range(12)], None, 2, [768, 800], 8, 2, 1, 256, 32, F16, E4M3, None),   # wide tiles of 256 channels
     ([900, 910, 930], None, 1, [768], 8, 2, 3, 192, 64, F32, I8, None),               # ... in tiles of 16
-    # windows: as long as the own tokens, into the shared ones, one token, longer than all
+    # windows (by themselves where these are short): as long as the own tokens, into the shared ones, one token
     ([1000, 990, 1020], None, 1, [960], 8, 2, 1, 128, 64, BF16, I8, 20),
     ([1000, 990, 1020, 980], None, 2, [960, 500], 8, 2, 1, 128, 64, F16, E4M3, 300),
     ([1000, 990, 1020], None, 1, [960], 8, 2, 1, 64, 64, BF16, E4M3, 1),
-    ([1000, 990], None, 1, [960], 8, 2, 1, 128, 64, F32, I8, 5000),
+    ([1000, 990], None, 1, [960], 8, 2, 1, 128, 64, F32, I8, 20000),
     ([1000 + 7 * i for i in range(20)], None, 1, [960], 8, 1, 1, 128, 16, BF16, E4M3, 100),   # wide tiles
     ([1000 + 7 * i for i in range(20)], None, 1, [960], 8, 1, 1, 64, 16, F32, I8, 200),
     ([800, 790, 780], [100, 9, 30], 1, [600], 4, 2, 100, 96, 48, BF16, I8, 150),
+    # ... long enough for runs to be read together: one launch, tiles of 32, 64 and 128 rows
+    ([6000 + 7 * i for i in range(16)], None, 1, [5984], 1, 1, 1, 128, 32, BF16, I8, 4200),
+    ([6000 + 7 * i for i in range(8)], [2, 1] * 4, 2, [5984, 5900], 4, 4, 2, 64, 16, F32, E4M3, 4200),
+    ([5500 + 7 * i for i in range(60)], None, 2, [5400, 5440], 2, 2, 1, 128, 32, BF16, E4M3, 5480),
+    ([5500 + 7 * i for i in range(60)], None, 1, [5440], 2, 2, 1, 128, 32, F16, I8, 5480),
+    ([9000 + 7 * i for i in range(72)], None, 1, [8960], 2, 2, 1, 64, 64, BF16, I8, 9110),
 ]
 
 
@@ -90,17 +111,27 @@ def test_shared(lengths, counts, runs, shared, N, heads, T, d, page, dtype, cach
     B = len(lengths)
     print("case shared", lengths[:6], counts, runs, shared, N, heads, T, d, page, dtype, cache_dtype, window, flush=True)
     starts = [n - (T if counts is None else counts[b]) for b, n in enumerate(lengths)]
-    cache = Cache(lengths, heads, page, d, cache_dtype, seed=B + d)
     size = B // runs
+    rows = size * T * N // heads
+    columns = max(_columns(B, heads, page, d, rows), -(-max(lengths) // page) + 2)
+    cache = Cache(lengths, heads, page, d, cache_dtype, seed=B + d, columns=columns)
     _share(cache, runs, [min([s for s in starts[r * size:(r + 1) * size] if s // page * page >= n // page * page] or [0])
                          if n > 0 else 0 for r, n in enumerate(shared)])
     q = _q(B, N, T, d, dtype, 7)
+    # (not where every sequence has more rows than fit a tile of 16 to 64, and not short windows)
+    fits = T * N // heads <= (16 if d > 128 else 48 if d > 64 else 64) or d > 128 and dtype == F32
+    seen = min(cache.pages.shape[1] * page, window + T if window else 1 << 31)
+    one_launch = rows <= 16 or d > 128 and dtype == F32
+    assert _shares(q, cache, runs, window) == (fits and 2 * d * seen * heads * B >= (16 if one_launch else 160) << 20)
+    assert _shares(q, cache, runs, window) == (fits and (window is None or window > 4000))
     ref, bound = attention_ref(q, cache, counts, window, d ** -0.5)
     args = (q.cuda(), *cache.on("cuda"), ints(lengths), window, d ** -0.5, None if counts is None else ints(counts))
     o = cache_attention(*args, ints(shared))
     _check(o, ref, bound, dtype, "shared")
     assert torch.equal(o, cache_attention(*args, ints(shared)))
     _check(cache_attention(*args), ref, bound, dtype, "not shared")
+    few = cache.pages[:, :max(-(-n // page) for n in lengths)].contiguous().cuda()   # a narrow table
+    _check(cache_attention(*args[:5], few, *args[6:], ints(shared)), ref, bound, dtype, "narrow")
     for b in range(B):
         assert (o[b, :, T if counts is None else counts[b]:] == 0).all()
 
@@ -111,7 +142,7 @@ def test_first_rows_of_a_run_that_ended():
     from e_natten_amd import cache_attention, cache_fork
     for size in (4, 80):
         lengths = [300 + i for i in range(size)]
-        cache = _share(Cache(lengths, 2, 16, 64, I8, seed=1, extra_columns=0), 1, [288])
+        cache = _share(Cache(lengths, 2, 16, 64, I8, seed=1, columns=_columns(size, 2, 16, 64, 2 * size)), 1, [288])
         cache.pages[cache.pages == 2 ** 31 - 1] = -1
         kc, vc, ks, vs, pages = cache.on("cuda")
         holders = torch.zeros(kc.shape[0], dtype=torch.int32, device="cuda")
@@ -121,6 +152,7 @@ def test_first_rows_of_a_run_that_ended():
         cache_fork(pages, n, holders, ints([-1] * gone + list(range(gone, size))), 16)
         counts = ints([0] * gone + [1] * (size - gone))
         q = _q(size, 4, 1, 64, BF16, 3)
+        assert _shares(q, cache, 1)
         cache.lengths = [0] * gone + lengths[gone:]
         ref, bound = attention_ref(q, cache, counts.tolist(), None, 0.125)
         o = cache_attention(q.cuda(), kc, vc, ks, vs, pages, n, None, 0.125, counts, ints([288]))
@@ -136,12 +168,14 @@ def test_numbers_and_pages_that_do_not_fit(rows):
     from e_natten_amd import cache_attention
     size = 4
     lengths = [400 + i for i in range(2 * size)]
-    cache = _share(Cache(lengths, 2, 16, 64, I8, seed=2), 2, [384, 384])
+    cache = Cache(lengths, 2, 16, 64, I8, seed=2, columns=_columns(2 * size, 2, 16, 64, size * rows))
+    _share(cache, 2, [384, 384])
     kc, vc, ks, vs, pages = cache.on("cuda")
     q = _q(2 * size, 2 * rows, 1, 64, BF16, 3).cuda()
+    assert _shares(q, cache, 2)
     good = cache_attention(q, kc, vc, ks, vs, pages, ints(lengths), None, 0.125, None, ints([384, 384]))
     bad = list(lengths)
-    bad[0], bad[5] = -3, 1 << 30
+    bad[0], bad[5] = -3, 2 ** 31 - 1
     o = cache_attention(q, kc, vc, ks, vs, pages, ints(bad), None, 0.125, None, ints([384, 384]))
     assert torch.isnan(o[[0, 5]]).all()
     rest = [1, 2, 3, 4, 6, 7]
@@ -165,9 +199,11 @@ def test_values_that_are_not_finite(rows):
     ensure_built()
     from e_natten_amd import cache_attention
     lengths = [400 + i for i in range(8)]
-    cache = _share(Cache(lengths, 2, 16, 128, E4M3, seed=2), 2, [384, 384])
+    cache = Cache(lengths, 2, 16, 128, E4M3, seed=2, columns=_columns(8, 2, 16, 128, 4 * rows))
+    _share(cache, 2, [384, 384])
     kc, vc, ks, vs, pages = cache.on("cuda")
     q = _q(8, 2 * rows, 1, 128, F16, 3).cuda()
+    assert _shares(q, cache, 2)
     args = (kc, vc, ks, vs, pages, ints(lengths), None, 0.125, None, ints([384, 384]))
     good = cache_attention(q, *args)
     for value in (math.inf, -math.inf, math.nan):
@@ -197,24 +233,27 @@ def test_large_logits_in_one_part_only():
     from e_natten_amd import cache_attention
     lengths = [140, 139]
     for where in (5, 136):
-        cache = Cache(lengths, 1, 16, 32, I8, seed=4, scale_spread=(1.0, 1.001))
+        cache = Cache(lengths, 1, 16, 32, I8, seed=4, scale_spread=(1.0, 1.001), columns=_columns(2, 1, 16, 32, 4))
         _share(cache, 1, [128])
         for b in range(2):
             p = int(cache.pages[b, where // 16])
             cache.codes[0].view(I8)[p, 0, where % 16] = 127
         q = torch.full((2, 2, 1, 32), 40.0, dtype=F32)
+        assert _shares(q, cache, 1)
         ref, bound = attention_ref(q, cache, None, None, 1.0)
         o = cache_attention(q.cuda(), *cache.on("cuda"), ints(lengths), None, 1.0, None, ints([128]))
         _check(o, ref, bound, F32, "token %d" % where)
 
 
-@pytest.mark.parametrize("T,N", [(1, 8), (70, 8)])
+@pytest.mark.parametrize("T,N", [(1, 8), (1, 16), (4, 16), (70, 8)])
 def test_streams_graphs_bindings_and_layouts(T, N):
     ensure_built()
     import e_natten_amd as E
     from e_natten_amd import sequence as S
     lengths = [700, 690, 720, 715]
-    cache = _share(Cache(lengths, 2, 32, 128, E4M3, seed=5), 2, [512, 608])
+    columns = _columns(4, 2, 32, 128, T * N)
+    cache = _share(Cache(lengths, 2, 32, 128, E4M3, seed=5, columns=columns), 2, [512, 608])
+    assert _shares(_q(4, N, T, 128, BF16, 6), cache, 2) == (T < 70)
     where = cache.on("cuda")
     q, n, shared = _q(4, N, T, 128, BF16, 6).cuda(), ints(lengths), ints([512, 608])
     want = E.cache_attention(q, *where, n, None, 0.1, None, shared)
@@ -245,7 +284,7 @@ def test_streams_graphs_bindings_and_layouts(T, N):
         torch.cuda.synchronize()
         assert torch.equal(o, E.cache_attention(x, *where, m, None, 0.1, None, c))
     if E.ops.NATIVE_BINDING:   # (the check multiplies its inputs, which torch does not do with float8)
-        where = _share(Cache(lengths, 2, 32, 128, I8, seed=5), 2, [512, 608]).on("cuda")
+        where = _share(Cache(lengths, 2, 32, 128, I8, seed=5, columns=columns), 2, [512, 608]).on("cuda")
         where = [x.nan_to_num(nan=1.0) if x.dtype == F32 else x for x in where]
         torch.library.opcheck(torch.ops.enatten.cache_attention.default, (q, *where, n, None, 0, 0.1, shared),
                               test_utils=("test_schema", "test_faketensor"))
@@ -260,7 +299,8 @@ def test_offsets_past_32_bits(T, N):
     far = (1 << 32) // (pages - 1) // 16 * 16 + (1 << 20)
     pool = torch.zeros(far * (pages - 1) + heads * page * d, dtype=torch.int8, device="cuda")
     view = pool.as_strided((pages, heads, page, d), (far, page * d, d, 1))
-    lengths, table = [64 * 3 + 5, 64 * 3 + 60], [[4, 1, 3, 0], [4, 1, 3, 2]]
+    columns = _columns(2, heads, page, d, T * N)
+    lengths, table = [64 * 3 + 5, 64 * 3 + 60], [[4, 1, 3, n] + [-1] * columns for n in (0, 2)]
     g = torch.Generator().manual_seed(1)
     small = [torch.randint(-127, 128, (pages, heads, page, d), generator=g, dtype=torch.int8) for _ in range(2)]
     scales = [torch.rand(pages, heads, generator=g) * 0.02 + 0.01 for _ in range(2)]

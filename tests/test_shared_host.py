@@ -58,17 +58,26 @@ def test_c_shared_validates_before_launch():
     lib = _lib.load()
     at, none = ctypes.c_void_p(16), None
 
+    wide = 1 << 16   # columns: so many that the sequences' codes could be 16 MB and more
+
     def call(shared=at, runs=2, B=6, heads=4, ws=at, o=at, D=32, lengths=at):
         return lib.enatten_cache_attention_shared(at, at, at, at, at, at, lengths, none, shared, runs, o, ws, B, heads, 2, 1, D,
-                                                  8, 16, 3, 0, _lib.BF16, _lib.I8, none, none, none, none, none, none, 3, 1.0, none)
+                                                  8, 16, wide, 0, _lib.BF16, _lib.I8, none, none, none, none, none, none, wide, 1.0, none)
 
     for bad in (dict(shared=none), dict(runs=0), dict(runs=-1), dict(runs=4), dict(runs=12), dict(ws=none),
                 dict(ws=ctypes.c_void_p(8)), dict(heads=3), dict(o=none), dict(D=24), dict(lengths=none), dict(B=0)):
         assert call(**bad) == 1 and "enatten_cache_attention_shared" in lib.enatten_last_error().decode(), bad
-    need = lambda B=6, runs=2, T=1, cols=3, heads=4: lib.enatten_cache_attention_shared_workspace_bytes(
-        B, heads, 2, T, 32, 16, cols, 0, _lib.BF16, runs)
-    rows = lambda B, T: (B * 4 * T * 34 + 3) // 4 * 16   # sums of values, maximum and sum of every row
-    assert need() >= rows(6, 1) and need(T=3) >= rows(6, 3) and need(cols=4096) > need()
+    def need(B=6, runs=2, T=1, cols=wide, heads=4, D=32, window=0, call=lib.enatten_cache_attention_shared_workspace_bytes):
+        return call(B, heads, 2, T, D, 16, cols, window, _lib.BF16, *((runs,) if call is not plain else ()))
+
+    plain = lib.enatten_cache_attention_workspace_bytes
+    rows = lambda B, T: B * 4 * T * 34 * 4   # a row's sums of values, maximum and sum, once for the run and once for itself
+    assert need() >= 2 * rows(6, 1) and need(T=3) >= 2 * rows(6, 3) and need(T=16) >= 2 * rows(6, 16)
+    # by themselves: few codes, short windows, tiles of 256 rows for every sequence
+    for alone in (dict(cols=3), dict(cols=1365), dict(window=21844), dict(T=100), dict(T=7, cols=13653), dict(T=16, cols=13653)):
+        assert need(**alone) == need(**alone, call=plain), alone
+    for together in (dict(cols=1366), dict(window=21845), dict(T=7, cols=13654), dict(T=16, cols=13654)):
+        assert need(**together) != need(**together, call=plain), together
     for bad in (dict(B=0), dict(runs=0), dict(runs=4), dict(T=0), dict(cols=0), dict(heads=3), dict(T=1 << 28)):
         assert need(**bad) == 0
 
@@ -81,8 +90,7 @@ def test_kernels_do_not_spill_beside_accumulation_registers():
     from test_sequence_host import _registers
     found = _registers()
     ours = {kind: {n: v for n, v in found.items() if re.match(r"_ZN7enatten12_GLOBAL__N_1%d%sI" % (len(kind), kind), n)}
-            for kind in ("run_attend", "run_rows", "run_join", "run_join_rows", "run_join_tiles")}
-    assert {kind: len(v) for kind, v in ours.items()} == {"run_attend": 48, "run_rows": 40 + 16, "run_join": 8 + 3,
-                                                          "run_join_rows": 8, "run_join_tiles": 3}
+            for kind in ("run_attend", "run_rows", "run_join", "run_join_tiles")}
+    assert {kind: len(v) for kind, v in ours.items()} == {"run_attend": 48, "run_rows": 40, "run_join": 8, "run_join_tiles": 3}
     for kind, kernels in ours.items():
         assert not {n: v for n, v in kernels.items() if v[1] and (v[0] or kind != "run_rows")}
