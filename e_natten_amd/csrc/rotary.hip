@@ -32,6 +32,7 @@ struct RotaryArgs {
     float sign;  // -1: the other way round
     double scale;
     int tiles, slices, slice;  // token tiles per sequence; slices of `slice` heads of q and k together
+    int batches;               // sequences of a workgroup, which have the same positions
 };
 
 template <typename S> struct Math { using type = float; };
@@ -62,22 +63,33 @@ __global__ __launch_bounds__(256) void rotary_turn(RotaryArgs a) {
     int block = blockIdx.x;
     const int slice = block % a.slices;
     block /= a.slices;
-    const int tile = block % a.tiles, b = block / a.tiles;
+    const int tile = block % a.tiles, b0 = block / a.tiles * a.batches, b1 = min(b0 + a.batches, a.B);
     const int t0 = tile * TOKENS, nt = min(TOKENS, a.T - t0), half = a.R / 2;
+    auto position = [&](int64_t at) {
+        return a.wide_positions ? (double)static_cast<const int64_t *>(a.positions)[at]
+                                : (double)static_cast<const int *>(a.positions)[at];
+    };
+    // Of several axes the tokens' positions come into LDS at once: asked for pair by pair, behind its axis, they are
+    // waited for in every round.
+    constexpr int STAGED = 256;
+    __shared__ double staged[STAGED];
+    const bool few = a.axes && TOKENS * a.num_axes <= STAGED;
+    if (few) {
+        for (int i = threadIdx.x; i < TOKENS * a.num_axes; i += 256)
+            staged[i] = position(i / TOKENS * a.axis_stride + b0 * a.positions_stride + t0 + min(i % TOKENS, nt - 1));
+        __syncthreads();
+    }
     for (int i = threadIdx.x; i < nt * half; i += 256) {
         const int t = i / half, f = i - t * half;
         const int axis = a.axes ? a.axes[f] : 0;
-        if (a.axes && (unsigned)axis >= (unsigned)a.num_axes) {  // (an axis that is not there)
-            table[i] = Turn{(C)NAN, (C)NAN};
-            continue;
-        }
-        const int64_t at = axis * a.axis_stride + b * a.positions_stride + t0 + t;
-        const double p = a.wide_positions ? (double)static_cast<const int64_t *>(a.positions)[at]
-                                          : (double)static_cast<const int *>(a.positions)[at];
         const double w = a.wide_frequencies ? static_cast<const double *>(a.frequencies)[f]
                                             : (double)static_cast<const float *>(a.frequencies)[f];
+        const bool there = !a.axes || (unsigned)axis < (unsigned)a.num_axes;
+        const int at = there ? axis : 0;
+        const double p = few ? staged[at * TOKENS + t] : position(at * a.axis_stride + b0 * a.positions_stride + t0 + t);
         C c, s;
         turn(p * w, c, s);
+        if (!there) c = s = (C)NAN;  // (an axis that is not there)
         table[i] = Turn{c * (C)a.scale, s * (C)a.scale * (C)a.sign};
     }
     __syncthreads();
@@ -86,6 +98,7 @@ __global__ __launch_bounds__(256) void rotary_turn(RotaryArgs a) {
     const int turned = IN_PACK ? a.R / VEC : half / VEC, units = turned + (a.D - a.R) / VEC;
     const int mate = INTERLEAVED ? 1 : half;          // where not: the second channel, so far behind the first
     const int h0 = slice * a.slice, h1 = min(h0 + a.slice, a.heads[0] + a.heads[1]);
+    for (int b = b0; b < b1; b++)
 #pragma unroll
     for (int which = 0; which < 2; which++) {
         const int lo = which ? max(h0 - a.heads[0], 0) : h0, hi = which ? h1 - a.heads[0] : min(h1, a.heads[0]);
@@ -168,7 +181,11 @@ int launch_tokens(const char *fn, RotaryArgs &a, hipStream_t st) {
         a.slice = (a.slice + 1) / 2;
         a.slices = (heads + a.slice - 1) / a.slice;
     }
-    const int64_t blocks = (int64_t)a.B * a.tiles * a.slices;
+    // Sequences with the same positions share a workgroup's sines and cosines where there are enough of those:
+    a.batches = 1;
+    if (a.positions_stride == 0)
+        while (a.batches < a.B && (int64_t)((a.B + 2 * a.batches - 1) / (2 * a.batches)) * a.tiles * a.slices >= 1024) a.batches *= 2;
+    const int64_t blocks = (int64_t)((a.B + a.batches - 1) / a.batches) * a.tiles * a.slices;
     if (blocks > 0xffffff) {  // (2^32 threads)
         set_error("%s: too many tokens", fn);
         return ENATTEN_EUNSUPPORTED;
