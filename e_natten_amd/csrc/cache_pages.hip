@@ -672,6 +672,35 @@ int set_table(const char *fn, int *pages, int B, int columns, int num_pages, int
     *t = PageTable{pages, B > 1 ? stride : 0, B, columns, num_pages, page};
     return ENATTEN_OK;
 }
+// What a call writes shares no memory with its other arguments.
+struct Ints {
+    const int *at;
+    int64_t n;
+};
+bool meet(const Ints &x, const Ints &y) {
+    const int64_t d = (const char *)y.at - (const char *)x.at;
+    return x.at && y.at && d < x.n * (int64_t)sizeof(int) && -d < y.n * (int64_t)sizeof(int);
+}
+bool meet(const PageTable &t, const Ints &x) {  // (x may lie between the rows of a wider table)
+    const int64_t unit = sizeof(int), row = t.columns * unit, stride = t.stride * unit, size = x.n * unit;
+    const int64_t d = (const char *)x.at - (const char *)t.pages;
+    if (!x.at || d >= (t.B - 1) * stride + row || -d >= size) return false;
+    if (d <= 0) return true;
+    const int64_t in_row = stride ? d % stride : d;
+    return in_row < row || in_row + size > stride;
+}
+int apart(const char *fn, const PageTable &t, std::initializer_list<Ints> written, std::initializer_list<Ints> read) {
+    bool met = false;
+    for (const Ints &x : written) {
+        met |= meet(t, x);
+        for (const Ints &y : written) met |= &x < &y && meet(x, y);
+        for (const Ints &y : read) met |= meet(x, y);
+    }
+    for (const Ints &y : read) met |= meet(t, y);
+    if (!met) return ENATTEN_OK;
+    set_error("%s: what is written must not share memory with other arguments", fn);
+    return ENATTEN_EINVAL;
+}
 int missing(const char *fn) {
     set_error("%s: an argument is NULL", fn);
     return ENATTEN_EINVAL;
@@ -695,6 +724,7 @@ int enatten_cache_fork(int *pages, int *lengths, int *holders, const int *parent
     ForkArgs a{};
     if (int rc = set_table(fn, pages, B, columns, num_pages, page, pages_stride, &a.t)) return rc;
     if (!lengths || !holders || !parents) return missing(fn);
+    if (int rc = apart(fn, a.t, {{lengths, B}, {holders, num_pages}}, {{parents, B}})) return rc;
     a.lengths = lengths;
     a.holders = holders;
     a.parents = parents;
@@ -730,6 +760,8 @@ int enatten_cache_reserve(int *pages, const int *lengths, const int *counts, int
     if (int rc = set_table(fn, pages, B, columns, num_pages, page, pages_stride, &a.t)) return rc;
     if (!lengths || !holders || !copies) return missing(fn);
     if (!workspace || (uintptr_t)workspace % 16) return bad_workspace(fn);
+    if (int rc = apart(fn, a.t, {{holders, num_pages}, {copies, (int64_t)3 * B}, {static_cast<int *>(workspace), num_pages}},
+                       {{lengths, B}, {counts, counts ? B : 0}})) return rc;
     a.lengths = lengths;
     a.counts = counts;
     a.count = count;
@@ -822,6 +854,8 @@ int enatten_cache_compact(int *pages, int *holders, int *copies, void *workspace
     a.slabs = (int)(((int64_t)num_pages + kSlab - 1) / kSlab);
     a.most = num_pages > 1 ? num_pages / 2 : 1;
     a.place = static_cast<int *>(workspace);
+    if (int rc = apart(fn, a.t, {{holders, num_pages}, {copies, (int64_t)3 * a.most}, {a.place, (int64_t)num_pages + a.slabs}}, {}))
+        return rc;
     a.counts = a.place + num_pages;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (num_pages <= kSmallPool && (int64_t)B * columns <= kSmallPool) {

@@ -101,6 +101,9 @@ void cache_copy(const Tensor &kc, const Tensor &vc, const Tensor &ks, const Tens
     for (const Tensor *t : {&vc, &ks, &vs, &copies_})
         TORCH_CHECK_VALUE(t->device() == kc.device(), what, ": all tensors must be on the same device");
     for (const Tensor *t : {&kc, &vc, &ks, &vs}) at::assert_no_internal_overlap(*t);
+    TORCH_CHECK_VALUE(!kc.is_same(vc) && !ks.is_same(vs) &&
+                          (kc.is_meta() || !(share_memory(kc, vc) || share_memory(ks, vs))),
+                      what, ": keys and values must not share a cache");
     TORCH_CHECK_VALUE(kc.size(lead) <= 0x7fffffff && kc.size(lead + 1) <= (1 << 20) && (lead == 0 || kc.size(0) <= (1 << 20)) &&
                           copies_.size(0) <= 0x7fffffff && kc.size(lead + 2) <= 1024 && kc.size(lead + 3) <= 256,
                       what, ": tensor too large, more than 1024 tokens in a page, or a head_dim above 256");

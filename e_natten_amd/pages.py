@@ -24,7 +24,7 @@ import torch
 
 from . import _lib
 from .ops import NATIVE_BINDING, _check, _require_gpu, _stream_of
-from .sequence import _CACHE_DTYPES, _no_gradient, _tensors
+from .sequence import _CACHE_DTYPES, _no_gradient, _share_memory, _tensors
 
 _OPS = {name: getattr(torch.ops.enatten, name).default
         for name in ("cache_fork", "cache_reserve", "cache_copy", "cache_compact")} if NATIVE_BINDING else None
@@ -137,6 +137,8 @@ def _copy_impl(k_cache, v_cache, k_scale, v_scale, copies) -> None:
     for t in written:
         if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
             raise RuntimeError("the cache must not share memory between its elements")
+    if _share_memory(k_cache, v_cache) or _share_memory(k_scale, v_scale):
+        raise ValueError("keys and values must not share a cache")
     lead = k_cache.dim() - 4
     layers = k_cache.shape[0] if lead else 1
     num, heads, page, D = k_cache.shape[lead:]

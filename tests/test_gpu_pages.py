@@ -84,6 +84,26 @@ def test_reserve(B, columns, page, spare, layout):
         assert n.tolist() == lengths
 
 
+def test_lengths_and_holders_between_the_rows_of_a_wider_table():
+    """One allocation for all of a program's numbers: refused only where elements are the same."""
+    ensure_built()
+    from e_natten_amd import cache_fork, cache_reserve
+    pages, lengths, holders = random_state(3, 4, 16, 5, 1)
+    n = len(holders)
+    state = torch.full((3, 4 + 3 + n), 7, dtype=torch.int32, device="cuda")
+    p, m, h = state[:, :4], state[0, 4:7], state[1, 7:]
+    p.copy_(ints(pages)), m.copy_(ints(lengths)), h.copy_(ints(holders))
+    want = fork_ref(pages, lengths, holders, [1, 1, 0], 16)
+    cache_fork(p, m, h, ints([1, 1, 0]), 16)
+    assert [x.tolist() for x in (p, m, h)] == list(want)
+    with pytest.raises(ValueError, match="share memory"):
+        cache_fork(p, m, h, m, 16)
+    with pytest.raises(ValueError, match="share memory"):
+        cache_reserve(state[:, :8], m, h, 16)
+    count = ints([5, 5, 5])
+    cache_reserve(p, count, h, 16, count)   # whole prompts: lengths and counts may be one tensor
+
+
 def test_reserve_gives_every_holder_of_a_page_its_own():
     """All rows that hold a page write to it: the last one keeps it.  A row that only reads it holds it on."""
     ensure_built()

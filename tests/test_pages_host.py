@@ -164,6 +164,26 @@ def test_pages_refuse(name, change, text):
             call(*_args(name, **change))
 
 
+_LAYERS = _z(4, 3, 2, 16, 32, dtype=I8).transpose(0, 1)     # layers, pages, heads, tokens, channels
+_POOL = _z(6, 2, 2, 16, 32, dtype=I8)                       # pages, keys and values, ...
+
+
+@pytest.mark.parametrize("shared,change", [
+    (True, dict(k_cache=_POOL[:4, 0], v_cache=_POOL[:4, 0])), (True, dict(k_cache=_POOL[:4, 0], v_cache=_POOL[2:, 0])),
+    (False, dict(k_cache=_POOL[:4, 0], v_cache=_POOL[:4, 1])),
+    (True, dict(k_cache=_LAYERS[:2], v_cache=_LAYERS[1:], k_scale=_z(2, 4, 2, dtype=F32), v_scale=_z(2, 4, 2, dtype=F32))),
+    (False, dict(k_cache=_LAYERS[:1], v_cache=_LAYERS[1:2], k_scale=_z(1, 4, 2, dtype=F32), v_scale=_z(1, 4, 2, dtype=F32))),
+    (True, dict(k_scale=_z(6, 2, dtype=F32)[:4], v_scale=0)),   # (v_scale: the same from page 2 on)
+])
+def test_copy_refuses_keys_and_values_that_share_some_memory(shared, change):
+    ensure_built()
+    if isinstance(change.get("v_scale"), int):
+        change = dict(change, v_scale=change["k_scale"]._base[2:])
+    for call in _impls("cache_copy"):
+        with pytest.raises((ValueError, RuntimeError), match="must not share a cache" if shared else "GPU"):
+            call(*_args("cache_copy", **change))
+
+
 def test_what_is_no_tensor_or_no_int():
     ensure_built()
     import e_natten_amd as E
@@ -285,6 +305,39 @@ def test_c_pages_validate_before_launch():
     for bad in ((0, 3, 4), (2, 0, 4), (2, 3, 0)):
         assert lib.enatten_cache_reserve_workspace_bytes(*bad) == 0
     assert lib.enatten_cache_compact_workspace_bytes(0) == 0
+
+
+def test_c_pages_refuse_memory_that_is_written_twice():
+    """Addresses that nothing is read from: a table [3, 4] of rows 10 entries apart, 20 pages."""
+    lib, _ = _lib()
+    none, base = ctypes.c_void_p(None), 1 << 20
+
+    def at(entry, byte=0):
+        return ctypes.c_void_p(base + 4 * entry + byte)
+
+    far = dict(lengths=at(100), holders=at(200), parents=at(300), copies=at(400), ws=at(500), counts=at(600))
+    sizes = (3, 4, 20, 16, 10, none)
+
+    def fork(lengths, holders, parents, **_):
+        return lib.enatten_cache_fork(at(0), lengths, holders, parents, *sizes)
+
+    def reserve(lengths, holders, copies, ws, counts, **_):
+        return lib.enatten_cache_reserve(at(0), lengths, counts, 1, holders, copies, ws, *sizes)
+
+    def compact(holders, copies, ws, **_):
+        return lib.enatten_cache_compact(at(0), holders, copies, ws, *sizes)
+
+    for call, bads in (
+            (fork, (dict(lengths=at(0)), dict(lengths=at(-2)), dict(lengths=at(3)), dict(lengths=at(8)), dict(lengths=at(23)),
+                    dict(holders=at(4)), dict(holders=at(-19)), dict(parents=at(11)), dict(parents=far["lengths"]),
+                    dict(parents=at(302), lengths=at(300)), dict(lengths=at(219)), dict(holders=at(300, -76)),
+                    dict(lengths=at(4, -1)), dict(lengths=at(7, 1)))),
+            (reserve, (dict(lengths=at(12)), dict(counts=at(23)), dict(counts=at(200)), dict(lengths=at(408)), dict(copies=at(0)),
+                       dict(copies=at(219)), dict(ws=at(400)), dict(ws=at(8)), dict(ws=at(596), counts=at(600)))),
+            (compact, (dict(holders=at(0)), dict(copies=at(20)), dict(copies=far["holders"]), dict(ws=at(180)),
+                       dict(copies=at(371), ws=at(400))))):
+        for bad in bads:
+            assert call(**dict(far, **bad)) == 1 and "must not share memory" in _text(lib), (call, bad)
 
 
 def test_c_copy_validates_before_launch():
