@@ -127,7 +127,7 @@ __global__ __launch_bounds__(1024) void fork_lengths(ForkArgs a) {
 struct ReserveArgs {
     PageTable t;
     const int *lengths, *counts;
-    int *holders, *copies, *keeper;  // keeper: workspace [num_pages]
+    int *holders, *copies, *keeper, *dropped;  // the last two: workspace [num_pages] each
     int count;
 };
 // The columns that a row's new tokens go to.
@@ -188,6 +188,37 @@ __device__ __forceinline__ int free_pages(const ReserveArgs &a, int wanted, int 
     return min(given, wanted);
 }
 
+// New tokens may meet a page that others hold where no older token is: a row's length went back behind tokens that it
+// shares.  Such entries become none, so that they get a page of their own; `dropped` counts them page by page, and the
+// holders lose them when all pages are given out, as a page that a copy still has to read is not free in this call.
+// Seldom, so that passes over the table and all pages do not matter.
+__device__ __forceinline__ void drop_entries(const ReserveArgs &a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int p = threadIdx.x; p < a.t.num_pages; p += 1024) a.dropped[p] = 0;
+    __threadfence();
+    __syncthreads();
+    for (int b = wave; b < a.t.B; b += 16) {
+        const Need n = need_of(a, b);
+        for (int c = lane + (n.older != 0); c < n.columns; c += 64) {
+            int &e = a.t.at(b, n.first + c);
+            const int page = load_now(&e);
+            if (!a.t.is_page(page) || load_now(a.holders + page) <= 1) continue;
+            atomicAdd(a.dropped + page, 1);
+            e = -1;
+        }
+    }
+    __threadfence();
+    __syncthreads();
+}
+__device__ __forceinline__ void take_dropped(const ReserveArgs &a) {
+    __threadfence();
+    __syncthreads();
+    for (int p = threadIdx.x; p < a.t.num_pages; p += 1024) {
+        const int n = load_now(a.dropped + p);
+        if (n) a.holders[p] = load_now(a.holders + p) - n;
+    }
+}
+
 constexpr int kShortRows = 1024, kShortColumns = 4;
 
 // Up to 1024 rows, a thread each.  A row whose first page e holds older tokens and is held by others too (held > 1)
@@ -218,30 +249,49 @@ __device__ __forceinline__ bool reserve_short(const ReserveArgs &a, int *part, i
 #pragma unroll
     for (int i = 0; i < kShortColumns; i++) e[i] = a.t.at(min(b, a.t.B - 1), n.first + min(i, max(n.columns - 1, 0)));
     if (__syncthreads_or(n.columns > kShortColumns)) return false;
-    const bool leaves = leaves_page(a, e[0], n.older && a.t.is_page(e[0]) ? a.holders[e[0]] : 0, page_of);
-    unsigned wants = leaves ? 1u : 0u;
+    bool met = false;  // (a page that others hold, with no older tokens: looked at again when all have left theirs)
 #pragma unroll
     for (int i = 0; i < kShortColumns; i++)
-        if (i < n.columns && !(i == 0 && n.older) && !a.t.is_page(e[i])) wants |= 1u << i;
-    int wanted;
-    int rank = block_sum<1024>(__popc(wants), part, wanted) - __popc(wants);
+        if (i < n.columns && !(i == 0 && n.older) && a.t.is_page(e[i])) met |= a.holders[e[i]] > 1;
+    const bool leaves = leaves_page(a, e[0], n.older && a.t.is_page(e[0]) ? a.holders[e[0]] : 0, page_of);
+    unsigned wants;
+    int wanted, rank;
+    auto count = [&] {
+        wants = leaves ? 1u : 0u;
+#pragma unroll
+        for (int i = 0; i < kShortColumns; i++)
+            if (i < n.columns && !(i == 0 && n.older) && !a.t.is_page(e[i])) wants |= 1u << i;
+        const int mine = __popc(wants) + (met ? 1 << 16 : 0);  // (4096 pages at most)
+        rank = (block_sum<1024>(mine, part, wanted) & 0xffff) - __popc(wants);
+    };
+    count();
+    const bool drops = wanted >> 16;
+    if (drops) {
+        drop_entries(a);
+        if (b < a.t.B)
+            for (int i = 0; i < n.columns; i++) e[i] = load_now(&a.t.at(b, n.first + i));
+        met = false;
+        count();
+    }
     int given = 0;
     if (wanted) {
         given = free_pages(a, wanted, part, [&](int r, int page) { fresh[r] = page; });
         __syncthreads();
     }
-    if (b >= a.t.B) return true;
-    int to = -1;
+    if (b < a.t.B) {
+        int to = -1;
 #pragma unroll
-    for (int i = 0; i < kShortColumns; i++) {
-        if (!(wants >> i & 1)) continue;
-        const int page = rank < given ? fresh[rank] : -1;
-        rank++;
-        a.t.at(b, n.first + i) = page;
-        if (page >= 0) a.holders[page] = 1;
-        if (i == 0 && leaves) to = page;
+        for (int i = 0; i < kShortColumns; i++) {
+            if (!(wants >> i & 1)) continue;
+            const int page = rank < given ? fresh[rank] : -1;
+            rank++;
+            a.t.at(b, n.first + i) = page;
+            if (page >= 0) a.holders[page] = 1;
+            if (i == 0 && leaves) to = page;
+        }
+        put_copy(a, b, to >= 0 ? e[0] : -1, to, to >= 0 ? n.older : 0);
     }
-    put_copy(a, b, to >= 0 ? e[0] : -1, to, to >= 0 ? n.older : 0);
+    if (drops) take_dropped(a);
     return true;
 }
 
@@ -268,7 +318,7 @@ __device__ __forceinline__ void wants_of(const ReserveArgs &a, int b, const Need
 // its rank.  (With a thread for every entry the one CU was bound by instructions: 8000 entries took 14 us.)
 __global__ __launch_bounds__(1024) void reserve_pages(ReserveArgs a) {
     extern __shared__ int lds[];
-    __shared__ int part[16], page_of[kShortRows], fresh_short[kShortRows * kShortColumns], long_rows;
+    __shared__ int part[16], page_of[kShortRows], fresh_short[kShortRows * kShortColumns], long_rows, met;
     if (reserve_short(a, part, page_of, fresh_short)) return;
     int *count = lds, *row_of = lds + a.t.B;  // [B] each: pages that a row wants, then of the rows before; the long rows
     unsigned *left = reinterpret_cast<unsigned *>(lds + 2 * a.t.B), *common = left + (a.t.B + 31) / 32;  // a bit for each row
@@ -276,7 +326,6 @@ __global__ __launch_bounds__(1024) void reserve_pages(ReserveArgs a) {
     auto bit = [](const unsigned *set, int b) { return (set[b / 32] >> (b % 32) & 1u) != 0; };
     auto mark = [](unsigned *set, int b) { atomicOr(set + b / 32, 1u << (b % 32)); };
     for (int i = tid; i < 2 * ((a.t.B + 31) / 32); i += 1024) left[i] = 0;
-    if (tid == 0) long_rows = 0;
     __syncthreads();
 
     // first pages that hold older tokens and that others hold
@@ -320,38 +369,59 @@ __global__ __launch_bounds__(1024) void reserve_pages(ReserveArgs a) {
     __syncthreads();
 
     constexpr int N = 8;  // (4: 1.5 us more in a call of 32 rows with 256 columns each)
-    for (int b = tid; b < a.t.B; b += 1024) {
-        const Need n = need_of(a, b);
-        if (n.columns > kShortColumns) {
-            row_of[atomicAdd(&long_rows, 1)] = b;
-            continue;
-        }
-        const bool leaves = bit(left, b);
-        int wants = 0;
-        for (int c = 0; c < n.columns; c++) wants += c == 0 && n.older ? leaves : !a.t.is_page(a.t.at(b, n.first + c));
-        count[b] = wants;
-        put_copy(a, b, -1, -1, 0);
-    }
-    __syncthreads();
-    for (int i = wave; i < long_rows; i += 16) {
-        const int b = __builtin_amdgcn_readfirstlane(row_of[i]);
-        const Need n = need_of(a, b);
-        const bool leaves = bit(left, b);
-        int wants = 0;
-        for (int c0 = 0; c0 < n.columns; c0 += 64 * N) {
-            int old[N];
-            unsigned long long who[N];
-            wants_of(a, b, n, leaves, c0, old, who);
-#pragma unroll
-            for (int j = 0; j < N; j++) wants += __popcll(who[j]);
-        }
-        if (lane == 0) {
+    auto count_all = [&] {
+        if (tid == 0) long_rows = met = 0;
+        __syncthreads();
+        for (int b = tid; b < a.t.B; b += 1024) {
+            const Need n = need_of(a, b);
+            if (n.columns > kShortColumns) {
+                row_of[atomicAdd(&long_rows, 1)] = b;
+                continue;
+            }
+            const bool leaves = bit(left, b);
+            int wants = 0;
+            for (int c = 0; c < n.columns; c++) {
+                const int old = a.t.at(b, n.first + c);
+                if (c == 0 && n.older) wants += leaves;
+                else if (!a.t.is_page(old)) wants++;
+                else if (a.holders[old] > 1) met = 1;
+            }
             count[b] = wants;
             put_copy(a, b, -1, -1, 0);
         }
+        __syncthreads();
+        for (int i = wave; i < long_rows; i += 16) {
+            const int b = __builtin_amdgcn_readfirstlane(row_of[i]);
+            const Need n = need_of(a, b);
+            const bool leaves = bit(left, b);
+            int wants = 0;
+            for (int c0 = 0; c0 < n.columns; c0 += 64 * N) {
+                int old[N];
+                unsigned long long who[N];
+                wants_of(a, b, n, leaves, c0, old, who);
+#pragma unroll
+                for (int j = 0; j < N; j++) wants += __popcll(who[j]);
+            }
+            if (wants < n.columns - (n.older && !leaves)) {  // (some pages are there)
+                for (int c = lane + (n.older != 0); c < n.columns; c += 64) {
+                    const int e = a.t.at(b, n.first + c);
+                    if (a.t.is_page(e) && a.holders[e] > 1) met = 1;
+                }
+            }
+            if (lane == 0) {
+                count[b] = wants;
+                put_copy(a, b, -1, -1, 0);
+            }
+        }
+        settle();
+        __syncthreads();
+    };
+    count_all();
+    const bool drops = met;
+    if (drops) {
+        drop_entries(a);
+        count_all();
     }
-    settle();
-    __syncthreads();
     int wanted = 0;
     for (int b0 = 0; b0 < a.t.B; b0 += 1024) {
         const int b = b0 + tid, mine = b < a.t.B ? count[b] : 0;
@@ -360,6 +430,7 @@ __global__ __launch_bounds__(1024) void reserve_pages(ReserveArgs a) {
         if (b < a.t.B) count[b] = wanted + sum - mine;
         wanted += total;
     }
+    // (with drops some pages are wanted)
     if (wanted == 0) return;
     // (the places of `keeper` are free again: pages in the order in which they are given out)
     int *fresh = a.keeper;
@@ -407,6 +478,7 @@ __global__ __launch_bounds__(1024) void reserve_pages(ReserveArgs a) {
                 if (who[j] >> lane & 1) give(b, n, c0 + j * 64 + lane, old[j], page[j]);
         }
     }
+    if (drops) take_dropped(a);
 }
 
 // ---- copies of pages ----------------------------------------------------------
@@ -749,7 +821,7 @@ int enatten_cache_fork(int *pages, int *lengths, int *holders, const int *parent
 
 size_t enatten_cache_reserve_workspace_bytes(int B, int columns, int num_pages) {
     if (B < 1 || columns < 1 || num_pages < 1) return 0;
-    return (size_t)num_pages * sizeof(int);
+    return (size_t)2 * num_pages * sizeof(int);
 }
 
 int enatten_cache_reserve(int *pages, const int *lengths, const int *counts, int count, int *holders, int *copies,
@@ -760,7 +832,7 @@ int enatten_cache_reserve(int *pages, const int *lengths, const int *counts, int
     if (int rc = set_table(fn, pages, B, columns, num_pages, page, pages_stride, &a.t)) return rc;
     if (!lengths || !holders || !copies) return missing(fn);
     if (!workspace || (uintptr_t)workspace % 16) return bad_workspace(fn);
-    if (int rc = apart(fn, a.t, {{holders, num_pages}, {copies, (int64_t)3 * B}, {static_cast<int *>(workspace), num_pages}},
+    if (int rc = apart(fn, a.t, {{holders, num_pages}, {copies, (int64_t)3 * B}, {static_cast<int *>(workspace), (int64_t)2 * num_pages}},
                        {{lengths, B}, {counts, counts ? B : 0}})) return rc;
     a.lengths = lengths;
     a.counts = counts;
@@ -768,6 +840,7 @@ int enatten_cache_reserve(int *pages, const int *lengths, const int *counts, int
     a.holders = holders;
     a.copies = copies;
     a.keeper = static_cast<int *>(workspace);
+    a.dropped = a.keeper + num_pages;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     ProfScope prof(ENATTEN_KERNEL_CACHE_PAGES, "reserve_pages", st);
     reserve_pages<<<1, 1024, (2 * B + 2 * ((B + 31) / 32)) * sizeof(int), st>>>(a);

@@ -184,6 +184,8 @@ def cache_reserve(pages, lengths, holders, page, counts=1):
     their order.  Where the first of them holds older tokens and other rows hold its page, the row gets a
     free page instead, and its line of ``copies`` is (page left, page got, older tokens), else (-1, -1, 0);
     if all that hold a page leave it in one call, the last row keeps it.
+    A page without older tokens that others hold even then, as where a row's length went back behind tokens
+    that it shares, is replaced without a copy; if nobody holds it any more it is free after the call.
 
     Where no page is free the entry becomes -1: :func:`cache_append` leaves its tokens out and
     :func:`cache_attention` gives NaN.  An entry that older tokens belong to and that is no page stays none.

@@ -413,7 +413,8 @@ int enatten_cache_fork(int *pages, int *lengths, int *holders, const int *parent
  * enatten_cache_reserve: a page of its own for every place of the last counts[b] of lengths[b] tokens of
  * row b (counts NULL: `count` each).  Entries that are no page get a free one.  A first page that holds
  * older tokens too and that others hold is left to them and replaced; if all its holders leave it in this
- * call, the last row keeps it.  copies [B, 3] is (page left, page got, older tokens) for a row that has
+ * call, the last row keeps it.  Then pages without older tokens that others hold are replaced too, those
+ * that nobody holds any more being free after the call.  copies [B, 3] is (page left, page got, older tokens) for a row that has
  * to be copied so, else (-1, -1, 0).  Where no free page is left the entry becomes -1, and one that should
  * hold older tokens but is no page stays none.  Rows whose numbers do not fit together are left out.
  *   workspace  enatten_cache_reserve_workspace_bytes(), 16-byte aligned; calls that may overlap need one each

@@ -35,29 +35,35 @@ def reserve_ref(pages, lengths, holders, page, counts):
     n, columns = len(holders), len(pages[0])
     pages, holders = [list(r) for r in pages], list(holders)
     free = [p for p in range(n) if holders[p] == 0]
-    copies = []
+    copies, dropped, places = [(-1, -1, 0)] * len(pages), [], []
     for b, (length, count) in enumerate(zip(lengths, counts)):
-        copy = (-1, -1, 0)
         if 0 < count <= length <= columns * page:
             start = length - count
-            for c in range(columns):
-                if (c + 1) * page <= start or c * page >= length:
-                    continue
-                e, there = pages[b][c], 0 <= pages[b][c] < n
-                older = max(start - c * page, 0)
-                if older and not (there and holders[e] > 1):
-                    continue            # its own, or tokens that are not there
-                if not older and there:
-                    continue
-                got = free.pop(0) if free else -1
-                if older:
-                    holders[e] -= 1
-                    if got >= 0:
-                        copy = (e, got, older)
-                if got >= 0:
-                    holders[got] = 1
-                pages[b][c] = got
-        copies.append(copy)
+            places += [(b, c, max(start - c * page, 0)) for c in range(start // page, -(-length // page))]
+    leave = set()
+    for b, c, older in places:
+        e = pages[b][c]
+        if older and 0 <= e < n and holders[e] > 1:
+            holders[e] -= 1
+            leave.add(b)
+    held = list(holders)
+    for b, c, older in places:
+        e = pages[b][c]
+        there = 0 <= e < n
+        if older and b not in leave:
+            continue            # its own, or tokens that are not there
+        if not older and there:
+            if held[e] < 2:
+                continue
+            dropped.append(e)   # (free when the call is over)
+        got = free.pop(0) if free else -1
+        if older and got >= 0:
+            copies[b] = (e, got, older)
+        if got >= 0:
+            holders[got] = 1
+        pages[b][c] = got
+    for e in dropped:
+        holders[e] -= 1
     return pages, holders, copies
 
 

@@ -123,6 +123,41 @@ def test_reserve_gives_every_holder_of_a_page_its_own():
         assert h.tolist() == [1, 1, 1, 1, 1, 0, 0, 0, 0, 5, 0, 0]
 
 
+@pytest.mark.parametrize("B,columns,page,spare", _SIZES)
+def test_lengths_that_went_back(B, columns, page, spare):
+    """Rows whose length went back behind tokens that they share, or have on pages of their own: new tokens never go to a
+    page that others hold."""
+    ensure_built()
+    from e_natten_amd import cache_reserve
+    print("case back", B, columns, page, spare, flush=True)
+    replaced = 0
+    for seed in range(4):
+        pages, lengths, holders = random_state(B, columns, page, spare, seed, sharing=0.8)
+        r = random.Random(seed)
+        for b in range(1, B):   # whole rows that others hold, as forks leave them
+            if r.random() < 0.4:
+                for e in pages[b]:
+                    holders[e] -= e >= 0
+                pages[b], lengths[b] = list(pages[b - 1]), lengths[b - 1]
+                for e in pages[b]:
+                    holders[e] += e >= 0
+        kept = [r.choice((n, n // page * page, r.randint(0, n), max(n - 3, 0))) for n in lengths]
+        # (few new tokens where all of a row have few columns, many else)
+        counts = [min(r.choice((0, 1, 2, page, 2 * page if seed % 2 else columns * page)), columns * page - k) for k in kept]
+        now = [k + c for k, c in zip(kept, counts)]
+        want = reserve_ref(pages, now, holders, page, counts)
+        p, h = ints(pages), ints(holders)
+        copies = cache_reserve(p, ints(now), h, page, ints(counts))
+        assert p.tolist() == want[0] and h.tolist() == want[1] and copies.tolist() == [list(x) for x in want[2]], seed
+        for b in range(B):
+            for c in range(kept[b] // page, -(-now[b] // page)):
+                e = want[0][b][c]
+                if counts[b] and e >= 0:
+                    assert want[1][e] == 1
+                    replaced += 0 <= pages[b][c] != e
+    assert replaced or B == 1
+
+
 def test_a_pool_that_runs_out():
     """The first rows get what there is; the others' entries are no pages, and stay none while they should hold
     older tokens."""

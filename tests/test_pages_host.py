@@ -299,7 +299,7 @@ def test_c_pages_validate_before_launch():
                        (compact, (dict(copies=none), dict(ws=none), dict(ws=ctypes.c_void_p(20))))):
         for bad in bads:
             assert call(**bad) == 1, (call, bad)
-    assert lib.enatten_cache_reserve_workspace_bytes(2, 3, 4) == 4 * 4
+    assert lib.enatten_cache_reserve_workspace_bytes(2, 3, 4) == 2 * 4 * 4
     assert lib.enatten_cache_compact_workspace_bytes(4096) == 4 * (4096 + 2)
     assert lib.enatten_cache_compact_workspace_bytes(2 ** 31 - 1) == 4 * (2 ** 31 - 1 + 2 ** 20)
     for bad in ((0, 3, 4), (2, 0, 4), (2, 3, 0)):
