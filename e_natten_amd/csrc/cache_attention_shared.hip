@@ -196,6 +196,10 @@ int enatten_cache_attention_shared(const void *q, const void *k_cache, const voi
         set_error("%s: workspace is NULL or not 16-byte aligned", fn);
         return ENATTEN_EINVAL;
     }
+    if (!p.many && (int64_t)B * heads * T > 0xffffff) {  // (2^32 threads that join the parts)
+        set_error("%s: too many rows", fn);
+        return ENATTEN_EUNSUPPORTED;
+    }
     a.shared = shared;
     a.runs = runs;
     a.size = B / runs;

@@ -12,8 +12,9 @@ __global__ __launch_bounds__(512, 2) void run_rows(SharedArgs args) {
     rows_body<DP, E4M3, DT, TG, TG == 1 ? 1 : TG == 8 && DP == 128 ? 4 : 2>(args);
 }
 
-// The parts of the first part's tiles joined, and with the second part's.  One workgroup per (tile, 16 rows, 32 channels): few tiles have many parts.  A
-// wave takes every fourth part: 16 lanes over the rows, 4 over neighbouring words of 4 channels.
+// The parts of the first part's tiles joined, and with the second part's.  One workgroup per (tile, 16 rows, 32
+// channels), as few tiles have many parts.  A wave takes every fourth part: 16 lanes over the rows, 4 over neighbouring
+// words of 4 channels.
 template <int DP, int DT>
 __global__ __launch_bounds__(256) void run_join(SharedArgs a, int tile_rows, int second_rows) {
     constexpr int WORDS = 2, SPLIT = DP / 32;
@@ -72,28 +73,26 @@ __global__ __launch_bounds__(256) void run_join(SharedArgs a, int tile_rows, int
         z += f * red[v][wave][lane];
     }
     const Place where = place_of(a, which, head, row, true);
-    {
-        int len, count;
-        const bool ok = sequence_of(a.tb, where.b, len, count);
-        if (!(ok && count > 0 && len - count >= shared_end(a, which))) {  // (it does not share them)
-            top = kFloor;
-            sum = 0.f;
-            z = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-        const int own = where.t * a.group + where.head - head * a.group, own_entry = where.b * a.row_tiles + own / second_rows;
-        const int own_row = own % second_rows;
-        const int *note = reinterpret_cast<const int *>(a.ws) + 2 * own_entry;
-        const int own_first = a.parts ? note[0] : own_entry, items = a.parts ? note[1] : 1;
-        for (int i = 0; i < items; i++) {
-            const float *p = part_of(a, second_rows, own_first + i, head, false);
-            const float m = p[own_row], most = fmaxf(top, m), f = __builtin_amdgcn_exp2f(top - most), g = __builtin_amdgcn_exp2f(m - most);
-            z = f * z + g * *reinterpret_cast<const f32x4 *>(p + 2 * second_rows + own_row * a.D + d);
-            sum = f * sum + g * p[second_rows + own_row];
-            top = most;
-        }
-        const float norm = sum == 0.f ? 0.f : 1.f / sum, poison = ok ? 0.f : __uint_as_float(0x7fc00000u);
-        store_channels<DT>(a.o, offset_of(a.o, where) + d, (where.t < count ? z * norm : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
+    int len, count;
+    const bool ok = sequence_of(a.tb, where.b, len, count);
+    if (!(ok && count > 0 && len - count >= shared_end(a, which))) {  // (it does not share them)
+        top = kFloor;
+        sum = 0.f;
+        z = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    const int own = where.t * a.group + where.head - head * a.group, own_entry = where.b * a.row_tiles + own / second_rows;
+    const int own_row = own % second_rows;
+    const int *note = reinterpret_cast<const int *>(a.ws) + 2 * own_entry;
+    const int own_first = a.parts ? note[0] : own_entry, items = a.parts ? note[1] : 1;
+    for (int i = 0; i < items; i++) {
+        const float *p = part_of(a, second_rows, own_first + i, head, false);
+        const float m = p[own_row], most = fmaxf(top, m), f = __builtin_amdgcn_exp2f(top - most), g = __builtin_amdgcn_exp2f(m - most);
+        z = f * z + g * *reinterpret_cast<const f32x4 *>(p + 2 * second_rows + own_row * a.D + d);
+        sum = f * sum + g * p[second_rows + own_row];
+        top = most;
+    }
+    const float norm = sum == 0.f ? 0.f : 1.f / sum, poison = ok ? 0.f : __uint_as_float(0x7fc00000u);
+    store_channels<DT>(a.o, offset_of(a.o, where) + d, (where.t < count ? z * norm : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
 }
 
 template <int DP, bool E4M3, int DT>

@@ -68,6 +68,9 @@ _CASES = [
     ([300, 310, 320, 290], None, 2, [-5, 2 ** 31 - 1], 4, 4, 1, 64, 32, BF16, I8, None),         # numbers out of any range
     ([300, 200, 320, 290], None, 1, [256], 8, 2, 1, 128, 64, BF16, E4M3, None),       # one is shorter: by itself
     ([200, 300, 320, 290], None, 1, [256], 8, 2, 1, 128, 64, BF16, E4M3, None),       # ... the first one
+    ([300, 400, 330], None, 3, [256, 399, 0], 8, 2, 1, 128, 64, BF16, E4M3, None),    # a sequence for itself in each run
+    ([300, 400], None, 2, [256, 384], 40, 2, 1, 64, 16, F16, I8, None),
+    ([500], None, 1, [448], 8, 2, 1, 128, 64, BF16, I8, None), ([500], None, 1, [448], 8, 2, 3, 80, 16, F32, E4M3, 100),
     ([0, 300, 0, 290], [0, 1, 0, 1], 1, [256], 8, 2, 1, 128, 64, BF16, I8, None),     # some without tokens
     ([300] * 4, [0, 2, 1, 2], 1, [256], 4, 2, 2, 80, 16, F32, E4M3, None),            # ... without new ones
     ([5000, 5050, 5020], None, 1, [4928], 4, 1, 1, 128, 64, BF16, I8, None),          # split along the tokens

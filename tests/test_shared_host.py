@@ -67,6 +67,11 @@ def test_c_shared_validates_before_launch():
     for bad in (dict(shared=none), dict(runs=0), dict(runs=-1), dict(runs=4), dict(runs=12), dict(ws=none),
                 dict(ws=ctypes.c_void_p(8)), dict(heads=3), dict(o=none), dict(D=24), dict(lengths=none), dict(B=0)):
         assert call(**bad) == 1 and "enatten_cache_attention_shared" in lib.enatten_last_error().decode(), bad
+    # rows above 128 channels in tiles of 16, each with a workgroup that joins its parts: 2^24 at most
+    assert lib.enatten_cache_attention_shared(at, at, at, at, at, at, at, none, at, 2, at, at, 64, 64, 1, 4096, 256, 8, 16, wide, 0,
+                                              _lib.F32, _lib.I8, none, none, none, none, none, none, wide, 1.0, none) not in (0, 1)
+    assert "too many rows" in lib.enatten_last_error().decode()
+
     def need(B=6, runs=2, T=1, cols=wide, heads=4, D=32, window=0, call=lib.enatten_cache_attention_shared_workspace_bytes):
         return call(B, heads, 2, T, D, 16, cols, window, _lib.BF16, *((runs,) if call is not plain else ()))
 
