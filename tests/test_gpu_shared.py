@@ -90,6 +90,11 @@ _CASES = [
     ([900, 910, 930], None, 1, [768], 8, 2, 1, 256, 64, BF16, I8, None),
     ([900 + i for i in range(12)], None, 2, [768, 800], 8, 2, 1, 256, 32, F16, E4M3, None),   # wide tiles of 256 channels
     ([900, 910, 930], None, 1, [768], 8, 2, 3, 192, 64, F32, I8, None),               # ... in tiles of 16
+    # more runs than lanes, and than workgroups that start at once; in tiles of many rows
+    ([200 + i % 90 for i in range(140)], None, 70, [160 + 16 * (i % 3) if i % 5 else 0 for i in range(70)], 2, 1, 1, 64, 16, BF16, I8, None),
+    ([60 + i % 40 for i in range(1200)], None, 600, [16 * (i % 4) for i in range(600)], 1, 1, 1, 32, 16, F16, E4M3, None),
+    ([200 + i % 90 for i in range(140)], None, 70, [160 + 16 * (i % 3) if i % 5 else 0 for i in range(70)], 12, 1, 1, 64, 16, BF16, E4M3, None),
+    ([90 + i % 40 for i in range(600)], [2 - i % 2 for i in range(600)], 300, [16 * (i % 5) for i in range(300)], 9, 1, 2, 128, 16, F16, I8, None),
     # windows (by themselves where these are short): as long as the own tokens, into the shared ones, one token
     ([1000, 990, 1020], None, 1, [960], 8, 2, 1, 128, 64, BF16, I8, 20),
     ([1000, 990, 1020, 980], None, 2, [960, 500], 8, 2, 1, 128, 64, F16, E4M3, 300),
