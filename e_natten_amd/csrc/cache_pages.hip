@@ -5,6 +5,11 @@
 // the number of entries that name it.  They read and write these once, some hundred kilobytes in a large
 // server, so launches and chains of loads bound them, not memory; what they write goes by their arguments
 // alone (sums by atomics of whole numbers, ranks by scans).  The copy moves codes: HBM.
+//
+// Measured on MI355X, single launches under the profiler.  4 beams, pages of 16: fork 2.4 us, reserve 5.1, copy 3.8.
+// 128 samples of 32 prompts, pages of 64, 4 layers of 8 heads of 128: 3.1, 7.1 and 13.8 (50 MB, 3.6 TB/s).  64 rows of
+// 1025 columns, half of which get prompts of up to 8192 tokens, pages of 16: 6.1 (two launches), 18.2 and 3.8.
+// compact: 216 pages 6.2 us; 1594 pages 6.7, and 23.6 for the copy that it asks for (100 MB, 4.2 TB/s).
 #include "sequence_common.h"
 
 namespace enatten {

@@ -13,6 +13,8 @@
 // [token, head] (4.8 TB/s, a plain copy of that size reaches 5.0), 46 us where they lie [head, token];
 // 16 + 4 heads of 128, 64 of them turned, 2 x 8192 tokens, float16: 29 us; 64 single tokens: 3.5 us.
 // 8 + 8 heads of 64 channels, 4 x 8192 tokens, by type: bfloat16 25 us, float32 48 (5.6 TB/s), float64 108 (5.0).
+// Two axes, 4 + 4 heads of 128 channels, 4 images of 128 x 128 as a projection leaves them, bfloat16: 53.6 us (5.0 TB/s);
+// three axes, 16 + 4 heads of 128, 96 of them turned, interleaved, 2 x 8192 tokens, float16: 30.6; 8 single tokens: 3.8.
 // Stores past the caches take 47 us instead of 56, but the reader that follows pays: with one pass over
 // both results behind it 114 us instead of 99.
 #include "sequence_common.h"
@@ -79,7 +81,7 @@ __global__ __launch_bounds__(256) void rotary_turn(RotaryArgs a) {
         // in every round.
         constexpr int STAGED = 256;
         __shared__ double staged[STAGED];
-        const bool few = TOKENS * a.num_axes <= STAGED;
+        const bool few = a.num_axes <= STAGED / TOKENS;
         if (few) {
             for (int i = threadIdx.x; i < TOKENS * a.num_axes; i += 256)
                 staged[i] = position(i / TOKENS * a.axis_stride + b0 * a.positions_stride + t0 + min(i % TOKENS, nt - 1));
@@ -193,11 +195,13 @@ int launch_tokens(const char *fn, RotaryArgs &a, hipStream_t st) {
         a.slice = (a.slice + 1) / 2;
         a.slices = (heads + a.slice - 1) / a.slice;
     }
-    // Sequences with the same positions share a workgroup's sines and cosines where there are enough of those:
+    // Sequences with the same positions share a workgroup's sines and cosines where 1024 workgroups are left: the 4
+    // images of the top take 53.6 us instead of 57.8.
+    const auto blocks_of = [&](int64_t batches) { return (a.B + batches - 1) / batches * a.tiles * a.slices; };
     a.batches = 1;
     if (a.positions_stride == 0)
-        while (a.batches < a.B && (int64_t)((a.B + 2 * a.batches - 1) / (2 * a.batches)) * a.tiles * a.slices >= 1024) a.batches *= 2;
-    const int64_t blocks = (int64_t)((a.B + a.batches - 1) / a.batches) * a.tiles * a.slices;
+        while (a.batches < a.B && blocks_of(2 * (int64_t)a.batches) >= 1024) a.batches *= 2;
+    const int64_t blocks = blocks_of(a.batches);
     if (blocks > 0xffffff) {  // (2^32 threads)
         set_error("%s: too many tokens", fn);
         return ENATTEN_EUNSUPPORTED;

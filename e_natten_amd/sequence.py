@@ -462,7 +462,8 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, kerne
     neighbours, B / runs each, and those of run r have their first ``shared[r]`` tokens on the same pages
     (:func:`cache_fork`).  These are read once for all rows of the run; whole pages of them count.  A sequence
     whose new tokens start before their end is computed by itself, and numbers below 1 share nothing, so
-    that the result is the same but for its rounding.
+    that the result is the same but for its rounding.  Where that would not pay, by the sizes of the call (few
+    codes in all that its columns could name or its window holds, many new tokens), every sequence reads for itself.
     """
     _tensors(q=q, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, pages=pages,
              lengths=lengths)

@@ -381,7 +381,8 @@ int enatten_cache_attention(const void *q, const void *k_cache, const void *v_ca
  * (int32 [runs], on the device; whole pages count, the rest of a page is each sequence's own).  These
  * tokens are read once for all rows of the run.  A sequence whose new tokens start before that end is
  * computed by itself, and a number below 1 shares nothing: results are enatten_cache_attention's but
- * for where they are rounded.  The pages are those of the run's first sequence that shares them.
+ * for where they are rounded.  The pages are those of the run's first sequence that shares them.  Where it
+ * would not pay, by the sizes of the call, every sequence reads for itself.
  */
 size_t enatten_cache_attention_shared_workspace_bytes(int B, int heads, int heads_kv, int T, int D,
                                                       int page, int columns, int kernel_size, int dtype,
