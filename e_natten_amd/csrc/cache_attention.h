@@ -518,9 +518,9 @@ int launch_attend_rows(const char *fn, const AttnArgs &a, bool e4m3, hipStream_t
 // Tiles of many rows of the first part, and the join behind both (cache_attention_shared_rows.hip)
 int launch_first_rows(const char *fn, const SharedArgs &a, int rows, bool e4m3, hipStream_t st);
 int launch_last_join(const char *fn, const SharedArgs &a, int rows, int second_rows, hipStream_t st);
-// A call without shared tokens, its arguments checked
+// A call without shared tokens, its arguments checked; plans without tiles of kWideRows rows are not `wide`
 int launch_plain(const char *fn, AttnArgs a, const Plan &p, void *workspace, bool e4m3, hipStream_t st);
-Plan plan_of(int B, int heads, int heads_kv, int T, int D, int page, int columns, int window, int dtype);
+Plan plan_of(int B, int heads, int heads_kv, int T, int D, int page, int columns, int window, int dtype, bool wide = true);
 size_t workspace_bytes(const Plan &p, int B, int heads_kv, int D);  // B: sequences, or runs
 // The arguments that all calls have, checked, but for row_tiles, parts and ws
 int set_attention(const char *fn, const void *q, const void *k_cache, const void *v_cache, const float *k_scale,

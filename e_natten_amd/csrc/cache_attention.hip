@@ -68,11 +68,11 @@ __global__ __launch_bounds__(256) void attend_join(AttnArgs a) {
 // tokens each of 16384 and 12288, 16 + 4 heads of 256 channels, take 783 us and 334 in bfloat16.
 // Workgroups.  Two per CU where their registers leave room for two waves per SIMD, else one: with 48 rows
 // of 128 channels a second one per CU only waits.
-Plan plan_of(int B, int heads, int heads_kv, int T, int D, int page, int columns, int window, int dtype) {
+Plan plan_of(int B, int heads, int heads_kv, int T, int D, int page, int columns, int window, int dtype, bool wide) {
     Plan p;
     const int64_t all = (int64_t)T * (heads / heads_kv);
     const int most = D > 128 ? 16 : D > 64 ? 48 : 64;
-    p.rows = all <= most ? (int)(all + 15) / 16 * 16 : D > 128 && dtype == ENATTEN_F32 ? 16 : kWideRows;
+    p.rows = all <= most ? (int)(all + 15) / 16 * 16 : !wide || (D > 128 && dtype == ENATTEN_F32) ? most : kWideRows;
     p.row_tiles = (int)((all + p.rows - 1) / p.rows);
     const int64_t entries = (int64_t)B * p.row_tiles;
     int64_t tokens = (int64_t)columns * page;

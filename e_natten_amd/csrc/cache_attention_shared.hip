@@ -82,14 +82,7 @@ __global__ __launch_bounds__(256) void run_join_tiles(SharedArgs a) {
     store_channels<DT>(a.o, b * a.o.sb + head * a.o.sh + t * a.o.st + c * 4, (t < count ? y * norm : f32x4{0.f, 0.f, 0.f, 0.f}) + poison);
 }
 
-// How a call is cut: both parts' plans, and where their workspaces lie (in floats).  Or not at all: the codes that
-// all sequences could have, read by each for itself, take about as long as what the launches cost in addition.
-// Measured, shared and by themselves, by those bytes.  One launch and the join, 16 rows: 7 MB 9.5 and 6.5 us, 13 MB 11.7
-// and 10.7, 38 MB 11.7 and 14.9, 139 MB 13.7 and 24.1.  Tiles of many rows, 32: 17 MB 25.5 and 13.1, 91 MB 31 and 28,
-// 288 MB 41 and 55; 48: 69 MB 27 and 20, 221 MB 32 and 36; 64 of 64 channels: 46 MB 23.5 and 17.4, 145 MB 28 and 31;
-// 256: 79 MB 26 and 12, 288 MB 29 and 30.  Sequences that have tiles of 256 rows each are bound by the matrix cores, whose
-// work is the same: 64 new tokens of 64 sequences behind 8192 take 412 and 328 us.
-constexpr int64_t kTilesFrom = 16 << 20, kRowsFrom = 160 << 20;
+// How a call is cut: both parts' plans, and where their workspaces lie (in floats).
 struct SharedPlan {
     Plan first, second;
     bool shares;
@@ -97,17 +90,44 @@ struct SharedPlan {
     int first_rows;  // of a place of its workspace
     int64_t second_at, floats;
 };
+// Whether a call is cut so at all: the codes that all sequences could have, read by each for itself, have to take longer
+// than the further launches.  Both ways measured, graph replays in us, together and by themselves; bytes are of codes
+// with head_dim rounded up to 64, 128 or 256, as the steps take their time by that (32 channels, 78 rows of 13
+// sequences, 110 MB or 220 rounded up: 26 and 44; 192 channels, 138 MB rounded up: 39 and 26).
+// One launch and the join, 16 rows: 7 MB 9.5 and 6.5, 13 MB 11.7 and 10.7, 17 MB 11.9 and 13.2, 38 MB 11.7 and 14.9, 139
+// MB 13.7 and 24.1.
+// Tiles of many rows, 32: 17 MB 25.5 and 13.1, 91 MB 31 and 28, 288 MB 41 and 55; 48: 69 MB 27 and 20, 221 MB 32 and 36;
+// 64 of 64 channels: 46 MB 23.5 and 17.4, 145 MB 28 and 31; 256: 79 MB 26 and 12, 288 MB 29 and 30.
+// Two sequences of up to 16 rows each have little to share: 270 MB 48 and 39 (three: 406 MB 47 and 67; two of 48 rows: 271
+// MB 72 and 85).
+// Sequences with too many rows for a tile of 16 to 64 have tiles of 256 by themselves, of which few rows are empty or
+// many: 64 rows of 128 channels, 238 MB 78 and 110; 96: 98 and 112; 128: 122 and 114; 256: 212 and 160.  Of 256 channels,
+// 96: 125 and 139.
+// Above 128 channels the first part has tiles of 256 rows too, and sequences of up to 16 rows have tiles of 16: 16 runs of 4
+// 541 MB 107 and 64; 6 and more: 276 MB 54 and 34, 346 MB 60 and 65, 811 MB 109 and 169, 1352 MB 118 and 211.
+constexpr int64_t kTilesFrom = 16 << 20, kRowsFrom = 160 << 20, kWideFrom = 320 << 20;
+bool pays(int64_t bytes, bool many, int size, int64_t rows, int D) {  // rows: of a sequence, per cache head
+    if (size == 1) return false;
+    // (float32 rows above 128 channels are in tiles of 16 however many: fewer tiles, or nothing is gained)
+    if (!many) return bytes >= kTilesFrom && (size * rows + 15) / 16 * 4 <= size * ((rows + 15) / 16) * 3;
+    if (rows > 96) return false;
+    if (D > 128 && rows <= 16) return bytes >= kWideFrom && size >= 6;
+    return bytes >= kRowsFrom && (size > 2 || rows > 16);
+}
 SharedPlan shared_plan(int B, int heads, int heads_kv, int T, int D, int page, int columns, int window, int dtype, int runs) {
     SharedPlan p;
     const int size = B / runs;
     const int64_t rows = (int64_t)T * size * (heads / heads_kv);
-    p.second = plan_of(B, heads, heads_kv, T, D, page, columns, window, dtype);
+    p.second = plan_of(B, heads, heads_kv, T, D, page, columns, window, dtype, false);
     p.first = plan_of(runs, heads, heads_kv, T * size, D, page, columns, window, dtype);
     p.many = p.first.rows > 16;
     int64_t tokens = (int64_t)columns * page;
     if (window && window + (int64_t)T < tokens) tokens = window + (int64_t)T;
-    p.shares = p.second.rows != kWideRows && 2 * D * tokens * heads_kv * B >= (p.many ? kRowsFrom : kTilesFrom);
-    if (!p.shares) return p;
+    p.shares = pays(2 * padded(D) * tokens * heads_kv * B, p.many, size, (int64_t)T * (heads / heads_kv), D);
+    if (!p.shares) {
+        p.second = plan_of(B, heads, heads_kv, T, D, page, columns, window, dtype);
+        return p;
+    }
     if (p.many) {
         p.first.rows = D > 128 ? kWideRows : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
         p.first.row_tiles = (int)((rows + p.first.rows - 1) / p.first.rows);

@@ -36,7 +36,7 @@ def _bits(t):
 
 def _columns(B, heads, page, d, rows):
     """A table so wide that its sequences could have the codes from which on a run's tokens are read together."""
-    return ((16 if rows <= 16 else 160) << 20) // (2 * d * page * heads * B) + 2
+    return ((16 if rows <= 16 else 160 if d <= 128 else 320) << 20) // (2 * max(d, 64) * page * heads * B) + 2
 
 
 @pytest.mark.parametrize("dtype,cache_dtype,d,page,size,N,heads,window,wide", [

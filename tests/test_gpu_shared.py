@@ -28,10 +28,28 @@ def _share(cache, runs, shared):
     return cache
 
 
+def _padded(d):
+    return 64 if d <= 64 else 128 if d <= 128 else 256
+
+
 def _columns(B, heads, page, d, rows):
     """A table so wide that its sequences could have the codes from which on a run's tokens are read together: 16 MB
-    with up to 16 rows, else 160."""
-    return ((16 if rows <= 16 else 160) << 20) // (2 * d * page * heads * B) + 2
+    with up to 16 rows, else 160, or 320 above 128 channels."""
+    return ((16 if rows <= 16 else 160 if d <= 128 else 320) << 20) // (2 * _padded(d) * page * heads * B) + 2
+
+
+def _pays(B, runs, N, heads, T, d, dtype, tokens):
+    """The rule: by the codes that all sequences could have, sequences in a run, and rows of a sequence."""
+    size, rows, mb = B // runs, T * N // heads, 2 * _padded(d) * tokens * heads * B / 2 ** 20
+    if size == 1:
+        return False
+    if size * rows <= 16 or d > 128 and dtype == F32:
+        return mb >= 16 and 4 * -(-size * rows // 16) <= 3 * size * -(-rows // 16)
+    if rows > 96:
+        return False
+    if d > 128 and rows <= 16:
+        return mb >= 320 and size >= 6
+    return mb >= 160 and (size > 2 or rows > 16)
 
 
 def _shares(q, cache, runs, window=0):
@@ -84,16 +102,27 @@ _CASES = [
     ([100] * 64 + [300 + i for i in range(6)], None, 1, [256], 2, 1, 1, 64, 32, BF16, I8, None),  # readers behind them
     ([600, 609, 650], [5, 3, 0], 1, [512], 8, 2, 5, 64, 128, BF16, E4M3, None),       # drafted tokens
     ([600, 609, 650, 700], [5, 3, 1, 4], 2, [500, 640], 15, 5, 5, 80, 48, F32, I8, None),
+    ([600, 609, 650, 700], [5, 3, 1, 4], 1, [500], 15, 5, 5, 80, 48, F32, I8, None),
+    ([620, 609, 650, 700], [5, 13, 1, 7], 2, [500, 640], 15, 5, 13, 80, 48, F32, I8, None),
+    # more rows than a sequence's tiles of 16 to 64, which it has several of: 64 of 80, 48 of 84 and 64, 16 of 96, 50, 20
+    ([700, 690, 800, 790], [20, 14, 1, 13], 2, [512, 700], 8, 2, 20, 64, 64, BF16, I8, None),
+    ([700, 690, 800, 790], [20, 14, 1, 13], 1, [512], 8, 2, 20, 48, 64, F32, E4M3, None),
+    ([700, 690, 800, 790], [21, 14, 1, 0], 2, [512, 700], 8, 2, 21, 128, 64, F16, E4M3, None),
+    ([700, 690, 800, 790], [16, 14, 1, 0], 1, [512], 8, 2, 16, 96, 32, F32, I8, None),
+    ([700, 690, 800, 790], [24, 14, 1, 0], 2, [512, 700], 8, 2, 24, 256, 64, BF16, I8, None),
+    ([700, 690, 800], [25, 14, 1], 1, [512], 4, 2, 25, 192, 16, F16, E4M3, None),
+    ([700, 690, 800], [5, 4, 1], 1, [512], 8, 2, 5, 256, 48, BF16, E4M3, None),
     ([700, 690, 800, 790], [70, 64, 1, 33], 2, [512, 700], 8, 2, 70, 128, 64, BF16, I8, None),  # chunks behind a prompt
     ([700, 690, 800, 790], [70, 64, 1, 33], 2, [512, 700], 8, 2, 70, 64, 64, F32, E4M3, None),
     ([520, 530], [257, 200], 1, [256], 4, 1, 257, 64, 16, BF16, I8, None),            # tiles of rows in both passes
     ([900, 910, 930], None, 1, [768], 8, 2, 1, 256, 64, BF16, I8, None),
     ([900 + i for i in range(12)], None, 2, [768, 800], 8, 2, 1, 256, 32, F16, E4M3, None),   # wide tiles of 256 channels
-    ([900, 910, 930], None, 1, [768], 8, 2, 3, 192, 64, F32, I8, None),               # ... in tiles of 16
+    ([900, 910, 930, 905], None, 1, [768], 8, 2, 3, 192, 64, F32, I8, None),          # ... in tiles of 16, three for four
+    ([900, 910, 930], None, 1, [768], 8, 2, 3, 192, 64, F32, I8, None),               # (three for three: by themselves)
     # more runs than lanes, and than workgroups that start at once; in tiles of many rows
     ([200 + i % 90 for i in range(140)], None, 70, [160 + 16 * (i % 3) if i % 5 else 0 for i in range(70)], 2, 1, 1, 64, 16, BF16, I8, None),
     ([60 + i % 40 for i in range(1200)], None, 600, [16 * (i % 4) for i in range(600)], 1, 1, 1, 32, 16, F16, E4M3, None),
-    ([200 + i % 90 for i in range(140)], None, 70, [160 + 16 * (i % 3) if i % 5 else 0 for i in range(70)], 12, 1, 1, 64, 16, BF16, E4M3, None),
+    ([200 + i % 90 for i in range(140)], None, 70, [160 + 16 * (i % 3) if i % 5 else 0 for i in range(70)], 20, 1, 1, 64, 16, BF16, E4M3, None),
     ([90 + i % 40 for i in range(600)], [2 - i % 2 for i in range(600)], 300, [16 * (i % 5) for i in range(300)], 9, 1, 2, 128, 16, F16, I8, None),
     # windows (by themselves where these are short): as long as the own tokens, into the shared ones, one token
     ([1000, 990, 1020], None, 1, [960], 8, 2, 1, 128, 64, BF16, I8, 20),
@@ -126,12 +155,9 @@ def test_shared(lengths, counts, runs, shared, N, heads, T, d, page, dtype, cach
     _share(cache, runs, [min([s for s in starts[r * size:(r + 1) * size] if s // page * page >= n // page * page] or [0])
                          if n > 0 else 0 for r, n in enumerate(shared)])
     q = _q(B, N, T, d, dtype, 7)
-    # (not where every sequence has more rows than fit a tile of 16 to 64, and not short windows)
-    fits = T * N // heads <= (16 if d > 128 else 48 if d > 64 else 64) or d > 128 and dtype == F32
-    seen = min(cache.pages.shape[1] * page, window + T if window else 1 << 31)
-    one_launch = rows <= 16 or d > 128 and dtype == F32
-    assert _shares(q, cache, runs, window) == (fits and 2 * d * seen * heads * B >= (16 if one_launch else 160) << 20)
-    assert _shares(q, cache, runs, window) == (fits and (window is None or window > 4000))
+    pays = _pays(B, runs, N, heads, T, d, dtype, min(cache.pages.shape[1] * page, window + T if window else 1 << 31))
+    assert _shares(q, cache, runs, window) == pays
+    assert pays or size == 1 or window and window < 4000 or T * N // heads > 96 or T == 5 or (size, d) == (3, 192)
     ref, bound = attention_ref(q, cache, counts, window, d ** -0.5)
     args = (q.cuda(), *cache.on("cuda"), ints(lengths), window, d ** -0.5, None if counts is None else ints(counts))
     o = cache_attention(*args, ints(shared))

@@ -67,9 +67,8 @@ def test_c_shared_validates_before_launch():
     for bad in (dict(shared=none), dict(runs=0), dict(runs=-1), dict(runs=4), dict(runs=12), dict(ws=none),
                 dict(ws=ctypes.c_void_p(8)), dict(heads=3), dict(o=none), dict(D=24), dict(lengths=none), dict(B=0)):
         assert call(**bad) == 1 and "enatten_cache_attention_shared" in lib.enatten_last_error().decode(), bad
-    # rows above 128 channels in tiles of 16, each with a workgroup that joins its parts: 2^24 at most
-    assert lib.enatten_cache_attention_shared(at, at, at, at, at, at, at, none, at, 2, at, at, 64, 64, 1, 4096, 256, 8, 16, wide, 0,
-                                              _lib.F32, _lib.I8, none, none, none, none, none, none, wide, 1.0, none) not in (0, 1)
+    # rows of runs with up to 16 have a workgroup each that joins their parts: fewer than 2^24
+    assert call(B=1 << 22, runs=1 << 21) not in (0, 1)
     assert "too many rows" in lib.enatten_last_error().decode()
 
     def need(B=6, runs=2, T=1, cols=wide, heads=4, D=32, window=0, call=lib.enatten_cache_attention_shared_workspace_bytes):
@@ -79,9 +78,11 @@ def test_c_shared_validates_before_launch():
     rows = lambda B, T: B * 4 * T * 34 * 4   # a row's sums of values, maximum and sum, once for the run and once for itself
     assert need() >= 2 * rows(6, 1) and need(T=3) >= 2 * rows(6, 3) and need(T=16) >= 2 * rows(6, 16)
     # by themselves: few codes, short windows, tiles of 256 rows for every sequence
-    for alone in (dict(cols=3), dict(cols=1365), dict(window=21844), dict(T=100), dict(T=7, cols=13653), dict(T=16, cols=13653)):
+    for alone in (dict(cols=3), dict(cols=682), dict(window=10921), dict(T=100), dict(T=49), dict(T=7, cols=6826),
+                  dict(T=16, cols=6826), dict(runs=6), dict(runs=3, T=7), dict(runs=2, T=3, D=256), dict(runs=1, T=3, D=256, cols=3413)):
         assert need(**alone) == need(**alone, call=plain), alone
-    for together in (dict(cols=1366), dict(window=21845), dict(T=7, cols=13654), dict(T=16, cols=13654)):
+    for together in (dict(cols=683), dict(window=10922), dict(T=7, cols=6827), dict(T=16, cols=6827), dict(T=48), dict(runs=3, T=16),
+                     dict(runs=3), dict(runs=1, T=3, D=256, cols=3414), dict(runs=2, T=9, D=256, cols=3414)):
         assert need(**together) != need(**together, call=plain), together
     for bad in (dict(B=0), dict(runs=0), dict(runs=4), dict(T=0), dict(cols=0), dict(heads=3), dict(T=1 << 28)):
         assert need(**bad) == 0
