@@ -101,17 +101,17 @@ struct SharedPlan {
 // Two sequences of up to 16 rows each have little to share: 270 MB 48 and 39 (three: 406 MB 47 and 67; two of 48 rows: 271
 // MB 72 and 85).
 // Sequences with too many rows for a tile of 16 to 64 have tiles of 256 by themselves, of which few rows are empty or
-// many: 64 rows of 128 channels, 238 MB 78 and 110; 96: 98 and 112; 128: 122 and 114; 256: 212 and 160.  Of 256 channels,
-// 96: 125 and 139.
+// many: 64 rows of 128 channels, 102 MB 57 and 61, 238 MB 78 and 110; 96: 98 and 112; 128: 122 and 114; 256: 212 and 160.
+// Of 256 channels, 64 rows: 28 MB 57 and 54, 65 MB 69 and 77, 204 MB 96 and 137; 96: 125 and 139.
 // Above 128 channels the first part has tiles of 256 rows too, and sequences of up to 16 rows have tiles of 16: 16 runs of 4
 // 541 MB 107 and 64; 6 and more: 276 MB 54 and 34, 346 MB 60 and 65, 811 MB 109 and 169, 1352 MB 118 and 211.
-constexpr int64_t kTilesFrom = 16 << 20, kRowsFrom = 160 << 20, kWideFrom = 320 << 20;
+constexpr int64_t kTilesFrom = 16 << 20, kRowsFrom = 160 << 20, kWideFrom = 320 << 20, kWideRowsFrom = 64 << 20;
 bool pays(int64_t bytes, bool many, int size, int64_t rows, int D) {  // rows: of a sequence, per cache head
     if (size == 1) return false;
     // (float32 rows above 128 channels are in tiles of 16 however many: fewer tiles, or nothing is gained)
     if (!many) return bytes >= kTilesFrom && (size * rows + 15) / 16 * 4 <= size * ((rows + 15) / 16) * 3;
     if (rows > 96) return false;
-    if (D > 128 && rows <= 16) return bytes >= kWideFrom && size >= 6;
+    if (D > 128) return rows > 16 ? bytes >= kWideRowsFrom : bytes >= kWideFrom && size >= 6;
     return bytes >= kRowsFrom && (size > 2 || rows > 16);
 }
 SharedPlan shared_plan(int B, int heads, int heads_kv, int T, int D, int page, int columns, int window, int dtype, int runs) {
@@ -227,6 +227,7 @@ int enatten_cache_attention_shared(const void *q, const void *k_cache, const voi
         set_error("%s: too many rows", fn);
         return ENATTEN_EUNSUPPORTED;
     }
+    if (a.window >= (int64_t)columns * page) a.window = 0;  // (hides nothing: no row has to be asked where its begins)
     a.shared = shared;
     a.runs = runs;
     a.size = B / runs;

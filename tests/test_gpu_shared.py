@@ -47,8 +47,8 @@ def _pays(B, runs, N, heads, T, d, dtype, tokens):
         return mb >= 16 and 4 * -(-size * rows // 16) <= 3 * size * -(-rows // 16)
     if rows > 96:
         return False
-    if d > 128 and rows <= 16:
-        return mb >= 320 and size >= 6
+    if d > 128:
+        return mb >= 64 if rows > 16 else mb >= 320 and size >= 6
     return mb >= 160 and (size > 2 or rows > 16)
 
 

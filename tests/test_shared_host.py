@@ -79,10 +79,11 @@ def test_c_shared_validates_before_launch():
     assert need() >= 2 * rows(6, 1) and need(T=3) >= 2 * rows(6, 3) and need(T=16) >= 2 * rows(6, 16)
     # by themselves: few codes, short windows, tiles of 256 rows for every sequence
     for alone in (dict(cols=3), dict(cols=682), dict(window=10921), dict(T=100), dict(T=49), dict(T=7, cols=6826),
-                  dict(T=16, cols=6826), dict(runs=6), dict(runs=3, T=7), dict(runs=2, T=3, D=256), dict(runs=1, T=3, D=256, cols=3413)):
+                  dict(T=16, cols=6826), dict(runs=6), dict(runs=3, T=7), dict(runs=2, T=3, D=256), dict(runs=1, T=3, D=256, cols=3413),
+                  dict(runs=2, T=9, D=256, cols=682)):
         assert need(**alone) == need(**alone, call=plain), alone
     for together in (dict(cols=683), dict(window=10922), dict(T=7, cols=6827), dict(T=16, cols=6827), dict(T=48), dict(runs=3, T=16),
-                     dict(runs=3), dict(runs=1, T=3, D=256, cols=3414), dict(runs=2, T=9, D=256, cols=3414)):
+                     dict(runs=3), dict(runs=1, T=3, D=256, cols=3414), dict(runs=2, T=9, D=256, cols=683)):
         assert need(**together) != need(**together, call=plain), together
     for bad in (dict(B=0), dict(runs=0), dict(runs=4), dict(T=0), dict(cols=0), dict(heads=3), dict(T=1 << 28)):
         assert need(**bad) == 0
