@@ -14,8 +14,8 @@
 //
 // Measured on MI355X, launches under the profiler, bfloat16, heads of 128 channels.  8 sequences, 16 + 16 heads, 480
 // shared tokens and up to 40 of their own, int8: 8.8 us and 4.0 for the join.  64 sequences, 32 + 8
-// heads, 16384 shared tokens and up to 500, E4M3: 36.6 us for the shared tokens (17.2 GFLOP, 470 TFLOP/s), 14.8 for the
-// others, join 7.2.  16 runs of 4, 32 + 4 heads, up to 8192 shared tokens each and up to 300, int8: 42.8, 13.5 and 5.9.
+// heads, 16384 shared tokens and up to 500, E4M3: 35.6 us for the shared tokens (17.2 GFLOP, 480 TFLOP/s), 15.2 for the
+// others, join 7.2.  16 runs of 4, 32 + 4 heads, up to 8192 shared tokens each and up to 300, int8: 42.1, 13.0 and 6.0.
 // Beside the first launches' steps, about 10 us each go to chains of loads (lengths, pages, codes, q) and the code's
 // first run.
 #include "cache_attention_body.h"

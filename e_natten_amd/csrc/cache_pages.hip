@@ -199,7 +199,7 @@ __device__ __forceinline__ int free_pages(const ReserveArgs &a, int wanted, int 
 // Seldom, so that passes over the table and all pages do not matter.
 __device__ __forceinline__ void drop_entries(const ReserveArgs &a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int p = threadIdx.x; p < a.t.num_pages; p += 1024) a.dropped[p] = 0;
+    for (int64_t p = threadIdx.x; p < a.t.num_pages; p += 1024) a.dropped[p] = 0;
     __threadfence();
     __syncthreads();
     for (int b = wave; b < a.t.B; b += 16) {
@@ -218,7 +218,7 @@ __device__ __forceinline__ void drop_entries(const ReserveArgs &a) {
 __device__ __forceinline__ void take_dropped(const ReserveArgs &a) {
     __threadfence();
     __syncthreads();
-    for (int p = threadIdx.x; p < a.t.num_pages; p += 1024) {
+    for (int64_t p = threadIdx.x; p < a.t.num_pages; p += 1024) {
         const int n = load_now(a.dropped + p);
         if (n) a.holders[p] = load_now(a.holders + p) - n;
     }
