@@ -9,10 +9,11 @@ namespace {
 // groups of waves share; above 128 channels, where LDS has no room for such steps, tiles of 256 rows.
 //
 // A workgroup takes 8.5 us to its first step (shares 1.4, who reads 1, pages and scales 1.3, rows of q 2.8, the first
-// codes 2) and 2 to 3 to leave its part.  Steps of 128 rows by 128 tokens of 128 channels take 2.9 us, in turn the codes'
-// widening 0.6, the next loads' requests 0.5, the products and exponentials 1.3 and the wait for the waves that turn
-// values; steps of 32 rows by 256 tokens 3.2 us, 64 KB per CU, as fast as HBM brings them (5.2 TB/s).  Half of the
-// waves one phase ahead of the others (products before widening) came to the same time, whichever half it was.
+// codes 2) and 2 to 3 to leave its part.  Steps of 128 rows by 128 tokens of 128 channels take 2.9 us, of which vector
+// instructions (exponentials, the codes' widening) fill two thirds and the matrix cores one: a wave's widening takes 0.4
+// to 0.7 us, the next loads' requests 0.3 to 0.6, products and exponentials 1.4.  Half of the waves one phase ahead of the
+// others (products before widening) came to the same time, whichever half it was.  Steps of 32 rows by 256 tokens take 3.2
+// us, 64 KB per CU, as fast as HBM brings them (5.2 TB/s).
 template <int DP, bool E4M3, int DT, int TG>
 __global__ __launch_bounds__(512, 2) void run_rows(SharedArgs args) {
     rows_body<DP, E4M3, DT, TG, TG == 1 ? 1 : TG == 8 && DP == 128 ? 4 : 2>(args);
