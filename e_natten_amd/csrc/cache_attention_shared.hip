@@ -106,7 +106,7 @@ struct SharedPlan {
 // Above 128 channels the first part has tiles of 256 rows too, and sequences of up to 16 rows have tiles of 16: 16 runs of 4
 // 541 MB 107 and 64; 6 and more: 276 MB 54 and 34, 346 MB 60 and 65, 811 MB 109 and 169, 1352 MB 118 and 211.
 constexpr int64_t kTilesFrom = 16 << 20, kRowsFrom = 160 << 20, kWideFrom = 320 << 20, kWideRowsFrom = 64 << 20;
-bool pays(int64_t bytes, bool many, int size, int64_t rows, int D) {  // rows: of a sequence, per cache head
+bool pays(double bytes, bool many, int size, int64_t rows, int D) {  // rows: of a sequence, per cache head
     if (size == 1) return false;
     // (float32 rows above 128 channels are in tiles of 16 however many: fewer tiles, or nothing is gained)
     if (!many) return bytes >= kTilesFrom && (size * rows + 15) / 16 * 4 <= size * ((rows + 15) / 16) * 3;
@@ -123,7 +123,7 @@ SharedPlan shared_plan(int B, int heads, int heads_kv, int T, int D, int page, i
     p.many = p.first.rows > 16;
     int64_t tokens = (int64_t)columns * page;
     if (window && window + (int64_t)T < tokens) tokens = window + (int64_t)T;
-    p.shares = pays(2 * padded(D) * tokens * heads_kv * B, p.many, size, (int64_t)T * (heads / heads_kv), D);
+    p.shares = pays(2.0 * padded(D) * tokens * heads_kv * B, p.many, size, (int64_t)T * (heads / heads_kv), D);
     if (!p.shares) {
         p.second = plan_of(B, heads, heads_kv, T, D, page, columns, window, dtype);
         return p;
