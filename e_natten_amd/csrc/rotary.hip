@@ -55,8 +55,10 @@ __device__ __forceinline__ void turn(double angle, double &c, double &s) { sinco
 // A unit of work is a pack of VEC channels: in the half layout one of the first channels of the pairs
 // together with the one of the second channels, interleaved a pack of VEC / 2 pairs (with VEC 1 a single
 // pair); behind the rotated channels a pack to copy.
-// (AXES: whether there are several axes; asking for that in the kernel takes a single token 2.80 us instead of 2.68)
-template <typename S, int VEC, bool INTERLEAVED, int TOKENS, bool AXES>
+// (AXES: whether there are several axes; asking for that in the kernel takes a single token 2.80 us instead of 2.68.
+// SHARED: whether a workgroup has several sequences; with the loop over its only one 32 x 1024 tokens of 32 + 8 heads of
+// 128 channels take 160 us instead of 142, and 65536 single tokens of one head with axes 87 instead of 72)
+template <typename S, int VEC, bool INTERLEAVED, int TOKENS, bool AXES, bool SHARED>
 __global__ __launch_bounds__(256) void rotary_turn(RotaryArgs a) {
     using C = typename Math<S>::type;
     struct alignas(2 * sizeof(C)) Turn { C c, s; };
@@ -66,7 +68,7 @@ __global__ __launch_bounds__(256) void rotary_turn(RotaryArgs a) {
     int block = blockIdx.x;
     const int slice = block % a.slices;
     block /= a.slices;
-    const int tile = block % a.tiles, b0 = block / a.tiles * a.batches, b1 = min(b0 + a.batches, a.B);
+    const int tile = block % a.tiles, b0 = SHARED ? block / a.tiles * a.batches : block / a.tiles;
     const int t0 = tile * TOKENS, nt = min(TOKENS, a.T - t0), half = a.R / 2;
     auto position = [&](int64_t at) {
         return a.wide_positions ? (double)static_cast<const int64_t *>(a.positions)[at]
@@ -112,7 +114,8 @@ __global__ __launch_bounds__(256) void rotary_turn(RotaryArgs a) {
     const int turned = IN_PACK ? a.R / VEC : half / VEC, units = turned + (a.D - a.R) / VEC;
     const int mate = INTERLEAVED ? 1 : half;          // where not: the second channel, so far behind the first
     const int h0 = slice * a.slice, h1 = min(h0 + a.slice, a.heads[0] + a.heads[1]);
-    for (int b = b0; b < b1; b++)
+    int b = b0;
+    do {
 #pragma unroll
     for (int which = 0; which < 2; which++) {
         const int lo = which ? max(h0 - a.heads[0], 0) : h0, hi = which ? h1 - a.heads[0] : min(h1, a.heads[0]);
@@ -176,6 +179,18 @@ __global__ __launch_bounds__(256) void rotary_turn(RotaryArgs a) {
             }
         }
     }
+    } while (SHARED && ++b < min(b0 + a.batches, a.B));
+}
+
+template <typename S, int VEC, bool INTERLEAVED, bool AXES, bool SHARED>
+void launch_turn(const RotaryArgs &a, int tokens, int blocks, size_t lds, hipStream_t st) {
+    switch (tokens) {
+        case 16: rotary_turn<S, VEC, INTERLEAVED, 16, AXES, SHARED><<<blocks, 256, lds, st>>>(a); break;
+        case 8: rotary_turn<S, VEC, INTERLEAVED, 8, AXES, SHARED><<<blocks, 256, lds, st>>>(a); break;
+        case 4: rotary_turn<S, VEC, INTERLEAVED, 4, AXES, SHARED><<<blocks, 256, lds, st>>>(a); break;
+        case 2: rotary_turn<S, VEC, INTERLEAVED, 2, AXES, SHARED><<<blocks, 256, lds, st>>>(a); break;
+        default: rotary_turn<S, VEC, INTERLEAVED, 1, AXES, SHARED><<<blocks, 256, lds, st>>>(a); break;
+    }
 }
 
 template <typename S, int VEC, bool INTERLEAVED, bool AXES>
@@ -195,12 +210,18 @@ int launch_tokens(const char *fn, RotaryArgs &a, hipStream_t st) {
         a.slice = (a.slice + 1) / 2;
         a.slices = (heads + a.slice - 1) / a.slice;
     }
-    // Sequences with the same positions share a workgroup's sines and cosines where 1024 workgroups are left: the 4
-    // images of the top take 53.6 us instead of 57.8.
+    // Up to four sequences with the same positions share a workgroup's sines and cosines where these count, with fewer
+    // than 8 heads, and 2048 workgroups are left.  Both sides measured, us of each sequence by itself and together,
+    // bfloat16 without axes: a head of 64 channels, 4 x 65536 tokens 30.5 and 19.1; 1 + 1 heads, 8 x 32768 tokens 37 and
+    // 28; 2 + 2, 8 x 16384 28.2 and 25.1; 3 + 2, 16 x 4096, float16 18.5 and 17.2; 1 + 1 of 128, 8192 single tokens 14.3
+    // and 13.8, but 27 with eight of them.  With more heads it does not pay: 4 + 4 of 128, 4 x 16384 tokens 46 and 48; 32 +
+    // 8, 32 x 1024 141 and 149; 16 + 4, 16384 single tokens 31 and, 16 of them, 38.  With fewer workgroups neither: one
+    // head of 128, 2048 single tokens 5.1 and 5.7.  With two axes 4 + 4 heads of 128, 4 x 16384 46.3 and 48.6; 3 + 2, 16 x
+    // 4096 20.0 and 17.7.
     const auto blocks_of = [&](int64_t batches) { return (a.B + batches - 1) / batches * a.tiles * a.slices; };
     a.batches = 1;
-    if (a.positions_stride == 0)
-        while (a.batches < a.B && blocks_of(2 * (int64_t)a.batches) >= 1024) a.batches *= 2;
+    if (a.positions_stride == 0 && heads < 8)
+        while (a.batches < 4 && a.batches < a.B && blocks_of(2 * (int64_t)a.batches) >= 2048) a.batches *= 2;
     const int64_t blocks = blocks_of(a.batches);
     if (blocks > 0xffffff) {  // (2^32 threads)
         set_error("%s: too many tokens", fn);
@@ -208,13 +229,8 @@ int launch_tokens(const char *fn, RotaryArgs &a, hipStream_t st) {
     }
     const size_t lds = (size_t)tokens * a.R * sizeof(typename Math<S>::type);
     ProfScope prof(ENATTEN_KERNEL_ROTARY, "rotary_turn", st);
-    switch (tokens) {
-        case 16: rotary_turn<S, VEC, INTERLEAVED, 16, AXES><<<(int)blocks, 256, lds, st>>>(a); break;
-        case 8: rotary_turn<S, VEC, INTERLEAVED, 8, AXES><<<(int)blocks, 256, lds, st>>>(a); break;
-        case 4: rotary_turn<S, VEC, INTERLEAVED, 4, AXES><<<(int)blocks, 256, lds, st>>>(a); break;
-        case 2: rotary_turn<S, VEC, INTERLEAVED, 2, AXES><<<(int)blocks, 256, lds, st>>>(a); break;
-        default: rotary_turn<S, VEC, INTERLEAVED, 1, AXES><<<(int)blocks, 256, lds, st>>>(a); break;
-    }
+    if (a.batches > 1) launch_turn<S, VEC, INTERLEAVED, AXES, true>(a, tokens, (int)blocks, lds, st);
+    else launch_turn<S, VEC, INTERLEAVED, AXES, false>(a, tokens, (int)blocks, lds, st);
     return launched(fn);
 }
 
