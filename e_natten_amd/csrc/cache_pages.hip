@@ -742,8 +742,10 @@ int set_table(const char *fn, int *pages, int B, int columns, int num_pages, int
         set_error("%s: the rows of pages must not overlap", fn);
         return ENATTEN_EINVAL;
     }
-    if (B > kMostRows || (int64_t)B * columns > 1 << 30 || (int64_t)columns * page > (1 << 30) - 4096) {
-        set_error("%s: more than 4096 rows, 2^30 entries, or 2^30 tokens in a row's pages", fn);
+    // (of 2^30 pages up to 2^29 move, whose lines of three numbers still have places of 32 bits; that many pages of
+    // 16 tokens of 16 channels are 512 GB of keys and values)
+    if (B > kMostRows || (int64_t)B * columns > 1 << 30 || num_pages > 1 << 30 || (int64_t)columns * page > (1 << 30) - 4096) {
+        set_error("%s: more than 4096 rows, 2^30 entries, 2^30 pages, or 2^30 tokens in a row's pages", fn);
         return ENATTEN_EUNSUPPORTED;
     }
     *t = PageTable{pages, B > 1 ? stride : 0, B, columns, num_pages, page};

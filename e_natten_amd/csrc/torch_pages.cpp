@@ -28,7 +28,7 @@ void validate_table(const char *what, const Tensor &pages, const Tensor &holders
     TORCH_CHECK_VALUE(page >= 16 && page <= 1024 && page % 16 == 0, what,
                       ": pages must hold a multiple of 16 tokens up to 1024, got ", page);
     validate_numbers(what, "holders", holders, -1, pages);
-    TORCH_CHECK_VALUE(pages.size(0) <= 0x7fffffff && pages.size(1) <= 0x7fffffff && holders.size(0) <= 0x7fffffff, what,
+    TORCH_CHECK_VALUE(pages.size(0) <= 0x7fffffff && pages.size(1) <= 0x7fffffff && holders.size(0) <= 1 << 30, what,
                       ": tensor too large");
 }
 Tensor workspace(size_t bytes, const Tensor &like) { return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)); }

@@ -13,7 +13,7 @@ a program keeps ``holders``, how many entries of the table name each page; a pag
 
 No call waits for the GPU, so a step can be captured into a graph; what they write depends on their
 arguments alone.  An entry of the table outside the cache's pages is no page (these calls write -1), and all
-of a row counts, also behind its last token: a table starts filled with -1.
+of a row counts, also behind its last token: a table starts filled with -1.  At most 2^30 pages.
 
 Like the others they run through the native torch binding where it is built (operators
 ``enatten::cache_fork``, ...), else through ctypes.
@@ -50,7 +50,7 @@ def _validate_table(pages, holders, page) -> None:
     if page < 16 or page > 1024 or page % 16:
         raise ValueError("pages must hold a multiple of 16 tokens up to 1024, got %d" % page)
     _numbers("holders", holders, None, pages)
-    if max(*pages.shape, holders.shape[0]) > 0x7fffffff:
+    if max(pages.shape) > 0x7fffffff or holders.shape[0] > 1 << 30:
         raise ValueError("tensor too large")
 
 
