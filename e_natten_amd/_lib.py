@@ -9,6 +9,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libenatten.so")
 
 ABI_VERSION = 5  # ENATTEN_ABI_VERSION of include/enatten.h
+EUNSUPPORTED = 2
 F32, BF16, F16, F64 = 0, 1, 2, 3
 I32, I64, I8, E4M3 = 16, 17, 18, 19
 STATIC_BWD_MAX_QUERIES = 1 << 20

@@ -87,6 +87,7 @@ struct SharedPlan {
     Plan first, second;
     bool shares;
     bool many;       // the first part has tiles of many rows
+    bool fits;       // no launch has 2^32 threads
     int first_rows;  // of a place of its workspace
     int64_t second_at, floats;
 };
@@ -145,6 +146,9 @@ SharedPlan shared_plan(int B, int heads, int heads_kv, int T, int D, int page, i
         p.first_rows = 16;
         p.second_at = head_floats(entries) + p.first.items * heads_kv * item_floats(16, D);
     }
+    const int64_t joins = p.many ? (int64_t)runs * p.first.row_tiles * heads_kv * (p.first_rows / 16) * (padded(D) / 32)
+                                 : (int64_t)B * heads * T;
+    p.fits = joins <= 0xffffff && (p.first.items + p.second.items) * heads_kv <= 0xffffff;
     p.floats = p.second_at + head_floats((int64_t)B * p.second.row_tiles) + p.second.items * heads_kv * item_floats(p.second.rows, D);
     return p;
 }
@@ -160,10 +164,6 @@ int launch_type(const char *fn, const SharedArgs &a, int64_t items, hipStream_t 
 }
 template <int DP, bool E4M3>
 int launch_tiles(const char *fn, const SharedArgs &a, int rows, int64_t items, hipStream_t st) {
-    if (items * a.heads_kv > 0xffffff) {  // (2^32 threads)
-        set_error("%s: too many row tiles", fn);
-        return ENATTEN_EUNSUPPORTED;
-    }
     if (rows == 16) return launch_type<DP, 1, E4M3>(fn, a, items, st);
     if constexpr (DP <= 128) {
         if (rows == 32) return launch_type<DP, 2, E4M3>(fn, a, items, st);
@@ -194,7 +194,7 @@ size_t enatten_cache_attention_shared_workspace_bytes(int B, int heads, int head
         kernel_size < 0 || runs < 1 || B % runs || (int64_t)B * heads * T > (1 << 30))
         return 0;
     const SharedPlan p = shared_plan(B, heads, heads_kv, T, D, page, columns, kernel_size, dtype, runs);
-    return p.shares ? p.floats * sizeof(float) : workspace_bytes(p.second, B, heads_kv, D);
+    return !p.shares ? workspace_bytes(p.second, B, heads_kv, D) : p.fits ? p.floats * sizeof(float) : 0;
 }
 
 int enatten_cache_attention_shared(const void *q, const void *k_cache, const void *v_cache, const float *k_scale,
@@ -219,13 +219,13 @@ int enatten_cache_attention_shared(const void *q, const void *k_cache, const voi
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const bool e = cache_dtype == ENATTEN_E4M3;
     if (!p.shares) return launch_plain(fn, a, p.second, workspace, e, st);
+    if (!p.fits) {
+        set_error("%s: too many rows for sequences that are read together", fn);
+        return ENATTEN_EUNSUPPORTED;
+    }
     if (!workspace || (uintptr_t)workspace % 16) {
         set_error("%s: workspace is NULL or not 16-byte aligned", fn);
         return ENATTEN_EINVAL;
-    }
-    if (!p.many && (int64_t)B * heads * T > 0xffffff) {  // (2^32 threads that join the parts)
-        set_error("%s: too many rows", fn);
-        return ENATTEN_EUNSUPPORTED;
     }
     if (a.window >= (int64_t)columns * page) a.window = 0;  // (hides nothing: no row has to be asked where its begins)
     a.shared = shared;
@@ -239,7 +239,7 @@ int enatten_cache_attention_shared(const void *q, const void *k_cache, const voi
     a.row_tiles = p.second.row_tiles;
     a.parts = p.second.parts;
     if (p.many && (rc = launch_first_rows(fn, a, p.first.rows, e, st))) return rc;
-    a.first_items = p.many ? 0 : (int)p.first.items;
+    a.first_items = (int)p.first.items;
     if ((rc = launch_attend(fn, a, p.second.rows, a.first_items + p.second.items, e, st))) return rc;
     if (p.many) return launch_last_join(fn, a, p.first.rows, p.second.rows, st);
     ProfScope prof(ENATTEN_KERNEL_CACHE_JOIN, "run_join_tiles", st);

@@ -116,13 +116,9 @@ int first_rows(const char *fn, const SharedArgs &a, int rows, hipStream_t st) {
 }
 template <int DP, int DT>
 int join(const char *fn, const SharedArgs &a, int rows, int second, hipStream_t st) {
-    const int64_t blocks = (int64_t)a.runs * a.first_tiles * a.heads_kv * (a.first_rows / 16) * (DP / 32);
-    if (blocks > 0xffffff) {  // (2^32 threads)
-        set_error("%s: too many rows", fn);
-        return ENATTEN_EUNSUPPORTED;
-    }
+    const int blocks = a.runs * a.first_tiles * a.heads_kv * (a.first_rows / 16) * (DP / 32);  // (fewer than 2^24)
     ProfScope prof(ENATTEN_KERNEL_CACHE_JOIN, "run_join", st);
-    run_join<DP, DT><<<(int)blocks, 256, 0, st>>>(a, rows, second);
+    run_join<DP, DT><<<blocks, 256, 0, st>>>(a, rows, second);
     return launched(fn);
 }
 

@@ -275,20 +275,26 @@ Tensor cache_attention(const Tensor &q_, const Tensor &kc, const Tensor &vc, con
     const int window = (int)std::min<int64_t>(kernel_size, 0x7fffffff);
     const int B = q.size(0), N = q.size(1), Nk = kc.size(1), T = q.size(2), D = q.size(3);
     const int page = kc.size(2), columns = pages.size(1);
-    const Tensor shared = shared_.has_value() ? shared_->contiguous() : Tensor();
-    const int runs = shared.defined() ? shared.size(0) : 0;
-    const size_t need = runs ? enatten_cache_attention_shared_workspace_bytes(B, N, Nk, T, D, page, columns, window, dtype_code(q), runs)
-                             : enatten_cache_attention_workspace_bytes(B, N, Nk, T, D, page, columns, window, dtype_code(q));
-    const Tensor ws = need ? at::empty({(int64_t)need}, q.options().dtype(at::kByte)) : Tensor();
-    if (runs) {
-        check_rc(enatten_cache_attention_shared(
+    const auto workspace = [&](size_t need) { return need ? at::empty({(int64_t)need}, q.options().dtype(at::kByte)) : Tensor(); };
+    if (shared_.has_value()) {
+        const Tensor shared = shared_->contiguous();
+        const int runs = shared.size(0);
+        const size_t need = enatten_cache_attention_shared_workspace_bytes(B, N, Nk, T, D, page, columns, window, dtype_code(q), runs);
+        const Tensor ws = workspace(need);
+        const int rc = enatten_cache_attention_shared(
             q.data_ptr(), kc.data_ptr(), vc.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(), pages.data_ptr<int>(),
             lengths.data_ptr<int>(), counts.defined() ? counts.data_ptr<int>() : nullptr, shared.data_ptr<int>(), runs,
             o.data_ptr(), need ? ws.data_ptr() : nullptr, B, N, Nk, T, D, kc.size(0), page, columns, window, dtype_code(q),
             cache_code(kc), q.strides().data(), o.strides().data(), kc.strides().data(), vc.strides().data(),
-            ks.strides().data(), vs.strides().data(), pages.stride(0), (float)scale, stream_now()));
-        return o;
+            ks.strides().data(), vs.strides().data(), pages.stride(0), (float)scale, stream_now());
+        // (too many rows for that, and nothing queued: every sequence reads for itself)
+        if (rc != ENATTEN_EUNSUPPORTED) {
+            check_rc(rc);
+            return o;
+        }
     }
+    const size_t need = enatten_cache_attention_workspace_bytes(B, N, Nk, T, D, page, columns, window, dtype_code(q));
+    const Tensor ws = workspace(need);
     check_rc(enatten_cache_attention(
         q.data_ptr(), kc.data_ptr(), vc.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(), pages.data_ptr<int>(),
         lengths.data_ptr<int>(), counts.defined() ? counts.data_ptr<int>() : nullptr, o.data_ptr(),

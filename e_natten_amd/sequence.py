@@ -391,20 +391,25 @@ def _attention_impl(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, count
     with torch.cuda.device(q.device):
         o = _aligned_rows(_kernel_layout(torch.empty_like(rows)))
         sizes = (B, N, heads, T, D, page, columns, window, _DTYPES[q.dtype])
-        need = (lib.enatten_cache_attention_workspace_bytes(*sizes) if shared is None
-                else lib.enatten_cache_attention_shared_workspace_bytes(*sizes, shared.shape[0]))
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         data = (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                 pages.data_ptr(), lengths.data_ptr(), None if counts is None else counts.data_ptr())
-        rest = (o.data_ptr(), ws.data_ptr() if need else None, B, N, heads, T, D, k_cache.shape[0], page, columns, window,
+        rest = (B, N, heads, T, D, k_cache.shape[0], page, columns, window,
                 _DTYPES[q.dtype], _CACHE_DTYPES[k_cache.dtype], _lib.strides3(q), _lib.strides3(o),
                 _lib.strides3(k_cache), _lib.strides3(v_cache), _lib.strides2(k_scale), _lib.strides2(v_scale),
                 pages.stride(0), float(scale), _stream_of(q))
-        if shared is None:
-            _check(lib.enatten_cache_attention(*data, *rest))
-        else:
+
+        def run(entry, need, *extra):
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+            return entry(*data, *extra, o.data_ptr(), ws.data_ptr() if need else None, *rest)
+
+        rc = _lib.EUNSUPPORTED
+        if shared is not None:
             shared = shared.contiguous()
-            _check(lib.enatten_cache_attention_shared(*data, shared.data_ptr(), shared.shape[0], *rest))
+            rc = run(lib.enatten_cache_attention_shared,
+                     lib.enatten_cache_attention_shared_workspace_bytes(*sizes, shared.shape[0]), shared.data_ptr(), shared.shape[0])
+        if rc == _lib.EUNSUPPORTED:   # (too many rows for sharing, and nothing queued: every sequence reads for itself)
+            rc = run(lib.enatten_cache_attention, lib.enatten_cache_attention_workspace_bytes(*sizes))
+        _check(rc)
     return o
 
 
