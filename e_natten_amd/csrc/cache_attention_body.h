@@ -85,6 +85,7 @@ __device__ __forceinline__ void attend_body(const Args &a) {
     int step0 = w.step0, step1 = w.step1;
     if constexpr (kShared<Args>) {
         if (first) {
+            if (s.hi == 0) return;  // (a run that shares nothing leaves nothing)
             b = reader_of(a, which, s.hi);
             if (b < 0) b = which * a.size, step0 = step1 = 0;  // (nobody reads them)
         } else {

@@ -77,6 +77,16 @@ __device__ __forceinline__ void rows_body(const Args &args) {
     for (; at_step < end; into = 0) {
     const Args &a = args_again<Args>();
     const Span s = span_of<ROWS>(a, entry, FIRST);
+    if constexpr (FIRST) {
+        if (s.hi == 0) {  // a run that shares nothing leaves nothing: its tile counts as one step
+            at_step++;
+            if (++entry == entries) {
+                entry = 0;
+                head++;
+            }
+            continue;
+        }
+    }
     const int total = steps_of<TOK>(s), counted = max(1, total), step0 = into;
     int step1 = line.whole ? total : min(total, (int)min((int64_t)counted, step0 + (end - at_step)));
     const bool parted = FIRST || (!line.whole && (into || step0 + (end - at_step) < counted));

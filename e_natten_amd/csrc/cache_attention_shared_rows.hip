@@ -35,7 +35,8 @@ __global__ __launch_bounds__(256) void run_join(SharedArgs a, int tile_rows, int
     const int which = entry / a.first_tiles, row = (entry - which * a.first_tiles) * tile_rows + r;
     if (row - n >= all_rows || split * 32 >= a.D) return;
     const int *ranges = reinterpret_cast<const int *>(a.first_ws) + 2 * tile;
-    const int first = ranges[0], parts = ranges[1] - first + 1;
+    const int end = shared_end(a, which);  // (0: the first part left nothing)
+    const int first = end ? ranges[0] : 0, parts = end ? ranges[1] - first + 1 : 0;
     // rows behind the last one have no sums: they go along with its
     const int from = min(r, all_rows - 1 - (row - r));
     auto part_at = [&](int q) { return stair_of(a, (int64_t)first + q + tile); };
@@ -82,7 +83,8 @@ __global__ __launch_bounds__(256) void run_join(SharedArgs a, int tile_rows, int
     const Place where = place_of(a, which, head, row, true);
     int len, count;
     const bool ok = sequence_of(a.tb, where.b, len, count);
-    if (!(ok && count > 0 && len - count >= shared_end(a, which))) {  // (it does not share them)
+    const bool shares = end && ok && count > 0 && len - count >= end;
+    if (!shares) {
         top = kFloor;
         sum = 0.f;
         z = f32x4{0.f, 0.f, 0.f, 0.f};

@@ -382,7 +382,8 @@ int enatten_cache_attention(const void *q, const void *k_cache, const void *v_ca
  * tokens are read once for all rows of the run.  A sequence whose new tokens start before that end is
  * computed by itself, and a number below 1 shares nothing: results are enatten_cache_attention's but
  * for where they are rounded.  The pages are those of the run's first sequence that shares them.  Where it
- * would not pay, by the sizes of the call, every sequence reads for itself.  With more rows than a launch
+ * would not pay, by the sizes of the call, every sequence reads for itself.  As lengths are not known on the host,
+ * `columns` stands for them: pass those that the longest sequence needs, with the table's stride.  With more rows than a launch
  * joins (2^24, or 2^24 groups of 16 rows and 32 channels where a run has more than 16) nothing is queued and
  * ENATTEN_EUNSUPPORTED returned, the workspace's size being 0: enatten_cache_attention takes such calls.
  */
