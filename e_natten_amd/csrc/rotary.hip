@@ -216,12 +216,15 @@ int launch_tokens(const char *fn, RotaryArgs &a, hipStream_t st) {
     // 28; 2 + 2, 8 x 16384 28.2 and 25.1; 3 + 2, 16 x 4096, float16 18.5 and 17.2; 1 + 1 of 128, 8192 single tokens 14.3
     // and 13.8, but 27 with eight of them.  With more heads it does not pay: 4 + 4 of 128, 4 x 16384 tokens 46 and 48; 32 +
     // 8, 32 x 1024 141 and 149; 16 + 4, 16384 single tokens 31 and, 16 of them, 38.  With fewer workgroups neither: one
-    // head of 128, 2048 single tokens 5.1 and 5.7.  With two axes 4 + 4 heads of 128, 4 x 16384 46.3 and 48.6; 3 + 2, 16 x
-    // 4096 20.0 and 17.7.
+    // head of 128, 2048 single tokens 5.1 and 5.7.
+    // With axes turns take longer, and it pays up to 8 heads and with 1024 workgroups left.  Two of them: the images of the
+    // top 59.9 and 57.6 (55.9 and 55.2 in a graph), 4 + 4 heads of 64, 256 x 128 15.8 and 14.8, 8 x 8192 24.3 and 23.8, 3 +
+    // 2, 16 x 4096, float16 20.0 and 17.7, but 4 + 4 of 128 that lie [token, head], 4 x 16384 46.3 and 48.6; 8 + 8 of
+    // 64, 4 x 16384 45.4 and 47.6; 32 + 8 of 128, 32 x 1024 142 and 149.
     const auto blocks_of = [&](int64_t batches) { return (a.B + batches - 1) / batches * a.tiles * a.slices; };
     a.batches = 1;
-    if (a.positions_stride == 0 && heads < 8)
-        while (a.batches < 4 && a.batches < a.B && blocks_of(2 * (int64_t)a.batches) >= 2048) a.batches *= 2;
+    if (a.positions_stride == 0 && heads <= (AXES ? 8 : 7))
+        while (a.batches < 4 && a.batches < a.B && blocks_of(2 * (int64_t)a.batches) >= (AXES ? 1024 : 2048)) a.batches *= 2;
     const int64_t blocks = blocks_of(a.batches);
     if (blocks > 0xffffff) {  // (2^32 threads)
         set_error("%s: too many tokens", fn);
