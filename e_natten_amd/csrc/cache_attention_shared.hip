@@ -13,9 +13,12 @@
 // holds as float16, and a launch of its own.
 //
 // Measured on MI355X, launches under the profiler, bfloat16, heads of 128 channels.  8 sequences, 16 + 16 heads, 480
-// shared tokens and up to 40 of their own, int8: 8.8 us and 4.0 for the join.  64 sequences, 32 + 8
-// heads, 16384 shared tokens and up to 500, E4M3: 35.6 us for the shared tokens (17.2 GFLOP, 480 TFLOP/s), 15.2 for the
-// others, join 7.2.  16 runs of 4, 32 + 4 heads, up to 8192 shared tokens each and up to 300, int8: 42.1, 13.0 and 6.0.
+// shared tokens and up to 40 of their own, int8: 8.8 us and 3.5 for the join.  64 sequences, 32 + 8
+// heads, 16384 shared tokens and up to 500, E4M3: 35.6 us for the shared tokens (17.2 GFLOP, 480 TFLOP/s), 14.8 for the
+// others, join 7.4.  16 runs of 4, 32 + 4 heads, up to 8192 shared tokens each and up to 300, int8: 41.5, 12.7 and 5.7.
+// float32, 16 sequences of 8192 shared tokens, 8 + 8 heads: 15.5 in all (float16 14.8); 64 of them, 16 + 4 heads: 47.6;
+// two runs of 14, 5 new tokens, 16 + 4 heads: float16 and bfloat16 52.7, with a window of 6000 tokens 51.8.
+// Probabilities take 11 bits into the second product, as in cache_attention.hip; tiles of many rows sum them before that.
 // Beside the first launches' steps, about 10 us each go to chains of loads (lengths, pages, codes, q) and the code's
 // first run.
 #include "cache_attention_body.h"

@@ -9,7 +9,8 @@
 // Measured on MI355X, single launches under the profiler.  4 beams, pages of 16: fork 2.4 us, reserve 5.1, copy 3.8.
 // 128 samples of 32 prompts, pages of 64, 4 layers of 8 heads of 128: 3.1, 7.1 and 13.8 (50 MB, 3.6 TB/s).  64 rows of
 // 1025 columns, half of which get prompts of up to 8192 tokens, pages of 16: 6.1 (two launches), 18.2 and 3.8.
-// compact: 216 pages 6.2 us; 1594 pages 6.7, and 23.6 for the copy that it asks for (100 MB, 4.2 TB/s).
+// compact: 216 pages 6.0 us; 1594 pages 6.7, and 24.3 for the copy that it asks for (100 MB, 4.1 TB/s); in a graph 15.0 for
+// 16384 pages and entries, and in three launches 10.2 for 3000 pages in a table of 64 x 1025, 12.4 for 65536, 34.8 for 10^6.
 #include "sequence_common.h"
 
 namespace enatten {

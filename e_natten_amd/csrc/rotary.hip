@@ -13,8 +13,8 @@
 // [token, head] (4.8 TB/s, a plain copy of that size reaches 5.0), 46 us where they lie [head, token];
 // 16 + 4 heads of 128, 64 of them turned, 2 x 8192 tokens, float16: 29 us; 64 single tokens: 3.5 us.
 // 8 + 8 heads of 64 channels, 4 x 8192 tokens, by type: bfloat16 25 us, float32 48 (5.6 TB/s), float64 108 (5.0).
-// Two axes, 4 + 4 heads of 128 channels, 4 images of 128 x 128 as a projection leaves them, bfloat16: 53.6 us (5.0 TB/s);
-// three axes, 16 + 4 heads of 128, 96 of them turned, interleaved, 2 x 8192 tokens, float16: 30.6; 8 single tokens: 3.8.
+// Two axes, 4 + 4 heads of 128 channels, 4 images of 128 x 128 as a projection leaves them, bfloat16: 55 us (4.9 TB/s);
+// three axes, 16 + 4 heads of 128, 96 of them turned, interleaved, 2 x 8192 tokens, float16: 30.9; 8 single tokens: 4.0.
 // Stores past the caches take 47 us instead of 56, but the reader that follows pays: with one pass over
 // both results behind it 114 us instead of 99.
 #include "sequence_common.h"

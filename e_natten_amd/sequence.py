@@ -472,7 +472,7 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, kerne
     These sizes are the table's, as lengths are not known here: with a table much wider than the sequences are long,
     a call takes some 20 us more than without ``shared``.  So pass the columns that the longest sequence needs,
     ``pages[:, :n]``, or leave ``shared`` out.  Where only the device knows, numbers of 0 take most of that back: 4 to
-    7 us are left for single tokens.  Reading together pays from 16 MB of codes that the sequences have in all, shared
+    8 us are left for single tokens.  Reading together pays from 16 MB of codes that the sequences have in all, shared
     ones counted for each of them, with up to 16 rows in a run (new tokens times heads of q for one of the cache),
     160 MB beyond.
     """
