@@ -12,8 +12,9 @@ a program keeps ``holders``, how many entries of the table name each page; a pag
     o = cache_attention(q, k_cache, v_cache, k_scale, v_scale, pages, lengths, None, scale, counts, shared)
 
 No call waits for the GPU, so a step can be captured into a graph; what they write depends on their
-arguments alone.  An entry of the table outside the cache's pages is no page (these calls write -1), and all
-of a row counts, also behind its last token: a table starts filled with -1.  At most 2^30 pages.
+arguments alone.  An entry of the table outside the cache's pages is no page (these calls write -1, but a
+row that continues another has its entries as they are), and all of a row counts, also behind its last
+token: a table starts filled with -1.  At most 2^30 pages.
 
 Like the others they run through the native torch binding where it is built (operators
 ``enatten::cache_fork``, ...), else through ctypes.

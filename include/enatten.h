@@ -403,10 +403,11 @@ int enatten_cache_attention_shared(const void *q, const void *k_cache, const voi
 /*
  * Pages that sequences share, leave and get.  Beside the table and the lengths:
  *   holders    int32 [num_pages]: how many entries of the table name each page; 0: free
- * An entry of the table outside 0 .. num_pages - 1 is no page (-1 is written).  All of a row counts, also
- * entries behind its last token.  What the calls write depends on their arguments alone: pages are given
- * out from the lowest free one on, to rows and columns in their order.  At most 4096 rows, 2^30
- * entries and 2^30 pages.  What a call writes must not share memory with its other arguments.
+ * An entry of the table outside 0 .. num_pages - 1 is no page (-1 is written, but a row that continues
+ * another has its entries as they are).  All of a row counts, also entries behind its last token.  What
+ * the calls write depends on their arguments alone: pages are given out from the lowest free one on, to
+ * rows and columns in their order.  At most 4096 rows, 2^30 entries and 2^30 pages.  What a call writes
+ * must not share memory with its other arguments.
  *
  * enatten_cache_fork: row b becomes what row parents[b] was: the pages of its lengths[parents[b]] tokens,
  * which both hold then, and its length.  -1 leaves it empty; its own number, or any other, as it is.
